@@ -498,6 +498,105 @@ int tccl_word_reached(int32_t word, int32_t need);
 int tccl_mfma_rate_probe(int32_t kind, const void* a_like, int64_t a_bytes, const void* b_like,
                          int64_t b_bytes, float* sink, int32_t steps, int32_t workgroups, void* stream);
 
+/* ---- between the GEMMs and collectives of a training step ----------------------------------------
+ * No counterpart in the reference, which ends at the GEMM and the collective.  Matrices are row-major with
+ * contiguous rows of any alignment and pitches (ld, elements) of at least `cols`; rows >= 0, cols >= 1.
+ *
+ * Activations in 8 bits.  A rows x cols tensor of TCCL_F16 or TCCL_BF16 is held in blocks of TCCL_HELD_ROWS x
+ * TCCL_HELD_COLS: with e the smallest whole number, not under -117, with max|x| <= 448 * 2^e over the block's finite
+ * values, a value is held as the e4m3 of x / 2^e (exact division, round to nearest even), what is not finite as NaN.
+ * The value that is held, q * 2^e, is exact in the tensor's type.  With RB = ceil(rows / 8), CB = ceil(cols / 128):
+ *   values  uint8[RB][128 * CB][8]     row block, column, row in the block; zeros beyond the tensor; on 16 bytes
+ *   scales  uint8[CB][SP]              e + 127 of column block, row block; SP = RB rounded up to 16; bytes from RB on
+ *                                      are not read */
+#define TCCL_HELD_ROWS 8
+#define TCCL_HELD_COLS 128
+typedef struct tccl_held_desc {
+  void* x;       /* tccl_hold: read; tccl_restore: written */
+  void* values;
+  void* scales;
+  int64_t ld;
+  int32_t rows, cols;
+  int32_t dtype; /* of x */
+} tccl_held_desc;
+int tccl_hold(const tccl_held_desc* held, void* stream);
+int tccl_restore(const tccl_held_desc* held, void* stream);
+
+/* Layer norm over the columns of each row: s = x, or x + residual rounded to x's type and stored to `summed`;
+ * out = (s - mean) * rstd * weight + bias with rstd = 1 / sqrt(var + eps), var the mean of (s - mean)^2.  Sums are
+ * fp32.  values / scales: s in 8 bits too (16-bit types; NULL: not wanted).  weight, bias NULL: one, zero.  `out` and
+ * `summed` may be x or residual themselves.  At most TCCL_NORM_MAX_COLS columns. */
+#define TCCL_NORM_MAX_COLS 32768
+typedef struct tccl_norm_desc {
+  const void* x;
+  const void* residual; /* or NULL */
+  void* summed;         /* with residual only */
+  void* out;
+  float* mean;          /* rows */
+  float* rstd;          /* rows */
+  const void* weight;   /* cols, affine_dtype */
+  const void* bias;
+  void* values;
+  void* scales;
+  int64_t ld_x, ld_residual, ld_summed, ld_out;
+  int32_t rows, cols;
+  int32_t dtype;        /* x, residual, summed, out: F16, BF16 or F32 */
+  int32_t affine_dtype; /* weight, bias: dtype, or F32 */
+  float eps;
+} tccl_norm_desc;
+int tccl_layer_norm(const tccl_norm_desc* norm, void* stream);
+
+/* Its gradients.  grad: that of `out`.  The norm's input s comes as x, or as values / scales with x NULL.
+ * dx = rstd * (g - mean(g) - xh * mean(g * xh)) + grad_summed with g = grad * weight, xh = (s - mean) * rstd, means over
+ * the row; dweight = sum over rows of grad * xh, dbeta = sum over rows of grad (fp32, NULL: not wanted), added in an
+ * order that depends on the sizes only.  dx may be grad or grad_summed itself.  `workspace`: device memory of
+ * tccl_layer_norm_grad_workspace(rows, cols, dtype, held) bytes on 16 bytes; `held`: whether values are given. */
+typedef struct tccl_norm_grad_desc {
+  const void* grad;
+  const void* x;
+  const void* values;
+  const void* scales;
+  const void* grad_summed; /* or NULL */
+  const float* mean;
+  const float* rstd;
+  const void* weight;
+  void* dx;
+  float* dweight;
+  float* dbias;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t ld_grad, ld_x, ld_grad_summed, ld_dx;
+  int32_t rows, cols;
+  int32_t dtype;
+  int32_t affine_dtype;
+} tccl_norm_grad_desc;
+int64_t tccl_layer_norm_grad_workspace(int32_t rows, int32_t cols, int32_t dtype, int32_t held);
+int tccl_layer_norm_grad(const tccl_norm_grad_desc* norm, void* stream);
+
+/* Weight gradient of a linear layer from its input in 8 bits: W[h][n] = sum over rows t of x[t][h] * grad[t][n]
+ * (+ add[h][n]), x the values that are held (rows x cols), grad rows x outputs of the type x was held from, in fp32
+ * with one rounding to out_dtype (F32 or that type).  transposed: out and add are outputs x cols (element (h, n) at
+ * n * ld + h), the layout of a weight that is multiplied as its .t() view.  `add` NULL: none; it may be `out`.
+ * grad's rows start on 16 bytes and are readable in whole 16-byte vectors, past the last of `outputs` columns too (what
+ * lies there has no part in the result).  `workspace`: device memory of
+ * tccl_weight_gradient_workspace(rows, cols, outputs) bytes on 16 bytes (0: none). */
+typedef struct tccl_weight_gradient_desc {
+  const void* values;
+  const void* scales;
+  const void* grad;
+  const void* add;
+  void* out;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t ld_grad, ld_add, ld_out;
+  int32_t rows, cols, outputs;
+  int32_t dtype;      /* grad: F16 or BF16 */
+  int32_t out_dtype;  /* add, out */
+  int32_t transposed;
+} tccl_weight_gradient_desc;
+int64_t tccl_weight_gradient_workspace(int32_t rows, int32_t cols, int32_t outputs);
+int tccl_weight_gradient(const tccl_weight_gradient_desc* wg, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

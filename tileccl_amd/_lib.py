@@ -133,6 +133,92 @@ class PackDesc(C.Structure):
     ]
 
 
+class HeldDesc(C.Structure):
+    """``tccl_held_desc``: a tensor and its 8-bit values."""
+
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("values", C.c_void_p),
+        ("scales", C.c_void_p),
+        ("ld", C.c_int64),
+        ("rows", C.c_int32),
+        ("cols", C.c_int32),
+        ("dtype", C.c_int32),
+    ]
+
+
+class NormDesc(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("residual", C.c_void_p),
+        ("summed", C.c_void_p),
+        ("out", C.c_void_p),
+        ("mean", C.c_void_p),
+        ("rstd", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("bias", C.c_void_p),
+        ("values", C.c_void_p),
+        ("scales", C.c_void_p),
+        ("ld_x", C.c_int64),
+        ("ld_residual", C.c_int64),
+        ("ld_summed", C.c_int64),
+        ("ld_out", C.c_int64),
+        ("rows", C.c_int32),
+        ("cols", C.c_int32),
+        ("dtype", C.c_int32),
+        ("affine_dtype", C.c_int32),
+        ("eps", C.c_float),
+    ]
+
+
+class NormGradDesc(C.Structure):
+    _fields_ = [
+        ("grad", C.c_void_p),
+        ("x", C.c_void_p),
+        ("values", C.c_void_p),
+        ("scales", C.c_void_p),
+        ("grad_summed", C.c_void_p),
+        ("mean", C.c_void_p),
+        ("rstd", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("dx", C.c_void_p),
+        ("dweight", C.c_void_p),
+        ("dbias", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+        ("ld_grad", C.c_int64),
+        ("ld_x", C.c_int64),
+        ("ld_grad_summed", C.c_int64),
+        ("ld_dx", C.c_int64),
+        ("rows", C.c_int32),
+        ("cols", C.c_int32),
+        ("dtype", C.c_int32),
+        ("affine_dtype", C.c_int32),
+    ]
+
+
+class WeightGradientDesc(C.Structure):
+    _fields_ = [
+        ("values", C.c_void_p),
+        ("scales", C.c_void_p),
+        ("grad", C.c_void_p),
+        ("add", C.c_void_p),
+        ("out", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+        ("ld_grad", C.c_int64),
+        ("ld_add", C.c_int64),
+        ("ld_out", C.c_int64),
+        ("rows", C.c_int32),
+        ("cols", C.c_int32),
+        ("outputs", C.c_int32),
+        ("dtype", C.c_int32),
+        ("out_dtype", C.c_int32),
+        ("transposed", C.c_int32),
+    ]
+
+
+HELD_ROWS, HELD_COLS, NORM_MAX_COLS = 8, 128, 32768  # TCCL_HELD_ROWS, TCCL_HELD_COLS, TCCL_NORM_MAX_COLS
 STATIC_MAX_TILES, STATIC_MAX_GROUPS = 16384, 64
 
 
@@ -206,6 +292,13 @@ SIGNATURES = {
     "tccl_static_call_words": (C.c_int, [C.c_uint32, _i32, _P(_i32), _P(_i32), _P(_i32)]),
     "tccl_word_reached": (C.c_int, [_i32, _i32]),
     "tccl_static_reset": (C.c_int, [_vp]),
+    "tccl_hold": (C.c_int, [_P(HeldDesc), _vp]),
+    "tccl_restore": (C.c_int, [_P(HeldDesc), _vp]),
+    "tccl_layer_norm": (C.c_int, [_P(NormDesc), _vp]),
+    "tccl_layer_norm_grad_workspace": (_i64, [_i32, _i32, _i32, _i32]),
+    "tccl_layer_norm_grad": (C.c_int, [_P(NormGradDesc), _vp]),
+    "tccl_weight_gradient_workspace": (_i64, [_i32, _i32, _i32]),
+    "tccl_weight_gradient": (C.c_int, [_P(WeightGradientDesc), _vp]),
     "tccl_mfma_rate_probe": (C.c_int, [_i32, _vp, _i64, _vp, _i64, _vp, _i32, _i32, _vp]),
     "tccl_gemm_reducescatter": (
         C.c_int,

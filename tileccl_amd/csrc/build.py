@@ -2,9 +2,10 @@
 
     python -m tileccl_amd.csrc.build
 
-The library is three translation units (``tccl_api.hip``: entry points and the kernels for
+The library is five translation units (``tccl_api.hip``: entry points and the kernels for
 row-major B; ``tccl_kmajor.hip``: the large-tile kernels for k-major B; ``tccl_stream.hip``: the
-streaming kernels) compiled side by side and linked.  Beside it the CPython extension ``_host.so``
+streaming kernels; ``tccl_norm.hip``: layer norm and activations in 8 bits; ``tccl_weight.hip``: weight
+gradients from them) compiled side by side and linked.  Beside it the CPython extension ``_host.so``
 (``tccl_host.cpp``, host code only) is built with the host compiler.  Both lie next to the Python
 package so that they travel with the source tree.
 """
@@ -21,9 +22,9 @@ HERE = Path(__file__).resolve().parent
 OUT = HERE.parent / "libtileccl_hip.so"
 HOST_OUT = HERE.parent / "_host.so"
 HOST_SOURCE = HERE / "tccl_host.cpp"
-SOURCES = [HERE / "tccl_api.hip", HERE / "tccl_kmajor.hip", HERE / "tccl_stream.hip"]
+SOURCES = [HERE / "tccl_api.hip", HERE / "tccl_kmajor.hip", HERE / "tccl_stream.hip", HERE / "tccl_norm.hip", HERE / "tccl_weight.hip"]
 HEADERS = [HERE / "tccl_device.h", HERE / "tccl_gemm.h", HERE / "tccl_gemm256.h", HERE / "tccl_kernels256.h", HERE / "tccl_comm.h", HERE / "tccl_bulk.h", HERE / "tccl_stream.h",
-           HERE / "tccl_staged.h", HERE / "tccl_probe.h", HERE.parent.parent / "include" / "tileccl_hip.h"]
+           HERE / "tccl_staged.h", HERE / "tccl_probe.h", HERE / "tccl_host.h", HERE / "tccl_norm.h", HERE / "tccl_weight.h", HERE.parent.parent / "include" / "tileccl_hip.h"]
 
 FLAGS = [
     "--offload-arch=gfx950",

@@ -1521,6 +1521,17 @@ __global__ void static_setup_kernel(StaticScratch* s, tccl_static_plan plan, int
 // ============================================================================================
 // extern "C"
 // ============================================================================================
+// For the entry points of the other translation units (tccl_host.h).
+namespace tccl {
+int report(int code, const char* text) { return fail(code, "%s", text); }
+int compute_units(int* out) {
+  tccl_device_info info;
+  const int rc = query_device(-1, &info);
+  *out = rc ? 0 : info.compute_units;
+  return rc;
+}
+}  // namespace tccl
+
 extern "C" {
 
 int tccl_abi_version(void) { return TCCL_ABI_VERSION; }

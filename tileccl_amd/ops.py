@@ -53,9 +53,27 @@ __all__ = [
     "GemmAllScatterPlan",
     "GemmAllScatterMixedLayoutPlan",
     "GemmAllScatterContract",
+    "ActivationCheckpoint",
+    "LayerNormResult",
+    "LayerNormGradients",
+    "layer_norm",
+    "layer_norm_backward",
+    "checkpoint_activation",
+    "restore_activation",
+    "weight_gradient",
 ]
 
 from tileccl_amd.ops_collective import gemm_allgather, gemm_reducescatter  # noqa: E402  (re-exported)
+from tileccl_amd.ops_training import (  # noqa: E402  (re-exported)
+    ActivationCheckpoint,
+    LayerNormGradients,
+    LayerNormResult,
+    checkpoint_activation,
+    layer_norm,
+    layer_norm_backward,
+    restore_activation,
+    weight_gradient,
+)
 from tileccl_amd.ops_plans import (  # noqa: E402  (re-exported)
     AllGatherGemmReduceScatterContract,
     AllGatherGemmReduceScatterPlan,
