@@ -6,7 +6,7 @@ The library is five translation units (``tccl_api.hip``: entry points and the ke
 row-major B; ``tccl_kmajor.hip``: the large-tile kernels for k-major B; ``tccl_stream.hip``: the
 streaming kernels; ``tccl_norm.hip``: layer norm and activations in 8 bits; ``tccl_weight.hip``: weight
 gradients from them) compiled side by side and linked.  Beside it the CPython extension ``_host.so``
-(``tccl_host.cpp``, host code only) is built with the host compiler.  Both lie next to the Python
+(``tccl_host.cpp`` and ``tccl_host_ops.cpp``, host code only) is built with the host compiler.  Both lie next to the Python
 package so that they travel with the source tree.
 """
 
@@ -21,7 +21,7 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 OUT = HERE.parent / "libtileccl_hip.so"
 HOST_OUT = HERE.parent / "_host.so"
-HOST_SOURCE = HERE / "tccl_host.cpp"
+HOST_SOURCES = [HERE / "tccl_host.cpp", HERE / "tccl_host_ops.cpp"]
 SOURCES = [HERE / "tccl_api.hip", HERE / "tccl_kmajor.hip", HERE / "tccl_stream.hip", HERE / "tccl_norm.hip", HERE / "tccl_weight.hip"]
 HEADERS = [HERE / "tccl_device.h", HERE / "tccl_gemm.h", HERE / "tccl_gemm256.h", HERE / "tccl_kernels256.h", HERE / "tccl_comm.h", HERE / "tccl_bulk.h", HERE / "tccl_stream.h",
            HERE / "tccl_staged.h", HERE / "tccl_probe.h", HERE / "tccl_host.h", HERE / "tccl_norm.h", HERE / "tccl_weight.h", HERE.parent.parent / "include" / "tileccl_hip.h"]
@@ -62,7 +62,7 @@ def host_command(out: Path = HOST_OUT) -> list[str]:
     return [
         "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
         f"-I{root / 'include'}", f"-I{root / 'include/torch/csrc/api/include'}", f"-I{sysconfig.get_paths()['include']}",
-        str(HOST_SOURCE), "-o", str(out), f"-L{root / 'lib'}", "-ltorch_python", "-lc10",
+        *map(str, HOST_SOURCES), "-o", str(out), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-ltorch_hip", "-lc10",
     ]
 
 

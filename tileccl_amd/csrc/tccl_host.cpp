@@ -25,6 +25,7 @@
 #include <vector>
 
 #include "../../include/tileccl_hip.h"
+#include "tccl_host_ops.h"
 
 namespace {
 
@@ -646,7 +647,7 @@ PyMODINIT_FUNC PyInit__host() {
   sRevision = PyUnicode_InternFromString("revision");
   device0 = PyLong_FromLong(0);  // every rank lives on device 0
   PyObject* m = PyModule_Create(&module_def);
-  if (!m) return nullptr;
+  if (!m || PyModule_AddFunctions(m, operator_methods()) < 0) return nullptr;
   Py_INCREF(&CallType);
   Py_INCREF(&TableType);
   Py_INCREF(kGemm);

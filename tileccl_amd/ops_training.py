@@ -17,8 +17,7 @@ Tensors may lie on a symmetric heap or elsewhere on the device; launches go to t
 from __future__ import annotations
 
 import ctypes as C
-from dataclasses import dataclass
-from typing import Any, NamedTuple
+from typing import Any, NamedTuple, NoReturn
 
 import torch
 
@@ -39,8 +38,7 @@ _HELD_TYPES = (torch.float16, torch.bfloat16)
 _TYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 
-@dataclass(frozen=True, slots=True)
-class ActivationCheckpoint:
+class ActivationCheckpoint(NamedTuple):
     """A ``rows x columns`` tensor of ``dtype`` in 8 bits.
 
     ``values``: uint8 ``[ceil(rows / 8), 128 * ceil(columns / 128), 8]``, the e4m3 codes by row block, column, row in the
@@ -84,6 +82,31 @@ class LayerNormGradients(NamedTuple):
     x: torch.Tensor
     weight: torch.Tensor | None
     bias: torch.Tensor | None
+
+
+_native = None  # the operators of the extension module, once they have been used
+
+
+def _bind() -> Any:
+    """The host side of the operators (``csrc/tccl_host_ops.cpp``): checks, outputs, workspace, launch."""
+    global _native
+    if _native is None:
+        host, lib = _lib.host(), _lib.load()
+        entries = (lib.tccl_layer_norm, lib.tccl_layer_norm_grad, lib.tccl_layer_norm_grad_workspace, lib.tccl_hold, lib.tccl_restore,
+                   lib.tccl_weight_gradient, lib.tccl_weight_gradient_workspace)
+        host.bind_operators(_launch._raw_stream or (lambda _device: _launch.stream_ptr()), _lib.check,
+                            (LayerNormResult, LayerNormGradients, ActivationCheckpoint), _TYPES,
+                            tuple(C.cast(e, C.c_void_p).value for e in entries))
+        _native = host
+    return _native
+
+
+# Each operator is one call of the extension module, which answers None to arguments that it does not take.  The functions
+# from here on say what is wrong with them.
+
+
+def _unexplained(op: str) -> NoReturn:
+    raise RuntimeError(f"{op}: arguments were refused for no reason that is known here")
 
 
 def _matrix(t: Any, name: str, op: str, *, like: torch.Tensor | None = None, shape: tuple[int, int] | None = None, dtype=None) -> int:
@@ -164,47 +187,33 @@ def layer_norm(
     ``checkpoint``: also hold the norm's input in 8 bits, for ``layer_norm_backward``.  ``out`` (for instance on the
     symmetric heap) may be ``x`` or ``residual`` itself.
     """
+    result = (_native or _bind()).layer_norm(x, weight, bias, eps, residual, checkpoint, out)
+    if result is None:
+        _refuse_layer_norm(x, weight, bias, residual, checkpoint, out)
+    return result
+
+
+def _refuse_layer_norm(x, weight, bias, residual, checkpoint, out) -> NoReturn:
     op = "layer_norm"
-    ld_x = _matrix(x, "x", op)
+    _matrix(x, "x", op)
     if x.dtype not in _TYPES:
         raise ValueError(f"{op}: x must be float16, bfloat16 or float32, got {x.dtype}")
-    rows, cols = x.shape
+    cols = x.shape[1]
+    if cols > _lib.NORM_MAX_COLS:
+        raise ValueError(f"{op}: {cols} columns, at most {_lib.NORM_MAX_COLS}")
     if checkpoint and x.dtype not in _HELD_TYPES:
         raise ValueError(f"{op}: a checkpoint holds float16 or bfloat16, not {x.dtype}")
-    d = _lib.NormDesc()
-    affine = None
     for t, name in ((weight, "weight"), (bias, "bias")):
         if t is not None:
             _vector(t, name, op, cols, x.device, (x.dtype,) if x.dtype == torch.float32 else (x.dtype, torch.float32))
-            if affine is not None and t.dtype != affine:
-                raise ValueError(f"{op}: weight and bias must share one dtype, got {affine} and {t.dtype}")
-            affine = t.dtype
-    summed = None
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError(f"{op}: weight and bias must share one dtype, got {weight.dtype} and {bias.dtype}")
     if residual is not None:
-        d.ld_residual = _matrix(residual, "residual", op, like=x)
-        summed = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-        d.residual, d.summed, d.ld_summed = residual.data_ptr(), summed.data_ptr(), cols
-    if out is None:
-        out = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-        d.ld_out = cols
-    else:
-        d.ld_out = _matrix(out, "out", op, like=x)
+        _matrix(residual, "residual", op, like=x)
+    if out is not None:
+        _matrix(out, "out", op, like=x)
         _apart(out, "out", op, x, residual)
-    mean = torch.empty(rows, dtype=torch.float32, device=x.device)
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
-    held = None
-    if checkpoint:
-        held = ActivationCheckpoint.empty(rows, cols, x.dtype, x.device)
-        d.values, d.scales = held.values.data_ptr(), held.scales.data_ptr()
-    d.x, d.out, d.mean, d.rstd = x.data_ptr(), out.data_ptr(), mean.data_ptr(), rstd.data_ptr()
-    d.weight, d.bias = _launch.ptr(weight), _launch.ptr(bias)
-    d.ld_x, d.rows, d.cols, d.eps = ld_x, rows, cols, eps
-    d.dtype = _launch.dtype_code(x.dtype)
-    d.affine_dtype = d.dtype if affine is None else _launch.dtype_code(affine)
-    rc = _lib.load().tccl_layer_norm(C.byref(d), _launch.stream_ptr())
-    if rc:
-        _lib.check(rc, "tccl_layer_norm")
-    return LayerNormResult(out, mean, rstd, summed, held)
+    _unexplained(op)
 
 
 def layer_norm_backward(
@@ -225,57 +234,37 @@ def layer_norm_backward(
     are float32, in an order that depends on the sizes only; ``affine=False`` leaves them out.  ``out`` may be ``grad`` or
     ``grad_summed`` itself.
     """
+    result = (_native or _bind()).layer_norm_backward(grad, x, mean, rstd, weight, grad_summed, affine, out)
+    if result is None:
+        _refuse_layer_norm_backward(grad, x, mean, rstd, weight, grad_summed, out)
+    return result
+
+
+def _refuse_layer_norm_backward(grad, x, mean, rstd, weight, grad_summed, out) -> NoReturn:
     op = "layer_norm_backward"
-    d = _lib.NormGradDesc()
-    d.ld_grad = _matrix(grad, "grad", op)
+    _matrix(grad, "grad", op)
     if grad.dtype not in _TYPES:
         raise ValueError(f"{op}: grad must be float16, bfloat16 or float32, got {grad.dtype}")
     rows, cols = grad.shape
-    device = grad.device
-    held = not isinstance(x, torch.Tensor)
-    if held:
-        _held(x, op, device)
+    if cols > _lib.NORM_MAX_COLS:
+        raise ValueError(f"{op}: {cols} columns, at most {_lib.NORM_MAX_COLS}")
+    full = isinstance(x, torch.Tensor)
+    if full:
+        _matrix(x, "x", op, like=grad)
+    else:
+        _held(x, op, grad.device)
         if (x.rows, x.columns) != (rows, cols) or x.dtype != grad.dtype:
             raise ValueError(f"{op}: the checkpoint is of {x.dtype} {(x.rows, x.columns)}, grad is {grad.dtype} {(rows, cols)}")
-        d.values, d.scales = x.values.data_ptr(), x.scales.data_ptr()
-    else:
-        d.ld_x = _matrix(x, "x", op, like=grad)
-        d.x = x.data_ptr()
-    _vector(mean, "mean", op, rows, device, (torch.float32,))
-    _vector(rstd, "rstd", op, rows, device, (torch.float32,))
-    d.dtype = d.affine_dtype = _launch.dtype_code(grad.dtype)
+    _vector(mean, "mean", op, rows, grad.device, (torch.float32,))
+    _vector(rstd, "rstd", op, rows, grad.device, (torch.float32,))
     if weight is not None:
-        _vector(weight, "weight", op, cols, device, (grad.dtype,) if grad.dtype == torch.float32 else (grad.dtype, torch.float32))
-        d.weight, d.affine_dtype = weight.data_ptr(), _launch.dtype_code(weight.dtype)
+        _vector(weight, "weight", op, cols, grad.device, (grad.dtype,) if grad.dtype == torch.float32 else (grad.dtype, torch.float32))
     if grad_summed is not None:
-        d.ld_grad_summed = _matrix(grad_summed, "grad_summed", op, like=grad)
-        d.grad_summed = grad_summed.data_ptr()
-    if out is None:
-        out = torch.empty((rows, cols), dtype=grad.dtype, device=device)
-        d.ld_dx = cols
-    else:
-        d.ld_dx = _matrix(out, "out", op, like=grad)
-        _apart(out, "out", op, grad, grad_summed, None if held else x)
-    sums = None
-    if affine:
-        sums = torch.empty((2, cols), dtype=torch.float32, device=device)
-        d.dweight, d.dbias = sums.data_ptr(), sums.data_ptr() + 4 * cols
-    lib = _lib.load()
-    need = lib.tccl_layer_norm_grad_workspace(rows, cols, d.dtype, int(held))
-    if need < 0:
-        _lib.check(_lib.ERR_UNSUPPORTED, "tccl_layer_norm_grad")
-    workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    d.grad, d.mean, d.rstd, d.dx = grad.data_ptr(), mean.data_ptr(), rstd.data_ptr(), out.data_ptr()
-    d.workspace, d.workspace_bytes = workspace.data_ptr(), need
-    d.rows, d.cols = rows, cols
-    rc = lib.tccl_layer_norm_grad(C.byref(d), _launch.stream_ptr())
-    if rc:
-        _lib.check(rc, "tccl_layer_norm_grad")
-    return LayerNormGradients(out, None if sums is None else sums[0], None if sums is None else sums[1])
-
-
-def _held_desc(t: torch.Tensor, pitch: int, held: ActivationCheckpoint) -> _lib.HeldDesc:
-    return _lib.HeldDesc(t.data_ptr(), held.values.data_ptr(), held.scales.data_ptr(), pitch, held.rows, held.columns, _launch.dtype_code(t.dtype))
+        _matrix(grad_summed, "grad_summed", op, like=grad)
+    if out is not None:
+        _matrix(out, "out", op, like=grad)
+        _apart(out, "out", op, grad, grad_summed, x if full else None)
+    _unexplained(op)
 
 
 def checkpoint_activation(x: torch.Tensor) -> ActivationCheckpoint:
@@ -285,32 +274,28 @@ def checkpoint_activation(x: torch.Tensor) -> ActivationCheckpoint:
     fits under (``448 * 2**e``); values are rounded to the nearest e4m3, ties to even (to the one below it where that is more
     than ``x``'s type can hold); what is not finite is held as NaN.
     """
-    op = "checkpoint_activation"
-    pitch = _matrix(x, "x", op)
-    if x.dtype not in _HELD_TYPES:
-        raise ValueError(f"{op}: x must be float16 or bfloat16, got {x.dtype}")
-    held = ActivationCheckpoint.empty(int(x.shape[0]), int(x.shape[1]), x.dtype, x.device)
-    rc = _lib.load().tccl_hold(C.byref(_held_desc(x, pitch, held)), _launch.stream_ptr())
-    if rc:
-        _lib.check(rc, "tccl_hold")
-    return held
+    result = (_native or _bind()).checkpoint_activation(x)
+    if result is None:
+        op = "checkpoint_activation"
+        _matrix(x, "x", op)
+        if x.dtype not in _HELD_TYPES:
+            raise ValueError(f"{op}: x must be float16 or bfloat16, got {x.dtype}")
+        _unexplained(op)
+    return result
 
 
 def restore_activation(held: ActivationCheckpoint, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """The values that a checkpoint stands for, in the type of the tensor it was made of (exactly)."""
-    op = "restore_activation"
-    _held(held, op)
-    if out is None:
-        out = torch.empty((held.rows, held.columns), dtype=held.dtype, device=held.values.device)
-        pitch = held.columns
-    else:
-        pitch = _matrix(out, "out", op, shape=(held.rows, held.columns), dtype=held.dtype)
-        if out.device != held.values.device:
-            raise ValueError(f"{op}: out must reside on {held.values.device}, got {out.device}")
-    rc = _lib.load().tccl_restore(C.byref(_held_desc(out, pitch, held)), _launch.stream_ptr())
-    if rc:
-        _lib.check(rc, "tccl_restore")
-    return out
+    result = (_native or _bind()).restore_activation(held, out)
+    if result is None:
+        op = "restore_activation"
+        _held(held, op)
+        if out is not None:
+            _matrix(out, "out", op, shape=(held.rows, held.columns), dtype=held.dtype)
+            if out.device != held.values.device:
+                raise ValueError(f"{op}: out must reside on {held.values.device}, got {out.device}")
+        _unexplained(op)
+    return result
 
 
 def weight_gradient(
@@ -326,53 +311,43 @@ def weight_gradient(
     gradient of its output, of the type that ``x`` was held from.
 
     ``layout``: ``"kn"`` (inputs, outputs), as the GEMMs here take a row-major B; ``"nk"`` (outputs, inputs), as a linear
-    layer holds it.  Sums are float32, rounded once to ``out_dtype`` (float32 or ``grad``'s type).  ``add``: what earlier
-    micro-batches have summed, of the result's shape and type; ``out`` may be ``add`` itself.
+    layer holds it.  Sums are float32, rounded once to ``out_dtype`` (float32 or ``grad``'s type; that of ``out`` or
+    ``add`` where one is given).  ``add``: what earlier micro-batches have summed, of the result's shape and type; ``out``
+    may be ``add`` itself.
     """
-    op = "weight_gradient"
     if layout not in ("kn", "nk"):
-        raise ValueError(f"{op}: layout must be 'kn' or 'nk', got {layout!r}")
-    pitch = _matrix(grad, "grad", op)
-    _held(x, op, grad.device)
-    rows, outputs = grad.shape
-    if grad.dtype != x.dtype or rows != x.rows:
-        raise ValueError(f"{op}: the checkpoint is of {x.dtype} with {x.rows} rows, grad is {grad.dtype} with {rows}")
+        raise ValueError(f"weight_gradient: layout must be 'kn' or 'nk', got {layout!r}")
     if out is not None:
         out_dtype = out.dtype
     elif add is not None:
         out_dtype = add.dtype
+    result = (_native or _bind()).weight_gradient(x, grad, None, layout == "nk", out_dtype, add, out)
+    if result is not None:
+        return result
+    op = "weight_gradient"
+    _matrix(grad, "grad", op)
+    _held(x, op, grad.device)
+    rows, outputs = grad.shape
+    if grad.dtype != x.dtype or rows != x.rows:
+        raise ValueError(f"{op}: the checkpoint is of {x.dtype} with {x.rows} rows, grad is {grad.dtype} with {rows}")
     if out_dtype not in (torch.float32, grad.dtype):
         raise ValueError(f"{op}: the result must be float32 or {grad.dtype}, got {out_dtype}")
     shape = (x.columns, outputs) if layout == "kn" else (outputs, x.columns)
-    d = _lib.WeightGradientDesc()
-    if add is not None:
-        d.ld_add = _matrix(add, "add", op, shape=shape, dtype=out_dtype)
-        d.add = add.data_ptr()
-    if out is None:
-        out = torch.empty(shape, dtype=out_dtype, device=grad.device)
-        d.ld_out = shape[1]
-    else:
-        d.ld_out = _matrix(out, "out", op, shape=shape, dtype=out_dtype)
-        if add is not None:
-            _apart(out, "out", op, add)
     for t, name in ((add, "add"), (out, "out")):
-        if t is not None and t.device != grad.device:
-            raise ValueError(f"{op}: {name} must reside on {grad.device}, got {t.device}")
-    if rows and (outputs % 8 or pitch % 8 or grad.data_ptr() % 16):
+        if t is not None:
+            _matrix(t, name, op, shape=shape, dtype=out_dtype)
+            if t.device != grad.device:
+                raise ValueError(f"{op}: {name} must reside on {grad.device}, got {t.device}")
+    if out is not None:
+        _apart(out, "out", op, add)
+        lo, hi = _span(out)
+        if lo < _span(grad)[1] and _span(grad)[0] < hi:
+            raise ValueError(f"{op}: out overlaps grad")
+    width = -(-outputs // 8) * 8
+    if rows and (width != outputs or grad.stride(0) % 8 or grad.data_ptr() % 16):
         # The kernel reads 16-byte vectors: a gradient without them is copied first, as the GEMMs' operands are.
-        width = -(-outputs // 8) * 8
-        (grad,) = _launch._pack([(grad, rows, width, "weight_gradient")])
-        pitch = width
-    lib = _lib.load()
-    need = lib.tccl_weight_gradient_workspace(rows, x.columns, outputs)
-    if need < 0:
-        _lib.check(_lib.ERR_INVALID, "tccl_weight_gradient")
-    workspace = torch.empty(need, dtype=torch.uint8, device=grad.device) if need else None
-    d.values, d.scales, d.grad, d.out = x.values.data_ptr(), x.scales.data_ptr(), grad.data_ptr(), out.data_ptr()
-    d.workspace, d.workspace_bytes = _launch.ptr(workspace), need
-    d.ld_grad, d.rows, d.cols, d.outputs = pitch, rows, x.columns, outputs
-    d.dtype, d.out_dtype, d.transposed = _launch.dtype_code(grad.dtype), _launch.dtype_code(out_dtype), int(layout == "nk")
-    rc = lib.tccl_weight_gradient(C.byref(d), _launch.stream_ptr())
-    if rc:
-        _lib.check(rc, "tccl_weight_gradient")
-    return out
+        (packed,) = _launch._pack([(grad, rows, width, "weight_gradient")])
+        result = _native.weight_gradient(x, packed, outputs, layout == "nk", out_dtype, add, out)
+    if result is None:
+        _unexplained(op)
+    return result
