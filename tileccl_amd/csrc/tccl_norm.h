@@ -26,6 +26,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "tccl_device.h"
 
 namespace tccl {
@@ -59,7 +61,9 @@ struct NormGradArgs {
   const float *mean, *rstd;
   const void* weight;
   char* dx;
-  float* partial;  // [slot][2][cols]
+  float* partial;  // [slot][2][cols]; nullptr: the sums over the rows are made by workgroups of their own
+  float *dgamma, *dbeta;  // of those workgroups
+  int column_wgs;         // how many there are, ahead of the others
   int64_t ld_grad, ld_x, ld_grad_summed, ld_dx;
   int64_t scale_pitch, value_pitch;
   int rows, cols, items;
@@ -78,6 +82,48 @@ struct HoldArgs {
 
 #if defined(__HIPCC__)
 
+TCCL_D void renew_words(u32x4n& w) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+v"(w));
+#endif
+}
+
+// The value exists here (and is not computed later from what it is made of, which would have to be kept).
+template <typename W>
+TCCL_D void renew_word(W& v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+v"(v));
+#endif
+}
+
+// Instructions stay on their side of this: without it the scheduler converts everything that a thread holds to fp32 first, and
+// spills.
+TCCL_D void step_by_step() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_sched_barrier(0);
+#endif
+}
+
+// Everything here lies in global memory.  (The compiler would take an address that went through a scalar register for one of
+// any kind, and wait for LDS at each access.)  kOnce: non-temporal accesses.  Where a wavefront's access covers whole lines,
+// which rows of 16-bit activations on 128-byte boundaries give, they copy 512 MiB at 6.4 TB/s instead of 5.8 and read two for
+// one written at 6.5 instead of 5.7; where each of several accesses takes a part of every line (8-bit patches, fp32 vectors,
+// unaligned rows) they cost a quarter to a third (16384 x 4096 to 8 bits 45 -> 58 us, back 30 -> 41).
+template <typename V, bool kOnce = false, typename P>
+TCCL_D V got(const P* p) {
+  typedef const V __attribute__((address_space(1))) Global;
+  if (kOnce) return __builtin_nontemporal_load((Global*)p);
+  return *(Global*)p;
+}
+template <typename V, bool kOnce = false, typename P>
+TCCL_D void put(P* p, V v) {
+  typedef V __attribute__((address_space(1))) Global;
+  if (kOnce)
+    __builtin_nontemporal_store(v, (Global*)p);
+  else
+    *(Global*)p = v;
+}
+
 // ---- eight neighbouring values of a row, as they lie in memory ---------------------------------
 // Rows may start at any address that their type allows: the accesses say so, and the compiler makes the
 // same 16-byte instructions of them.
@@ -86,20 +132,26 @@ struct Eight {
   typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
   u32x4n w;
   TCCL_D void zero() { w = (u32x4n){0, 0, 0, 0}; }
-  TCCL_D void load(const T* p) { w = *(const Words*)p; }
-  TCCL_D void store(T* p) const { *(Words*)p = w; }
+  // What is computed from the values again after this is computed again, not kept in registers in between.
+  TCCL_D void renew() { renew_words(w); }
+  template <bool kOnce>
+  TCCL_D void load(const T* p) { w = got<Words, kOnce>(p); }
+  template <bool kOnce>
+  TCCL_D void store(T* p) const { put<Words, kOnce>(p, w); }
   TCCL_D f32x2n pair(int i) const;
   TCCL_D void set(int i, float a, float b);
   TCCL_D void load_some(const T* p, int n) {
-    zero();
+    // The last element stands in for those that do not exist, so that the loads need no branches.
+    uint32_t h[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) w[i >> 1] |= (uint32_t)((const uint16_t*)p)[i] << (16 * (i & 1));
+    for (int i = 0; i < 8; ++i) h[i] = got<uint16_t>((const uint16_t*)p + (i < n ? i : n - 1));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (2 * i < n ? h[2 * i] : 0u) | (2 * i + 1 < n ? h[2 * i + 1] << 16 : 0u);
   }
   TCCL_D void store_some(T* p, int n) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < n) ((uint16_t*)p)[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+      if (i < n) put<uint16_t>((uint16_t*)p + i, (uint16_t)(w[i >> 1] >> (16 * (i & 1))));
   }
 };
 template <>
@@ -127,58 +179,85 @@ struct Eight<float> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = 0.f;
   }
+  template <bool kOnce>
   TCCL_D void load(const float* p) {
-    const Words a = *(const Words*)p, b = *(const Words*)(p + 4);
+    const Words a = got<Words, kOnce>(p), b = got<Words, kOnce>(p + 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
   }
+  template <bool kOnce>
   TCCL_D void store(float* p) const {
-    *(Words*)p = (Words){v[0], v[1], v[2], v[3]};
-    *(Words*)(p + 4) = (Words){v[4], v[5], v[6], v[7]};
+    put<Words, kOnce>(p, (Words){v[0], v[1], v[2], v[3]});
+    put<Words, kOnce>(p + 4, (Words){v[4], v[5], v[6], v[7]});
+  }
+  TCCL_D void renew() {
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(v[i]));
+#endif
   }
   TCCL_D f32x2n pair(int i) const { return (f32x2n){v[2 * i], v[2 * i + 1]}; }
   TCCL_D void set(int i, float a, float b) { v[2 * i] = a, v[2 * i + 1] = b; }
   TCCL_D void load_some(const float* p, int n) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.f;
+    for (int i = 0; i < 8; ++i) v[i] = got<float>(p + (i < n ? i : n - 1));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? v[i] : 0.f;
   }
   TCCL_D void store_some(float* p, int n) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = v[i];
+      if (i < n) put<float>(p + i, v[i]);
   }
 };
 
-// n: how many of the eight columns exist (8, or fewer at the end of a row; <= 0: none)
-template <typename T>
+// A thread's place in a row whose start is uniform: scalar base, 32-bit offset.  (The compiler would add the offset to the
+// tensors' addresses ahead of the loop and keep two vector registers for each.)
+template <typename T, typename Byte>
+TCCL_D auto in_row(Byte* row, uint32_t off) {
+  typedef typename std::conditional<std::is_const<Byte>::value, const T, T>::type Element;
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+s"(row));
+#endif
+  return (Element*)(row + off);
+}
+
+// What the matrices' rows are: of any length and alignment, whole 16-byte vectors on 16-byte boundaries, or those on lines.
+enum RowKind { kAnyRows = 0, kVectorRows = 1, kLineRows = 2 };
+
+// n: how many of the eight columns exist (8, or fewer at the end of a row; <= 0: none).
+template <int kRows, bool kOnce = true, typename T>
 TCCL_D void load_n(Eight<T>& e, const T* p, int n) {
   if (n >= 8)
-    e.load(p);
-  else
+    e.template load<kOnce && kRows == kLineRows && sizeof(T) == 2>(p);
+  else if (kRows == kAnyRows && n > 0)
     e.load_some(p, n);
+  else
+    e.zero();
 }
-template <typename T>
+template <int kRows, typename T>
 TCCL_D void store_n(const Eight<T>& e, T* p, int n) {
   if (n >= 8)
-    e.store(p);
-  else
+    e.template store<kRows == kLineRows && sizeof(T) == 2>(p);
+  else if (kRows == kAnyRows)
     e.store_some(p, n);
 }
 
-// gamma or beta of eight columns, in the activations' type or in fp32; `missing` where there is none
-template <typename T>
+// gamma or beta of eight columns, in the activations' type or in fp32; `missing` where there is none.  They are read by
+// every workgroup: kept in the caches.
+template <typename T, int kRows>
 TCCL_D void load_affine(float (&v)[8], const void* p, int f32, int col, int n, float missing) {
   if (!p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = missing;
   } else if (f32) {
     Eight<float> e;
-    load_n(e, (const float*)p + col, n);
+    load_n<kRows, false>(e, in_row<float>((const char*)p, 4u * (uint32_t)col), n);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = e.v[i];
   } else {
     Eight<T> e;
-    load_n(e, (const T*)p + col, n);
+    load_n<kRows, false>(e, in_row<T>((const char*)p, (uint32_t)sizeof(T) * (uint32_t)col), n);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const f32x2n q = e.pair(i);
@@ -279,6 +358,7 @@ TCCL_D void hold_patch(const Eight<T> (&p)[8], uint8_t* values, uint8_t* scale, 
       hi[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[2][1] * inv, v[3][1] * inv, hi[h], true);
     }
     q[c] = (u32x4n){(uint32_t)lo[0], (uint32_t)lo[1], (uint32_t)hi[0], (uint32_t)hi[1]};
+    step_by_step();
   }
   if (!all_finite) {
 #pragma unroll
@@ -299,23 +379,23 @@ TCCL_D void hold_patch(const Eight<T> (&p)[8], uint8_t* values, uint8_t* scale, 
   }
   if (live) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) ((u32x4n*)values)[c] = q[c];
+    for (int c = 0; c < 4; ++c) put<u32x4n>((u32x4n*)values + c, q[c]);
     if (first) *scale = (uint8_t)(e + 127);
   }
 }
 
-// Rows 4h .. 4h + 3 of a column pair of a held patch: q[c] as hold_patch() writes it.
-TCCL_D void held_quad(const u32x4n& q, int h, float scale, f32x2n (&v)[4]) {
-  const f32x2n a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[h], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[h], true);
-  const f32x2n c = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[2 + h], false), d = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[2 + h], true);
+// Four rows of two neighbouring columns, from the four codes of each.
+TCCL_D void held_quad(uint32_t left, uint32_t right, float scale, f32x2n (&v)[4]) {
+  const f32x2n a = __builtin_amdgcn_cvt_pk_f32_fp8((int)left, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)left, true);
+  const f32x2n c = __builtin_amdgcn_cvt_pk_f32_fp8((int)right, false), d = __builtin_amdgcn_cvt_pk_f32_fp8((int)right, true);
   v[0] = (f32x2n){a[0] * scale, c[0] * scale}, v[1] = (f32x2n){a[1] * scale, c[1] * scale};
   v[2] = (f32x2n){b[0] * scale, d[0] * scale}, v[3] = (f32x2n){b[1] * scale, d[1] * scale};
 }
 
 // ---- forward ---------------------------------------------------------------------------------------
 // blockDim = (64 W, G): G groups of W wavefronts, each with R rows at a time.
-template <typename T, int R, int NV, bool kHold, int kThreads>
-__global__ __launch_bounds__(kThreads) void layer_norm_kernel(NormArgs a) {
+template <typename T, int R, int NV, bool kHold, int kRows>
+__global__ __launch_bounds__(1024, 4) void layer_norm_kernel(NormArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   __shared__ f32x2n part[2][16][R];  // (sum, sum of squares around the wavefront's mean) of wavefront w, by turns
   const int lane = (int)(threadIdx.x & 63);
@@ -323,9 +403,11 @@ __global__ __launch_bounds__(kThreads) void layer_norm_kernel(NormArgs a) {
   const int group = __builtin_amdgcn_readfirstlane((int)threadIdx.y), groups = (int)blockDim.y;
   const int first_part = group * waves;
   int col[NV], left[NV], wave_n = 0;
+  uint32_t off[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     col[j] = (int)(j * blockDim.x + threadIdx.x) * 8;
+    off[j] = (uint32_t)col[j] * (uint32_t)sizeof(T);
     left[j] = a.cols - col[j];
     const int n = a.cols - (j * waves + wave) * 512;
     wave_n += n < 0 ? 0 : n > 512 ? 512 : n;
@@ -340,10 +422,10 @@ __global__ __launch_bounds__(kThreads) void layer_norm_kernel(NormArgs a) {
   }
   const float inv_join_n = join_n ? 1.f / (float)join_n : 0.f;
   constexpr bool kKeep = NV == 1;  // gamma and beta stay in registers
-  float gamma[NV][8], beta[NV][8];
+  float gamma[kKeep ? NV : 1][8], beta[kKeep ? NV : 1][8];
   if (kKeep) {
-    load_affine<T>(gamma[0], a.weight, a.affine_f32, col[0], left[0], 1.f);
-    load_affine<T>(beta[0], a.bias, a.affine_f32, col[0], left[0], 0.f);
+    load_affine<T, kRows>(gamma[0], a.weight, a.affine_f32, col[0], left[0], 1.f);
+    load_affine<T, kRows>(beta[0], a.bias, a.affine_f32, col[0], left[0], 0.f);
   }
   int turn = 0;
   for (int base = (int)blockIdx.x * groups; base < a.items; base += (int)gridDim.x * groups, turn ^= 1) {
@@ -354,7 +436,7 @@ __global__ __launch_bounds__(kThreads) void layer_norm_kernel(NormArgs a) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         if (row0 + r < a.rows && left[j] > 0)
-          load_n(s[r][j], (const T*)(a.x + (int64_t)(row0 + r) * a.ld_x) + col[j], left[j]);
+          load_n<kRows>(s[r][j], in_row<T>(a.x + (int64_t)(row0 + r) * a.ld_x, off[j]), left[j]);
         else
           s[r][j].zero();
       }
@@ -365,7 +447,7 @@ __global__ __launch_bounds__(kThreads) void layer_norm_kernel(NormArgs a) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           if (row0 + r < a.rows && left[j] > 0)
-            load_n(t[r][j], (const T*)(a.residual + (int64_t)(row0 + r) * a.ld_residual) + col[j], left[j]);
+            load_n<kRows>(t[r][j], in_row<T>(a.residual + (int64_t)(row0 + r) * a.ld_residual, off[j]), left[j]);
           else
             t[r][j].zero();
         }
@@ -378,7 +460,7 @@ __global__ __launch_bounds__(kThreads) void layer_norm_kernel(NormArgs a) {
             const f32x2n u = s[r][j].pair(i), v = t[r][j].pair(i);
             s[r][j].set(i, u[0] + v[0], u[1] + v[1]);  // rounded to x's type: the norm is that of the sum that is stored
           }
-          if (row0 + r < a.rows && left[j] > 0) store_n(s[r][j], (T*)(a.summed + (int64_t)(row0 + r) * a.ld_summed) + col[j], left[j]);
+          if (row0 + r < a.rows && left[j] > 0) store_n<kRows>(s[r][j], in_row<T>(a.summed + (int64_t)(row0 + r) * a.ld_summed, off[j]), left[j]);
         }
     }
     float sum[R], m2[R];
@@ -439,6 +521,10 @@ __global__ __launch_bounds__(kThreads) void layer_norm_kernel(NormArgs a) {
           if (r4 + k < R) mean[r4 + k] = lane_value(mu, 16 * k), rstd[r4 + k] = lane_value(inv, 16 * k);
       }
     }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) s[r][j].renew();
     if (threadIdx.x == 0) {
 #pragma unroll
       for (int r = 0; r < R; ++r)
@@ -446,9 +532,10 @@ __global__ __launch_bounds__(kThreads) void layer_norm_kernel(NormArgs a) {
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
+      const int m = kKeep ? j : 0;
       if (!kKeep) {
-        load_affine<T>(gamma[j], a.weight, a.affine_f32, col[j], left[j], 1.f);
-        load_affine<T>(beta[j], a.bias, a.affine_f32, col[j], left[j], 0.f);
+        load_affine<T, kRows>(gamma[m], a.weight, a.affine_f32, col[j], left[j], 1.f);
+        load_affine<T, kRows>(beta[m], a.bias, a.affine_f32, col[j], left[j], 0.f);
       }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -456,11 +543,12 @@ __global__ __launch_bounds__(kThreads) void layer_norm_kernel(NormArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const f32x2n p = s[r][j].pair(i);
-          o.set(i, (p[0] - mean[r]) * rstd[r] * gamma[j][2 * i] + beta[j][2 * i],
-                (p[1] - mean[r]) * rstd[r] * gamma[j][2 * i + 1] + beta[j][2 * i + 1]);
+          o.set(i, (p[0] - mean[r]) * rstd[r] * gamma[m][2 * i] + beta[m][2 * i],
+                (p[1] - mean[r]) * rstd[r] * gamma[m][2 * i + 1] + beta[m][2 * i + 1]);
         }
-        if (row0 + r < a.rows && left[j] > 0) store_n(o, (T*)(a.out + (int64_t)(row0 + r) * a.ld_out) + col[j], left[j]);
+        if (row0 + r < a.rows && left[j] > 0) store_n<kRows>(o, in_row<T>(a.out + (int64_t)(row0 + r) * a.ld_out, off[j]), left[j]);
       }
+      if (NV > 1) step_by_step();
     }
     if constexpr (kHold) {
       static_assert(!kHold || R == kHoldRows, "a row block at a time");
@@ -481,90 +569,198 @@ __global__ __launch_bounds__(kThreads) void layer_norm_kernel(NormArgs a) {
 }
 
 // ---- backward --------------------------------------------------------------------------------------
-// kHeld: s comes from its 8-bit values (then R == 8).
-template <typename T, int R, int NV, bool kHeld, int kThreads>
-__global__ __launch_bounds__(kThreads) void layer_norm_grad_kernel(NormGradArgs a) {
+// Few rows: workgroup `wg` sums 32 columns over all rows, reading grad and s a second time (from the caches) instead of
+// waiting for the other workgroups' partial sums in a second launch.  4 lanes side by side, the others below each other.
+template <typename T, bool kHeld, int kRows>
+TCCL_D void sum_columns(const NormGradArgs& a, int wg, float* joined) {
+  constexpr int kStep = kHeld ? kHoldRows : 4, Q = 4;
+  const int thread = (int)(threadIdx.y * blockDim.x + threadIdx.x), threads = (int)(blockDim.x * blockDim.y);
+  const int lane = thread & 63, wave = thread >> 6, waves = threads >> 6;
+  const int col = wg * 32 + (thread & 3) * 8, left = a.cols - col;
+  const uint32_t off = (uint32_t)col * (uint32_t)sizeof(T);
+  float dgamma[8], dbeta[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) dgamma[i] = dbeta[i] = 0.f;
+  for (int row0 = (thread >> 2) * kStep; row0 < a.rows; row0 += (threads >> 2) * kStep) {
+    u32x4n q[4];
+    float scale = 0.f;
+    if (kHeld) {
+      const int rb = row0 / kHoldRows;
+      const uint8_t* v = a.values + rb * a.value_pitch + (int64_t)col * kHoldRows;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) q[c] = left > 0 ? got<u32x4n>((const u32x4n*)v + c) : (u32x4n){0, 0, 0, 0};
+      if (left > 0) scale = __uint_as_float((uint32_t)a.scales[(col / kHoldCols) * a.scale_pitch + rb] << 23);
+    }
+#pragma unroll
+    for (int h = 0; h < (kHeld ? 2 : 1); ++h) {
+      Eight<T> g[Q], s[kHeld ? 1 : Q];
+      float mean[Q], rstd[Q];
+#pragma unroll
+      for (int e = 0; e < Q; ++e) {
+        const int row = row0 + 4 * h + e;
+        if (row < a.rows) {
+          load_n<kRows, false>(g[e], (const T*)(a.grad + (int64_t)row * a.ld_grad + off), left);
+          if (!kHeld) load_n<kRows, false>(s[kHeld ? 0 : e], (const T*)(a.x + (int64_t)row * a.ld_x + off), left);
+          mean[e] = a.mean[row], rstd[e] = a.rstd[row];
+        } else {
+          g[e].zero(), mean[e] = rstd[e] = 0.f;
+          if (!kHeld) s[kHeld ? 0 : e].zero();
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f32x2n v[Q];
+        if (kHeld)
+          held_quad(q[i][h], q[i][2 + h], scale, v);
+        else
+#pragma unroll
+          for (int e = 0; e < Q; ++e) v[e] = s[kHeld ? 0 : e].pair(i);
+#pragma unroll
+        for (int e = 0; e < Q; ++e) {
+          const f32x2n d = g[e].pair(i);
+#pragma unroll
+          for (int o = 0; o < 2; ++o) dgamma[2 * i + o] += d[o] * ((v[e][o] - mean[e]) * rstd[e]), dbeta[2 * i + o] += d[o];
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int m = 4; m < 64; m *= 2) dgamma[i] += __shfl_xor(dgamma[i], m), dbeta[i] += __shfl_xor(dbeta[i], m);
+  if (lane < 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) joined[wave * 64 + lane * 8 + i] = dgamma[i], joined[wave * 64 + 32 + lane * 8 + i] = dbeta[i];
+  }
+  __syncthreads();
+  if (thread < 64) {
+    float t = 0.f;
+    for (int w = 0; w < waves; ++w) t += joined[w * 64 + thread];
+    const int c = wg * 32 + (thread & 31);
+    float* to = thread < 32 ? a.dgamma : a.dbeta;
+    if (c < a.cols && to) to[c] = t;
+  }
+}
+
+// kHeld: s comes from its 8-bit values, R is a row block or half of one.
+template <typename T, int R, int NV, bool kHeld, int kRows>
+__global__ __launch_bounds__(1024, 4) void layer_norm_grad_kernel(NormGradArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  constexpr int Q = R < 4 ? R : 4;   // rows taken together
-  __shared__ f32x2n part[2][16][R];  // (sum g, sum g xh) of wavefront w, by turns
+  constexpr int Q = R < 4 ? R : 4;          // rows taken together
+  constexpr bool kTwice = kHeld && NV > 2;  // four rows of more than 16384 columns are more than the registers: read again
+  constexpr int kQuads = kHeld ? R / 4 : 1;  // rows of codes, four in a word
+  constexpr bool kKeep = NV == 1;           // gamma stays in registers
+  constexpr int KJ = kTwice ? 1 : NV;
+  __shared__ f32x2n part[2][16][R];         // (sum g, sum g xh) of wavefront w, by turns
+  __shared__ float merged[NV == 1 ? 7 * 1024 : 16 * 64];  // of the groups of a workgroup, or of sum_columns()
+  if constexpr (kRows != kAnyRows)
+    if ((int)blockIdx.x < a.column_wgs) return sum_columns<T, kHeld, kRows>(a, (int)blockIdx.x, merged);
+  const int block = (int)blockIdx.x - a.column_wgs, blocks = (int)gridDim.x - a.column_wgs;
   const int lane = (int)(threadIdx.x & 63);
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), waves = (int)(blockDim.x >> 6);
   const int group = __builtin_amdgcn_readfirstlane((int)threadIdx.y), groups = (int)blockDim.y;
   const int first_part = group * waves;
   int col[NV], left[NV];
-  float gamma[NV][8], dgamma[NV][8], dbeta[NV][8];
+  uint32_t off[NV];
+  float gamma[kKeep ? NV : 1][8], dgamma[NV][8], dbeta[NV][8];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     col[j] = (int)(j * blockDim.x + threadIdx.x) * 8;
+    off[j] = (uint32_t)col[j] * (uint32_t)sizeof(T);
     left[j] = a.cols - col[j];
-    load_affine<T>(gamma[j], a.weight, a.affine_f32, col[j], left[j], 1.f);
+    if (kKeep) load_affine<T, kRows>(gamma[j], a.weight, a.affine_f32, col[j], left[j], 1.f);
 #pragma unroll
     for (int i = 0; i < 8; ++i) dgamma[j][i] = dbeta[j][i] = 0.f;
   }
   int turn = 0;
-  for (int base = (int)blockIdx.x * groups; base < a.items; base += (int)gridDim.x * groups, turn ^= 1) {
+  for (int base = block * groups; base < a.items; base += blocks * groups, turn ^= 1) {
     const int row0 = (base + group) * R;
-    Eight<T> g[R][NV], s[kHeld ? 1 : R][NV];
-    u32x4n q[kHeld ? NV : 1][4];
-    float scale[NV], mean[R], rstd[R];
+    Eight<T> g[R][KJ], s[kHeld ? 1 : R][KJ];
+    uint32_t q[kHeld ? KJ : 1][4][kQuads][2];  // column pair, rows, column
+    float scale[KJ], mean[R], rstd[R];
+    auto fetch = [&](int j, int k) {  // vectors j into place k
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        if (row0 + r < a.rows && left[j] > 0) {
-          load_n(g[r][j], (const T*)(a.grad + (int64_t)(row0 + r) * a.ld_grad) + col[j], left[j]);
-          if (!kHeld) load_n(s[kHeld ? 0 : r][j], (const T*)(a.x + (int64_t)(row0 + r) * a.ld_x) + col[j], left[j]);
+      for (int r = 0; r < R; ++r) {
+        if (row0 + r < a.rows) {
+          load_n<kRows>(g[r][k], in_row<T>(a.grad + (int64_t)(row0 + r) * a.ld_grad, off[j]), left[j]);
+          if (!kHeld) load_n<kRows>(s[kHeld ? 0 : r][k], in_row<T>(a.x + (int64_t)(row0 + r) * a.ld_x, off[j]), left[j]);
         } else {
-          g[r][j].zero();
-          if (!kHeld) s[kHeld ? 0 : r][j].zero();
+          g[r][k].zero();
+          if (!kHeld) s[kHeld ? 0 : r][k].zero();
         }
       }
-    if (kHeld) {
-      const int rb = base + group;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
+      if (kHeld) {
+        const int rb = row0 / kHoldRows, half = R == 4 ? row0 / 4 % 2 : 0;
         const bool live = row0 < a.rows && left[j] > 0;
-        const uint8_t* v = a.values + rb * a.value_pitch + (int64_t)col[j] * kHoldRows;
+        const uint8_t* v = in_row<const uint8_t>(a.values + rb * a.value_pitch, (uint32_t)col[j] * kHoldRows);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) q[j][c] = live ? ((const u32x4n*)v)[c] : (u32x4n){0, 0, 0, 0};
-        scale[j] = live ? __uint_as_float((uint32_t)a.scales[(col[j] / kHoldCols) * a.scale_pitch + rb] << 23) : 0.f;
+        for (int c = 0; c < 4; ++c) {
+          const u32x4n codes = live ? got<u32x4n>((const u32x4n*)v + c) : (u32x4n){0, 0, 0, 0};
+#pragma unroll
+          for (int o = 0; o < 2; ++o) {
+            if (R == 4) {
+              q[kHeld ? k : 0][c][0][o] = half ? codes[2 * o + 1] : codes[2 * o];
+            } else {
+#pragma unroll
+              for (int h = 0; h < kQuads; ++h) q[kHeld ? k : 0][c][h][o] = codes[2 * o + h];
+            }
+          }
+        }
+        scale[k] = live ? __uint_as_float((uint32_t)a.scales[(col[j] / kHoldCols) * a.scale_pitch + rb] << 23) : 0.f;
       }
-    }
+    };
+    auto values = [&](int k, int i, int h, f32x2n(&v)[4]) {  // s of columns 2i, 2i + 1, rows h Q ..
+      if (kHeld)
+        held_quad(q[kHeld ? k : 0][i][kHeld ? h : 0][0], q[kHeld ? k : 0][i][kHeld ? h : 0][1], scale[k], v);
+      else
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const bool live = row0 + r < a.rows;
-      mean[r] = live ? a.mean[row0 + r] : 0.f, rstd[r] = live ? a.rstd[row0 + r] : 0.f;
+        for (int e = 0; e < Q; ++e) v[e] = s[kHeld ? 0 : h * Q + e][k].pair(i);
+    };
+    if (!kTwice) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) fetch(j, j);
+    }
+    {  // a row's statistics per lane, then uniform
+      const bool live = lane < R && row0 + lane < a.rows;
+      const float m = live ? a.mean[row0 + lane] : 0.f, v = live ? a.rstd[row0 + lane] : 0.f;
+#pragma unroll
+      for (int r = 0; r < R; ++r) mean[r] = lane_value(m, r), rstd[r] = lane_value(v, r);
     }
     float c1[R], c2[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) c1[r] = c2[r] = 0.f;
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) {
+      const int k = kTwice ? 0 : j, m = kKeep ? j : 0;
+      if (kTwice) fetch(j, 0);
+      if (!kKeep) load_affine<T, kRows>(gamma[m], a.weight, a.affine_f32, col[j], left[j], 1.f);
 #pragma unroll
       for (int h = 0; h < R / Q; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           f32x2n v[4];
-          if (kHeld)
-            held_quad(q[kHeld ? j : 0][i], h, scale[j], v);
-          else
+          values(k, i, h, v);
 #pragma unroll
-            for (int k = 0; k < Q; ++k) v[k] = s[kHeld ? 0 : h * Q + k][j].pair(i);
-#pragma unroll
-          for (int k = 0; k < Q; ++k) {
-            const int r = h * Q + k;
-            const f32x2n d = g[r][j].pair(i);
+          for (int e = 0; e < Q; ++e) {
+            const int r = h * Q + e;
+            const f32x2n d = g[r][k].pair(i);
 #pragma unroll
             for (int o = 0; o < 2; ++o) {
-              const float xh = (v[k][o] - mean[r]) * rstd[r];
-              const float gd = d[o] * gamma[j][2 * i + o];  // 0 in columns that do not exist
+              const float xh = (v[e][o] - mean[r]) * rstd[r];
+              const float gd = d[o] * gamma[m][2 * i + o];  // 0 in columns that do not exist
               c1[r] += gd;
               c2[r] += gd * xh;
               dgamma[j][2 * i + o] += d[o] * xh;
               dbeta[j][2 * i + o] += d[o];
             }
           }
+#pragma unroll
+          for (int o = 0; o < 2; ++o) renew_word(dgamma[j][2 * i + o]), renew_word(dbeta[j][2 * i + o]);
+#pragma unroll
+          for (int e = 0; e < Q; ++e) renew_word(c1[h * Q + e]), renew_word(c2[h * Q + e]);
+          step_by_step();
         }
+    }
 #pragma unroll
     for (int r = 0; r < R; ++r) c1[r] = sum64(c1[r]), c2[r] = sum64(c2[r]);
     if (waves > 1) {
@@ -587,59 +783,93 @@ __global__ __launch_bounds__(kThreads) void layer_norm_grad_kernel(NormGradArgs 
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) c1[r] *= a.inv_cols, c2[r] *= a.inv_cols;
+    if (!kTwice) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < KJ; ++j) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          g[r][j].renew();
+          if (!kHeld) s[kHeld ? 0 : r][j].renew();
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int h = 0; h < kQuads; ++h)
+            if (kHeld) renew_word(q[kHeld ? j : 0][c][h][0]), renew_word(q[kHeld ? j : 0][c][h][1]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int k = kTwice ? 0 : j, m = kKeep ? j : 0;
+      if (kTwice) fetch(j, 0);
+      if (!kKeep) load_affine<T, kRows>(gamma[m], a.weight, a.affine_f32, col[j], left[j], 1.f);
 #pragma unroll
       for (int h = 0; h < R / Q; ++h) {
         Eight<T> o[Q];
 #pragma unroll
-        for (int k = 0; k < Q; ++k) {
-          const int r = h * Q + k;
-          if (a.grad_summed && row0 + r < a.rows && left[j] > 0)
-            load_n(o[k], (const T*)(a.grad_summed + (int64_t)(row0 + r) * a.ld_grad_summed) + col[j], left[j]);
+        for (int e = 0; e < Q; ++e) {
+          const int r = h * Q + e;
+          if (a.grad_summed && row0 + r < a.rows)
+            load_n<kRows>(o[e], in_row<T>(a.grad_summed + (int64_t)(row0 + r) * a.ld_grad_summed, off[j]), left[j]);
           else
-            o[k].zero();
+            o[e].zero();
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           f32x2n v[4];
-          if (kHeld)
-            held_quad(q[kHeld ? j : 0][i], h, scale[j], v);
-          else
+          values(k, i, h, v);
 #pragma unroll
-            for (int k = 0; k < Q; ++k) v[k] = s[kHeld ? 0 : h * Q + k][j].pair(i);
-#pragma unroll
-          for (int k = 0; k < Q; ++k) {
-            const int r = h * Q + k;
-            const f32x2n d = g[r][j].pair(i), more = o[k].pair(i);
+          for (int e = 0; e < Q; ++e) {
+            const int r = h * Q + e;
+            const f32x2n d = g[r][k].pair(i), more = o[e].pair(i);
             float dx[2];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float xh = (v[k][e] - mean[r]) * rstd[r];
-              dx[e] = rstd[r] * (d[e] * gamma[j][2 * i + e] - c1[r] - xh * c2[r]) + more[e];
+            for (int u = 0; u < 2; ++u) {
+              const float xh = (v[e][u] - mean[r]) * rstd[r];
+              dx[u] = rstd[r] * (d[u] * gamma[m][2 * i + u] - c1[r] - xh * c2[r]) + more[u];
             }
-            o[k].set(i, dx[0], dx[1]);
+            o[e].set(i, dx[0], dx[1]);
           }
+          step_by_step();
         }
 #pragma unroll
-        for (int k = 0; k < Q; ++k) {
-          const int r = h * Q + k;
-          if (row0 + r < a.rows && left[j] > 0) store_n(o[k], (T*)(a.dx + (int64_t)(row0 + r) * a.ld_dx) + col[j], left[j]);
+        for (int e = 0; e < Q; ++e) {
+          const int r = h * Q + e;
+          if (row0 + r < a.rows && left[j] > 0) store_n<kRows>(o[e], in_row<T>(a.dx + (int64_t)(row0 + r) * a.ld_dx, off[j]), left[j]);
         }
       }
+    }
   }
-  const int64_t slot = (int64_t)blockIdx.x * groups + group;
+  if (!a.partial) return;
+  // The sums of the groups of a workgroup are joined in LDS (there is more than one only of up to 2048 columns).
+  if constexpr (NV == 1) {
+    if (groups > 1) {
+      const int width = (int)blockDim.x * 8;
+      float* mine = merged + (group - 1) * 2 * width + col[0];
+      if (group > 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mine[i] = dgamma[0][i], mine[width + i] = dbeta[0][i];
+      }
+      __syncthreads();
+      if (group > 0) return;
+      for (int o = 0; o < groups - 1; ++o) {
+        const float* other = merged + o * 2 * width + col[0];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dgamma[0][i] += other[i], dbeta[0][i] += other[width + i];
+      }
+    }
+  }
 #pragma unroll
   for (int j = 0; j < NV; ++j)
     if (left[j] > 0) {
-      float* to = a.partial + slot * 2 * a.cols + col[j];
+      float* to = a.partial + (int64_t)block * 2 * a.cols + col[j];
       Eight<float> e;
 #pragma unroll
       for (int i = 0; i < 8; ++i) e.v[i] = dgamma[j][i];
-      store_n(e, to, left[j]);
+      store_n<kAnyRows>(e, to, left[j]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) e.v[i] = dbeta[j][i];
-      store_n(e, to + a.cols, left[j]);
+      store_n<kAnyRows>(e, to + a.cols, left[j]);
     }
 #endif
 }
@@ -676,10 +906,11 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(const float* partial,
 
 // ---- to 8 bits and back ------------------------------------------------------------------------------
 // 256 threads: a patch of 8 rows x 8 columns each; blockIdx.x over 2048 columns, blockIdx.y over row blocks.
-template <typename T>
+template <typename T, int kRows>
 __global__ __launch_bounds__(256) void hold_kernel(HoldArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   const int col = (int)(blockIdx.x * 256 + threadIdx.x) * 8, left = a.cols - col;
+  const uint32_t off = (uint32_t)col * (uint32_t)sizeof(T);
   const int row_blocks = (a.rows + kHoldRows - 1) / kHoldRows;
   for (int rb = (int)blockIdx.y; rb < row_blocks; rb += (int)gridDim.y) {
     Eight<T> p[8];
@@ -687,7 +918,7 @@ __global__ __launch_bounds__(256) void hold_kernel(HoldArgs a) {
     for (int r = 0; r < 8; ++r) {
       const int row = rb * kHoldRows + r;
       if (row < a.rows && left > 0)
-        load_n(p[r], (const T*)(a.x + (int64_t)row * a.ld) + col, left);
+        load_n<kRows>(p[r], in_row<T>(a.x + (int64_t)row * a.ld, off), left);
       else
         p[r].zero();
     }
@@ -698,17 +929,18 @@ __global__ __launch_bounds__(256) void hold_kernel(HoldArgs a) {
 #endif
 }
 
-template <typename T>
+template <typename T, int kRows>
 __global__ __launch_bounds__(256) void restore_kernel(HoldArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   const int col = (int)(blockIdx.x * 256 + threadIdx.x) * 8, left = a.cols - col;
+  const uint32_t off = (uint32_t)col * (uint32_t)sizeof(T);
   const int row_blocks = (a.rows + kHoldRows - 1) / kHoldRows;
   if (left <= 0) return;
   for (int rb = (int)blockIdx.y; rb < row_blocks; rb += (int)gridDim.y) {
     const uint8_t* v = a.values + rb * a.value_pitch + (int64_t)col * kHoldRows;
     u32x4n q[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) q[c] = ((const u32x4n*)v)[c];
+    for (int c = 0; c < 4; ++c) q[c] = got<u32x4n>((const u32x4n*)v + c);
     const float scale = __uint_as_float((uint32_t)a.scales[(col / kHoldCols) * a.scale_pitch + rb] << 23);
     Eight<T> o[8];
 #pragma unroll
@@ -716,14 +948,14 @@ __global__ __launch_bounds__(256) void restore_kernel(HoldArgs a) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         f32x2n x[4];
-        held_quad(q[c], h, scale, x);
+        held_quad(q[c][h], q[c][2 + h], scale, x);
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[4 * h + k].set(c, x[k][0], x[k][1]);
       }
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
       const int row = rb * kHoldRows + r;
-      if (row < a.rows) store_n(o[r], (T*)(a.out + (int64_t)row * a.ld) + col, left);
+      if (row < a.rows) store_n<kRows>(o[r], in_row<T>(a.out + (int64_t)row * a.ld, off), left);
     }
   }
 #endif

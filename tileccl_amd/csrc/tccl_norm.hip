@@ -1,6 +1,8 @@
 // Layer norm, its gradients and activations in 8 bits: argument checks, launch shapes and the entry points.
 #include <hip/hip_runtime.h>
 
+#include <initializer_list>
+
 #pragma GCC visibility push(default)
 #include "../../include/tileccl_hip.h"
 #pragma GCC visibility pop
@@ -13,11 +15,32 @@ namespace {
 
 using namespace tccl;
 
+
 bool on16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 int size_of(int dtype) { return dtype == TCCL_F32 ? 4 : dtype == TCCL_F16 || dtype == TCCL_BF16 ? 2 : 0; }
 int64_t row_blocks(int rows) { return ((int64_t)rows + kHoldRows - 1) / kHoldRows; }
 int64_t scale_pitch(int rows) { return (row_blocks(rows) + 15) / 16 * 16; }
 int64_t value_pitch(int cols) { return ((int64_t)cols + kHoldCols - 1) / kHoldCols * kHoldCols * kHoldRows; }
+
+struct Rows {
+  const void* at;
+  int64_t ld;
+};
+// What the rows of all matrices that are there are.
+int rows_of(int cols, int size, std::initializer_list<Rows> matrices) {
+  if (cols % 8) return kAnyRows;
+  uintptr_t bits = 0;
+  for (const Rows& m : matrices)
+    if (m.at) bits |= (uintptr_t)m.at | (uintptr_t)(m.ld * size);
+  return bits % 16 ? kAnyRows : bits % 128 ? kVectorRows : kLineRows;
+}
+
+// Whether two matrices of these sizes have no memory in common (their spans: rows between rows count as common).
+bool lie_apart(const void* p, int64_t ld_p, const void* q, int64_t ld_q, int rows, int cols, int size) {
+  const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
+  const uintptr_t end_a = a + ((int64_t)(rows - 1) * ld_p + cols) * size, end_b = b + ((int64_t)(rows - 1) * ld_q + cols) * size;
+  return end_a <= b || end_b <= a;
+}
 
 // How a launch of rows x cols is cut: groups of `waves` wavefronts with R rows and NV vectors each, `groups` of them in
 // a workgroup.
@@ -38,66 +61,81 @@ Shape shape_of(int rows, int cols, int R, int cus, int per_cu_threads) {
   return s;
 }
 
-// Rows of a group: as many as four, unless the rows do not fill the device that way.
-Shape choose(int rows, int cols, int dtype, bool held, int cus, int per_cu_threads) {
-  if (held) return shape_of(rows, cols, kHoldRows, cus, per_cu_threads);
-  Shape s = shape_of(rows, cols, 1, cus, per_cu_threads);
-  const int most = s.NV > 1 ? 1 : dtype == TCCL_F32 ? 2 : 4;
-  for (int R = most; R > 1; R /= 2) {
-    const Shape t = shape_of(rows, cols, R, cus, per_cu_threads);
-    if (t.items >= cus * 2 * t.groups) return t;
+// Forward: two rows of a group where they fill the device that way, workgroups for 1536 threads of a CU.  Measured with
+// one, two and four rows and 1024 to 4096 threads, or a workgroup for each group of rows: 8192 x 4096 bf16 24.6 us (25.2 with four rows, 30.1 with
+// one, 26.3 with all workgroups at once), with a residual 45.5 (48.8, 48.8, 45.3), 16384 x 1024 24.4 (23.8, 26.2, 24.6).
+Shape forward_shape(int rows, int cols, bool held, int cus) {
+  if (held) return shape_of(rows, cols, kHoldRows, cus, 1024);
+  const Shape two = shape_of(rows, cols, 2, cus, 1536);
+  return two.NV == 1 && two.items >= 2 * cus * two.groups ? two : shape_of(rows, cols, 1, cus, 1536);
+}
+
+// Whether the sums over the rows are made by workgroups of their own (sum_columns) rather than in a second launch.  They read
+// a whole column one after the other: 512 x 512 8.8 -> 7.0 us, 1024 x 1024 8.9 -> 7.2, 1024 x 4096 18.3 -> 17.0; but
+// 2048 x 1024 10.1 -> 19.4.
+bool columns_apart(int rows) { return rows <= 1024; }
+
+// Backward: as many as four rows (two of fp32) as long as there are four groups of them for each CU, workgroups of up to 512 threads whose
+// groups join their sums, 1024 threads of a CU at most and four turns each if that leaves every CU one: each
+// workgroup's sums are written and read again.  2048 x 4096 bf16 26.6 us with 512 workgroups, 23.8 with 256; 12000 x 128 13.6
+// with eight groups each, 25.9 with one.
+Shape backward_shape(int rows, int cols, int dtype, bool held, int cus) {
+  Shape s;
+  for (int R = held ? kHoldRows : dtype == TCCL_F32 ? 2 : 4;; R /= 2) {
+    s = shape_of(rows, cols, R, cus, 1024);
+    if (s.NV > 1 && R > (held ? 4 : 1)) continue;
+    if (R == (held ? 4 : 1) || s.items >= (held ? 2 : 4) * cus) break;
   }
+  s.groups = s.waves <= 4 ? 8 / s.waves : 1;
+  // (sum_columns is quicker with at least 256 threads: 1003 x 1000 from 8 bits 10.3 us with 128 of them)
+  while (s.groups > (columns_apart(rows) ? (3 + s.waves) / s.waves : 1) && s.items < cus / 2 * s.groups) s.groups /= 2;
+  s.threads = 64 * s.waves * s.groups;
+  const int wanted = (s.items + s.groups - 1) / s.groups, most = cus * (s.threads <= 512 ? 1024 / s.threads : 1);
+  s.wgs = columns_apart(rows) ? wanted : wanted / 4 < cus ? cus : wanted / 4;
+  if (s.wgs > most && !columns_apart(rows)) s.wgs = most;
+  if (s.wgs > wanted) s.wgs = wanted;
   return s;
 }
 
-template <typename T, int R, int NV, bool kHold>
+template <typename T, int R, int NV, bool kHold, int kRows>
 void launch_forward(const NormArgs& a, const Shape& s, hipStream_t stream) {
   const dim3 block(64 * s.waves, s.groups);
-  if constexpr (NV == 1)
-    if (s.threads <= 512) {
-      hipLaunchKernelGGL((layer_norm_kernel<T, R, NV, kHold, 512>), dim3(s.wgs), block, 0, stream, a);
-      return;
-    }
-  hipLaunchKernelGGL((layer_norm_kernel<T, R, NV, kHold, 1024>), dim3(s.wgs), block, 0, stream, a);
+  hipLaunchKernelGGL((layer_norm_kernel<T, R, NV, kHold, kRows>), dim3(s.wgs), block, 0, stream, a);
 }
 
-template <typename T>
+template <typename T, int kRows>
 void forward(const NormArgs& a, const Shape& s, hipStream_t stream) {
   if constexpr (sizeof(T) == 2) {
-    if (a.values) return launch_forward<T, 8, 1, true>(a, s, stream);
-    if (s.R == 4) return launch_forward<T, 4, 1, false>(a, s, stream);
+    if (a.values) return launch_forward<T, 8, 1, true, kRows>(a, s, stream);
+    if (s.R == 4) return launch_forward<T, 4, 1, false, kRows>(a, s, stream);
   }
-  if (s.R == 2) return launch_forward<T, 2, 1, false>(a, s, stream);
-  if (s.NV == 1) return launch_forward<T, 1, 1, false>(a, s, stream);
-  if (s.NV == 2) return launch_forward<T, 1, 2, false>(a, s, stream);
-  return launch_forward<T, 1, 4, false>(a, s, stream);
+  if (s.R == 2) return launch_forward<T, 2, 1, false, kRows>(a, s, stream);
+  if (s.NV == 1) return launch_forward<T, 1, 1, false, kRows>(a, s, stream);
+  if (s.NV == 2) return launch_forward<T, 1, 2, false, kRows>(a, s, stream);
+  return launch_forward<T, 1, 4, false, kRows>(a, s, stream);
 }
 
-template <typename T, int R, int NV, bool kHeld>
+template <typename T, int R, int NV, bool kHeld, int kRows>
 void launch_backward(const NormGradArgs& a, const Shape& s, hipStream_t stream) {
   const dim3 block(64 * s.waves, s.groups);
-  if constexpr (NV == 1)
-    if (s.threads <= 512) {
-      hipLaunchKernelGGL((layer_norm_grad_kernel<T, R, NV, kHeld, 512>), dim3(s.wgs), block, 0, stream, a);
-      return;
-    }
-  hipLaunchKernelGGL((layer_norm_grad_kernel<T, R, NV, kHeld, 1024>), dim3(s.wgs), block, 0, stream, a);
+  hipLaunchKernelGGL((layer_norm_grad_kernel<T, R, NV, kHeld, kRows>), dim3(s.wgs + a.column_wgs), block, 0, stream, a);
 }
 
-template <typename T>
+template <typename T, int kRows>
 void backward(const NormGradArgs& a, const Shape& s, hipStream_t stream) {
   if constexpr (sizeof(T) == 2) {
     if (a.values) {
-      if (s.NV == 1) return launch_backward<T, 8, 1, true>(a, s, stream);
-      if (s.NV == 2) return launch_backward<T, 8, 2, true>(a, s, stream);
-      return launch_backward<T, 8, 4, true>(a, s, stream);
+      if (s.R == 8) return launch_backward<T, 8, 1, true, kRows>(a, s, stream);
+      if (s.NV == 1) return launch_backward<T, 4, 1, true, kRows>(a, s, stream);
+      if (s.NV == 2) return launch_backward<T, 4, 2, true, kRows>(a, s, stream);
+      return launch_backward<T, 4, 4, true, kRows>(a, s, stream);
     }
-    if (s.R == 4) return launch_backward<T, 4, 1, false>(a, s, stream);
+    if (s.R == 4) return launch_backward<T, 4, 1, false, kRows>(a, s, stream);
   }
-  if (s.R == 2) return launch_backward<T, 2, 1, false>(a, s, stream);
-  if (s.NV == 1) return launch_backward<T, 1, 1, false>(a, s, stream);
-  if (s.NV == 2) return launch_backward<T, 1, 2, false>(a, s, stream);
-  return launch_backward<T, 1, 4, false>(a, s, stream);
+  if (s.R == 2) return launch_backward<T, 2, 1, false, kRows>(a, s, stream);
+  if (s.NV == 1) return launch_backward<T, 1, 1, false, kRows>(a, s, stream);
+  if (s.NV == 2) return launch_backward<T, 1, 2, false, kRows>(a, s, stream);
+  return launch_backward<T, 1, 4, false, kRows>(a, s, stream);
 }
 
 int check_sizes(const char* what, int rows, int cols, int dtype, int most_cols) {
@@ -148,8 +186,6 @@ int check_hold(const char* what, const tccl_held_desc* d) {
   return 0;
 }
 
-Shape grad_shape(int rows, int cols, int dtype, bool held, int cus) { return choose(rows, cols, dtype, held, cus, 1024); }
-
 }  // namespace
 
 extern "C" {
@@ -160,10 +196,11 @@ int tccl_hold(const tccl_held_desc* d, void* stream) {
   dim3 grid;
   hold_grid(d, &grid);
   const HoldArgs a = hold_args(d);
+  const int kind = rows_of(d->cols, 2, {{d->x, d->ld}});
   if (d->dtype == TCCL_BF16)
-    hipLaunchKernelGGL((hold_kernel<__bf16>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL((kind == kAnyRows ? hold_kernel<__bf16, kAnyRows> : kind == kVectorRows ? hold_kernel<__bf16, kVectorRows> : hold_kernel<__bf16, kLineRows>), grid, dim3(256), 0, (hipStream_t)stream, a);
   else
-    hipLaunchKernelGGL((hold_kernel<_Float16>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL((kind == kAnyRows ? hold_kernel<_Float16, kAnyRows> : kind == kVectorRows ? hold_kernel<_Float16, kVectorRows> : hold_kernel<_Float16, kLineRows>), grid, dim3(256), 0, (hipStream_t)stream, a);
   return launched("hold");
 }
 
@@ -173,10 +210,11 @@ int tccl_restore(const tccl_held_desc* d, void* stream) {
   dim3 grid;
   hold_grid(d, &grid);
   const HoldArgs a = hold_args(d);
+  const int kind = rows_of(d->cols, 2, {{d->x, d->ld}});
   if (d->dtype == TCCL_BF16)
-    hipLaunchKernelGGL((restore_kernel<__bf16>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL((kind == kAnyRows ? restore_kernel<__bf16, kAnyRows> : kind == kVectorRows ? restore_kernel<__bf16, kVectorRows> : restore_kernel<__bf16, kLineRows>), grid, dim3(256), 0, (hipStream_t)stream, a);
   else
-    hipLaunchKernelGGL((restore_kernel<_Float16>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL((kind == kAnyRows ? restore_kernel<_Float16, kAnyRows> : kind == kVectorRows ? restore_kernel<_Float16, kVectorRows> : restore_kernel<_Float16, kLineRows>), grid, dim3(256), 0, (hipStream_t)stream, a);
   return launched("restore");
 }
 
@@ -211,14 +249,19 @@ int tccl_layer_norm(const tccl_norm_desc* d, void* stream) {
   // of their own.
   const bool apart = d->values && d->cols > 8192;
   a.values = apart ? nullptr : (uint8_t*)d->values, a.scales = apart ? nullptr : (uint8_t*)d->scales;
-  const Shape s = choose(d->rows, d->cols, d->dtype, a.values != nullptr, cus, 2048);
+  const Shape s = forward_shape(d->rows, d->cols, a.values != nullptr, cus);
   a.items = s.items;
+  const int kind = rows_of(d->cols, size, {{d->x, d->ld_x}, {d->residual, d->ld_residual}, {d->summed, d->ld_summed}, {d->out, d->ld_out}});
+#define TCCL_FORWARD(T)                                                            \
+  (kind == kAnyRows      ? forward<T, kAnyRows>(a, s, (hipStream_t)stream)         \
+   : kind == kVectorRows ? forward<T, kVectorRows>(a, s, (hipStream_t)stream)      \
+                         : forward<T, kLineRows>(a, s, (hipStream_t)stream))
   if (d->dtype == TCCL_F32)
-    forward<float>(a, s, (hipStream_t)stream);
+    TCCL_FORWARD(float);
   else if (d->dtype == TCCL_BF16)
-    forward<__bf16>(a, s, (hipStream_t)stream);
+    TCCL_FORWARD(__bf16);
   else
-    forward<_Float16>(a, s, (hipStream_t)stream);
+    TCCL_FORWARD(_Float16);
   TCCL_TRY(launched(what));
   if (!apart) return 0;
   const tccl_held_desc h = {d->residual ? d->summed : const_cast<void*>(d->x), d->values, d->scales, d->residual ? d->ld_summed : d->ld_x,
@@ -229,8 +272,8 @@ int tccl_layer_norm(const tccl_norm_desc* d, void* stream) {
 int64_t tccl_layer_norm_grad_workspace(int32_t rows, int32_t cols, int32_t dtype, int32_t held) {
   int cus = 0;
   if (check_sizes("layer_norm_grad", rows, cols, dtype, TCCL_NORM_MAX_COLS) || compute_units(&cus)) return -1;
-  const Shape s = grad_shape(rows, cols, dtype, held != 0, cus);
-  return (int64_t)s.wgs * s.groups * 2 * cols * 4;
+  const Shape s = backward_shape(rows, cols, dtype, held != 0, cus);
+  return (int64_t)s.wgs * 2 * cols * 4;
 }
 
 int tccl_layer_norm_grad(const tccl_norm_grad_desc* d, void* stream) {
@@ -248,29 +291,39 @@ int tccl_layer_norm_grad(const tccl_norm_grad_desc* d, void* stream) {
   if ((uintptr_t)d->weight % size_of(d->affine_dtype)) return reportf(TCCL_ERR_INVALID, "%s: weight is not aligned to its type", what);
   int cus = 0;
   TCCL_TRY(compute_units(&cus));
-  const Shape s = grad_shape(d->rows, d->cols, d->dtype, d->values != nullptr, cus);
-  const int slots = s.wgs * s.groups;
+  const Shape s = backward_shape(d->rows, d->cols, d->dtype, d->values != nullptr, cus);
+  const int slots = s.wgs;
+  const bool sums = d->dweight || d->dbias;
   if (d->rows && (!d->workspace || !on16(d->workspace) || d->workspace_bytes < (int64_t)slots * 2 * d->cols * 4))
     return reportf(TCCL_ERR_INVALID, "%s: the workspace has %lld bytes, %lld on 16 are needed", what, (long long)d->workspace_bytes, (long long)slots * 2 * d->cols * 4);
   const int size = size_of(d->dtype);
+  const int kind = rows_of(d->cols, size, {{d->grad, d->ld_grad}, {d->x, d->ld_x}, {d->grad_summed, d->ld_grad_summed}, {d->dx, d->ld_dx}});
+  // They read grad and x while dx is written: not where those share memory.
+  const bool apart = kind != kAnyRows && d->rows && columns_apart(d->rows) && lie_apart(d->dx, d->ld_dx, d->grad, d->ld_grad, d->rows, d->cols, size) &&
+                     (!d->x || lie_apart(d->dx, d->ld_dx, d->x, d->ld_x, d->rows, d->cols, size));
   NormGradArgs a;
   a.grad = (const char*)d->grad, a.x = (const char*)d->x, a.grad_summed = (const char*)d->grad_summed;
   a.values = (const uint8_t*)d->values, a.scales = (const uint8_t*)d->scales;
-  a.mean = d->mean, a.rstd = d->rstd, a.weight = d->weight, a.dx = (char*)d->dx, a.partial = (float*)d->workspace;
+  a.mean = d->mean, a.rstd = d->rstd, a.weight = d->weight, a.dx = (char*)d->dx, a.partial = apart ? nullptr : (float*)d->workspace;
+  a.dgamma = d->dweight, a.dbeta = d->dbias, a.column_wgs = apart && sums ? (d->cols + 31) / 32 : 0;
   a.ld_grad = d->ld_grad * size, a.ld_x = d->ld_x * size, a.ld_grad_summed = d->ld_grad_summed * size, a.ld_dx = d->ld_dx * size;
   a.scale_pitch = scale_pitch(d->rows), a.value_pitch = value_pitch(d->cols);
   a.rows = d->rows, a.cols = d->cols, a.items = s.items, a.affine_f32 = d->affine_dtype == TCCL_F32;
   a.inv_cols = 1.f / (float)d->cols;
   if (d->rows) {
+#define TCCL_BACKWARD(T)                                                           \
+  (kind == kAnyRows      ? backward<T, kAnyRows>(a, s, (hipStream_t)stream)        \
+   : kind == kVectorRows ? backward<T, kVectorRows>(a, s, (hipStream_t)stream)     \
+                         : backward<T, kLineRows>(a, s, (hipStream_t)stream))
     if (d->dtype == TCCL_F32)
-      backward<float>(a, s, (hipStream_t)stream);
+      TCCL_BACKWARD(float);
     else if (d->dtype == TCCL_BF16)
-      backward<__bf16>(a, s, (hipStream_t)stream);
+      TCCL_BACKWARD(__bf16);
     else
-      backward<_Float16>(a, s, (hipStream_t)stream);
+      TCCL_BACKWARD(_Float16);
     TCCL_TRY(launched(what));
   }
-  if (d->dweight || d->dbias)
+  if (sums && !apart)
     hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((2 * (int64_t)d->cols + 63) / 64)), dim3(1024), 0, (hipStream_t)stream, a.partial, d->dweight,
                        d->dbias, slots, d->cols);
   return launched(what);
