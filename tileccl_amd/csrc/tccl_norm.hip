@@ -76,7 +76,7 @@ Shape forward_shape(int rows, int cols, bool held, int cus) {
 bool columns_apart(int rows) { return rows <= 1024; }
 
 // Backward: as many as four rows (two of fp32) as long as there are four groups of them for each CU, workgroups of up to 512 threads whose
-// groups join their sums, 1024 threads of a CU at most and four turns each if that leaves every CU one: each
+// groups join their sums, 1024 threads of a CU at most and four turns each (of eight rows, two) if that leaves every CU one: each
 // workgroup's sums are written and read again.  2048 x 4096 bf16 26.6 us with 512 workgroups, 23.8 with 256; 12000 x 128 13.6
 // with eight groups each, 25.9 with one.
 Shape backward_shape(int rows, int cols, int dtype, bool held, int cus) {
@@ -91,7 +91,8 @@ Shape backward_shape(int rows, int cols, int dtype, bool held, int cus) {
   while (s.groups > (columns_apart(rows) ? (3 + s.waves) / s.waves : 1) && s.items < cus / 2 * s.groups) s.groups /= 2;
   s.threads = 64 * s.waves * s.groups;
   const int wanted = (s.items + s.groups - 1) / s.groups, most = cus * (s.threads <= 512 ? 1024 / s.threads : 1);
-  s.wgs = columns_apart(rows) ? wanted : wanted / 4 < cus ? cus : wanted / 4;
+  const int few = wanted / (held ? 2 : 4);  // (8192 x 4096 from 8 bits 50.4 us with two turns, 58.0 with four)
+  s.wgs = columns_apart(rows) ? wanted : few < cus ? cus : few;
   if (s.wgs > most && !columns_apart(rows)) s.wgs = most;
   if (s.wgs > wanted) s.wgs = wanted;
   return s;
