@@ -25,6 +25,8 @@ struct WeightArgs {
   int tiles_h, tiles_n;
   int steps, splits;            // steps of 64 tokens; a split takes steps_per_split of them
   int steps_per_split;
+  int xcds, span;               // slot -> tile (tile_for_slot)
+  int band;                     // tile rows of a band (tile_coords)
   int wide;                     // rows of out and add start on four elements
 };
 
@@ -76,62 +78,102 @@ TCCL_D void put4(const f32x4& v, const char* add, int64_t add_at, char* out, int
 }
 
 // kTileH x kTileN outputs, wavefronts 2 x kTileN / 64, each kTileH / 2 x 64.
+//
+// Three LDS stages of 64 tokens; step t computes from one while the loads of step t + 2 go to the one that step t - 1 has
+// left.  The loads are written out (copy_pair), so that the waits on them are counted here.
+//
+// 256 x 256, eight wavefronts, one workgroup per CU: a step is four phases (row half, token half), in each a wavefront first
+// moves data (two loads, LDS reads, the conversions of the phase's operands) and then multiplies (16 MFMAs, 256
+// clocks), with a barrier behind either; wavefronts 4..7 run one such slot behind wavefronts 0..3, so that of a SIMD's two
+// wavefronts one multiplies while the other moves data.  8-bit operands are read a phase ahead, so that nothing waits for
+// LDS within a slot.
+// 128 x 128, four wavefronts, two workgroups per CU: one barrier per step; each workgroup's waits are covered by the other.
 template <typename T, typename OutT, int kTileH, int kTileN, bool kTransposed>
 struct WeightGemm {
   typedef typename Mfma<T>::Vec Vec;
   typedef __attribute__((address_space(3))) void LdsVoid;
   typedef short s16x4 __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) s16x4 LdsQuad;
-  static constexpr int kWavesN = kTileN / 64, kWaves = 2 * kWavesN, kThreadsW = 64 * kWaves;
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  typedef uint32_t Words4 __attribute__((ext_vector_type(4)));
+  static constexpr bool kSides = kTileH == 256;
+  static constexpr int kWavesN = kTileN / 64, kWaves = 2 * kWavesN;
   static constexpr int kStepT = 64;                  // tokens of a step
   static constexpr int kRowsX = kTileH * 8;          // bytes of a row block of a stage
   static constexpr int kPitchG = kTileN * 2;         // bytes of a token of a stage
   static constexpr int kStageX = kRowsX * (kStepT / 8), kStageG = kPitchG * kStepT, kStage = kStageX + kStageG;
-  static constexpr int kStages = 3;
-  static constexpr int kLds = kStages * kStage;
-  static constexpr int kLoadsX = kStageX / 1024 / kWaves, kLoadsG = kStageG / 1024 / kWaves, kLoads = kLoadsX + kLoadsG;
+  static constexpr int kLds = 3 * kStage;
   static constexpr int kBlocksH = kTileH / 32, kBlocksN = 4;  // 16 x 16 blocks of a wavefront
+  static_assert(kStageX / 1024 / kWaves == 2 && kStageG / 1024 / kWaves == 4, "loads of a wavefront and step");
 
   const WeightArgs& a;
   char* lds;
   const int lane, wave, wh, wn;
   int h0, n0;
-  uint32_t off_x[kLoadsX], off_g[kLoadsG];
+  uint32_t off_x[2], off_g[2][2];  // this lane's byte offsets within a step
 
   TCCL_D WeightGemm(const WeightArgs& args, char* mem)
       : a(args), lds(mem), lane((int)(threadIdx.x & 63)), wave(__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6))), wh(wave / kWavesN), wn(wave % kWavesN) {}
 
-  static TCCL_D uint32_t clamped(int64_t bytes) { return bytes <= 0 ? 0u : bytes > 0xfffffff0ll ? 0xfffffff0u : (uint32_t)bytes; }
+  static TCCL_D Words4 window(const void* p, int64_t bytes) {
+    const uint64_t at = (uint64_t)(uintptr_t)p;
+    Words4 d;
+    d[0] = __builtin_amdgcn_readfirstlane((uint32_t)at);
+    d[1] = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32) & 0xffffu);
+    d[2] = __builtin_amdgcn_readfirstlane(bytes <= 0 ? 0u : bytes > 0xfffffff0ll ? 0xfffffff0u : (uint32_t)bytes);
+    d[3] = 0x00020000u;
+    return d;
+  }
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  // Two loads of 16 bytes per lane, global -> LDS, lane l's to `to` + 16 l and `to` + 1024 + 16 l; zero past the window.  Written out
+  // because the compiler makes every later read of an LDS array wait for all loads into it.  M0 wants an instruction between
+  // its write and the load; a scalar register that a vector instruction has written wants five wait states before a vector memory
+  // instruction reads it, which the block spends itself.
+  static TCCL_D void copy_pair(char* to, Words4 from, const uint32_t (&off)[2]) {
+    const uint32_t first = (uint32_t)(uintptr_t)(LdsVoid*)to, second = first + 1024u;
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %2, %4, 0 offen lds\n\t"
+        "s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %4, 0 offen lds" ::"s"(first), "s"(second), "v"(off[0]), "v"(off[1]), "s"(from)
+        : "memory", "m0");
+  }
+#pragma clang diagnostic pop
 
-  // The loads of step `t` into a stage.  Tokens past the last read as zero: they lie past the end of the window.
-  TCCL_D void issue(char* stage, int t) const {
-    const int64_t from_x = (int64_t)t * (kStepT / 8) * a.value_pitch + (int64_t)h0 * 8;
-    const int64_t from_g = ((int64_t)t * kStepT * a.ld_grad + n0) * 2;
-    const int64_t all_x = a.row_blocks * a.value_pitch, all_g = ((int64_t)(a.tokens - 1) * a.ld_grad + (a.outputs + 7) / 8 * 8) * 2;
-    const __amdgpu_buffer_rsrc_t x = __builtin_amdgcn_make_buffer_rsrc((void*)(a.values + from_x), 0, clamped(all_x - from_x), 0x00020000);
-    const __amdgpu_buffer_rsrc_t g = __builtin_amdgcn_make_buffer_rsrc((void*)(a.grad + from_g), 0, clamped(all_g - from_g), 0x00020000);
-#pragma unroll
-    for (int i = 0; i < kLoadsX; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(x, (LdsVoid*)(stage + (kLoadsX * wave + i) * 1024), 16, off_x[i], 0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < kLoadsG; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(g, (LdsVoid*)(stage + kStageX + (kLoadsG * wave + i) * 1024), 16, off_g[i], 0, 0, 0);
+  // Part p of the loads of step t into `stage`: 0 the 8-bit values, 1 and 2 the gradient.  Tokens past the last read as zero:
+  // they lie past the end of the window.
+  TCCL_D void issue(char* stage, int t, int p) const {
+    if (p == 0) {
+      const int64_t from = (int64_t)t * (kStepT / 8) * a.value_pitch + (int64_t)h0 * 8;
+      copy_pair(stage + 2 * wave * 1024, window(a.values + from, a.row_blocks * a.value_pitch - from), off_x);
+    } else {
+      const int64_t from = ((int64_t)t * kStepT * a.ld_grad + n0) * 2;
+      const int64_t all = ((int64_t)(a.tokens - 1) * a.ld_grad + (a.outputs + 7) / 8 * 8) * 2;
+      copy_pair(stage + kStageX + (4 * wave + 2 * (p - 1)) * 1024, window(a.grad + from, all - from), off_g[p - 1]);
+    }
   }
 
-  // The scale of the lane's row block of step t, half h (32 tokens).
-  TCCL_D uint32_t scale_bits(int t, int h) const {
-    int rb = t * (kStepT / 8) + 4 * h + (lane >> 4);
-    rb = rb < a.row_blocks ? rb : a.row_blocks - 1;
+  // The scales of the eight row blocks of step t (of the last step, past it).
+  TCCL_D u32x2 scales_of(int t) const {
+    typedef u32x2 Unaligned __attribute__((aligned(1)));
     int cb = (h0 + wh * (kTileH / 2)) / 128;
     const int last = (int)(a.value_pitch / 1024) - 1;
     cb = cb < last ? cb : last;
-    return a.scales[cb * a.scale_pitch + rb];
+    t = t < a.steps ? t : a.steps - 1;
+    return *(const Unaligned __attribute__((address_space(1)))*)(a.scales + cb * a.scale_pitch + t * (kStepT / 8));
+  }
+  // That of the lane's row block in token half h.  (255 is no scale: what lies behind the last row block may be anything.)
+  TCCL_D float scale_of(u32x2 s, int h) const {
+    const uint32_t e = (s[h] >> (8 * (lane >> 4))) & 255u;
+    return __uint_as_float((e < 254u ? e : 254u) << 23);
   }
 
-  TCCL_D Vec operand_x(const char* stage, int h, int b, float scale) const {
-    const int i = lane & 15, g = lane >> 4, rb = 4 * h + g;
-    const int chunk = (wh * kBlocksH + b) ^ (rb & 1);  // 16 columns, 128 bytes
-    const u32x2 q = *(const u32x2*)(stage + rb * kRowsX + chunk * 128 + i * 8);
+  // The codes of 16 x 16 x 32 operand b, token half h: the lane's eight tokens of one column.
+  TCCL_D u32x2 codes(const char* stage, int h, int b) const {
+    const int i = lane & 15, g = lane >> 4;
+    const int chunk = (wh * kBlocksH + b) ^ (g & 1);  // 16 columns, 128 bytes
+    return *(const u32x2*)(stage + (4 * h + g) * kRowsX + chunk * 128 + i * 8);
+  }
+  static TCCL_D Vec operand(u32x2 q, float scale) {
     typedef typename FromHeld<T>::Pair Pair;
     const Pair p0 = FromHeld<T>::template pair<false>(q[0], scale), p1 = FromHeld<T>::template pair<true>(q[0], scale);
     const Pair p2 = FromHeld<T>::template pair<false>(q[1], scale), p3 = FromHeld<T>::template pair<true>(q[1], scale);
@@ -145,20 +187,115 @@ struct WeightGemm {
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad*)(p + 4 * kPitchG));
     return __builtin_bit_cast(Vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
-  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-  TCCL_D void run(int tile, int split) {
-    h0 = (tile / a.tiles_n) * kTileH, n0 = (tile % a.tiles_n) * kTileN;
-#pragma unroll
-    for (int i = 0; i < kLoadsX; ++i) {
-      const int byte = (kLoadsX * wave + i) * 1024 + lane * 16, rb = byte / kRowsX, at = byte % kRowsX;
-      off_x[i] = (uint32_t)(rb * a.value_pitch + (at ^ (128 * (rb & 1))));
+  static TCCL_D void between() { __builtin_amdgcn_sched_barrier(0); }
+  static TCCL_D void barrier() {
+    between();
+    __builtin_amdgcn_s_barrier();
+    between();
+    asm volatile("" ::: "memory");
+  }
+  template <int kLeft>
+  static TCCL_D void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLeft) : "memory");
+  }
+
+  TCCL_D void multiply(f32x4 (&acc)[kBlocksH][kBlocksN], int first, const Vec (&x)[4], const Vec (&g)[4]) const {
+    if (kSides) {
+      barrier();
+      __builtin_amdgcn_s_setprio(1);
     }
 #pragma unroll
-    for (int i = 0; i < kLoadsG; ++i) {
-      const int byte = (kLoadsG * wave + i) * 1024 + lane * 16, k = byte / kPitchG, slot = byte % kPitchG / 16;
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        acc[first + i][j] = kTransposed ? Mfma<T>::run16(x[i], g[j], acc[first + i][j]) : Mfma<T>::run16(g[j], x[i], acc[first + i][j]);
+    if (kSides) {
+      __builtin_amdgcn_s_setprio(0);
+      barrier();
+    }
+  }
+
+  struct Running {
+    u32x2 q[2][4];   // codes of this phase and of the next
+    Vec g[2][4];     // the gradient's operands of either token half
+    u32x2 scales, next_scales;
+  };
+
+  // Step t of the large tile.  A stage is last read in phase 2 (codes) and 1 (gradient) of its step and refilled from phase 1 of the next
+  // one on: behind two barriers.  The loads of step t + 1 are waited for in phase 2, behind them those of step t + 2 that
+  // phases 1 and 2 have issued; they are first read in phase 3.
+  TCCL_D void step_sides(const char* cur, const char* nxt, char* far, int t, f32x4 (&acc)[kBlocksH][kBlocksN], Running& f) const {
+    const float s0 = scale_of(f.scales, 0), s1 = scale_of(f.scales, 1);
+    Vec x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f.g[0][j] = operand_g(cur, 0, j);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.q[1][i] = codes(cur, 1, i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = operand(f.q[0][i], s0);
+    multiply(acc, 0, x, f.g[0]);
+    issue(far, t + 2, 0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f.g[1][j] = operand_g(cur, 1, j);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.q[0][i] = codes(cur, 0, 4 + i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = operand(f.q[1][i], s1);
+    multiply(acc, 0, x, f.g[1]);
+    issue(far, t + 2, 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.q[1][i] = codes(cur, 1, 4 + i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = operand(f.q[0][i], s0);
+    wait_loads<4>();
+    multiply(acc, 4, x, f.g[0]);
+    f.scales = f.next_scales;
+    f.next_scales = scales_of(t + 2);
+    issue(far, t + 2, 2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.q[0][i] = codes(nxt, 0, i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = operand(f.q[1][i], s1);
+    multiply(acc, 4, x, f.g[1]);
+  }
+
+  // Step t of the small tile.
+  TCCL_D void step_one(const char* cur, char* far, int t, f32x4 (&acc)[kBlocksH][kBlocksN], Running& f) const {
+    // The loads of this step have landed (the six of the next may be under way), everybody has left `far`.
+    asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)" ::: "memory");
+    barrier();
+    const u32x2 scales = f.scales;
+    f.scales = f.next_scales;
+    f.next_scales = scales_of(t + 2);
+    issue(far, t + 2, 0);
+    issue(far, t + 2, 1);
+    issue(far, t + 2, 2);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float s = scale_of(scales, h);
+      Vec x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f.g[h][j] = operand_g(cur, h, j);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = operand(codes(cur, h, i), s);
+      multiply(acc, 0, x, f.g[h]);
+    }
+  }
+
+  TCCL_D void run(int tile, int split) {
+    const TileCoord at = tile_coords(tile, a.tiles_h, a.tiles_n, a.band);
+    h0 = at.m * kTileH, n0 = at.n * kTileN;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int byte = (2 * wave + i) * 1024 + lane * 16, rb = byte / kRowsX, in = byte % kRowsX;
+      off_x[i] = (uint32_t)(rb * a.value_pitch + (in ^ (128 * (rb & 1))));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int byte = (4 * wave + i) * 1024 + lane * 16, k = byte / kPitchG, slot = byte % kPitchG / 16;
       const int chunk = slot ^ (4 * (k & 3)) ^ (2 * ((k >> 3) & 1));
-      off_g[i] = (uint32_t)(k * a.ld_grad * 2 + chunk * 16);
+      off_g[i >> 1][i & 1] = (uint32_t)(k * a.ld_grad * 2 + chunk * 16);
     }
     const int first = split * a.steps_per_split, end = first + a.steps_per_split < a.steps ? first + a.steps_per_split : a.steps;
     f32x4 acc[kBlocksH][kBlocksN];
@@ -166,40 +303,33 @@ struct WeightGemm {
     for (int i = 0; i < kBlocksH; ++i)
 #pragma unroll
       for (int j = 0; j < kBlocksN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    uint32_t bits[2] = {0, 0}, next_bits[2] = {0, 0};
-    if (first < end) {  // no tokens: no scales either
-      bits[0] = scale_bits(first, 0), bits[1] = scale_bits(first, 1);
-      issue(lds, first);
-      issue(lds + kStage, first + 1);
-    }
-    int cur = 0;
-    for (int t = first; t < end; ++t) {
-      // The loads of this step have landed (those of the next may be under way), everybody has left the stage
-      // that is filled next.
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLoads) : "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      const int far = cur == 0 ? 2 : cur - 1;
-      next_bits[0] = scale_bits(t + 1, 0), next_bits[1] = scale_bits(t + 1, 1);
-      issue(lds + far * kStage, t + 2);
-      const char* stage = lds + cur * kStage;
+    if (first < end) {  // (no tokens: no scales either)
+      Running f;
+      f.scales = scales_of(first);
+      f.next_scales = scales_of(first + 1);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float scale = __uint_as_float(bits[h] << 23);
-        Vec g[kBlocksN];
+      for (int p = 0; p < 3; ++p) issue(lds, first, p);
 #pragma unroll
-        for (int j = 0; j < kBlocksN; ++j) g[j] = operand_g(stage, h, j);
+      for (int p = 0; p < 3; ++p) issue(lds + kStage, first + 1, p);
+      int cur = 0;
+      if (kSides) {
+        wait_loads<6>();
+        barrier();
 #pragma unroll
-        for (int i = 0; i < kBlocksH; ++i) {
-          const Vec x = operand_x(stage, h, i, scale);
-#pragma unroll
-          for (int j = 0; j < kBlocksN; ++j) acc[i][j] = kTransposed ? Mfma<T>::run16(x, g[j], acc[i][j]) : Mfma<T>::run16(g[j], x, acc[i][j]);
-        }
+        for (int i = 0; i < 4; ++i) f.q[0][i] = codes(lds, 0, i);
+        if (wave >= kWaves / 2) barrier();  // one slot behind
       }
-      bits[0] = next_bits[0], bits[1] = next_bits[1];
-      cur = cur == 2 ? 0 : cur + 1;
+      for (int t = first; t < end; ++t) {
+        const int nxt = cur == 2 ? 0 : cur + 1, far = cur == 0 ? 2 : cur - 1;
+        if constexpr (kSides)
+          step_sides(lds + cur * kStage, lds + nxt * kStage, lds + far * kStage, t, acc, f);
+        else
+          step_one(lds + cur * kStage, lds + far * kStage, t, acc, f);
+        cur = nxt;
+      }
+      if (kSides && wave < kWaves / 2) barrier();
+      wait_loads<0>();
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     store(acc, split);
   }
 
@@ -225,14 +355,14 @@ struct WeightGemm {
 };
 
 template <typename T, typename OutT, int kTileH, int kTileN, bool kTransposed>
-__global__ __launch_bounds__(2 * kTileN, 1) void weight_gradient_kernel(WeightArgs a) {
+__global__ __launch_bounds__(2 * kTileN, 2) void weight_gradient_kernel(WeightArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef WeightGemm<T, OutT, kTileH, kTileN, kTransposed> Gemm;
   __shared__ __attribute__((aligned(1024))) char weight_lds[Gemm::kLds];
   const int tiles = a.tiles_h * a.tiles_n;
-  const int slot = (int)blockIdx.x;
+  const int slot = (int)blockIdx.x % tiles;
   Gemm gemm(a, weight_lds);
-  gemm.run(slot % tiles, slot / tiles);
+  gemm.run(tile_for_slot(slot, tiles, a.xcds, a.span), (int)blockIdx.x / tiles);
 #endif
 }
 

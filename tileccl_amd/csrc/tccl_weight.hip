@@ -89,6 +89,7 @@ int tccl_weight_gradient(const tccl_weight_gradient_desc* d, void* stream) {
   if (!d) return reportf(TCCL_ERR_INVALID, "%s: the descriptor is NULL", what);
   if (d->rows < 0 || d->cols < 1 || d->outputs < 1)
     return reportf(TCCL_ERR_INVALID, "%s: rows must not be negative, cols and outputs must be positive (got %d, %d, %d)", what, d->rows, d->cols, d->outputs);
+  if (d->cols > 1 << 24 || d->outputs > 1 << 24) return reportf(TCCL_ERR_UNSUPPORTED, "%s: %d x %d outputs, at most %d of either", what, d->cols, d->outputs, 1 << 24);
   if (d->dtype != TCCL_F16 && d->dtype != TCCL_BF16) return reportf(TCCL_ERR_UNSUPPORTED, "%s: grad is F16 or BF16", what);
   if (d->out_dtype != d->dtype && d->out_dtype != TCCL_F32) return reportf(TCCL_ERR_UNSUPPORTED, "%s: out is of grad's type or F32", what);
   if (!d->out) return reportf(TCCL_ERR_INVALID, "%s: out is NULL", what);
@@ -117,6 +118,8 @@ int tccl_weight_gradient(const tccl_weight_gradient_desc* d, void* stream) {
   a.value_pitch = ((int64_t)d->cols + 127) / 128 * 1024, a.scale_pitch = ((int64_t)a.row_blocks + 15) / 16 * 16;
   a.ld_grad = d->rows > 1 ? d->ld_grad : (d->outputs + 7) / 8 * 8, a.ld_add = d->ld_add, a.ld_out = d->ld_out, a.ld_partial = partial_pitch(cols);
   a.tiles_h = c.tiles_h, a.tiles_n = c.tiles_n, a.steps = c.steps, a.splits = c.splits, a.steps_per_split = c.steps_per_split;
+  // An XCD takes a patch of tiles: 4 rows of them by as many columns as its CUs give.
+  a.band = 4, a.xcds = cus % 8 ? 1 : 8, a.span = cus / a.xcds;
   a.wide = ((uintptr_t)d->out | (uintptr_t)d->add) % (4 * osize) == 0 && (rows == 1 || (d->ld_out % 4 == 0 && (!d->add || d->ld_add % 4 == 0)));
   if (c.splits > 1) {
     const int64_t need = 4 * c.splits * partial_rows(rows, cols);
