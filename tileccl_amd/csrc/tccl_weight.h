@@ -26,6 +26,7 @@ struct WeightArgs {
   int steps, splits;            // steps of 64 tokens; a split takes steps_per_split of them
   int steps_per_split;
   int xcds, span;               // slot -> tile (tile_for_slot)
+  int staged;                   // `add` is there, fp32, wide, its rows within reach: store_staged()
   int band;                     // tile rows of a band (tile_coords)
   int wide;                     // rows of out and add start on four elements
 };
@@ -55,25 +56,33 @@ struct FromHeld<_Float16> {
   static TCCL_D Pair pair(uint32_t q, float scale) { return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)q, scale, kHigh); }
 };
 
-// Four neighbouring outputs; `left` (1 ..) columns exist from the first on.
+// Four neighbouring outputs, of which `left` (1 ..) exist.  `wide`: rows start on four elements.
 template <typename OutT>
-TCCL_D void put4(const f32x4& v, const char* add, int64_t add_at, char* out, int64_t out_at, int left, bool wide) {
+TCCL_D f32x4 get4(const char* from, int64_t at, int left, bool wide) {
   typedef OutT Quad __attribute__((ext_vector_type(4)));
-  f32x4 s = v;
+  typedef const Quad __attribute__((address_space(1))) GlobalQuad;
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
   if (wide && left >= 4) {
-    if (add) {
-      const Quad o = *(const Quad*)((const OutT*)add + add_at);
+    const Quad o = *(GlobalQuad*)((const OutT*)from + at);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[e] += (float)o[e];
-    }
-    *(Quad*)((OutT*)out + out_at) = (Quad){to_out<OutT>(s[0]), to_out<OutT>(s[1]), to_out<OutT>(s[2]), to_out<OutT>(s[3])};
+    for (int e = 0; e < 4; ++e) s[e] = (float)o[e];
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (e < left) {
-        if (add) s[e] += (float)((const OutT*)add)[add_at + e];
-        ((OutT*)out)[out_at + e] = to_out<OutT>(s[e]);
-      }
+      if (e < left) s[e] = (float)((const OutT*)from)[at + e];
+  }
+  return s;
+}
+template <typename OutT>
+TCCL_D void put4(const f32x4& s, char* to, int64_t at, int left, bool wide) {
+  typedef OutT Quad __attribute__((ext_vector_type(4)));
+  typedef Quad __attribute__((address_space(1))) GlobalQuad;
+  if (wide && left >= 4) {
+    *(GlobalQuad*)((OutT*)to + at) = (Quad){to_out<OutT>(s[0]), to_out<OutT>(s[1]), to_out<OutT>(s[2]), to_out<OutT>(s[3])};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left) ((OutT*)to)[at + e] = to_out<OutT>(s[e]);
   }
 }
 
@@ -139,31 +148,50 @@ struct WeightGemm {
   }
 #pragma clang diagnostic pop
 
-  // Part p of the loads of step t into `stage`: 0 the 8-bit values, 1 and 2 the gradient.  Tokens past the last read as zero:
-  // they lie past the end of the window.
-  TCCL_D void issue(char* stage, int t, int p) const {
+  // Where the next step's operands lie, and how many bytes there are from there on.
+  struct Source {
+    const uint8_t* x;
+    const char* g;
+    int64_t left_x, left_g;
+  };
+  TCCL_D Source source(int step) const {
+    const int64_t from_x = (int64_t)step * (kStepT / 8) * a.value_pitch + (int64_t)h0 * 8, from_g = ((int64_t)step * kStepT * a.ld_grad + n0) * 2;
+    return Source{a.values + from_x, a.grad + from_g, a.row_blocks * a.value_pitch - from_x,
+                  ((int64_t)(a.tokens - 1) * a.ld_grad + (a.outputs + 7) / 8 * 8) * 2 - from_g};
+  }
+  // Part p of the loads of a step into `stage`: 0 the 8-bit values, 1 and 2 the gradient; behind part 2 the source is the next
+  // step's.  Tokens past the last read as zero: they lie past the end of the window.
+  TCCL_D void issue(char* stage, Source& s, int p) const {
     if (p == 0) {
-      const int64_t from = (int64_t)t * (kStepT / 8) * a.value_pitch + (int64_t)h0 * 8;
-      copy_pair(stage + 2 * wave * 1024, window(a.values + from, a.row_blocks * a.value_pitch - from), off_x);
+      copy_pair(stage + 2 * wave * 1024, window(s.x, s.left_x), off_x);
+      s.x += (kStepT / 8) * a.value_pitch, s.left_x -= (kStepT / 8) * a.value_pitch;
     } else {
-      const int64_t from = ((int64_t)t * kStepT * a.ld_grad + n0) * 2;
-      const int64_t all = ((int64_t)(a.tokens - 1) * a.ld_grad + (a.outputs + 7) / 8 * 8) * 2;
-      copy_pair(stage + kStageX + (4 * wave + 2 * (p - 1)) * 1024, window(a.grad + from, all - from), off_g[p - 1]);
+      copy_pair(stage + kStageX + (4 * wave + 2 * (p - 1)) * 1024, window(s.g, s.left_g), off_g[p - 1]);
+      if (p == 2) s.g += kStepT * 2 * a.ld_grad, s.left_g -= kStepT * 2 * a.ld_grad;
     }
   }
 
-  // The scales of the eight row blocks of step t (of the last step, past it).
-  TCCL_D u32x2 scales_of(int t) const {
-    typedef u32x2 Unaligned __attribute__((aligned(1)));
+  // The scales of the wavefront's column block for kScaleSteps steps from `first` on: lane l has those of row blocks 16 l ..
+  // 16 l + 15.  One load for 8192 tokens: an ordinary load in every step would be waited for with everything behind it, the copies
+  // of the next stages (the compiler does not count those).
+  static constexpr int kScaleSteps = 128;
+  TCCL_D Words4 scales_from(int first) const {
+    typedef Words4 Unaligned __attribute__((aligned(1)));
+    typedef const Unaligned __attribute__((address_space(1))) Global;
     int cb = (h0 + wh * (kTileH / 2)) / 128;
     const int last = (int)(a.value_pitch / 1024) - 1;
     cb = cb < last ? cb : last;
-    t = t < a.steps ? t : a.steps - 1;
-    return *(const Unaligned __attribute__((address_space(1)))*)(a.scales + cb * a.scale_pitch + t * (kStepT / 8));
+    const int64_t at = (int64_t)first * (kStepT / 8) + 16 * lane;
+    Words4 s = {0, 0, 0, 0};
+    if (at < a.scale_pitch) s = *(Global*)(a.scales + cb * a.scale_pitch + at);
+    asm volatile("" : "+v"(s));  // waited for here, not in the loop
+    return s;
   }
-  // That of the lane's row block in token half h.  (255 is no scale: what lies behind the last row block may be anything.)
-  TCCL_D float scale_of(u32x2 s, int h) const {
-    const uint32_t e = (s[h] >> (8 * (lane >> 4))) & 255u;
+  // That of the lane's row block in token half h of the step that is `n` steps behind the first.  (255 is no scale: what lies
+  // behind the last row block may be anything.)
+  TCCL_D float scale_of(const Words4& s, int n, int h) const {
+    const uint32_t even = __builtin_amdgcn_readlane(s[h], n >> 1), odd = __builtin_amdgcn_readlane(s[2 + h], n >> 1);
+    const uint32_t e = ((n & 1 ? odd : even) >> (8 * (lane >> 4))) & 255u;
     return __uint_as_float((e < 254u ? e : 254u) << 23);
   }
 
@@ -173,12 +201,11 @@ struct WeightGemm {
     const int chunk = (wh * kBlocksH + b) ^ (g & 1);  // 16 columns, 128 bytes
     return *(const u32x2*)(stage + (4 * h + g) * kRowsX + chunk * 128 + i * 8);
   }
-  static TCCL_D Vec operand(u32x2 q, float scale) {
-    typedef typename FromHeld<T>::Pair Pair;
-    const Pair p0 = FromHeld<T>::template pair<false>(q[0], scale), p1 = FromHeld<T>::template pair<true>(q[0], scale);
-    const Pair p2 = FromHeld<T>::template pair<false>(q[1], scale), p3 = FromHeld<T>::template pair<true>(q[1], scale);
-    return (Vec){p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
+  // Dword w (tokens 2w, 2w + 1) of the operand that codes are converted to.
+  static TCCL_D uint32_t converted(u32x2 q, int w, float scale) {
+    return __builtin_bit_cast(uint32_t, w & 1 ? FromHeld<T>::template pair<true>(q[w >> 1], scale) : FromHeld<T>::template pair<false>(q[w >> 1], scale));
   }
+  static TCCL_D Words4 operand(u32x2 q, float scale) { return (Words4){converted(q, 0, scale), converted(q, 1, scale), converted(q, 2, scale), converted(q, 3, scale)}; }
   TCCL_D Vec operand_g(const char* stage, int h, int b) const {
     const int i = lane & 15, g = lane >> 4, t = i >> 2, cq = i & 3;
     const int chunk = (wn * 8 + 2 * b + (cq >> 1)) ^ (4 * t) ^ (2 * (g & 1));
@@ -200,86 +227,81 @@ struct WeightGemm {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLeft) : "memory");
   }
 
-  TCCL_D void multiply(f32x4 (&acc)[kBlocksH][kBlocksN], int first, const Vec (&x)[4], const Vec (&g)[4]) const {
-    if (kSides) {
-      barrier();
-      __builtin_amdgcn_s_setprio(1);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        acc[first + i][j] = kTransposed ? Mfma<T>::run16(x[i], g[j], acc[first + i][j]) : Mfma<T>::run16(g[j], x[i], acc[first + i][j]);
-    if (kSides) {
-      __builtin_amdgcn_s_setprio(0);
-      barrier();
-    }
+  static TCCL_D f32x4 product(Words4 x, Vec g, f32x4 c) {
+    const Vec v = __builtin_bit_cast(Vec, x);
+    return kTransposed ? Mfma<T>::run16(v, g, c) : Mfma<T>::run16(g, v, c);
   }
 
   struct Running {
-    u32x2 q[2][4];   // codes of this phase and of the next
+    u32x2 q[4];      // codes of the next phase
+    Words4 x[2][4];  // 8-bit operands, converted, of this phase and the next
     Vec g[2][4];     // the gradient's operands of either token half
-    u32x2 scales, next_scales;
+    Words4 scales;   // from step scales_at on
+    int scales_at;
   };
 
-  // Step t of the large tile.  A stage is last read in phase 2 (codes) and 1 (gradient) of its step and refilled from phase 1 of the next
-  // one on: behind two barriers.  The loads of step t + 1 are waited for in phase 2, behind them those of step t + 2 that
-  // phases 1 and 2 have issued; they are first read in phase 3.
-  TCCL_D void step_sides(const char* cur, const char* nxt, char* far, int t, f32x4 (&acc)[kBlocksH][kBlocksN], Running& f) const {
-    const float s0 = scale_of(f.scales, 0), s1 = scale_of(f.scales, 1);
-    Vec x[4];
+  // The multiplying slot of phase `kPhase`: 16 MFMAs, behind each the conversion of two of the next phase's values.
+  template <int kPhase>
+  TCCL_D void multiply(f32x4 (&acc)[kBlocksH][kBlocksN], Running& f, float next_scale) const {
+    constexpr int first = kPhase < 2 ? 0 : 4;
+    barrier();
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f.g[0][j] = operand_g(cur, 0, j);
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f.q[1][i] = codes(cur, 1, i);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = operand(f.q[0][i], s0);
-    multiply(acc, 0, x, f.g[0]);
-    issue(far, t + 2, 0);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) f.g[1][j] = operand_g(cur, 1, j);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f.q[0][i] = codes(cur, 0, 4 + i);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = operand(f.q[1][i], s1);
-    multiply(acc, 0, x, f.g[1]);
-    issue(far, t + 2, 1);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f.q[1][i] = codes(cur, 1, 4 + i);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = operand(f.q[0][i], s0);
-    wait_loads<4>();
-    multiply(acc, 4, x, f.g[0]);
-    f.scales = f.next_scales;
-    f.next_scales = scales_of(t + 2);
-    issue(far, t + 2, 2);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f.q[0][i] = codes(nxt, 0, i);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = operand(f.q[1][i], s1);
-    multiply(acc, 4, x, f.g[1]);
+      for (int i = 0; i < 4; ++i) {
+        acc[first + i][j] = product(f.x[kPhase & 1][i], f.g[kPhase & 1][j], acc[first + i][j]);
+        f.x[1 - (kPhase & 1)][j][i] = converted(f.q[j], i, next_scale);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 1, 0);
+      }
+    __builtin_amdgcn_s_setprio(0);
+    barrier();
   }
 
-  // Step t of the small tile.
-  TCCL_D void step_one(const char* cur, char* far, int t, f32x4 (&acc)[kBlocksH][kBlocksN], Running& f) const {
+  // Step t of the large tile; `next`: the scale of the next step's first half.  A stage is last read in phase 2 (codes) and 1
+  // (gradient) of its step and refilled from phase 1 of the next one on: behind two barriers.  The loads of step t + 1 are waited for in
+  // phase 2, behind them those of step t + 2 that phases 1 and 2 have issued; they are first read in phase 3.
+  TCCL_D void step_sides(const char* cur, const char* nxt, char* far, Source& src, float s0, float s1, float next, f32x4 (&acc)[kBlocksH][kBlocksN], Running& f) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.q[i] = codes(cur, 1, i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f.g[0][j] = operand_g(cur, 0, j);
+    multiply<0>(acc, f, s1);
+    issue(far, src, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.q[i] = codes(cur, 0, 4 + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f.g[1][j] = operand_g(cur, 1, j);
+    multiply<1>(acc, f, s0);
+    issue(far, src, 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.q[i] = codes(cur, 1, 4 + i);
+    wait_loads<4>();
+    multiply<2>(acc, f, s1);
+    issue(far, src, 2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.q[i] = codes(nxt, 0, i);
+    multiply<3>(acc, f, next);
+  }
+
+  // A step of the small tile.
+  TCCL_D void step_one(const char* cur, char* far, Source& src, float s0, float s1, f32x4 (&acc)[kBlocksH][kBlocksN], Running& f) const {
     // The loads of this step have landed (the six of the next may be under way), everybody has left `far`.
     asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)" ::: "memory");
     barrier();
-    const u32x2 scales = f.scales;
-    f.scales = f.next_scales;
-    f.next_scales = scales_of(t + 2);
-    issue(far, t + 2, 0);
-    issue(far, t + 2, 1);
-    issue(far, t + 2, 2);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) issue(far, src, p);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float s = scale_of(scales, h);
-      Vec x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f.x[h][i] = operand(codes(cur, h, i), h ? s1 : s0);
 #pragma unroll
       for (int j = 0; j < 4; ++j) f.g[h][j] = operand_g(cur, h, j);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = operand(codes(cur, h, i), s);
-      multiply(acc, 0, x, f.g[h]);
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i][j] = product(f.x[h][i], f.g[h][j], acc[i][j]);
     }
   }
 
@@ -305,52 +327,137 @@ struct WeightGemm {
       for (int j = 0; j < kBlocksN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
     if (first < end) {  // (no tokens: no scales either)
       Running f;
-      f.scales = scales_of(first);
-      f.next_scales = scales_of(first + 1);
+      Source src = source(first);
 #pragma unroll
-      for (int p = 0; p < 3; ++p) issue(lds, first, p);
+      for (int p = 0; p < 3; ++p) issue(lds, src, p);
 #pragma unroll
-      for (int p = 0; p < 3; ++p) issue(lds + kStage, first + 1, p);
+      for (int p = 0; p < 3; ++p) issue(lds + kStage, src, p);
+      f.scales = scales_from(first);
+      f.scales_at = first;
       int cur = 0;
+      float s0 = scale_of(f.scales, 0, 0);
       if (kSides) {
         wait_loads<6>();
         barrier();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f.q[0][i] = codes(lds, 0, i);
+        for (int i = 0; i < 4; ++i) f.x[0][i] = operand(codes(lds, 0, i), s0);
         if (wave >= kWaves / 2) barrier();  // one slot behind
       }
       for (int t = first; t < end; ++t) {
         const int nxt = cur == 2 ? 0 : cur + 1, far = cur == 0 ? 2 : cur - 1;
+        const float s1 = scale_of(f.scales, t - f.scales_at, 1);
+        if (t + 1 - f.scales_at == kScaleSteps) {
+          f.scales = scales_from(t + 1);
+          f.scales_at = t + 1;
+        }
+        const float next = scale_of(f.scales, t + 1 - f.scales_at, 0);
         if constexpr (kSides)
-          step_sides(lds + cur * kStage, lds + nxt * kStage, lds + far * kStage, t, acc, f);
+          step_sides(lds + cur * kStage, lds + nxt * kStage, lds + far * kStage, src, s0, s1, next, acc, f);
         else
-          step_one(lds + cur * kStage, lds + far * kStage, t, acc, f);
+          step_one(lds + cur * kStage, lds + far * kStage, src, s0, s1, acc, f);
+        s0 = next;
         cur = nxt;
       }
       if (kSides && wave < kWaves / 2) barrier();
       wait_loads<0>();
     }
+    if constexpr (kSides && sizeof(OutT) == 4)
+      if (a.staged && h0 + kTileH <= a.cols && n0 + kTileN <= a.outputs) return store_staged(acc);
     store(acc, split);
   }
 
-  // Lane l has out-row i % 16 of a block and 4 neighbouring columns 4 * (l / 16) .. of the row.
-  TCCL_D void store(const f32x4 (&acc)[kBlocksH][kBlocksN], int split) const {
+  // A whole 256 x 256 tile of fp32 on top of `add`: the tile's rows of `add` come through LDS, 128 of them (1 KiB each, one
+  // load) in either of two rounds; round 1 is on its way while round 0 is added and stored.  Round r has the rows of the
+  // wavefronts' blocks i (transposed: j) of half r.  16-byte chunk c of row k lies in slot c ^ (k % 16), which spreads the
+  // 16 rows that a read takes over the banks.  Read block by block, 64 bytes of 16 rows at a time, 64 MiB that are not in a
+  // cache cost 8192 x 4096 x 4096 34 us.
+  TCCL_D void store_staged(f32x4 (&acc)[kBlocksH][kBlocksN]) const {
+    const int i16 = lane & 15, g = lane >> 4;
+    const int row0 = kTransposed ? n0 : h0, col0 = kTransposed ? h0 : n0;
+    constexpr int kPart = kTransposed ? 32 : 64;  // consecutive rows of a round
+    const Words4 from = window((const float*)a.add + row0 * a.ld_add + col0, 0xfffffff0ll);
+    auto fetch = [&](int r) {
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        uint32_t off[2];
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          const int k = 16 * wave + 2 * p + o, row = k / kPart * (2 * kPart) + r * kPart + k % kPart;
+          off[o] = (uint32_t)(row * a.ld_add * 4) + (uint32_t)((lane ^ (k & 15)) * 16);
+        }
+        copy_pair(lds + (16 * wave + 2 * p) * 1024, from, off);
+      }
+    };
+    constexpr int kI = kTransposed ? kBlocksH : 4, kJ = kTransposed ? 2 : 4;  // blocks of a round
+    barrier();  // everybody has read the last stage
+    fetch(0);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      f32x4 more[kI][kJ];
+      wait_loads<0>();
+      barrier();
+#pragma unroll
+      for (int i = 0; i < kI; ++i)
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) {
+          const int k = (kTransposed ? wn * 32 + 16 * j : wh * 64 + 16 * i) + i16;
+          const int c = (kTransposed ? wh * 32 + 4 * i : wn * 16 + 4 * j) + g;
+          more[i][j] = *(const f32x4*)(lds + k * 1024 + ((c ^ i16) * 16));
+        }
+      if (r == 0) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        barrier();
+        fetch(1);
+      }
+#pragma unroll
+      for (int i = 0; i < kI; ++i)
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) {
+          const int bi = kTransposed ? i : 4 * r + i, bj = kTransposed ? 2 * r + j : j;
+          const int h = h0 + wh * (kTileH / 2) + 16 * bi, n = n0 + wn * 64 + 16 * bj;
+          const int64_t row = (kTransposed ? n : h) + i16, col = (kTransposed ? h : n) + 4 * g;
+          put4<float>(acc[bi][bj] + more[i][j], a.out, row * a.ld_out + col, 4, true);
+        }
+    }
+  }
+
+  // Lane l has out-row l % 16 of a block and 4 neighbouring columns 4 * (l / 16) .. of the row.  What is added is read
+  // for four rows of blocks at once: one trip to memory for each half of a wavefront's outputs instead of one for each few.
+  TCCL_D void store(f32x4 (&acc)[kBlocksH][kBlocksN], int split) const {
     const int i16 = lane & 15, g = lane >> 4;
     const int rows = kTransposed ? a.outputs : a.cols, cols = kTransposed ? a.cols : a.outputs;
 #pragma unroll
-    for (int i = 0; i < kBlocksH; ++i)
+    for (int half = 0; half < kBlocksH; half += 4) {
+      const int h1 = h0 + wh * (kTileH / 2) + 16 * half, n1 = n0 + wn * 64;
+      if (a.splits == 1 && a.add) {
+        f32x4 more[4][kBlocksN];
 #pragma unroll
-      for (int j = 0; j < kBlocksN; ++j) {
-        const int h = h0 + wh * (kTileH / 2) + 16 * i, n = n0 + wn * 64 + 16 * j;
-        const int row = kTransposed ? n + i16 : h + i16, col = (kTransposed ? h : n) + 4 * g;
-        if (row < rows && col < cols) store4(acc[i][j], row, col, cols - col, split, rows);
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < kBlocksN; ++j) {
+            const int h = h1 + 16 * i, n = n1 + 16 * j, row = kTransposed ? n + i16 : h + i16, col = (kTransposed ? h : n) + 4 * g;
+            more[i][j] = row < rows && col < cols ? get4<OutT>(a.add, row * a.ld_add + col, cols - col, a.wide) : (f32x4){0.f, 0.f, 0.f, 0.f};
+          }
+        between();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < kBlocksN; ++j) acc[half + i][j] += more[i][j];
       }
-  }
-  TCCL_D void store4(f32x4 v, int row, int col, int left, int split, int rows) const {
-    if (a.splits > 1)
-      put4<float>(v, nullptr, 0, (char*)(a.partial + (int64_t)split * rows * a.ld_partial), row * a.ld_partial + col, left, true);
-    else
-      put4<OutT>(v, a.add, row * a.ld_add + col, a.out, row * a.ld_out + col, left, a.wide);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < kBlocksN; ++j) {
+          const int h = h1 + 16 * i, n = n1 + 16 * j, row = kTransposed ? n + i16 : h + i16, col = (kTransposed ? h : n) + 4 * g;
+          if (row < rows && col < cols) {
+            if (a.splits > 1)
+              put4<float>(acc[half + i][j], (char*)(a.partial + (int64_t)split * rows * a.ld_partial), row * a.ld_partial + col, cols - col, true);
+            else
+              put4<OutT>(acc[half + i][j], a.out, row * a.ld_out + col, cols - col, a.wide);
+          }
+        }
+      between();
+    }
   }
 };
 
@@ -377,7 +484,8 @@ __global__ __launch_bounds__(256) void weight_sum_kernel(WeightSumArgs a) {
     const float* p = a.partial + row * a.ld_partial + col;
     f32x4 s = *(const f32x4*)p;
     for (int k = 1; k < a.splits; ++k) s += *(const f32x4*)(p + k * a.slice);
-    put4<OutT>(s, a.add, row * a.ld_add + col, a.out, row * a.ld_out + col, a.cols - col, a.wide);
+    if (a.add) s += get4<OutT>(a.add, row * a.ld_add + col, a.cols - col, a.wide);
+    put4<OutT>(s, a.out, row * a.ld_out + col, a.cols - col, a.wide);
   }
 #endif
 }

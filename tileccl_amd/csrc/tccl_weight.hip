@@ -121,6 +121,7 @@ int tccl_weight_gradient(const tccl_weight_gradient_desc* d, void* stream) {
   // An XCD takes a patch of tiles: 4 rows of them by as many columns as its CUs give.
   a.band = 4, a.xcds = cus % 8 ? 1 : 8, a.span = cus / a.xcds;
   a.wide = ((uintptr_t)d->out | (uintptr_t)d->add) % (4 * osize) == 0 && (rows == 1 || (d->ld_out % 4 == 0 && (!d->add || d->ld_add % 4 == 0)));
+  a.staged = d->add && a.wide && c.splits == 1 && d->out_dtype == TCCL_F32 && d->ld_add <= 1 << 22;
   if (c.splits > 1) {
     const int64_t need = 4 * c.splits * partial_rows(rows, cols);
     if (!d->workspace || ((uintptr_t)d->workspace & 15) || d->workspace_bytes < need)
