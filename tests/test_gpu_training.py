@@ -259,6 +259,23 @@ def test_weight_gradient_of_any_pitch_and_start(lib, layout, pitch, offset, out_
     check_weight(out if layout == "kn" else out.t(), ref.held(x), dy, None, F32)
 
 
+@pytest.mark.parametrize("rows, cols, outputs", [(100, 128, 64), (190, 256, 136), (1090, 64, 264), (9000, 64, 64), (9000, 512, 384)])
+def test_weight_gradient_of_blocks_with_scales_of_their_own(lib, rows, cols, outputs):
+    """Neighbouring blocks' scales differ by up to 2^10; the tokens are cut at odd and even steps of 64."""
+    x, dy = rand((rows, cols), 1, BF16), rand((rows, outputs), 2, BF16)
+    x *= torch.exp2(((torch.arange(rows) // 8)[:, None] * 7 + (torch.arange(cols) // 128)[None] * 3) % 11 - 5).to(BF16)
+    held = ops.checkpoint_activation(x.cuda())
+    check_weight(ops.weight_gradient(held, dy.cuda()), ref.held(x), dy, None, F32)
+
+
+@pytest.mark.parametrize("rows, cols, outputs", [(1, 8192, 8192), (65, 8192, 264), (100, 8192, 264), (100, 264, 8192)])
+def test_weight_gradient_of_fewer_steps_than_stages(lib, rows, cols, outputs):
+    """Few tokens of wide layers: what the pipeline would load next, and the last scales of a cut at an odd step, lie behind the operands."""
+    x, dy = rand((rows, cols), 1, BF16), rand((rows, outputs), 2, BF16)
+    held = ops.checkpoint_activation(x.cuda())
+    check_weight(ops.weight_gradient(held, dy.cuda()), ref.held(x), dy, None, F32)
+
+
 def test_what_is_not_finite_stays_in_its_row_and_column(lib):
     """NaN and infinities beside and behind the operands (the memory around them is NaN) and in them."""
     rows, cols, outputs = 100, 200, 136

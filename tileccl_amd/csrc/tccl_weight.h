@@ -25,7 +25,7 @@ struct WeightArgs {
   int tiles_h, tiles_n;
   int steps, splits;            // steps of 64 tokens; a split takes steps_per_split of them
   int steps_per_split;
-  int xcds, span;               // slot -> tile (tile_for_slot)
+  int xcds, per_xcd;            // dies with an L2 of their own; (split, tile) pairs of one
   int staged;                   // `add` is there, fp32, wide, its rows within reach: store_staged()
   int band;                     // tile rows of a band (tile_coords)
   int wide;                     // rows of out and add start on four elements
@@ -97,7 +97,9 @@ TCCL_D void put4(const f32x4& s, char* to, int64_t at, int left, bool wide) {
 // wavefronts one multiplies while the other moves data.  8-bit operands are read a phase ahead, so that nothing waits for
 // LDS within a slot.
 // 128 x 128, four wavefronts, two workgroups per CU: one barrier per step; each workgroup's waits are covered by the other.
-template <typename T, typename OutT, int kTileH, int kTileN, bool kTransposed>
+// kGroups = 2: 128 x 128 with eight wavefronts, of which either half takes half of the tokens with stages of its own; the
+// halves' sums meet in LDS.  For few tiles: the work of two workgroups on one tile, without partial sums in memory.
+template <typename T, typename OutT, int kTileH, int kTileN, bool kTransposed, int kGroups>
 struct WeightGemm {
   typedef typename Mfma<T>::Vec Vec;
   typedef __attribute__((address_space(3))) void LdsVoid;
@@ -111,25 +113,27 @@ struct WeightGemm {
   static constexpr int kRowsX = kTileH * 8;          // bytes of a row block of a stage
   static constexpr int kPitchG = kTileN * 2;         // bytes of a token of a stage
   static constexpr int kStageX = kRowsX * (kStepT / 8), kStageG = kPitchG * kStepT, kStage = kStageX + kStageG;
-  static constexpr int kLds = 3 * kStage;
+  static constexpr int kLds = kGroups * 3 * kStage;
   static constexpr int kBlocksH = kTileH / 32, kBlocksN = 4;  // 16 x 16 blocks of a wavefront
   static_assert(kStageX / 1024 / kWaves == 2 && kStageG / 1024 / kWaves == 4, "loads of a wavefront and step");
 
   const WeightArgs& a;
   char* lds;
-  const int lane, wave, wh, wn;
+  const int lane, group, wave, wh, wn;
   int h0, n0;
   uint32_t off_x[2], off_g[2][2];  // this lane's byte offsets within a step
 
   TCCL_D WeightGemm(const WeightArgs& args, char* mem)
-      : a(args), lds(mem), lane((int)(threadIdx.x & 63)), wave(__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6))), wh(wave / kWavesN), wn(wave % kWavesN) {}
+      : a(args), lds(mem + (kGroups > 1 ? __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) / kWaves * 3 * kStage : 0)), lane((int)(threadIdx.x & 63)),
+        group(kGroups > 1 ? __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) / kWaves : 0),
+        wave(__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) % kWaves), wh(wave / kWavesN), wn(wave % kWavesN) {}
 
   static TCCL_D Words4 window(const void* p, int64_t bytes) {
     const uint64_t at = (uint64_t)(uintptr_t)p;
     Words4 d;
     d[0] = __builtin_amdgcn_readfirstlane((uint32_t)at);
     d[1] = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32) & 0xffffu);
-    d[2] = __builtin_amdgcn_readfirstlane(bytes <= 0 ? 0u : bytes > 0xfffffff0ll ? 0xfffffff0u : (uint32_t)bytes);
+    d[2] = __builtin_amdgcn_readfirstlane(bytes > 0xfffffff0ll ? 0xfffffff0u : (uint32_t)bytes);  // (there are always some)
     d[3] = 0x00020000u;
     return d;
   }
@@ -148,35 +152,43 @@ struct WeightGemm {
   }
 #pragma clang diagnostic pop
 
-  // Where the next step's operands lie, and how many bytes there are from there on.
+  // Where the next step's operands lie, and how many bytes there are from there on.  Steps past the last are the last one again,
+  // so that no window begins behind its operand.
   struct Source {
     const uint8_t* x;
     const char* g;
     int64_t left_x, left_g;
+    int more;  // steps behind this one
   };
   TCCL_D Source source(int step) const {
+    step = step < a.steps ? step : a.steps - 1;
     const int64_t from_x = (int64_t)step * (kStepT / 8) * a.value_pitch + (int64_t)h0 * 8, from_g = ((int64_t)step * kStepT * a.ld_grad + n0) * 2;
     return Source{a.values + from_x, a.grad + from_g, a.row_blocks * a.value_pitch - from_x,
-                  ((int64_t)(a.tokens - 1) * a.ld_grad + (a.outputs + 7) / 8 * 8) * 2 - from_g};
+                  ((int64_t)(a.tokens - 1) * a.ld_grad + (a.outputs + 7) / 8 * 8) * 2 - from_g, a.steps - 1 - step};
   }
   // Part p of the loads of a step into `stage`: 0 the 8-bit values, 1 and 2 the gradient; behind part 2 the source is the next
   // step's.  Tokens past the last read as zero: they lie past the end of the window.
   TCCL_D void issue(char* stage, Source& s, int p) const {
     if (p == 0) {
       copy_pair(stage + 2 * wave * 1024, window(s.x, s.left_x), off_x);
-      s.x += (kStepT / 8) * a.value_pitch, s.left_x -= (kStepT / 8) * a.value_pitch;
     } else {
       copy_pair(stage + kStageX + (4 * wave + 2 * (p - 1)) * 1024, window(s.g, s.left_g), off_g[p - 1]);
-      if (p == 2) s.g += kStepT * 2 * a.ld_grad, s.left_g -= kStepT * 2 * a.ld_grad;
+      if (p == 2) {
+        const int64_t step_x = s.more > 0 ? (kStepT / 8) * a.value_pitch : 0, step_g = s.more > 0 ? kStepT * 2 * a.ld_grad : 0;
+        s.x += step_x, s.left_x -= step_x;
+        s.g += step_g, s.left_g -= step_g;
+        --s.more;
+      }
     }
   }
 
   // The scales of the wavefront's column block for kScaleSteps steps from `first` on: lane l has those of row blocks 16 l ..
-  // 16 l + 15.  One load for 8192 tokens: an ordinary load in every step would be waited for with everything behind it, the copies
+  // 16 l + 15.  `first` is even: a step has 8 row blocks, and a 16-byte read from an odd one would end 8 bytes behind the row, for
+  // the last column block behind the scales.  One load for 8192 tokens: an ordinary load in every step would be waited for with everything behind it, the copies
   // of the next stages (the compiler does not count those).
   static constexpr int kScaleSteps = 128;
   TCCL_D Words4 scales_from(int first) const {
-    typedef Words4 Unaligned __attribute__((aligned(1)));
+    typedef Words4 Unaligned __attribute__((aligned(1)));  // (the scales' address may be any)
     typedef const Unaligned __attribute__((address_space(1))) Global;
     int cb = (h0 + wh * (kTileH / 2)) / 128;
     const int last = (int)(a.value_pitch / 1024) - 1;
@@ -240,22 +252,26 @@ struct WeightGemm {
     int scales_at;
   };
 
-  // The multiplying slot of phase `kPhase`: 16 MFMAs, behind each the conversion of two of the next phase's values.
-  template <int kPhase>
-  TCCL_D void multiply(f32x4 (&acc)[kBlocksH][kBlocksN], Running& f, float next_scale) const {
-    constexpr int first = kPhase < 2 ? 0 : 4;
-    barrier();
+  // 16 MFMAs from operand sets kX and kG, behind each the conversion of two values of the next operands.
+  template <int kX, int kG>
+  TCCL_D void multiply(f32x4 (&acc)[kBlocksH][kBlocksN], int first, Running& f, float next_scale) const {
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        acc[first + i][j] = product(f.x[kPhase & 1][i], f.g[kPhase & 1][j], acc[first + i][j]);
-        f.x[1 - (kPhase & 1)][j][i] = converted(f.q[j], i, next_scale);
+        acc[first + i][j] = product(f.x[kX][i], f.g[kG][j], acc[first + i][j]);
+        f.x[1 - kX][j][i] = converted(f.q[j], i, next_scale);
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x002, 1, 0);
       }
     __builtin_amdgcn_s_setprio(0);
+  }
+  // The multiplying slot of phase `kPhase` of the large tile.
+  template <int kPhase>
+  TCCL_D void slot(f32x4 (&acc)[kBlocksH][kBlocksN], Running& f, float next_scale) const {
+    barrier();
+    multiply<kPhase & 1, kPhase & 1>(acc, kPhase < 2 ? 0 : 4, f, next_scale);
     barrier();
   }
 
@@ -267,42 +283,46 @@ struct WeightGemm {
     for (int i = 0; i < 4; ++i) f.q[i] = codes(cur, 1, i);
 #pragma unroll
     for (int j = 0; j < 4; ++j) f.g[0][j] = operand_g(cur, 0, j);
-    multiply<0>(acc, f, s1);
+    slot<0>(acc, f, s1);
     issue(far, src, 0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) f.q[i] = codes(cur, 0, 4 + i);
 #pragma unroll
     for (int j = 0; j < 4; ++j) f.g[1][j] = operand_g(cur, 1, j);
-    multiply<1>(acc, f, s0);
+    slot<1>(acc, f, s0);
     issue(far, src, 1);
 #pragma unroll
     for (int i = 0; i < 4; ++i) f.q[i] = codes(cur, 1, 4 + i);
     wait_loads<4>();
-    multiply<2>(acc, f, s1);
+    slot<2>(acc, f, s1);
     issue(far, src, 2);
 #pragma unroll
     for (int i = 0; i < 4; ++i) f.q[i] = codes(nxt, 0, i);
-    multiply<3>(acc, f, next);
+    slot<3>(acc, f, next);
   }
 
-  // A step of the small tile.
-  TCCL_D void step_one(const char* cur, char* far, Source& src, float s0, float s1, f32x4 (&acc)[kBlocksH][kBlocksN], Running& f) const {
-    // The loads of this step have landed (the six of the next may be under way), everybody has left `far`.
+  // A step of the small tile, whose first half's operands are there.  Either half reads the next one's while it multiplies; the loads of
+  // the next step are waited for in between, and those of the step after the next two go to the stage that everybody has left then.
+  // `live`: false where the other group has a step more.
+  TCCL_D void step_one(char* cur, const char* nxt, Source& src, float s1, float next, f32x4 (&acc)[kBlocksH][kBlocksN], Running& f, bool live) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.q[i] = codes(cur, 1, i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f.g[1][j] = operand_g(cur, 1, j);
+    between();
+    if (kGroups == 1 || live) multiply<0, 0>(acc, 0, f, s1);
+    between();
     asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)" ::: "memory");
     barrier();
 #pragma unroll
-    for (int p = 0; p < 3; ++p) issue(far, src, p);
+    for (int i = 0; i < 4; ++i) f.q[i] = codes(nxt, 0, i);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int j = 0; j < 4; ++j) f.g[0][j] = operand_g(nxt, 0, j);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f.x[h][i] = operand(codes(cur, h, i), h ? s1 : s0);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) f.g[h][j] = operand_g(cur, h, j);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i][j] = product(f.x[h][i], f.g[h][j], acc[i][j]);
-    }
+    for (int p = 0; p < 3; ++p) issue(cur, src, p);
+    between();
+    if (kGroups == 1 || live) multiply<1, 1>(acc, 0, f, next);
+    between();
   }
 
   TCCL_D void run(int tile, int split) {
@@ -319,31 +339,46 @@ struct WeightGemm {
       const int chunk = slot ^ (4 * (k & 3)) ^ (2 * ((k >> 3) & 1));
       off_g[i >> 1][i & 1] = (uint32_t)(k * a.ld_grad * 2 + chunk * 16);
     }
-    const int first = split * a.steps_per_split, end = first + a.steps_per_split < a.steps ? first + a.steps_per_split : a.steps;
+    int first = split * a.steps_per_split, end = first + a.steps_per_split < a.steps ? first + a.steps_per_split : a.steps;
+    int turns = end - first;
+    if (kGroups > 1) {  // either group takes as many turns; the second one may have a step fewer
+      turns = (end - first + 1) / 2;
+      first += group * turns;
+      end = group ? end : first + turns;
+    }
     f32x4 acc[kBlocksH][kBlocksN];
 #pragma unroll
     for (int i = 0; i < kBlocksH; ++i)
 #pragma unroll
       for (int j = 0; j < kBlocksN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    if (first < end) {  // (no tokens: no scales either)
+    if (turns > 0) {  // (no tokens: no scales either)
       Running f;
       Source src = source(first);
 #pragma unroll
       for (int p = 0; p < 3; ++p) issue(lds, src, p);
 #pragma unroll
       for (int p = 0; p < 3; ++p) issue(lds + kStage, src, p);
-      f.scales = scales_from(first);
-      f.scales_at = first;
+      if (!kSides) {
+#pragma unroll
+        for (int p = 0; p < 3; ++p) issue(lds + 2 * kStage, src, p);
+      }
+      f.scales_at = first & ~1;
+      f.scales = scales_from(f.scales_at);
       int cur = 0;
-      float s0 = scale_of(f.scales, 0, 0);
-      if (kSides) {
-        wait_loads<6>();
-        barrier();
+      float s0 = scale_of(f.scales, first - f.scales_at, 0);
+      wait_loads<kSides ? 6 : 12>();
+      barrier();
+      if (!kSides) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f.x[0][i] = operand(codes(lds, 0, i), s0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f.g[0][j] = operand_g(lds, 0, j);
+      } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) f.x[0][i] = operand(codes(lds, 0, i), s0);
         if (wave >= kWaves / 2) barrier();  // one slot behind
       }
-      for (int t = first; t < end; ++t) {
+      for (int t = first; t < first + turns; ++t) {
         const int nxt = cur == 2 ? 0 : cur + 1, far = cur == 0 ? 2 : cur - 1;
         const float s1 = scale_of(f.scales, t - f.scales_at, 1);
         if (t + 1 - f.scales_at == kScaleSteps) {
@@ -354,16 +389,21 @@ struct WeightGemm {
         if constexpr (kSides)
           step_sides(lds + cur * kStage, lds + nxt * kStage, lds + far * kStage, src, s0, s1, next, acc, f);
         else
-          step_one(lds + cur * kStage, lds + far * kStage, src, s0, s1, acc, f);
+          step_one(lds + cur * kStage, lds + nxt * kStage, src, s1, next, acc, f, t < end);
         s0 = next;
         cur = nxt;
       }
       if (kSides && wave < kWaves / 2) barrier();
       wait_loads<0>();
     }
+    if constexpr (kGroups > 1) {
+      join(acc);
+      store<kBlocksH / 2>(acc, split, group * (kBlocksH / 2));
+      return;
+    }
     if constexpr (kSides && sizeof(OutT) == 4)
       if (a.staged && h0 + kTileH <= a.cols && n0 + kTileN <= a.outputs) return store_staged(acc);
-    store(acc, split);
+    store<kBlocksH>(acc, split, 0);
   }
 
   // A whole 256 x 256 tile of fp32 on top of `add`: the tile's rows of `add` come through LDS, 128 of them (1 KiB each, one
@@ -421,18 +461,42 @@ struct WeightGemm {
     }
   }
 
-  // Lane l has out-row l % 16 of a block and 4 neighbouring columns 4 * (l / 16) .. of the row.  What is added is read
-  // for four rows of blocks at once: one trip to memory for each half of a wavefront's outputs instead of one for each few.
-  TCCL_D void store(f32x4 (&acc)[kBlocksH][kBlocksN], int split) const {
+  // The two groups' sums: each gives the other half of its rows of blocks away and has the other half, group 0 the first.
+  TCCL_D void join(f32x4 (&acc)[kBlocksH][kBlocksN]) const {
+    char* base = lds - group * 3 * kStage;
+    constexpr int kHalf = kBlocksH / 2 * kBlocksN;
+    barrier();  // everybody has read the last stages
+#pragma unroll
+    for (int i = 0; i < kBlocksH / 2; ++i)
+#pragma unroll
+      for (int j = 0; j < kBlocksN; ++j)
+        *(f32x4*)(base + (((group * kWaves + wave) * kHalf + i * kBlocksN + j) * 64 + lane) * 16) = group ? acc[i][j] : acc[kBlocksH / 2 + i][j];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kBlocksH / 2; ++i)
+#pragma unroll
+      for (int j = 0; j < kBlocksN; ++j) {
+        const f32x4 other = *(const f32x4*)(base + ((((1 - group) * kWaves + wave) * kHalf + i * kBlocksN + j) * 64 + lane) * 16);
+        // (group 0's half of the tokens first, whoever adds)
+        acc[i][j] = group ? other + acc[kBlocksH / 2 + i][j] : acc[i][j] + other;
+      }
+  }
+
+  // Rows of blocks 0 .. kRows - 1 of `acc`, which are `from` .. of the wavefront's.  Lane l has out-row l % 16 of a block and 4
+  // neighbouring columns 4 * (l / 16) .. of the row.  What is added is read for several rows of blocks at once: one trip to memory
+  // for each half of a wavefront's outputs instead of one for each few.
+  template <int kRows>
+  TCCL_D void store(f32x4 (&acc)[kBlocksH][kBlocksN], int split, int from) const {
     const int i16 = lane & 15, g = lane >> 4;
     const int rows = kTransposed ? a.outputs : a.cols, cols = kTransposed ? a.cols : a.outputs;
+    constexpr int kAtOnce = kRows < 4 ? kRows : 4;
 #pragma unroll
-    for (int half = 0; half < kBlocksH; half += 4) {
-      const int h1 = h0 + wh * (kTileH / 2) + 16 * half, n1 = n0 + wn * 64;
+    for (int half = 0; half < kRows; half += kAtOnce) {
+      const int h1 = h0 + wh * (kTileH / 2) + 16 * (from + half), n1 = n0 + wn * 64;
       if (a.splits == 1 && a.add) {
-        f32x4 more[4][kBlocksN];
+        f32x4 more[kAtOnce][kBlocksN];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < kAtOnce; ++i)
 #pragma unroll
           for (int j = 0; j < kBlocksN; ++j) {
             const int h = h1 + 16 * i, n = n1 + 16 * j, row = kTransposed ? n + i16 : h + i16, col = (kTransposed ? h : n) + 4 * g;
@@ -440,12 +504,12 @@ struct WeightGemm {
           }
         between();
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < kAtOnce; ++i)
 #pragma unroll
           for (int j = 0; j < kBlocksN; ++j) acc[half + i][j] += more[i][j];
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < kAtOnce; ++i)
 #pragma unroll
         for (int j = 0; j < kBlocksN; ++j) {
           const int h = h1 + 16 * i, n = n1 + 16 * j, row = kTransposed ? n + i16 : h + i16, col = (kTransposed ? h : n) + 4 * g;
@@ -461,15 +525,17 @@ struct WeightGemm {
   }
 };
 
-template <typename T, typename OutT, int kTileH, int kTileN, bool kTransposed>
-__global__ __launch_bounds__(2 * kTileN, 2) void weight_gradient_kernel(WeightArgs a) {
+template <typename T, typename OutT, int kTileH, int kTileN, bool kTransposed, int kGroups>
+__global__ __launch_bounds__(2 * kTileN * kGroups, 2) void weight_gradient_kernel(WeightArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  typedef WeightGemm<T, OutT, kTileH, kTileN, kTransposed> Gemm;
+  typedef WeightGemm<T, OutT, kTileH, kTileN, kTransposed, kGroups> Gemm;
   __shared__ __attribute__((aligned(1024))) char weight_lds[Gemm::kLds];
-  const int tiles = a.tiles_h * a.tiles_n;
-  const int slot = (int)blockIdx.x % tiles;
+  // Workgroups go to the XCDs in turn.  XCD x takes a run of the (split, tile) pairs: the tiles of a split, neighbours of each
+  // other, which read the same rows of the operands, find them in one L2 (16384 x 1024 x 512: 30.9 -> 29.3 us).
+  const int tiles = a.tiles_h * a.tiles_n, item = (int)blockIdx.x % a.xcds * a.per_xcd + (int)blockIdx.x / a.xcds;
+  if (item >= tiles * a.splits) return;
   Gemm gemm(a, weight_lds);
-  gemm.run(tile_for_slot(slot, tiles, a.xcds, a.span), (int)blockIdx.x / tiles);
+  gemm.run(item % tiles, item / tiles);
 #endif
 }
 

@@ -1,5 +1,6 @@
 // Weight gradients from activations in 8 bits: argument checks, launch shapes and the entry points.
 #include <hip/hip_runtime.h>
+#include <initializer_list>
 
 #pragma GCC visibility push(default)
 #include "../../include/tileccl_hip.h"
@@ -11,15 +12,18 @@ namespace {
 
 using namespace tccl;
 
+// The kernels: 256 x 256 tiles; 128 x 128 by eight wavefronts (two groups); 128 x 128 by four, two workgroups per CU.
+enum Kind { kLarge, kPairs, kSmall };
+
 struct Cut {
-  bool large;  // 256 x 256 tiles, else 128 x 128
+  Kind kind;
   int tiles_h, tiles_n, steps, splits, steps_per_split;
 };
 
-Cut cut_of(bool large, int splits, int rows, int cols, int outputs) {
-  const int edge = large ? 256 : 128;
+Cut cut_of(Kind kind, int splits, int rows, int cols, int outputs) {
+  const int edge = kind == kLarge ? 256 : 128;
   Cut c;
-  c.large = large;
+  c.kind = kind;
   c.tiles_h = (cols + edge - 1) / edge, c.tiles_n = (outputs + edge - 1) / edge;
   c.steps = (rows + 63) / 64;
   c.steps_per_split = (c.steps + splits - 1) / splits;
@@ -27,16 +31,34 @@ Cut cut_of(bool large, int splits, int rows, int cols, int outputs) {
   return c;
 }
 
+// An estimate of a launch's microseconds, fitted to sixteen shapes (64 to 16384 tokens, 64 to 4096 inputs and outputs) with
+// every kind and up to 128 splits; what it chose took at most 6 % longer than the best.  A step of 64 tokens: 1.53 us of a 256 tile, 1.0
+// of two 128 tiles' worth by two groups or (0.95) two workgroups on a CU, 0.65 of one workgroup alone.
+double estimate(const Cut& c, int cols, int outputs, int cus) {
+  const int64_t wgs = (int64_t)c.tiles_h * c.tiles_n * c.splits, steps = c.steps_per_split;
+  const double out_mb = 4e-6 * cols * outputs;
+  double us = 5.0 + out_mb / 5.0;
+  if (c.kind == kLarge)
+    us += (wgs + cus - 1) / cus * 1.53 * steps;
+  else if (c.kind == kPairs)
+    us += 1.0 + (wgs + cus - 1) / cus * ((steps + 1) / 2);
+  else
+    us += wgs / (2 * cus) * 0.95 * steps + (wgs % (2 * cus) > cus ? 0.95 : wgs % (2 * cus) ? 0.65 : 0.0) * steps;
+  if (c.splits > 1) us += 3.5 + 2.0 * c.splits * out_mb / 5.0;  // the partial sums there and back, and a second launch
+  return us;
+}
+
 Cut choose(int rows, int cols, int outputs, int cus) {
-  const Cut large = cut_of(true, 1, rows, cols, outputs);
-  const int64_t tiles = (int64_t)large.tiles_h * large.tiles_n;
-  if (tiles * 2 > cus) return large;
-  const Cut small = cut_of(false, 1, rows, cols, outputs);
-  const int64_t n = (int64_t)small.tiles_h * small.tiles_n;
-  int splits = (int)(2 * cus / n);
-  const int most = small.steps / 4;
-  if (splits > most) splits = most;
-  return cut_of(false, splits > 1 ? splits : 1, rows, cols, outputs);
+  Cut best = cut_of(kSmall, 1, rows, cols, outputs);
+  double least = estimate(best, cols, outputs, cus);
+  for (const Kind kind : {kLarge, kPairs, kSmall})
+    for (const int splits : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+      if (splits > 1 && (rows + 63) / 64 < 2 * splits) break;
+      const Cut c = cut_of(kind, splits, rows, cols, outputs);
+      const double us = estimate(c, cols, outputs, cus);
+      if (us < least) best = c, least = us;
+    }
+  return best;
 }
 
 int64_t partial_pitch(int cols) { return ((int64_t)cols + 3) / 4 * 4; }
@@ -44,11 +66,13 @@ int64_t partial_rows(int rows, int cols) { return (int64_t)rows * partial_pitch(
 
 template <typename T, typename OutT, bool kTransposed>
 int launch(const WeightArgs& a, const Cut& c, hipStream_t stream) {
-  const dim3 wgs((unsigned)(c.tiles_h * c.tiles_n * c.splits));
-  if (c.large)
-    hipLaunchKernelGGL((weight_gradient_kernel<T, OutT, 256, 256, kTransposed>), wgs, dim3(512), 0, stream, a);
+  const dim3 wgs((unsigned)(a.xcds * a.per_xcd));
+  if (c.kind == kLarge)
+    hipLaunchKernelGGL((weight_gradient_kernel<T, OutT, 256, 256, kTransposed, 1>), wgs, dim3(512), 0, stream, a);
+  else if (c.kind == kPairs)
+    hipLaunchKernelGGL((weight_gradient_kernel<T, OutT, 128, 128, kTransposed, 2>), wgs, dim3(512), 0, stream, a);
   else
-    hipLaunchKernelGGL((weight_gradient_kernel<T, OutT, 128, 128, kTransposed>), wgs, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((weight_gradient_kernel<T, OutT, 128, 128, kTransposed, 1>), wgs, dim3(256), 0, stream, a);
   return launched("weight_gradient");
 }
 
@@ -118,8 +142,8 @@ int tccl_weight_gradient(const tccl_weight_gradient_desc* d, void* stream) {
   a.value_pitch = ((int64_t)d->cols + 127) / 128 * 1024, a.scale_pitch = ((int64_t)a.row_blocks + 15) / 16 * 16;
   a.ld_grad = d->rows > 1 ? d->ld_grad : (d->outputs + 7) / 8 * 8, a.ld_add = d->ld_add, a.ld_out = d->ld_out, a.ld_partial = partial_pitch(cols);
   a.tiles_h = c.tiles_h, a.tiles_n = c.tiles_n, a.steps = c.steps, a.splits = c.splits, a.steps_per_split = c.steps_per_split;
-  // An XCD takes a patch of tiles: 4 rows of them by as many columns as its CUs give.
-  a.band = 4, a.xcds = cus % 8 ? 1 : 8, a.span = cus / a.xcds;
+  a.xcds = cus % 8 ? 1 : 8, a.per_xcd = (c.tiles_h * c.tiles_n * c.splits + a.xcds - 1) / a.xcds;
+  a.band = 4;  // an XCD's run of tiles is four rows of them by as many columns as its CUs give
   a.wide = ((uintptr_t)d->out | (uintptr_t)d->add) % (4 * osize) == 0 && (rows == 1 || (d->ld_out % 4 == 0 && (!d->add || d->ld_add % 4 == 0)));
   a.staged = d->add && a.wide && c.splits == 1 && d->out_dtype == TCCL_F32 && d->ld_add <= 1 << 22;
   if (c.splits > 1) {
