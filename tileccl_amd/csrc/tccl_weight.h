@@ -549,7 +549,14 @@ __global__ __launch_bounds__(256) void weight_sum_kernel(WeightSumArgs a) {
     const int row = (int)(u / quads), col = (int)(u % quads) * 4;
     const float* p = a.partial + row * a.ld_partial + col;
     f32x4 s = *(const f32x4*)p;
-    for (int k = 1; k < a.splits; ++k) s += *(const f32x4*)(p + k * a.slice);
+    for (int first = 1; first < a.splits; first += 8) {  // eight on their way at a time (16384 x 256 x 256: 24 -> 20 us)
+      f32x4 more[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) more[k] = first + k < a.splits ? *(const f32x4*)(p + (first + k) * a.slice) : (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (first + k < a.splits) s += more[k];
+    }
     if (a.add) s += get4<OutT>(a.add, row * a.ld_add + col, a.cols - col, a.wide);
     put4<OutT>(s, a.out, row * a.ld_out + col, a.cols - col, a.wide);
   }

@@ -31,19 +31,20 @@ Cut cut_of(Kind kind, int splits, int rows, int cols, int outputs) {
   return c;
 }
 
-// An estimate of a launch's microseconds, fitted to sixteen shapes (64 to 16384 tokens, 64 to 4096 inputs and outputs) with
-// every kind and up to 128 splits; what it chose took at most 6 % longer than the best.  A step of 64 tokens: 1.53 us of a 256 tile, 1.0
-// of two 128 tiles' worth by two groups or (0.95) two workgroups on a CU, 0.65 of one workgroup alone.
+// An estimate of a launch's microseconds, fitted to shapes of 64 to 16384 tokens and 64 to 7168 inputs and outputs with every kind and up
+// to 128 splits.  Of the thirty it was then checked at, what it chose took at most 7 % longer than the best (9000 x 130 x 3000: 28.2, best
+// 26.4 us).  A step of 64 tokens: 1.53 us of a 256 tile (less where CUs are idle: the clock is higher), 1.0 of two steps by two groups,
+// 0.95 of two workgroups on a CU, 0.65 of one alone there; what is left over behind full rounds fills gaps of theirs, 0.45.
 double estimate(const Cut& c, int cols, int outputs, int cus) {
   const int64_t wgs = (int64_t)c.tiles_h * c.tiles_n * c.splits, steps = c.steps_per_split;
   const double out_mb = 4e-6 * cols * outputs;
   double us = 5.0 + out_mb / 5.0;
   if (c.kind == kLarge)
-    us += (wgs + cus - 1) / cus * 1.53 * steps;
+    us += (wgs + cus - 1) / cus * (wgs < cus ? 1.2 + 0.33 * wgs / cus : 1.53) * steps;
   else if (c.kind == kPairs)
     us += 1.0 + (wgs + cus - 1) / cus * ((steps + 1) / 2);
   else
-    us += wgs / (2 * cus) * 0.95 * steps + (wgs % (2 * cus) > cus ? 0.95 : wgs % (2 * cus) ? 0.65 : 0.0) * steps;
+    us += wgs / (2 * cus) * 0.95 * steps + (wgs % (2 * cus) > cus ? 0.95 : wgs % (2 * cus) == 0 ? 0.0 : wgs > 2 * cus ? 0.45 : 0.65) * steps;
   if (c.splits > 1) us += 3.5 + 2.0 * c.splits * out_mb / 5.0;  // the partial sums there and back, and a second launch
   return us;
 }
