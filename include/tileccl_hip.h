@@ -508,7 +508,7 @@ int tccl_mfma_rate_probe(int32_t kind, const void* a_like, int64_t a_bytes, cons
  * The value that is held, q * 2^e, is exact in the tensor's type.  With RB = ceil(rows / 8), CB = ceil(cols / 128):
  *   values  uint8[RB][128 * CB][8]     row block, column, row in the block; zeros beyond the tensor; on 16 bytes
  *   scales  uint8[CB][SP]              e + 127 of column block, row block; SP = RB rounded up to 16; bytes from RB on
- *                                      are not read */
+ *                                      may hold anything */
 #define TCCL_HELD_ROWS 8
 #define TCCL_HELD_COLS 128
 typedef struct tccl_held_desc {

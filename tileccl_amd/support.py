@@ -3,7 +3,7 @@
 Same shape as ``/root/reference/tileccl/support.py:29-88`` (``SupportStatus``,
 ``RuntimeSupportMatrix.to_dict()`` with its ``context / ops / contracts / execution_paths /
 collectives / memory`` sections), filled for the surface built here: the three GEMM +
-collective operations on hand-written HIP kernels, one process, ranks emulated as slices of
+collective operations and the norm, checkpoint and weight-gradient operators on hand-written HIP kernels, one process, ranks emulated as slices of
 one device arena, plus the stand-alone collectives in their direct-write / peer-read form.
 """
 
@@ -90,6 +90,9 @@ def describe_runtime_support(ctx=None) -> RuntimeSupportMatrix:
             "gemm_allgather": SupportStatus(needs_heap, "column shards through the all-scatter launch; row blocks through tileccl_v2-style FusedGemmAllGather"),
             "gemm_reducescatter": SupportStatus(needs_heap, "column shards: per-owner GEMM + fp32 row reduce; row shards through FusedGemmReduceScatter"),
             "chained_ag_gemm_rs": SupportStatus(needs_heap, "gather launch, then GEMM with the scatter from its epilogue"),
+            "layer_norm": yes("fp16 / bf16 / fp32 rows of up to 32768 columns, with a residual and an 8-bit checkpoint of its input; layer_norm_backward from either"),
+            "checkpoint_activation": yes("fp16 / bf16 in e4m3 with a power-of-two scale per 8 x 128 block; restore_activation"),
+            "weight_gradient": yes("from a checkpoint and a fp16 / bf16 gradient; fp32 or 16-bit result, optionally added to"),
         },
         contracts={
             "full/full": yes("default public contract"),
