@@ -151,6 +151,33 @@ def test_backward(lib, rows, cols, dtype, affine, more, held):
     assert torch.equal(only.x, d.x) and only.weight is None and only.bias is None
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("rows, cols", [(1025, 5), (1030, 100), (9000, 1003), (5001, 2052), (3000, 4096), (1100, 4100), (2500, 6001), (1027, 8190), (1026, 8200)])
+def test_backward_of_many_rows(lib, rows, cols, dtype):
+    """Workgroups that take several groups of rows, with rows that end inside a vector; dx in the place of either gradient."""
+    s, dy, more = rand((rows, cols), 1, dtype, 2.0, 0.5), rand((rows, cols), 2, dtype, 0.1), rand((rows, cols), 3, dtype, 0.1)
+    weight = rand((cols,), 4, dtype, 0.2, 1.0)
+    _, mean, rstd = ref.layer_norm(s)
+    mean, rstd = mean.float().cuda(), rstd.float().cuda()
+    d = ops.layer_norm_backward(dy.cuda(), s.cuda(), mean, rstd, weight.cuda(), grad_summed=more.cuda())
+    check_backward(d, dy, s, mean, rstd, weight, more)
+    for place in (0, 1):
+        g, m = dy.cuda(), more.cuda()
+        there = ops.layer_norm_backward(g, s.cuda(), mean, rstd, weight.cuda(), grad_summed=m, out=(g, m)[place])
+        assert torch.equal(there.x, d.x) and torch.equal(there.weight, d.weight) and torch.equal(there.bias, d.bias)
+
+
+@pytest.mark.parametrize("held", [False, True])
+@pytest.mark.parametrize("rows, cols", [(16, 16384), (60, 12001), (250, 2056), (257, 2056), (1000, 260), (1024, 9)])
+def test_sums_of_few_rows(lib, rows, cols, held):
+    """Column sums by workgroups of their own: wide and narrow ones, one pass over the rows and several, part of a vector at the end."""
+    s, dy = rand((rows, cols), 1, BF16, 2.0, 0.5), rand((rows, cols), 2, BF16, 0.1)
+    _, mean, rstd = ref.layer_norm(s)
+    mean, rstd = mean.float().cuda(), rstd.float().cuda()
+    x = ops.checkpoint_activation(s.cuda()) if held else s.cuda()
+    check_backward(ops.layer_norm_backward(dy.cuda(), x, mean, rstd), dy, ref.held(s) if held else s, mean, rstd, None, None)
+
+
 def test_backward_against_differences(lib):
     """The gradients of the forward kernel itself, in fp32: its outputs are some 1e-7 of themselves off, so differences
     over steps of 2^-6 are about 2^6 * 48 * 4e-7 = 1.3e-3 off, and the terms of second order in the step 2^-12 * 10 = 2.5e-3."""

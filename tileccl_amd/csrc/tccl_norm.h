@@ -63,7 +63,7 @@ struct NormGradArgs {
   char* dx;
   float* partial;  // [slot][2][cols]; nullptr: the sums over the rows are made by workgroups of their own
   float *dgamma, *dbeta;  // of those workgroups
-  int column_wgs;         // how many there are, ahead of the others
+  int column_wgs, column_lanes;  // how many there are, ahead of the others; an eighth of their columns
   int64_t ld_grad, ld_x, ld_grad_summed, ld_dx;
   int64_t scale_pitch, value_pitch;
   int rows, cols, items;
@@ -148,6 +148,15 @@ struct Eight {
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = (2 * i < n ? h[2 * i] : 0u) | (2 * i + 1 < n ? h[2 * i + 1] << 16 : 0u);
   }
+  // From the eight values that end with the row's last to the n (under eight) that the columns from here on have, zeros behind them.
+  TCCL_D void settle(int n) {
+    const int before = n < 8 ? 8 - n : 0;
+    u32x4n v = w;
+    if (before & 4) v = (u32x4n){v[2], v[3], 0, 0};
+    if (before & 2) v = (u32x4n){v[1], v[2], v[3], 0};
+    if (before & 1) v = (u32x4n){v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+    w = v;
+  }
   TCCL_D void store_some(T* p, int n) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -204,6 +213,14 @@ struct Eight<float> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = i < n ? v[i] : 0.f;
   }
+  TCCL_D void settle(int n) {
+    const int before = n < 8 ? 8 - n : 0;
+#pragma unroll
+    for (int b = 4; b; b /= 2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = before & b ? (i + b < 8 ? v[i + b < 8 ? i + b : 0] : 0.f) : v[i];
+    }
+  }
   TCCL_D void store_some(float* p, int n) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -225,15 +242,31 @@ TCCL_D auto in_row(Byte* row, uint32_t off) {
 // What the matrices' rows are: of any length and alignment, whole 16-byte vectors on 16-byte boundaries, or those on lines.
 enum RowKind { kAnyRows = 0, kVectorRows = 1, kLineRows = 2 };
 
-// n: how many of the eight columns exist (8, or fewer at the end of a row; <= 0: none).
+// The ends of rows that are no whole vectors.  A thread whose columns are the last ones and fewer than eight loads the eight
+// that end with them, and moves them to their places once all its loads are on their way: `from` is where it loads, `tail`
+// whether its wavefront has such a thread.  (Loads of single values in a branch of their own are waited for row by row:
+// 16384 x 1003 backward 58.7 us, so 39.7.)  Rows of fewer than eight columns (narrow) are loaded value by value.
+template <int kRows>
+struct RowEnds {
+  bool narrow;
+  TCCL_D RowEnds(int cols) : narrow(kRows == kAnyRows && cols < 8) {}
+  template <typename T>
+  TCCL_D uint32_t from(int col, int n) const {
+    return (uint32_t)(kRows == kAnyRows && !narrow && n > 0 && n < 8 ? col - (8 - n) : col) * (uint32_t)sizeof(T);
+  }
+  TCCL_D bool tail(int n) const { return kRows == kAnyRows && !narrow && __ballot(n > 0 && n < 8) != 0; }
+};
+// n: how many of the eight columns exist (8, or fewer at the end of a row; <= 0: none).  Followed by settle(n) where there is a tail.
 template <int kRows, bool kOnce = true, typename T>
-TCCL_D void load_n(Eight<T>& e, const T* p, int n) {
-  if (n >= 8)
-    e.template load<kOnce && kRows == kLineRows && sizeof(T) == 2>(p);
-  else if (kRows == kAnyRows && n > 0)
-    e.load_some(p, n);
-  else
+TCCL_D void load_n(Eight<T>& e, const T* p, int n, const RowEnds<kRows>& ends) {
+  if (kRows == kAnyRows ? n > 0 : n >= 8) {
+    if (kRows == kAnyRows && ends.narrow)
+      e.load_some(p, n);
+    else
+      e.template load<kOnce && kRows == kLineRows && sizeof(T) == 2>(p);
+  } else {
     e.zero();
+  }
 }
 template <int kRows, typename T>
 TCCL_D void store_n(const Eight<T>& e, T* p, int n) {
@@ -246,18 +279,20 @@ TCCL_D void store_n(const Eight<T>& e, T* p, int n) {
 // gamma or beta of eight columns, in the activations' type or in fp32; `missing` where there is none.  They are read by
 // every workgroup: kept in the caches.
 template <typename T, int kRows>
-TCCL_D void load_affine(float (&v)[8], const void* p, int f32, int col, int n, float missing) {
+TCCL_D void load_affine(float (&v)[8], const void* p, int f32, int col, int n, float missing, const RowEnds<kRows>& ends) {
   if (!p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = missing;
   } else if (f32) {
     Eight<float> e;
-    load_n<kRows, false>(e, in_row<float>((const char*)p, 4u * (uint32_t)col), n);
+    load_n<kRows, false>(e, in_row<float>((const char*)p, ends.template from<float>(col, n)), n, ends);
+    if (ends.tail(n)) e.settle(n);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = e.v[i];
   } else {
     Eight<T> e;
-    load_n<kRows, false>(e, in_row<T>((const char*)p, (uint32_t)sizeof(T) * (uint32_t)col), n);
+    load_n<kRows, false>(e, in_row<T>((const char*)p, ends.template from<T>(col, n)), n, ends);
+    if (ends.tail(n)) e.settle(n);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const f32x2n q = e.pair(i);
@@ -402,13 +437,17 @@ __global__ __launch_bounds__(1024, 4) void layer_norm_kernel(NormArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), waves = (int)(blockDim.x >> 6);
   const int group = __builtin_amdgcn_readfirstlane((int)threadIdx.y), groups = (int)blockDim.y;
   const int first_part = group * waves;
+  const RowEnds<kRows> ends(a.cols);
   int col[NV], left[NV], wave_n = 0;
-  uint32_t off[NV];
+  uint32_t off[NV], from[NV];
+  bool tail = false;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     col[j] = (int)(j * blockDim.x + threadIdx.x) * 8;
     off[j] = (uint32_t)col[j] * (uint32_t)sizeof(T);
     left[j] = a.cols - col[j];
+    from[j] = ends.template from<T>(col[j], left[j]);
+    tail |= ends.tail(left[j]);
     const int n = a.cols - (j * waves + wave) * 512;
     wave_n += n < 0 ? 0 : n > 512 ? 512 : n;
   }
@@ -424,8 +463,8 @@ __global__ __launch_bounds__(1024, 4) void layer_norm_kernel(NormArgs a) {
   constexpr bool kKeep = NV == 1;  // gamma and beta stay in registers
   float gamma[kKeep ? NV : 1][8], beta[kKeep ? NV : 1][8];
   if (kKeep) {
-    load_affine<T, kRows>(gamma[0], a.weight, a.affine_f32, col[0], left[0], 1.f);
-    load_affine<T, kRows>(beta[0], a.bias, a.affine_f32, col[0], left[0], 0.f);
+    load_affine<T, kRows>(gamma[0], a.weight, a.affine_f32, col[0], left[0], 1.f, ends);
+    load_affine<T, kRows>(beta[0], a.bias, a.affine_f32, col[0], left[0], 0.f, ends);
   }
   int turn = 0;
   for (int base = (int)blockIdx.x * groups; base < a.items; base += (int)gridDim.x * groups, turn ^= 1) {
@@ -436,7 +475,7 @@ __global__ __launch_bounds__(1024, 4) void layer_norm_kernel(NormArgs a) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         if (row0 + r < a.rows && left[j] > 0)
-          load_n<kRows>(s[r][j], in_row<T>(a.x + (int64_t)(row0 + r) * a.ld_x, off[j]), left[j]);
+          load_n<kRows>(s[r][j], in_row<T>(a.x + (int64_t)(row0 + r) * a.ld_x, from[j]), left[j], ends);
         else
           s[r][j].zero();
       }
@@ -447,10 +486,16 @@ __global__ __launch_bounds__(1024, 4) void layer_norm_kernel(NormArgs a) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           if (row0 + r < a.rows && left[j] > 0)
-            load_n<kRows>(t[r][j], in_row<T>(a.residual + (int64_t)(row0 + r) * a.ld_residual, off[j]), left[j]);
+            load_n<kRows>(t[r][j], in_row<T>(a.residual + (int64_t)(row0 + r) * a.ld_residual, from[j]), left[j], ends);
           else
             t[r][j].zero();
         }
+      if (tail) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int j = 0; j < NV; ++j) s[r][j].settle(left[j]), t[r][j].settle(left[j]);
+      }
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -462,6 +507,12 @@ __global__ __launch_bounds__(1024, 4) void layer_norm_kernel(NormArgs a) {
           }
           if (row0 + r < a.rows && left[j] > 0) store_n<kRows>(s[r][j], in_row<T>(a.summed + (int64_t)(row0 + r) * a.ld_summed, off[j]), left[j]);
         }
+    }
+    if (tail && !a.residual) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < NV; ++j) s[r][j].settle(left[j]);
     }
     float sum[R], m2[R];
 #pragma unroll
@@ -534,8 +585,8 @@ __global__ __launch_bounds__(1024, 4) void layer_norm_kernel(NormArgs a) {
     for (int j = 0; j < NV; ++j) {
       const int m = kKeep ? j : 0;
       if (!kKeep) {
-        load_affine<T, kRows>(gamma[m], a.weight, a.affine_f32, col[j], left[j], 1.f);
-        load_affine<T, kRows>(beta[m], a.bias, a.affine_f32, col[j], left[j], 0.f);
+        load_affine<T, kRows>(gamma[m], a.weight, a.affine_f32, col[j], left[j], 1.f, ends);
+        load_affine<T, kRows>(beta[m], a.bias, a.affine_f32, col[j], left[j], 0.f, ends);
       }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -569,19 +620,24 @@ __global__ __launch_bounds__(1024, 4) void layer_norm_kernel(NormArgs a) {
 }
 
 // ---- backward --------------------------------------------------------------------------------------
-// Few rows: workgroup `wg` sums 32 columns over all rows, reading grad and s a second time (from the caches) instead of
-// waiting for the other workgroups' partial sums in a second launch.  4 lanes side by side, the others below each other.
+// Few rows: workgroup `wg` sums 8 a.column_lanes columns over all rows, reading grad and s a second time (from the caches) instead
+// of waiting for the other workgroups' partial sums in a second launch.  column_lanes (4 or 16) lanes side by side, the others
+// below each other.  (Eight rows' loads of s in full at a time instead of four: 1000 x 2048 12.4 -> 14.7 us, fewer wavefronts fit.)
+constexpr int kMostColumnLanes = 16;
 template <typename T, bool kHeld, int kRows>
 TCCL_D void sum_columns(const NormGradArgs& a, int wg, float* joined) {
   constexpr int kStep = kHeld ? kHoldRows : 4, Q = 4;
+  const int lanes = a.column_lanes, shift = lanes == 4 ? 2 : 4, width = 8 * lanes;
   const int thread = (int)(threadIdx.y * blockDim.x + threadIdx.x), threads = (int)(blockDim.x * blockDim.y);
   const int lane = thread & 63, wave = thread >> 6, waves = threads >> 6;
-  const int col = wg * 32 + (thread & 3) * 8, left = a.cols - col;
-  const uint32_t off = (uint32_t)col * (uint32_t)sizeof(T);
+  const int col = wg * width + (thread & (lanes - 1)) * 8, left = a.cols - col;
+  const RowEnds<kRows> ends(8);  // (the rows have that many)
+  const uint32_t off = ends.template from<T>(col, left);
+  const bool tail = ends.tail(left);
   float dgamma[8], dbeta[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) dgamma[i] = dbeta[i] = 0.f;
-  for (int row0 = (thread >> 2) * kStep; row0 < a.rows; row0 += (threads >> 2) * kStep) {
+  for (int row0 = (thread >> shift) * kStep; row0 < a.rows; row0 += (threads >> shift) * kStep) {
     u32x4n q[4];
     float scale = 0.f;
     if (kHeld) {
@@ -599,12 +655,19 @@ TCCL_D void sum_columns(const NormGradArgs& a, int wg, float* joined) {
       for (int e = 0; e < Q; ++e) {
         const int row = row0 + 4 * h + e;
         if (row < a.rows) {
-          load_n<kRows, false>(g[e], (const T*)(a.grad + (int64_t)row * a.ld_grad + off), left);
-          if (!kHeld) load_n<kRows, false>(s[kHeld ? 0 : e], (const T*)(a.x + (int64_t)row * a.ld_x + off), left);
+          load_n<kRows, false>(g[e], (const T*)(a.grad + (int64_t)row * a.ld_grad + off), left, ends);
+          if (!kHeld) load_n<kRows, false>(s[kHeld ? 0 : e], (const T*)(a.x + (int64_t)row * a.ld_x + off), left, ends);
           mean[e] = a.mean[row], rstd[e] = a.rstd[row];
         } else {
           g[e].zero(), mean[e] = rstd[e] = 0.f;
           if (!kHeld) s[kHeld ? 0 : e].zero();
+        }
+      }
+      if (tail) {
+#pragma unroll
+        for (int e = 0; e < Q; ++e) {
+          g[e].settle(left);
+          if (!kHeld) s[kHeld ? 0 : e].settle(left);
         }
       }
 #pragma unroll
@@ -625,106 +688,142 @@ TCCL_D void sum_columns(const NormGradArgs& a, int wg, float* joined) {
     }
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int m = 4; m < 64; m *= 2)
+    if (m >= lanes) {
 #pragma unroll
-    for (int m = 4; m < 64; m *= 2) dgamma[i] += __shfl_xor(dgamma[i], m), dbeta[i] += __shfl_xor(dbeta[i], m);
-  if (lane < 4) {
+      for (int i = 0; i < 8; ++i) dgamma[i] += __shfl_xor(dgamma[i], m), dbeta[i] += __shfl_xor(dbeta[i], m);
+    }
+  if (lane < lanes) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) joined[wave * 64 + lane * 8 + i] = dgamma[i], joined[wave * 64 + 32 + lane * 8 + i] = dbeta[i];
+    for (int i = 0; i < 8; ++i) joined[wave * 2 * width + lane * 8 + i] = dgamma[i], joined[(wave * 2 + 1) * width + lane * 8 + i] = dbeta[i];
   }
   __syncthreads();
-  if (thread < 64) {
+  for (int u = thread; u < 2 * width; u += threads) {
     float t = 0.f;
-    for (int w = 0; w < waves; ++w) t += joined[w * 64 + thread];
-    const int c = wg * 32 + (thread & 31);
-    float* to = thread < 32 ? a.dgamma : a.dbeta;
+    for (int w = 0; w < waves; ++w) t += joined[w * 2 * width + u];
+    const int c = wg * width + (u & (width - 1));
+    float* to = u < width ? a.dgamma : a.dbeta;
     if (c < a.cols && to) to[c] = t;
   }
 }
 
 // kHeld: s comes from its 8-bit values, R is a row block or half of one.
-template <typename T, int R, int NV, bool kHeld, int kRows>
-__global__ __launch_bounds__(1024, 4) void layer_norm_grad_kernel(NormGradArgs a) {
+// kAhead: workgroups of up to 512 threads, one on a CU, whose 256 registers hold two turns: a turn's operands are on their way while the
+// turn before is computed.  Many rows, from 16-bit s: 2048 x 4096 24.4 -> 20.4 us, 4096 x 4096 37.3 -> 32.4, 16384 x 4096 102.6 -> 97.9,
+// 8192 x 8192 106 -> 101.5.  Two turns of 8-bit s, of more than 8192 columns or of fp32 are more than the registers and lose (16384 x
+// 4096 from 8 bits 89 -> 128, 4096 x 16384 119 -> 170, 4096 x 4096 fp32 53 -> 71).
+template <typename T, int R, int NV, bool kHeld, int kRows, bool kAhead>
+__global__ __launch_bounds__(kAhead ? 512 : 1024, kAhead ? 2 : 4) void layer_norm_grad_kernel(NormGradArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int Q = R < 4 ? R : 4;          // rows taken together
-  constexpr bool kTwice = kHeld && NV > 2;  // four rows of more than 16384 columns are more than the registers: read again
+  constexpr bool kTwice = kHeld && NV > 1;  // four rows are more than 128 registers: read again
   constexpr int kQuads = kHeld ? R / 4 : 1;  // rows of codes, four in a word
-  constexpr bool kKeep = NV == 1;           // gamma stays in registers
+  constexpr bool kKeep = NV == 1 || kAhead;  // gamma stays in registers (a load of it would be waited for with those of the next turn)
   constexpr int KJ = kTwice ? 1 : NV;
   __shared__ f32x2n part[2][16][R];         // (sum g, sum g xh) of wavefront w, by turns
-  __shared__ float merged[NV == 1 ? 7 * 1024 : 16 * 64];  // of the groups of a workgroup, or of sum_columns()
-  if constexpr (kRows != kAnyRows)
-    if ((int)blockIdx.x < a.column_wgs) return sum_columns<T, kHeld, kRows>(a, (int)blockIdx.x, merged);
+  __shared__ float merged[NV == 1 ? 7 * 1024 : 16 * 16 * kMostColumnLanes];  // of the groups of a workgroup, or of sum_columns()
+  if (!kAhead && (int)blockIdx.x < a.column_wgs) return sum_columns<T, kHeld, kRows>(a, (int)blockIdx.x, merged);
   const int block = (int)blockIdx.x - a.column_wgs, blocks = (int)gridDim.x - a.column_wgs;
   const int lane = (int)(threadIdx.x & 63);
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), waves = (int)(blockDim.x >> 6);
   const int group = __builtin_amdgcn_readfirstlane((int)threadIdx.y), groups = (int)blockDim.y;
   const int first_part = group * waves;
+  const RowEnds<kRows> ends(a.cols);
   int col[NV], left[NV];
-  uint32_t off[NV];
+  uint32_t off[NV], from[NV];
+  bool tail = false;
   float gamma[kKeep ? NV : 1][8], dgamma[NV][8], dbeta[NV][8];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     col[j] = (int)(j * blockDim.x + threadIdx.x) * 8;
     off[j] = (uint32_t)col[j] * (uint32_t)sizeof(T);
     left[j] = a.cols - col[j];
-    if (kKeep) load_affine<T, kRows>(gamma[j], a.weight, a.affine_f32, col[j], left[j], 1.f);
+    from[j] = ends.template from<T>(col[j], left[j]);
+    tail |= ends.tail(left[j]);
+    if (kKeep) load_affine<T, kRows>(gamma[j], a.weight, a.affine_f32, col[j], left[j], 1.f, ends);
 #pragma unroll
     for (int i = 0; i < 8; ++i) dgamma[j][i] = dbeta[j][i] = 0.f;
   }
-  int turn = 0;
-  for (int base = block * groups; base < a.items; base += blocks * groups, turn ^= 1) {
-    const int row0 = (base + group) * R;
-    Eight<T> g[R][KJ], s[kHeld ? 1 : R][KJ];
+  struct Turn {
+    int row0;
+    Eight<T> g[R][KJ], s[kHeld ? 1 : R][KJ], o[kAhead ? R : 1][kAhead ? NV : 1];
     uint32_t q[kHeld ? KJ : 1][4][kQuads][2];  // column pair, rows, column
-    float scale[KJ], mean[R], rstd[R];
-    auto fetch = [&](int j, int k) {  // vectors j into place k
+    float scale[KJ], mean, rstd;               // the statistics of row `lane`
+  };
+  auto fetch = [&](Turn& t, int j, int k) __attribute__((always_inline)) {  // vectors j into place k
+    const int row0 = t.row0;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        if (row0 + r < a.rows) {
-          load_n<kRows>(g[r][k], in_row<T>(a.grad + (int64_t)(row0 + r) * a.ld_grad, off[j]), left[j]);
-          if (!kHeld) load_n<kRows>(s[kHeld ? 0 : r][k], in_row<T>(a.x + (int64_t)(row0 + r) * a.ld_x, off[j]), left[j]);
-        } else {
-          g[r][k].zero();
-          if (!kHeld) s[kHeld ? 0 : r][k].zero();
-        }
+    for (int r = 0; r < R; ++r) {
+      if (row0 + r < a.rows) {
+        load_n<kRows>(t.g[r][k], in_row<T>(a.grad + (int64_t)(row0 + r) * a.ld_grad, from[j]), left[j], ends);
+        if (!kHeld) load_n<kRows>(t.s[kHeld ? 0 : r][k], in_row<T>(a.x + (int64_t)(row0 + r) * a.ld_x, from[j]), left[j], ends);
+      } else {
+        t.g[r][k].zero();
+        if (!kHeld) t.s[kHeld ? 0 : r][k].zero();
       }
-      if (kHeld) {
-        const int rb = row0 / kHoldRows, half = R == 4 ? row0 / 4 % 2 : 0;
-        const bool live = row0 < a.rows && left[j] > 0;
-        const uint8_t* v = in_row<const uint8_t>(a.values + rb * a.value_pitch, (uint32_t)col[j] * kHoldRows);
+    }
+    if (kHeld) {
+      const int rb = row0 / kHoldRows, half = R == 4 ? row0 / 4 % 2 : 0;
+      const bool live = row0 < a.rows && left[j] > 0;
+      const uint8_t* v = in_row<const uint8_t>(a.values + rb * a.value_pitch, (uint32_t)col[j] * kHoldRows);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const u32x4n codes = live ? got<u32x4n>((const u32x4n*)v + c) : (u32x4n){0, 0, 0, 0};
+      for (int c = 0; c < 4; ++c) {
+        const u32x4n codes = live ? got<u32x4n>((const u32x4n*)v + c) : (u32x4n){0, 0, 0, 0};
 #pragma unroll
-          for (int o = 0; o < 2; ++o) {
-            if (R == 4) {
-              q[kHeld ? k : 0][c][0][o] = half ? codes[2 * o + 1] : codes[2 * o];
-            } else {
+        for (int o = 0; o < 2; ++o) {
+          if (R == 4) {
+            t.q[kHeld ? k : 0][c][0][o] = half ? codes[2 * o + 1] : codes[2 * o];
+          } else {
 #pragma unroll
-              for (int h = 0; h < kQuads; ++h) q[kHeld ? k : 0][c][h][o] = codes[2 * o + h];
-            }
+            for (int h = 0; h < kQuads; ++h) t.q[kHeld ? k : 0][c][h][o] = codes[2 * o + h];
           }
         }
-        scale[k] = live ? __uint_as_float((uint32_t)a.scales[(col[j] / kHoldCols) * a.scale_pitch + rb] << 23) : 0.f;
       }
-    };
-    auto values = [&](int k, int i, int h, f32x2n(&v)[4]) {  // s of columns 2i, 2i + 1, rows h Q ..
-      if (kHeld)
-        held_quad(q[kHeld ? k : 0][i][kHeld ? h : 0][0], q[kHeld ? k : 0][i][kHeld ? h : 0][1], scale[k], v);
-      else
-#pragma unroll
-        for (int e = 0; e < Q; ++e) v[e] = s[kHeld ? 0 : h * Q + e][k].pair(i);
-    };
+      t.scale[k] = live ? __uint_as_float((uint32_t)a.scales[(col[j] / kHoldCols) * a.scale_pitch + rb] << 23) : 0.f;
+    }
+  };
+  auto begin = [&](Turn& t, int base) __attribute__((always_inline)) {
+    t.row0 = (base + group) * R;
     if (!kTwice) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) fetch(j, j);
+      for (int j = 0; j < NV; ++j) fetch(t, j, j);
     }
-    {  // a row's statistics per lane, then uniform
-      const bool live = lane < R && row0 + lane < a.rows;
-      const float m = live ? a.mean[row0 + lane] : 0.f, v = live ? a.rstd[row0 + lane] : 0.f;
+    if (kAhead && a.grad_summed) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) mean[r] = lane_value(m, r), rstd[r] = lane_value(v, r);
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (t.row0 + r < a.rows)
+            load_n<kRows>(t.o[kAhead ? r : 0][kAhead ? j : 0], in_row<T>(a.grad_summed + (int64_t)(t.row0 + r) * a.ld_grad_summed, from[j]), left[j], ends);
+    }
+    const bool live = lane < R && t.row0 + lane < a.rows;
+    t.mean = live ? a.mean[t.row0 + lane] : 0.f, t.rstd = live ? a.rstd[t.row0 + lane] : 0.f;
+  };
+  int turn = 0;
+  auto finish = [&](Turn& t) __attribute__((always_inline)) {
+    const int row0 = t.row0;
+    auto settle = [&](int j, int k) __attribute__((always_inline)) {
+      if (tail) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          t.g[r][k].settle(left[j]);
+          if (!kHeld) t.s[kHeld ? 0 : r][k].settle(left[j]);
+        }
+      }
+    };
+    auto values = [&](int k, int i, int h, f32x2n(&v)[4]) __attribute__((always_inline)) {  // s of columns 2i, 2i + 1, rows h Q ..
+      if (kHeld)
+        held_quad(t.q[kHeld ? k : 0][i][kHeld ? h : 0][0], t.q[kHeld ? k : 0][i][kHeld ? h : 0][1], t.scale[k], v);
+      else
+#pragma unroll
+        for (int e = 0; e < Q; ++e) v[e] = t.s[kHeld ? 0 : h * Q + e][k].pair(i);
+    };
+    float mean[R], rstd[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) mean[r] = lane_value(t.mean, r), rstd[r] = lane_value(t.rstd, r);
+    if (!kTwice) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) settle(j, j);
     }
     float c1[R], c2[R];
 #pragma unroll
@@ -732,8 +831,8 @@ __global__ __launch_bounds__(1024, 4) void layer_norm_grad_kernel(NormGradArgs a
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int k = kTwice ? 0 : j, m = kKeep ? j : 0;
-      if (kTwice) fetch(j, 0);
-      if (!kKeep) load_affine<T, kRows>(gamma[m], a.weight, a.affine_f32, col[j], left[j], 1.f);
+      if (kTwice) fetch(t, j, 0), settle(j, 0);
+      if (!kKeep) load_affine<T, kRows>(gamma[m], a.weight, a.affine_f32, col[j], left[j], 1.f, ends);
 #pragma unroll
       for (int h = 0; h < R / Q; ++h)
 #pragma unroll
@@ -743,7 +842,7 @@ __global__ __launch_bounds__(1024, 4) void layer_norm_grad_kernel(NormGradArgs a
 #pragma unroll
           for (int e = 0; e < Q; ++e) {
             const int r = h * Q + e;
-            const f32x2n d = g[r][k].pair(i);
+            const f32x2n d = t.g[r][k].pair(i);
 #pragma unroll
             for (int o = 0; o < 2; ++o) {
               const float xh = (v[e][o] - mean[r]) * rstd[r];
@@ -788,31 +887,37 @@ __global__ __launch_bounds__(1024, 4) void layer_norm_grad_kernel(NormGradArgs a
       for (int j = 0; j < KJ; ++j) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          g[r][j].renew();
-          if (!kHeld) s[kHeld ? 0 : r][j].renew();
+          t.g[r][j].renew();
+          if (!kHeld) t.s[kHeld ? 0 : r][j].renew();
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int h = 0; h < kQuads; ++h)
-            if (kHeld) renew_word(q[kHeld ? j : 0][c][h][0]), renew_word(q[kHeld ? j : 0][c][h][1]);
+            if (kHeld) renew_word(t.q[kHeld ? j : 0][c][h][0]), renew_word(t.q[kHeld ? j : 0][c][h][1]);
       }
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int k = kTwice ? 0 : j, m = kKeep ? j : 0;
-      if (kTwice) fetch(j, 0);
-      if (!kKeep) load_affine<T, kRows>(gamma[m], a.weight, a.affine_f32, col[j], left[j], 1.f);
+      if (kTwice) fetch(t, j, 0), settle(j, 0);
+      if (!kKeep) load_affine<T, kRows>(gamma[m], a.weight, a.affine_f32, col[j], left[j], 1.f, ends);
 #pragma unroll
       for (int h = 0; h < R / Q; ++h) {
         Eight<T> o[Q];
 #pragma unroll
         for (int e = 0; e < Q; ++e) {
           const int r = h * Q + e;
-          if (a.grad_summed && row0 + r < a.rows)
-            load_n<kRows>(o[e], in_row<T>(a.grad_summed + (int64_t)(row0 + r) * a.ld_grad_summed, off[j]), left[j]);
-          else
+          if (!a.grad_summed || row0 + r >= a.rows)
             o[e].zero();
+          else if (kAhead)
+            o[e] = t.o[kAhead ? r : 0][kAhead ? j : 0];
+          else
+            load_n<kRows>(o[e], in_row<T>(a.grad_summed + (int64_t)(row0 + r) * a.ld_grad_summed, from[j]), left[j], ends);
+        }
+        if (tail && a.grad_summed) {
+#pragma unroll
+          for (int e = 0; e < Q; ++e) o[e].settle(left[j]);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -821,7 +926,7 @@ __global__ __launch_bounds__(1024, 4) void layer_norm_grad_kernel(NormGradArgs a
 #pragma unroll
           for (int e = 0; e < Q; ++e) {
             const int r = h * Q + e;
-            const f32x2n d = g[r][k].pair(i), more = o[e].pair(i);
+            const f32x2n d = t.g[r][k].pair(i), more = o[e].pair(i);
             float dx[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -838,6 +943,39 @@ __global__ __launch_bounds__(1024, 4) void layer_norm_grad_kernel(NormGradArgs a
           if (row0 + r < a.rows && left[j] > 0) store_n<kRows>(o[e], in_row<T>(a.dx + (int64_t)(row0 + r) * a.ld_dx, off[j]), left[j]);
         }
       }
+    }
+    turn ^= 1;
+  };
+  const int step = blocks * groups;
+  if constexpr (kAhead) {
+    Turn even, odd;
+    int base = block * groups;
+    if (base < a.items) {
+      begin(even, base);
+      for (;;) {
+        base += step;
+        if (base >= a.items) {
+          finish(even);
+          break;
+        }
+        begin(odd, base);
+        step_by_step();
+        finish(even);
+        base += step;
+        if (base >= a.items) {
+          finish(odd);
+          break;
+        }
+        begin(even, base);
+        step_by_step();
+        finish(odd);
+      }
+    }
+  } else {
+    for (int base = block * groups; base < a.items; base += step) {
+      Turn t;
+      begin(t, base);
+      finish(t);
     }
   }
   if (!a.partial) return;
@@ -910,7 +1048,9 @@ template <typename T, int kRows>
 __global__ __launch_bounds__(256) void hold_kernel(HoldArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   const int col = (int)(blockIdx.x * 256 + threadIdx.x) * 8, left = a.cols - col;
-  const uint32_t off = (uint32_t)col * (uint32_t)sizeof(T);
+  const RowEnds<kRows> ends(a.cols);
+  const uint32_t off = ends.template from<T>(col, left);
+  const bool tail = ends.tail(left);
   const int row_blocks = (a.rows + kHoldRows - 1) / kHoldRows;
   for (int rb = (int)blockIdx.y; rb < row_blocks; rb += (int)gridDim.y) {
     Eight<T> p[8];
@@ -918,9 +1058,13 @@ __global__ __launch_bounds__(256) void hold_kernel(HoldArgs a) {
     for (int r = 0; r < 8; ++r) {
       const int row = rb * kHoldRows + r;
       if (row < a.rows && left > 0)
-        load_n<kRows>(p[r], in_row<T>(a.x + (int64_t)row * a.ld, off), left);
+        load_n<kRows>(p[r], in_row<T>(a.x + (int64_t)row * a.ld, off), left, ends);
       else
         p[r].zero();
+    }
+    if (tail) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) p[r].settle(left);
     }
     const bool live = (int64_t)col * kHoldRows < a.value_pitch;
     hold_patch<T>(p, a.values + rb * a.value_pitch + (int64_t)col * kHoldRows, a.scales + (col / kHoldCols) * a.scale_pitch + rb, live,
