@@ -17,6 +17,10 @@
 // pass in registers; the column sums of all groups are added by a second launch in a fixed order, so that results
 // do not depend on which workgroup comes first.
 //
+// What bounds them: memory where there are many rows (bf16: 8192 x 4096 forward 24.6 us, 5.4 TB/s with the launch, where a copy reaches 6.45
+// without; 16384 x 4096 backward with a residual's gradient 98 us, 5.5; 16384 x 4096 to 8 bits 39 us, back 29), a launch and one or two trips to
+// memory where there are few (16 x 4096 6.2 us, of which an empty launch is 3.5).
+//
 // 8 rows x 8 columns of a thread are also the unit of the 8-bit layout: values lie as [row block][column][row in block], so a
 // thread's patch is 64 contiguous bytes, two neighbouring rows of a column go into one conversion, and the weight gradient
 // finds the 8 consecutive rows that a lane of a matrix instruction takes as 8 contiguous bytes, with no transposition.

@@ -99,6 +99,11 @@ TCCL_D void put4(const f32x4& s, char* to, int64_t at, int left, bool wide) {
 // 128 x 128, four wavefronts, two workgroups per CU: one barrier per step; each workgroup's waits are covered by the other.
 // kGroups = 2: 128 x 128 with eight wavefronts, of which either half takes half of the tokens with stages of its own; the
 // halves' sums meet in LDS.  For few tiles: the work of two workgroups on one tile, without partial sums in memory.
+//
+// What bounds them.  256 x 256: power (8192 x 4096 x 4096 bf16 207 us, 220 with `add`; 1.41 PFLOP/s in the K loop); what is added and stored
+// takes 25 us that one tile per CU cannot hide.  128 x 128, two groups (8192 x 2048 x 2048 69 us): multiplication and operands that
+// do not hide each other wholly: 64 us with operands that stay in the L2, 55 with no loads at all, 46 with no multiplication.  Conversions later in
+// a half, when their codes are there for certain, change nothing (16384 x 1024 x 512 30.6 -> 31.0).
 template <typename T, typename OutT, int kTileH, int kTileN, bool kTransposed, int kGroups>
 struct WeightGemm {
   typedef typename Mfma<T>::Vec Vec;
