@@ -152,7 +152,7 @@ def test_backward(lib, rows, cols, dtype, affine, more, held):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
-@pytest.mark.parametrize("rows, cols", [(1025, 5), (1030, 100), (9000, 1003), (5001, 2052), (3000, 4096), (1100, 4100), (2500, 6001), (1027, 8190), (1026, 8200)])
+@pytest.mark.parametrize("rows, cols", [(1025, 5), (1030, 100), (9000, 1003), (5001, 2052), (3000, 4096), (1100, 4100), (2500, 6001), (1027, 8190), (1026, 8200), (1100, 16383), (1030, 16400)])
 def test_backward_of_many_rows(lib, rows, cols, dtype):
     """Workgroups that take several groups of rows, with rows that end inside a vector; dx in the place of either gradient."""
     s, dy, more = rand((rows, cols), 1, dtype, 2.0, 0.5), rand((rows, cols), 2, dtype, 0.1), rand((rows, cols), 3, dtype, 0.1)
@@ -165,6 +165,22 @@ def test_backward_of_many_rows(lib, rows, cols, dtype):
         g, m = dy.cuda(), more.cuda()
         there = ops.layer_norm_backward(g, s.cuda(), mean, rstd, weight.cuda(), grad_summed=m, out=(g, m)[place])
         assert torch.equal(there.x, d.x) and torch.equal(there.weight, d.weight) and torch.equal(there.bias, d.bias)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows, cols", [(1025, 5), (1027, 100), (1030, 4096), (9001, 1003), (5006, 2052), (2500, 4100)])
+def test_backward_of_many_rows_from_8_bits(lib, rows, cols, dtype):
+    """Blocks with scales of their own, the last of them cut in its first or second half."""
+    s, dy, more = rand((rows, cols), 1, dtype, 0.1, 0.1), rand((rows, cols), 2, dtype, 0.1), rand((rows, cols), 3, dtype, 0.1)
+    s *= torch.exp2(((torch.arange(rows) // 8)[:, None] * 7 + (torch.arange(cols) // 128)[None] * 3) % 5).to(dtype)
+    _, mean, rstd = ref.layer_norm(s)
+    mean, rstd = mean.float().cuda(), rstd.float().cuda()
+    held = ops.checkpoint_activation(s.cuda())
+    d = ops.layer_norm_backward(dy.cuda(), held, mean, rstd, grad_summed=more.cuda())
+    check_backward(d, dy, ref.held(s), mean, rstd, None, more)
+    m = more.cuda()
+    there = ops.layer_norm_backward(dy.cuda(), held, mean, rstd, grad_summed=m, out=m)
+    assert torch.equal(there.x, d.x) and torch.equal(there.weight, d.weight) and torch.equal(there.bias, d.bias)
 
 
 @pytest.mark.parametrize("held", [False, True])

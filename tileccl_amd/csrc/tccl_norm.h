@@ -18,7 +18,7 @@
 // do not depend on which workgroup comes first.
 //
 // What bounds them: memory where there are many rows (bf16: 8192 x 4096 forward 24.6 us, 5.4 TB/s with the launch, where a copy reaches 6.45
-// without; 16384 x 4096 backward with a residual's gradient 98 us, 5.5; 16384 x 4096 to 8 bits 39 us, back 29), a launch and one or two trips to
+// without; 16384 x 4096 backward with a residual's gradient 99 us, 5.4; 16384 x 4096 to 8 bits 39 us, back 29), a launch and one or two trips to
 // memory where there are few (16 x 4096 6.2 us, of which an empty launch is 3.5).
 //
 // 8 rows x 8 columns of a thread are also the unit of the 8-bit layout: values lie as [row block][column][row in block], so a
@@ -712,20 +712,23 @@ TCCL_D void sum_columns(const NormGradArgs& a, int wg, float* joined) {
 }
 
 // kHeld: s comes from its 8-bit values, R is a row block or half of one.
-// kAhead: workgroups of up to 512 threads, one on a CU, whose 256 registers hold two turns: a turn's operands are on their way while the
-// turn before is computed.  Many rows, from 16-bit s: 2048 x 4096 24.4 -> 20.4 us, 4096 x 4096 37.3 -> 32.4, 16384 x 4096 102.6 -> 97.9,
-// 8192 x 8192 106 -> 101.5.  Two turns of 8-bit s, of more than 8192 columns or of fp32 are more than the registers and lose (16384 x
-// 4096 from 8 bits 89 -> 128, 4096 x 16384 119 -> 170, 4096 x 4096 fp32 53 -> 71).
+// kAhead: workgroups of up to 512 threads, 512 threads of a CU, whose 256 registers hold two turns: a turn's operands are on their way
+// while the turn before is computed (from 8 bits the turns are the halves of a row block, whose codes come with the first).  bf16
+// 4096 x 4096 37.3 -> 33.0 us, 4096 x 16384 119 -> 105, from 8 bits 34.6 -> 29.1 and 1030 x 4096 21.1 -> 14.9; fp32 4096 x 4096
+// 63 -> 52.  Whole row blocks a turn ahead are more than the registers (16384 x 4096 from 8 bits 89 -> 128 us, so 87), and so are two rows of
+// one fp32 vector instead of a row of two (8192 x 4096 119 -> 128 us, so 104).
 template <typename T, int R, int NV, bool kHeld, int kRows, bool kAhead>
 __global__ __launch_bounds__(kAhead ? 512 : 1024, kAhead ? 2 : 4) void layer_norm_grad_kernel(NormGradArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int Q = R < 4 ? R : 4;          // rows taken together
+  constexpr bool kHalves = kHeld && kAhead;  // turns are the halves of a row block, whose codes are loaded with the first
   constexpr bool kTwice = kHeld && NV > 1;  // four rows are more than 128 registers: read again
   constexpr int kQuads = kHeld ? R / 4 : 1;  // rows of codes, four in a word
   constexpr bool kKeep = NV == 1 || kAhead;  // gamma stays in registers (a load of it would be waited for with those of the next turn)
   constexpr int KJ = kTwice ? 1 : NV;
   __shared__ f32x2n part[2][16][R];         // (sum g, sum g xh) of wavefront w, by turns
-  __shared__ float merged[NV == 1 ? 7 * 1024 : 16 * 16 * kMostColumnLanes];  // of the groups of a workgroup, or of sum_columns()
+  constexpr bool kGroups = NV == 1 || (kAhead && sizeof(T) == 4);  // whether there may be several groups: of up to eight wavefronts in all
+  __shared__ float merged[kGroups ? NV * 7 * 1024 : 16 * 16 * kMostColumnLanes];  // of the groups of a workgroup, or of sum_columns()
   if (!kAhead && (int)blockIdx.x < a.column_wgs) return sum_columns<T, kHeld, kRows>(a, (int)blockIdx.x, merged);
   const int block = (int)blockIdx.x - a.column_wgs, blocks = (int)gridDim.x - a.column_wgs;
   const int lane = (int)(threadIdx.x & 63);
@@ -754,6 +757,8 @@ __global__ __launch_bounds__(kAhead ? 512 : 1024, kAhead ? 2 : 4) void layer_nor
     uint32_t q[kHeld ? KJ : 1][4][kQuads][2];  // column pair, rows, column
     float scale[KJ], mean, rstd;               // the statistics of row `lane`
   };
+  uint32_t codes[4][2][2], next_codes[4][2][2];  // kHalves: of this row block and the next; column pair, half, column
+  float codes_scale = 0.f, next_scale = 0.f;
   auto fetch = [&](Turn& t, int j, int k) __attribute__((always_inline)) {  // vectors j into place k
     const int row0 = t.row0;
 #pragma unroll
@@ -766,28 +771,40 @@ __global__ __launch_bounds__(kAhead ? 512 : 1024, kAhead ? 2 : 4) void layer_nor
         if (!kHeld) t.s[kHeld ? 0 : r][k].zero();
       }
     }
-    if (kHeld) {
+    if (kHeld && !kHalves) {
       const int rb = row0 / kHoldRows, half = R == 4 ? row0 / 4 % 2 : 0;
       const bool live = row0 < a.rows && left[j] > 0;
       const uint8_t* v = in_row<const uint8_t>(a.values + rb * a.value_pitch, (uint32_t)col[j] * kHoldRows);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const u32x4n codes = live ? got<u32x4n>((const u32x4n*)v + c) : (u32x4n){0, 0, 0, 0};
+        const u32x4n four = live ? got<u32x4n>((const u32x4n*)v + c) : (u32x4n){0, 0, 0, 0};
 #pragma unroll
         for (int o = 0; o < 2; ++o) {
           if (R == 4) {
-            t.q[kHeld ? k : 0][c][0][o] = half ? codes[2 * o + 1] : codes[2 * o];
+            t.q[kHeld ? k : 0][c][0][o] = half ? four[2 * o + 1] : four[2 * o];
           } else {
 #pragma unroll
-            for (int h = 0; h < kQuads; ++h) t.q[kHeld ? k : 0][c][h][o] = codes[2 * o + h];
+            for (int h = 0; h < kQuads; ++h) t.q[kHeld ? k : 0][c][h][o] = four[2 * o + h];
           }
         }
       }
       t.scale[k] = live ? __uint_as_float((uint32_t)a.scales[(col[j] / kHoldCols) * a.scale_pitch + rb] << 23) : 0.f;
     }
   };
-  auto begin = [&](Turn& t, int base) __attribute__((always_inline)) {
-    t.row0 = (base + group) * R;
+  auto begin = [&](Turn& t, int base, int half) __attribute__((always_inline)) {
+    t.row0 = kHalves ? (base + group) * kHoldRows + 4 * half : (base + group) * R;
+    if (kHalves && half == 0) {
+      const int rb = base + group;
+      const bool live = rb * kHoldRows < a.rows && left[0] > 0;
+      const uint8_t* v = in_row<const uint8_t>(a.values + rb * a.value_pitch, (uint32_t)col[0] * kHoldRows);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const u32x4n four = live ? got<u32x4n>((const u32x4n*)v + c) : (u32x4n){0, 0, 0, 0};
+#pragma unroll
+        for (int o = 0; o < 2; ++o) next_codes[c][0][o] = four[2 * o], next_codes[c][1][o] = four[2 * o + 1];
+      }
+      next_scale = live ? __uint_as_float((uint32_t)a.scales[(col[0] / kHoldCols) * a.scale_pitch + rb] << 23) : 0.f;
+    }
     if (!kTwice) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) fetch(t, j, j);
@@ -804,8 +821,15 @@ __global__ __launch_bounds__(kAhead ? 512 : 1024, kAhead ? 2 : 4) void layer_nor
     t.mean = live ? a.mean[t.row0 + lane] : 0.f, t.rstd = live ? a.rstd[t.row0 + lane] : 0.f;
   };
   int turn = 0;
-  auto finish = [&](Turn& t) __attribute__((always_inline)) {
+  auto finish = [&](Turn& t, int half) __attribute__((always_inline)) {
     const int row0 = t.row0;
+    if (kHalves && half == 0) {
+      codes_scale = next_scale;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) codes[c][h][0] = next_codes[c][h][0], codes[c][h][1] = next_codes[c][h][1];
+    }
     auto settle = [&](int j, int k) __attribute__((always_inline)) {
       if (tail) {
 #pragma unroll
@@ -816,7 +840,9 @@ __global__ __launch_bounds__(kAhead ? 512 : 1024, kAhead ? 2 : 4) void layer_nor
       }
     };
     auto values = [&](int k, int i, int h, f32x2n(&v)[4]) __attribute__((always_inline)) {  // s of columns 2i, 2i + 1, rows h Q ..
-      if (kHeld)
+      if (kHalves)
+        held_quad(codes[i][half][0], codes[i][half][1], codes_scale, v);
+      else if (kHeld)
         held_quad(t.q[kHeld ? k : 0][i][kHeld ? h : 0][0], t.q[kHeld ? k : 0][i][kHeld ? h : 0][1], t.scale[k], v);
       else
 #pragma unroll
@@ -898,7 +924,10 @@ __global__ __launch_bounds__(kAhead ? 512 : 1024, kAhead ? 2 : 4) void layer_nor
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int h = 0; h < kQuads; ++h)
-            if (kHeld) renew_word(t.q[kHeld ? j : 0][c][h][0]), renew_word(t.q[kHeld ? j : 0][c][h][1]);
+            if (kHalves)
+              renew_word(codes[c][half][0]), renew_word(codes[c][half][1]);
+            else if (kHeld)
+              renew_word(t.q[kHeld ? j : 0][c][h][0]), renew_word(t.q[kHeld ? j : 0][c][h][1]);
       }
     }
 #pragma unroll
@@ -951,53 +980,66 @@ __global__ __launch_bounds__(kAhead ? 512 : 1024, kAhead ? 2 : 4) void layer_nor
     turn ^= 1;
   };
   const int step = blocks * groups;
-  if constexpr (kAhead) {
+  if constexpr (kHalves) {
     Turn even, odd;
     int base = block * groups;
-    if (base < a.items) {
-      begin(even, base);
-      for (;;) {
-        base += step;
-        if (base >= a.items) {
-          finish(even);
-          break;
-        }
-        begin(odd, base);
-        step_by_step();
-        finish(even);
-        base += step;
-        if (base >= a.items) {
-          finish(odd);
-          break;
-        }
-        begin(even, base);
-        step_by_step();
-        finish(odd);
-      }
+    bool more = base < a.items;
+    if (more) begin(even, base, 0);
+    while (more) {
+      begin(odd, base, 1);
+      step_by_step();
+      finish(even, 0);
+      base += step;
+      more = base < a.items;
+      if (more) begin(even, base, 0);
+      step_by_step();
+      finish(odd, 1);
+    }
+  } else if constexpr (kAhead) {
+    Turn even, odd;
+    int base = block * groups;
+    bool more = base < a.items;
+    if (more) begin(even, base, 0);
+    while (more) {
+      base += step;
+      more = base < a.items;
+      if (more) begin(odd, base, 0);
+      step_by_step();
+      finish(even, 0);
+      if (!more) break;
+      base += step;
+      more = base < a.items;
+      if (more) begin(even, base, 0);
+      step_by_step();
+      finish(odd, 0);
     }
   } else {
     for (int base = block * groups; base < a.items; base += step) {
       Turn t;
-      begin(t, base);
-      finish(t);
+      begin(t, base, 0);
+      finish(t, 0);
     }
   }
   if (!a.partial) return;
-  // The sums of the groups of a workgroup are joined in LDS (there is more than one only of up to 2048 columns).
-  if constexpr (NV == 1) {
+  // The sums of the groups of a workgroup are joined in LDS.
+  if constexpr (kGroups) {
     if (groups > 1) {
-      const int width = (int)blockDim.x * 8;
-      float* mine = merged + (group - 1) * 2 * width + col[0];
+      const int width = NV * (int)blockDim.x * 8;
+      float* mine = merged + (group - 1) * 2 * width;
       if (group > 0) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mine[i] = dgamma[0][i], mine[width + i] = dbeta[0][i];
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) mine[col[j] + i] = dgamma[j][i], mine[width + col[j] + i] = dbeta[j][i];
       }
       __syncthreads();
       if (group > 0) return;
       for (int o = 0; o < groups - 1; ++o) {
-        const float* other = merged + o * 2 * width + col[0];
+        const float* other = merged + o * 2 * width;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) dgamma[0][i] += other[i], dbeta[0][i] += other[width + i];
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dgamma[j][i] += other[col[j] + i], dbeta[j][i] += other[width + col[j] + i];
       }
     }
   }

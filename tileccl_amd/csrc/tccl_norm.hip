@@ -76,15 +76,17 @@ Shape forward_shape(int rows, int cols, bool held, int cus) {
 // 2048 x 1024 10.1 -> 19.4.
 bool columns_apart(int rows) { return rows <= 1024; }
 
-// Backward: as many as four rows (two of fp32) as long as there are four groups of them for each CU, workgroups of up to 512 threads whose
-// groups join their sums, 1024 threads of a CU at most and four turns each (of eight rows, two) if that leaves every CU one: each
-// workgroup's sums are written and read again.  2048 x 4096 bf16 26.6 us with 512 workgroups, 23.8 with 256; 12000 x 128 13.6
-// with eight groups each, 25.9 with one.
+// Backward.  Many rows: workgroups of up to 512 threads, 512 of a CU, whose threads are a turn ahead (kAhead), where two turns of
+// four vectors (fp32: two; from 8 bits: a row block's halves of four) are no more than 256 registers.  Otherwise one row, or from 8 bits
+// eight as long as there are two groups of them for each CU, else four; workgroups of up to 512 threads whose groups join their
+// sums, 1024 threads of a CU at most and four turns each (of eight rows, two) if that leaves every CU one: each workgroup's sums are
+// written and read again (8192 x 4096 from 8 bits: 50.4 us with two turns, 58.0 with four).
 Shape backward_shape(int rows, int cols, int dtype, bool held, int cus) {
   Shape s;
-  if (!columns_apart(rows) && !held && dtype != TCCL_F32 && cols <= 8192) {  // kAhead: one workgroup, or several small ones, on a CU
+  const bool f32 = dtype == TCCL_F32;
+  if (!columns_apart(rows) && cols <= (held ? 4096 : f32 ? 8192 : 16384)) {
     s.ahead = true;
-    s.NV = cols > 4096 ? 2 : 1, s.R = 4 / s.NV;
+    s.NV = cols > 8192 ? 4 : cols > 4096 || f32 ? 2 : 1, s.R = held ? kHoldRows : (f32 ? 2 : 4) / s.NV;
     s.waves = (cols + 512 * s.NV - 1) / (512 * s.NV);
     s.items = (int)(((int64_t)rows + s.R - 1) / s.R);
     s.groups = 8 / s.waves;
@@ -94,17 +96,14 @@ Shape backward_shape(int rows, int cols, int dtype, bool held, int cus) {
     s.wgs = wanted < most ? wanted : most;
     return s;
   }
-  for (int R = held ? kHoldRows : dtype == TCCL_F32 ? 2 : 4;; R /= 2) {
-    s = shape_of(rows, cols, R, cus, 1024);
-    if (s.NV > 1 && R > (held ? 4 : 1)) continue;
-    if (R == (held ? 4 : 1) || s.items >= (held ? 2 : 4) * cus) break;
-  }
+  s = shape_of(rows, cols, held ? kHoldRows : 1, cus, 1024);
+  if (held && (s.NV > 1 || s.items < 2 * cus)) s = shape_of(rows, cols, 4, cus, 1024);
   s.groups = s.waves <= 4 ? 8 / s.waves : 1;
   // (sum_columns is quicker with at least 256 threads: 1003 x 1000 from 8 bits 10.3 us with 128 of them)
   while (s.groups > (columns_apart(rows) ? (3 + s.waves) / s.waves : 1) && s.items < cus / 2 * s.groups) s.groups /= 2;
   s.threads = 64 * s.waves * s.groups;
   const int wanted = (s.items + s.groups - 1) / s.groups, most = cus * (s.threads <= 512 ? 1024 / s.threads : 1);
-  const int few = wanted / (held ? 2 : 4);  // (8192 x 4096 from 8 bits 50.4 us with two turns, 58.0 with four)
+  const int few = wanted / (held ? 2 : 4);
   s.wgs = columns_apart(rows) ? wanted : few < cus ? cus : few;
   if (s.wgs > most && !columns_apart(rows)) s.wgs = most;
   if (s.wgs > wanted) s.wgs = wanted;
@@ -139,16 +138,18 @@ template <typename T, int kRows>
 void backward(const NormGradArgs& a, const Shape& s, hipStream_t stream) {
   if constexpr (sizeof(T) == 2) {
     if (a.values) {
+      if (s.ahead) return launch_backward<T, 4, 1, true, kRows, true>(a, s, stream);
       if (s.R == 8) return launch_backward<T, 8, 1, true, kRows>(a, s, stream);
       if (s.NV == 1) return launch_backward<T, 4, 1, true, kRows>(a, s, stream);
       if (s.NV == 2) return launch_backward<T, 4, 2, true, kRows>(a, s, stream);
       return launch_backward<T, 4, 4, true, kRows>(a, s, stream);
     }
     if (s.ahead && s.NV == 1) return launch_backward<T, 4, 1, false, kRows, true>(a, s, stream);
-    if (s.ahead) return launch_backward<T, 2, 2, false, kRows, true>(a, s, stream);
-    if (s.R == 4) return launch_backward<T, 4, 1, false, kRows>(a, s, stream);
+    if (s.ahead && s.NV == 2) return launch_backward<T, 2, 2, false, kRows, true>(a, s, stream);
+    if (s.ahead) return launch_backward<T, 1, 4, false, kRows, true>(a, s, stream);
+  } else {
+    if (s.ahead) return launch_backward<T, 1, 2, false, kRows, true>(a, s, stream);
   }
-  if (s.R == 2) return launch_backward<T, 2, 1, false, kRows>(a, s, stream);
   if (s.NV == 1) return launch_backward<T, 1, 1, false, kRows>(a, s, stream);
   if (s.NV == 2) return launch_backward<T, 1, 2, false, kRows>(a, s, stream);
   return launch_backward<T, 1, 4, false, kRows>(a, s, stream);
