@@ -18,7 +18,7 @@
 // do not depend on which workgroup comes first.
 //
 // What bounds them: memory where there are many rows (bf16: 8192 x 4096 forward 24.6 us, 5.4 TB/s with the launch, where a copy reaches 6.45
-// without; 16384 x 4096 backward with a residual's gradient 99 us, 5.4; 16384 x 4096 to 8 bits 39 us, back 29), a launch and one or two trips to
+// without; 16384 x 4096 backward with a residual's gradient 99 us, 5.4; 16384 x 4096 to 8 bits 34 us, back 29), a launch and one or two trips to
 // memory where there are few (16 x 4096 6.2 us, of which an empty launch is 3.5).
 //
 // 8 rows x 8 columns of a thread are also the unit of the 8-bit layout: values lie as [row block][column][row in block], so a
@@ -359,7 +359,9 @@ TCCL_D int held_exponent(float amax) {
 
 // The patch of one lane; 16 neighbouring lanes hold a block.  rows 0..7 of the patch in p[0..7]; what lies outside the
 // tensor is zero.  Writes the lane's 64 bytes and, from the first of the 16 lanes, the scale.
-template <typename T>
+// kTurn: four neighbouring lanes turn their 4 x 4 vectors around first, so that a store has 64 bytes in a row of each four, not 16
+// of each lane (16384 x 4096 to 8 bits 38.5 -> 34.4 us; in the norm's kernel, short of registers, 8192 x 4096 57.5 -> 59.7).
+template <typename T, bool kTurn>
 TCCL_D void hold_patch(const Eight<T> (&p)[8], uint8_t* values, uint8_t* scale, bool live, bool first) {
   u16x2n top = {0, 0};
 #pragma unroll
@@ -416,9 +418,25 @@ TCCL_D void hold_patch(const Eight<T> (&p)[8], uint8_t* values, uint8_t* scale, 
         for (int b = 0; b < 32; b += 8)
           if (((q[c][k] >> b) & 0x7fu) == 0x78u) q[c][k] -= 1u << b;
   }
-  if (live) {
+  const int lane = (int)(threadIdx.x & 63);
+  if (kTurn) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) put<u32x4n>((u32x4n*)values + c, q[c]);
+    for (int m = 1; m <= 2; m *= 2)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if (c & m) continue;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int sent = (int)(lane & m ? q[c][k] : q[c + m][k]);
+          const uint32_t came = (uint32_t)(m == 1 ? __builtin_amdgcn_update_dpp(0, sent, 0xB1, 0xf, 0xf, false) : __builtin_amdgcn_update_dpp(0, sent, 0x4E, 0xf, 0xf, false));
+          q[c][k] = lane & m ? came : q[c][k], q[c + m][k] = lane & m ? q[c + m][k] : came;
+        }
+      }
+  }
+  if (live) {
+    uint8_t* to = kTurn ? values - (lane & 3) * 48 : values;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) put<u32x4n>((u32x4n*)(to + c * (kTurn ? 64 : 16)), q[c]);
     if (first) *scale = (uint8_t)(e + 127);
   }
 }
@@ -616,7 +634,7 @@ __global__ __launch_bounds__(1024, 4) void layer_norm_kernel(NormArgs a) {
         const int cb = col[j] / kHoldCols;
         // The columns up to a whole block are written too, as zeros.
         const bool live = row0 < a.rows && (int64_t)col[j] * kHoldRows < a.value_pitch;
-        hold_patch<T>(p, a.values + rb * a.value_pitch + (int64_t)col[j] * kHoldRows, a.scales + cb * a.scale_pitch + rb, live, (lane & 15) == 0);
+        hold_patch<T, false>(p, a.values + rb * a.value_pitch + (int64_t)col[j] * kHoldRows, a.scales + cb * a.scale_pitch + rb, live, (lane & 15) == 0);
       }
     }
   }
@@ -1113,7 +1131,7 @@ __global__ __launch_bounds__(256) void hold_kernel(HoldArgs a) {
       for (int r = 0; r < 8; ++r) p[r].settle(left);
     }
     const bool live = (int64_t)col * kHoldRows < a.value_pitch;
-    hold_patch<T>(p, a.values + rb * a.value_pitch + (int64_t)col * kHoldRows, a.scales + (col / kHoldCols) * a.scale_pitch + rb, live,
+    hold_patch<T, true>(p, a.values + rb * a.value_pitch + (int64_t)col * kHoldRows, a.scales + (col / kHoldCols) * a.scale_pitch + rb, live,
                   (threadIdx.x & 15) == 0);
   }
 #endif
