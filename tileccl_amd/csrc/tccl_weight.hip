@@ -85,7 +85,7 @@ int launch_out(const WeightArgs& a, const Cut& c, bool transposed, hipStream_t s
   s.rows = transposed ? a.outputs : a.cols, s.cols = transposed ? a.cols : a.outputs;
   s.partial = a.partial, s.add = a.add, s.out = a.out;
   s.ld_partial = a.ld_partial, s.ld_add = a.ld_add, s.ld_out = a.ld_out, s.slice = s.rows * a.ld_partial;
-  s.splits = c.splits, s.wide = a.wide;
+  s.splits = c.splits;
   const int64_t units = (int64_t)s.rows * ((s.cols + 3) / 4);
   const int64_t wgs = (units + 255) / 256;
   hipLaunchKernelGGL((weight_sum_kernel<OutT>), dim3((unsigned)(wgs < 4096 ? wgs : 4096)), dim3(256), 0, stream, s);
@@ -145,8 +145,8 @@ int tccl_weight_gradient(const tccl_weight_gradient_desc* d, void* stream) {
   a.tiles_h = c.tiles_h, a.tiles_n = c.tiles_n, a.steps = c.steps, a.splits = c.splits, a.steps_per_split = c.steps_per_split;
   a.xcds = cus % 8 ? 1 : 8, a.per_xcd = (c.tiles_h * c.tiles_n * c.splits + a.xcds - 1) / a.xcds;
   a.band = 4;  // an XCD's run of tiles is four rows of them by as many columns as its CUs give
-  a.wide = ((uintptr_t)d->out | (uintptr_t)d->add) % (4 * osize) == 0 && (rows == 1 || (d->ld_out % 4 == 0 && (!d->add || d->ld_add % 4 == 0)));
-  a.staged = d->add && a.wide && c.splits == 1 && d->out_dtype == TCCL_F32 && d->ld_add <= 1 << 22;
+  const bool wide = ((uintptr_t)d->out | (uintptr_t)d->add) % (4 * osize) == 0 && (rows == 1 || (d->ld_out % 4 == 0 && d->ld_add % 4 == 0));
+  a.staged = d->add && wide && c.splits == 1 && d->out_dtype == TCCL_F32 && d->ld_add <= 1 << 22;
   if (c.splits > 1) {
     const int64_t need = 4 * c.splits * partial_rows(rows, cols);
     if (!d->workspace || ((uintptr_t)d->workspace & 15) || d->workspace_bytes < need)
