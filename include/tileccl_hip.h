@@ -525,7 +525,7 @@ int tccl_restore(const tccl_held_desc* held, void* stream);
 /* Layer norm over the columns of each row: s = x, or x + residual rounded to x's type and stored to `summed`;
  * out = (s - mean) * rstd * weight + bias with rstd = 1 / sqrt(var + eps), var the mean of (s - mean)^2.  Sums are
  * fp32.  values / scales: s in 8 bits too (16-bit types; NULL: not wanted).  weight, bias NULL: one, zero.  `out` and
- * `summed` may be x or residual themselves.  At most TCCL_NORM_MAX_COLS columns. */
+ * `summed` may be x or residual themselves (the 8-bit values are those of s also then), but not each other.  At most TCCL_NORM_MAX_COLS columns. */
 #define TCCL_NORM_MAX_COLS 32768
 typedef struct tccl_norm_desc {
   const void* x;

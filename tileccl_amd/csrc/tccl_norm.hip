@@ -252,6 +252,7 @@ int tccl_layer_norm(const tccl_norm_desc* d, void* stream) {
     return reportf(TCCL_ERR_INVALID, "%s: weight or bias is not aligned to its type", what);
   if (d->values || d->scales) TCCL_TRY(check_held(what, d->values, d->scales, d->dtype));
   if (!d->rows) return 0;
+  if (d->out == d->summed) return reportf(TCCL_ERR_INVALID, "%s: out and summed are the same memory", what);
   int cus = 0;
   TCCL_TRY(compute_units(&cus));
   const int size = size_of(d->dtype);
@@ -269,6 +270,10 @@ int tccl_layer_norm(const tccl_norm_desc* d, void* stream) {
   a.values = apart ? nullptr : (uint8_t*)d->values, a.scales = apart ? nullptr : (uint8_t*)d->scales;
   const Shape s = forward_shape(d->rows, d->cols, a.values != nullptr, cus);
   a.items = s.items;
+  // That launch reads the norm's input: x, ahead of the norm, which may write `out` over it, or `summed`, which the norm makes.
+  const tccl_held_desc h = {d->residual ? d->summed : const_cast<void*>(d->x), d->values, d->scales, d->residual ? d->ld_summed : d->ld_x,
+                            d->rows, d->cols, d->dtype};
+  if (apart && !d->residual) TCCL_TRY(tccl_hold(&h, stream));
 #define TCCL_FORWARD(T)                                                            \
   (kind == kAnyRows      ? forward<T, kAnyRows>(a, s, (hipStream_t)stream)         \
    : kind == kVectorRows ? forward<T, kVectorRows>(a, s, (hipStream_t)stream)      \
@@ -280,10 +285,7 @@ int tccl_layer_norm(const tccl_norm_desc* d, void* stream) {
   else
     TCCL_FORWARD(_Float16);
   TCCL_TRY(launched(what));
-  if (!apart) return 0;
-  const tccl_held_desc h = {d->residual ? d->summed : const_cast<void*>(d->x), d->values, d->scales, d->residual ? d->ld_summed : d->ld_x,
-                            d->rows, d->cols, d->dtype};
-  return tccl_hold(&h, stream);
+  return apart && d->residual ? tccl_hold(&h, stream) : 0;
 }
 
 int64_t tccl_layer_norm_grad_workspace(int32_t rows, int32_t cols, int32_t dtype, int32_t held) {

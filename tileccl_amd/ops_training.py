@@ -185,7 +185,7 @@ def layer_norm(
     With ``residual`` the norm is that of ``x + residual``, rounded once to ``x``'s type and returned as ``summed``.
     ``weight`` and ``bias`` are of ``x``'s type or float32.  ``mean`` and ``rstd`` are float32; sums are float32.
     ``checkpoint``: also hold the norm's input in 8 bits, for ``layer_norm_backward``.  ``out`` (for instance on the
-    symmetric heap) may be ``x`` or ``residual`` itself.
+    symmetric heap) may be ``x`` or ``residual`` itself; the checkpoint is that of the norm's input as it was.
     """
     result = (_native or _bind()).layer_norm(x, weight, bias, eps, residual, checkpoint, out)
     if result is None:
