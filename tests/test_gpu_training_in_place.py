@@ -28,3 +28,12 @@ def test_checkpoint_of_an_input_that_is_overwritten(lib, cols, pitch, offset, pl
     assert torch.equal(ops.restore_activation(r.checkpoint).cpu().double(), ref.held(s)), "not the checkpoint of the norm's input"
     assert more is None or torch.equal(r.summed.cpu(), s)
     check_forward(r, s, w, b)
+
+
+@pytest.mark.parametrize("rows", [64, 61])
+def test_weight_gradient_in_the_gradients_place_is_refused(lib, rows):
+    """As many inputs as tokens: the result has the gradient's shape, and other tiles still read what one has written."""
+    grad = rand((rows, 72), 1, BF16).cuda()
+    held = ops.checkpoint_activation(rand((rows, rows), 2, BF16).cuda())
+    with pytest.raises(ValueError, match="out overlaps grad"):
+        ops.weight_gradient(held, grad, out=grad)

@@ -70,10 +70,10 @@ struct Matrix {
   }
   bool like(const Matrix& m) const { return rows == m.rows && cols == m.cols && t->scalar_type() == m.t->scalar_type() && t->device() == m.t->device(); }
   char* end() const { return rows ? at + ((rows - 1) * pitch + cols) * t->element_size() : at; }
+  // No memory in common (rows between rows count as the matrix's).
+  bool elsewhere(const Matrix& m) const { return !(at < m.end() && m.at < end()); }
   // The same elements in the same places, or none in common.
-  bool apart(const Matrix& m) const {
-    return !m.t || !(at < m.end() && m.at < end()) || (at == m.at && pitch == m.pitch && t->scalar_type() == m.t->scalar_type());
-  }
+  bool apart(const Matrix& m) const { return !m.t || elsewhere(m) || (at == m.at && pitch == m.pitch && t->scalar_type() == m.t->scalar_type()); }
 };
 
 bool vector_of(PyObject* o, int64_t n, const at::Device& device, const at::Tensor*& t) {
@@ -376,7 +376,7 @@ PyObject* weight_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
     at::Tensor made;
     if (args[6] != Py_None) {
-      if (!out.open(args[6]) || out.rows != rows || out.cols != cols || out.t->scalar_type() != result || out.t->device() != device || !out.apart(add) || !out.apart(grad)) return none();
+      if (!out.open(args[6]) || out.rows != rows || out.cols != cols || out.t->scalar_type() != result || out.t->device() != device || !out.apart(add) || !out.elsewhere(grad)) return none();
       d.out = out.at, d.ld_out = out.pitch;
     } else {
       made = empty({rows, cols}, result, device);
