@@ -500,7 +500,8 @@ int tccl_mfma_rate_probe(int32_t kind, const void* a_like, int64_t a_bytes, cons
 
 /* ---- between the GEMMs and collectives of a training step ----------------------------------------
  * No counterpart in the reference, which ends at the GEMM and the collective.  Matrices are row-major with
- * contiguous rows of any alignment and pitches (ld, elements) of at least `cols`; rows >= 0, cols >= 1.
+ * contiguous rows of any alignment and pitches (ld, elements) of at least `cols`; rows >= 0, cols >= 1.  What is written
+ * shares no memory with any other operand, but where it is said that it may be one.
  *
  * Activations in 8 bits.  A rows x cols tensor of TCCL_F16 or TCCL_BF16 is held in blocks of TCCL_HELD_ROWS x
  * TCCL_HELD_COLS: with e the smallest whole number, not under -117, with max|x| <= 448 * 2^e over the block's finite

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle import training as ref
-from tests.test_gpu_training import BF16, F16, check_forward, placed, rand
+from tests.test_gpu_training import BF16, F16, F32, check_forward, placed, rand
 from tileccl_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -37,3 +37,45 @@ def test_weight_gradient_in_the_gradients_place_is_refused(lib, rows):
     held = ops.checkpoint_activation(rand((rows, rows), 2, BF16).cuda())
     with pytest.raises(ValueError, match="out overlaps grad"):
         ops.weight_gradient(held, grad, out=grad)
+
+
+def test_results_across_other_operands(lib):
+    """Every operand has a place in one allocation.  Results that begin in it, end in it or have one row there are refused before
+    anything is written; right in front of it, right behind it and with rows on either side they are what they are elsewhere."""
+    rows, cols = 24, 64
+    g, a = rand((rows, cols), 1, BF16).cuda(), rand((rows, cols), 2, BF16).cuda()
+    memory, places = torch.zeros(2 << 20, dtype=torch.uint8, device="cuda"), iter(range(1 << 20, 2 << 20, 1 << 14))
+
+    def put(t):
+        place = memory[next(places):][: t.numel() * t.element_size()]
+        place.copy_(t.contiguous().view(-1).view(torch.uint8))
+        return place.view(t.dtype).view(t.shape)
+
+    w, mean, rstd = put(rand((cols,), 3, F32, 0.2, 1.0).cuda()), put(rand((rows,), 4).cuda()), put(rand((rows,), 5, F32, 0.1, 1.0).cuda())
+    h = ops.checkpoint_activation(a)
+    held = ops.ActivationCheckpoint(put(h.values), put(h.scales), rows, cols, BF16)
+    before = memory.clone()
+    eight_bits = {"the checkpoint's values": held.values, "the checkpoint's scales": held.scales}
+    statistics = {"mean": mean, "rstd": rstd, "weight": w}
+    calls = [
+        (rows, {"weight": w}, lambda out: ops.layer_norm(a, w, out=out).out),
+        (rows, {"bias": w}, lambda out: ops.layer_norm(a, bias=w, out=out).out),
+        (rows, statistics, lambda out: ops.layer_norm_backward(g, a, mean, rstd, w, out=out).x),
+        (rows, statistics | eight_bits, lambda out: ops.layer_norm_backward(g, held, mean, rstd, w, out=out).x),
+        (rows, eight_bits, lambda out: ops.restore_activation(held, out=out)),
+        (cols, eight_bits, lambda out: ops.weight_gradient(held, g, out_dtype=BF16, out=out)),
+    ]
+    for out_rows, operands, call in calls:
+        def at(first, pitch=cols):
+            return memory[first:first // 2 * 2 + 2 * ((out_rows - 1) * pitch + cols)].view(BF16).as_strided((out_rows, cols), (pitch, 1))
+
+        want = call(None)
+        for name, t in operands.items():
+            first, behind, size = t.data_ptr() - memory.data_ptr(), t.data_ptr() - memory.data_ptr() + t.numel() * t.element_size(), out_rows * cols * 2
+            for out in (at(first), at(behind - 16), at(first + 16 - size), at(first - 3 * 8192, 4096)):
+                with pytest.raises(ValueError, match=f"out overlaps ({'|'.join(operands)})"):
+                    call(out)
+            assert torch.equal(memory, before), "a refused call has written"
+            for out in (at(first - size), at(behind), at(first + 4096 - 3 * 8192, 4096)):
+                assert torch.equal(call(out), want), name
+                memory.copy_(before)

@@ -72,6 +72,15 @@ struct Matrix {
   char* end() const { return rows ? at + ((rows - 1) * pitch + cols) * t->element_size() : at; }
   // No memory in common (rows between rows count as the matrix's).
   bool elsewhere(const Matrix& m) const { return !(at < m.end() && m.at < end()); }
+  // No byte of the matrix's rows lies in a contiguous tensor.
+  bool clear_of(const at::Tensor& o) const {
+    if (!rows || !o.numel()) return true;
+    const int64_t step = pitch * (int64_t)t->element_size(), width = cols * (int64_t)t->element_size();
+    const int64_t from = (char*)o.data_ptr() - at, to = from + (int64_t)o.nbytes();  // seen from the first row
+    const int64_t row = from < width ? 0 : (from - width) / step + 1;               // the first one that ends behind `from`
+    return row >= rows || row * step >= to;
+  }
+  bool clear_of(const at::Tensor* o) const { return !o || clear_of(*o); }
   // The same elements in the same places, or none in common.
   bool apart(const Matrix& m) const { return !m.t || elsewhere(m) || (at == m.at && pitch == m.pitch && t->scalar_type() == m.t->scalar_type()); }
 };
@@ -193,9 +202,10 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const int code = code_of(type);
     if (code < 0 || x.cols > TCCL_NORM_MAX_COLS) return none();
     d.dtype = d.affine_dtype = code;
+    const at::Tensor* affine[2] = {nullptr, nullptr};
     for (int i = 1; i <= 2; ++i) {
       if (args[i] == Py_None) continue;
-      const at::Tensor* t;
+      const at::Tensor*& t = affine[i - 1];
       if (!vector_of(args[i], x.cols, device, t) || (t->scalar_type() != type && t->scalar_type() != at::kFloat)) return none();
       if (i == 2 && d.weight && d.affine_dtype != code_of(t->scalar_type())) return none();
       d.affine_dtype = code_of(t->scalar_type());
@@ -206,7 +216,8 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (PyErr_Occurred()) return nullptr;
     if (wanted && type == at::kFloat) return none();
     if (args[4] != Py_None && (!residual.open(args[4]) || !residual.like(x))) return none();
-    if (args[6] != Py_None && (!out.open(args[6]) || !out.like(x) || !out.apart(x) || !out.apart(residual))) return none();
+    if (args[6] != Py_None && (!out.open(args[6]) || !out.like(x) || !out.apart(x) || !out.apart(residual) || !out.clear_of(affine[0]) || !out.clear_of(affine[1])))
+      return none();
     at::Tensor made, summed, stats = empty({2 * x.rows}, at::kFloat, device);
     HeldOut held;
     d.x = x.at, d.ld_x = x.pitch, d.rows = (int32_t)x.rows, d.cols = (int32_t)x.cols;
@@ -260,7 +271,7 @@ PyObject* layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs
       if (!open_held(args[1], held) || held.rows != grad.rows || held.cols != grad.cols || held.type != type || held.values->device() != device) return none();
       d.values = held.values->data_ptr(), d.scales = held.scales->data_ptr();
     }
-    const at::Tensor *mean, *rstd, *weight;
+    const at::Tensor *mean, *rstd, *weight = nullptr;
     if (!vector_of(args[2], grad.rows, device, mean) || mean->scalar_type() != at::kFloat) return none();
     if (!vector_of(args[3], grad.rows, device, rstd) || rstd->scalar_type() != at::kFloat) return none();
     d.mean = (const float*)mean->data_ptr(), d.rstd = (const float*)rstd->data_ptr();
@@ -275,7 +286,9 @@ PyObject* layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs
     }
     const int affine = PyObject_IsTrue(args[6]);
     if (affine < 0) return nullptr;
-    if (args[7] != Py_None && (!out.open(args[7]) || !out.like(grad) || !out.apart(grad) || !out.apart(more) || !out.apart(x))) return none();
+    if (args[7] != Py_None && (!out.open(args[7]) || !out.like(grad) || !out.apart(grad) || !out.apart(more) || !out.apart(x) || !out.clear_of(held.values) ||
+                               !out.clear_of(held.scales) || !out.clear_of(mean) || !out.clear_of(rstd) || !out.clear_of(weight)))
+      return none();
     at::Tensor made, sums;
     d.grad = grad.at, d.ld_grad = grad.pitch, d.rows = (int32_t)grad.rows, d.cols = (int32_t)grad.cols;
     if (!out.t) {
@@ -333,7 +346,9 @@ PyObject* restore_activation(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     if (!open_held(args[0], held)) return none();
     tccl_held_desc d = {nullptr, held.values->data_ptr(), held.scales->data_ptr(), held.cols, (int32_t)held.rows, (int32_t)held.cols, code_of(held.type)};
     if (args[1] != Py_None) {
-      if (!out.open(args[1]) || out.rows != held.rows || out.cols != held.cols || out.t->scalar_type() != held.type || out.t->device() != held.values->device()) return none();
+      if (!out.open(args[1]) || out.rows != held.rows || out.cols != held.cols || out.t->scalar_type() != held.type || out.t->device() != held.values->device() ||
+          !out.clear_of(held.values) || !out.clear_of(held.scales))
+        return none();
       d.x = out.at, d.ld = out.pitch;
     } else {
       made = empty({held.rows, held.cols}, held.type, held.values->device());
@@ -376,7 +391,9 @@ PyObject* weight_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
     at::Tensor made;
     if (args[6] != Py_None) {
-      if (!out.open(args[6]) || out.rows != rows || out.cols != cols || out.t->scalar_type() != result || out.t->device() != device || !out.apart(add) || !out.elsewhere(grad)) return none();
+      if (!out.open(args[6]) || out.rows != rows || out.cols != cols || out.t->scalar_type() != result || out.t->device() != device || !out.apart(add) || !out.elsewhere(grad) ||
+          !out.clear_of(held.values) || !out.clear_of(held.scales))
+        return none();
       d.out = out.at, d.ld_out = out.pitch;
     } else {
       made = empty({rows, cols}, result, device);

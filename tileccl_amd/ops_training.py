@@ -170,6 +170,23 @@ def _apart(out: torch.Tensor, name: str, op: str, *inputs: torch.Tensor | None) 
             raise ValueError(f"{op}: {name} overlaps an input without being the same tensor")
 
 
+def _bytes_of(c: ActivationCheckpoint) -> dict[str, torch.Tensor]:
+    return {"the checkpoint's values": c.values, "the checkpoint's scales": c.scales}
+
+
+def _clear(out: torch.Tensor, op: str, **inputs: torch.Tensor | None) -> None:
+    """No row of ``out`` lies across a contiguous input that is not made of its rows."""
+    lo, size = out.data_ptr(), out.element_size()
+    width, step = out.shape[1] * size, (out.stride(0) if out.shape[0] > 1 else out.shape[1]) * size
+    for name, t in inputs.items():
+        if t is None or not t.numel() or not out.shape[0]:
+            continue
+        start = t.data_ptr() - lo
+        row = 0 if start < width else (start - width) // step + 1  # the first one that ends behind the input's start
+        if row < out.shape[0] and row * step < start + t.numel() * t.element_size():
+            raise ValueError(f"{op}: out overlaps {name}")
+
+
 def layer_norm(
     x: torch.Tensor,
     weight: torch.Tensor | None = None,
@@ -185,7 +202,8 @@ def layer_norm(
     With ``residual`` the norm is that of ``x + residual``, rounded once to ``x``'s type and returned as ``summed``.
     ``weight`` and ``bias`` are of ``x``'s type or float32.  ``mean`` and ``rstd`` are float32; sums are float32.
     ``checkpoint``: also hold the norm's input in 8 bits, for ``layer_norm_backward``.  ``out`` (for instance on the
-    symmetric heap) may be ``x`` or ``residual`` itself; the checkpoint is that of the norm's input as it was.
+    symmetric heap) may be ``x`` or ``residual`` itself (the checkpoint is that of the norm's input as it was), and lies
+    across no other operand.
     """
     result = (_native or _bind()).layer_norm(x, weight, bias, eps, residual, checkpoint, out)
     if result is None:
@@ -213,6 +231,7 @@ def _refuse_layer_norm(x, weight, bias, residual, checkpoint, out) -> NoReturn:
     if out is not None:
         _matrix(out, "out", op, like=x)
         _apart(out, "out", op, x, residual)
+        _clear(out, op, weight=weight, bias=bias)
     _unexplained(op)
 
 
@@ -232,7 +251,7 @@ def layer_norm_backward(
     ``x``: the norm's input (``summed`` where there was a residual), or the checkpoint of it.  ``grad_summed``: the
     gradient that reaches the norm's input along the residual stream, added to the result.  The sums for weight and bias
     are float32, in a fixed order (the same call gives the same bits); ``affine=False`` leaves them out.  ``out`` may be ``grad`` or
-    ``grad_summed`` itself.
+    ``grad_summed`` itself, and lies across no other operand.
     """
     result = (_native or _bind()).layer_norm_backward(grad, x, mean, rstd, weight, grad_summed, affine, out)
     if result is None:
@@ -264,6 +283,7 @@ def _refuse_layer_norm_backward(grad, x, mean, rstd, weight, grad_summed, out) -
     if out is not None:
         _matrix(out, "out", op, like=grad)
         _apart(out, "out", op, grad, grad_summed, x if full else None)
+        _clear(out, op, mean=mean, rstd=rstd, weight=weight, **({} if full else _bytes_of(x)))
     _unexplained(op)
 
 
@@ -285,7 +305,8 @@ def checkpoint_activation(x: torch.Tensor) -> ActivationCheckpoint:
 
 
 def restore_activation(held: ActivationCheckpoint, *, out: torch.Tensor | None = None) -> torch.Tensor:
-    """The values that a checkpoint stands for, in the type of the tensor it was made of (exactly)."""
+    """The values that a checkpoint stands for, in the type of the tensor it was made of (exactly).  ``out`` lies
+    across neither the values nor the scales."""
     result = (_native or _bind()).restore_activation(held, out)
     if result is None:
         op = "restore_activation"
@@ -294,6 +315,7 @@ def restore_activation(held: ActivationCheckpoint, *, out: torch.Tensor | None =
             _matrix(out, "out", op, shape=(held.rows, held.columns), dtype=held.dtype)
             if out.device != held.values.device:
                 raise ValueError(f"{op}: out must reside on {held.values.device}, got {out.device}")
+            _clear(out, op, **_bytes_of(held))
         _unexplained(op)
     return result
 
@@ -313,7 +335,7 @@ def weight_gradient(
     ``layout``: ``"kn"`` (inputs, outputs), as the GEMMs here take a row-major B; ``"nk"`` (outputs, inputs), as a linear
     layer holds it.  Sums are float32, rounded once to ``out_dtype`` (float32 or ``grad``'s type; that of ``out`` or
     ``add`` where one is given).  ``add``: what earlier micro-batches have summed, of the result's shape and type; ``out``
-    may be ``add`` itself.
+    may be ``add`` itself, and lies across no other operand.
     """
     if layout not in ("kn", "nk"):
         raise ValueError(f"weight_gradient: layout must be 'kn' or 'nk', got {layout!r}")
@@ -343,6 +365,7 @@ def weight_gradient(
         lo, hi = _span(out)
         if lo < _span(grad)[1] and _span(grad)[0] < hi:
             raise ValueError(f"{op}: out overlaps grad")
+        _clear(out, op, **_bytes_of(x))
     width = -(-outputs // 8) * 8
     if rows and (width != outputs or grad.stride(0) % 8 or grad.data_ptr() % 16):
         # The kernel reads 16-byte vectors: a gradient without them is copied first, as the GEMMs' operands are.
