@@ -549,9 +549,10 @@ int tccl_layer_norm(const tccl_norm_desc* norm, void* stream);
 
 /* Its gradients.  grad: that of `out`.  The norm's input s comes as x, or as values / scales with x NULL.
  * dx = rstd * (g - mean(g) - xh * mean(g * xh)) + grad_summed with g = grad * weight, xh = (s - mean) * rstd, means over
- * the row; dweight = sum over rows of grad * xh, dbeta = sum over rows of grad (fp32, NULL: not wanted), added in a
- * fixed order: the same call gives the same bits (one with dx in grad's place may add in another).  dx may be grad or grad_summed itself.  `workspace`: device memory of
- * tccl_layer_norm_grad_workspace(rows, cols, dtype, held) bytes on 16 bytes; `held`: whether values are given. */
+ * the row; dweight = sum over rows of grad * xh, dbias = sum over rows of grad (fp32, NULL: not wanted), added in a
+ * fixed order: the same call gives the same bits (one with dx in grad's place may add in another).  dx may be grad or
+ * grad_summed itself.  `workspace`: device memory of tccl_layer_norm_grad_workspace(rows, cols, dtype, held) bytes on 16 bytes,
+ * which a call that wants neither sum leaves as it is; `held`: whether values are given. */
 typedef struct tccl_norm_grad_desc {
   const void* grad;
   const void* x;

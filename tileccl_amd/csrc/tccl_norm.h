@@ -65,7 +65,7 @@ struct NormGradArgs {
   const float *mean, *rstd;
   const void* weight;
   char* dx;
-  float* partial;  // [slot][2][cols]; nullptr: the sums over the rows are made by workgroups of their own
+  float* partial;  // [slot][2][cols]; nullptr: the sums over the rows are made by workgroups of their own, or not wanted
   float *dgamma, *dbeta;  // of those workgroups
   int column_wgs, column_lanes;  // how many there are, ahead of the others; an eighth of their columns
   int64_t ld_grad, ld_x, ld_grad_summed, ld_dx;

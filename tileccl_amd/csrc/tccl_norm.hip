@@ -323,8 +323,8 @@ int tccl_layer_norm_grad(const tccl_norm_grad_desc* d, void* stream) {
   NormGradArgs a;
   a.grad = (const char*)d->grad, a.x = (const char*)d->x, a.grad_summed = (const char*)d->grad_summed;
   a.values = (const uint8_t*)d->values, a.scales = (const uint8_t*)d->scales;
-  a.mean = d->mean, a.rstd = d->rstd, a.weight = d->weight, a.dx = (char*)d->dx, a.partial = apart ? nullptr : (float*)d->workspace;
-  a.dgamma = d->dweight, a.dbeta = d->dbias, 
+  a.mean = d->mean, a.rstd = d->rstd, a.weight = d->weight, a.dx = (char*)d->dx, a.partial = apart || !sums ? nullptr : (float*)d->workspace;
+  a.dgamma = d->dweight, a.dbeta = d->dbias;
   // As many columns as leave every thread of the workgroup one step of rows (16 x 16384: 13.7 us with 32 of them, 7.1 with 128).
   a.column_lanes = (int64_t)d->rows * kMostColumnLanes <= s.threads * (d->values ? kHoldRows : 4) ? kMostColumnLanes : 4;
   a.column_wgs = apart && sums ? (d->cols + 8 * a.column_lanes - 1) / (8 * a.column_lanes) : 0;

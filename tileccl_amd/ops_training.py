@@ -250,7 +250,7 @@ def layer_norm_backward(
 
     ``x``: the norm's input (``summed`` where there was a residual), or the checkpoint of it.  ``grad_summed``: the
     gradient that reaches the norm's input along the residual stream, added to the result.  The sums for weight and bias
-    are float32, in a fixed order (the same call gives the same bits); ``affine=False`` leaves them out.  ``out`` may be ``grad`` or
+    are float32, in a fixed order (the same call gives the same bits); ``affine=False``: nothing of them is stored or added up.  ``out`` may be ``grad`` or
     ``grad_summed`` itself, and lies across no other operand.
     """
     result = (_native or _bind()).layer_norm_backward(grad, x, mean, rstd, weight, grad_summed, affine, out)
