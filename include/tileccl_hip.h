@@ -500,7 +500,8 @@ int tccl_mfma_rate_probe(int32_t kind, const void* a_like, int64_t a_bytes, cons
 
 /* ---- between the GEMMs and collectives of a training step ----------------------------------------
  * No counterpart in the reference, which ends at the GEMM and the collective.  Matrices are row-major with
- * contiguous rows of any alignment and pitches (ld, elements) of at least `cols`; rows >= 0, cols >= 1.  What is written
+ * contiguous rows of any alignment and pitches (ld, elements) of at least `cols`; 0 <= rows <= TCCL_TRAINING_MAX_ROWS (a grid's
+ * last turns count up to 2^16 rows past the last, in 32 bits), cols >= 1.  What is written
  * shares no memory with any other operand, but where it is said that it may be one.
  *
  * Activations in 8 bits.  A rows x cols tensor of TCCL_F16 or TCCL_BF16 is held in blocks of TCCL_HELD_ROWS x
@@ -509,7 +510,9 @@ int tccl_mfma_rate_probe(int32_t kind, const void* a_like, int64_t a_bytes, cons
  * The value that is held, q * 2^e, is exact in the tensor's type.  With RB = ceil(rows / 8), CB = ceil(cols / 128):
  *   values  uint8[RB][128 * CB][8]     row block, column, row in the block; zeros beyond the tensor; on 16 bytes
  *   scales  uint8[CB][SP]              e + 127 of column block, row block; SP = RB rounded up to 16; bytes from RB on
- *                                      may hold anything */
+ *                                      may hold anything
+ * At most 2^27 columns. */
+#define TCCL_TRAINING_MAX_ROWS 2147418111
 #define TCCL_HELD_ROWS 8
 #define TCCL_HELD_COLS 128
 typedef struct tccl_held_desc {
@@ -580,7 +583,7 @@ int tccl_layer_norm_grad(const tccl_norm_grad_desc* norm, void* stream);
  * with one rounding to out_dtype (F32 or that type).  transposed: out and add are outputs x cols (element (h, n) at
  * n * ld + h), the layout of a weight that is multiplied as its .t() view.  `add` NULL: none; it may be `out`.
  * grad's rows start on 16 bytes and are readable in whole 16-byte vectors, past the last of `outputs` columns too (what
- * lies there has no part in the result).  `workspace`: device memory of
+ * lies there has no part in the result).  At most 2^24 cols, outputs and elements of grad's pitch.  `workspace`: device memory of
  * tccl_weight_gradient_workspace(rows, cols, outputs) bytes on 16 bytes (0: none). */
 typedef struct tccl_weight_gradient_desc {
   const void* values;

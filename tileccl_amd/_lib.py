@@ -219,6 +219,7 @@ class WeightGradientDesc(C.Structure):
 
 
 HELD_ROWS, HELD_COLS, NORM_MAX_COLS = 8, 128, 32768  # TCCL_HELD_ROWS, TCCL_HELD_COLS, TCCL_NORM_MAX_COLS
+TRAINING_MAX_ROWS = 2147418111  # TCCL_TRAINING_MAX_ROWS
 STATIC_MAX_TILES, STATIC_MAX_GROUPS = 16384, 64
 
 

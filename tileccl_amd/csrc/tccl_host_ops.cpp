@@ -63,7 +63,7 @@ struct Matrix {
     t = &THPVariable_Unpack(o);
     if (!t->is_cuda() || t->layout() != at::kStrided || t->dim() != 2) return false;
     rows = t->size(0), cols = t->size(1);
-    if (cols < 1 || rows > INT32_MAX || cols > INT32_MAX || (cols > 1 && t->stride(1) != 1)) return false;
+    if (cols < 1 || rows > TCCL_TRAINING_MAX_ROWS || cols > INT32_MAX || (cols > 1 && t->stride(1) != 1)) return false;
     pitch = rows > 1 ? t->stride(0) : cols;
     at = (char*)t->data_ptr();
     return pitch >= cols;
@@ -115,7 +115,7 @@ bool open_held(PyObject* o, Held& h) {
     return false;
   }
   h.type = d == f16 ? at::kHalf : at::kBFloat16;
-  if (h.rows < 0 || h.cols < 1 || h.rows > INT32_MAX || h.cols > INT32_MAX) return false;
+  if (h.rows < 0 || h.cols < 1 || h.rows > TCCL_TRAINING_MAX_ROWS || h.cols > INT32_MAX) return false;
   const at::Device device = h.values->device();
   const int64_t rb = row_blocks(h.rows), cb = col_blocks(h.cols);
   return bytes_of(*h.values, device) && bytes_of(*h.scales, device) && h.values->dim() == 3 && h.values->size(0) == rb && h.values->size(1) == cb * TCCL_HELD_COLS &&

@@ -157,6 +157,7 @@ void backward(const NormGradArgs& a, const Shape& s, hipStream_t stream) {
 
 int check_sizes(const char* what, int rows, int cols, int dtype, int most_cols) {
   if (rows < 0 || cols < 1) return reportf(TCCL_ERR_INVALID, "%s: rows must not be negative and cols must be positive (got %d, %d)", what, rows, cols);
+  if (rows > TCCL_TRAINING_MAX_ROWS) return reportf(TCCL_ERR_UNSUPPORTED, "%s: rows=%d, at most %d", what, rows, TCCL_TRAINING_MAX_ROWS);
   if (cols > most_cols) return reportf(TCCL_ERR_UNSUPPORTED, "%s: cols=%d, at most %d", what, cols, most_cols);
   if (!size_of(dtype)) return reportf(TCCL_ERR_UNSUPPORTED, "%s: dtype %d is not F16, BF16 or F32", what, dtype);
   return 0;

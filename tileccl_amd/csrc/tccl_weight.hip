@@ -92,6 +92,14 @@ int launch_out(const WeightArgs& a, const Cut& c, bool transposed, hipStream_t s
   return launched("weight_gradient");
 }
 
+int check_sizes(const char* what, int rows, int cols, int outputs) {
+  if (rows < 0 || cols < 1 || outputs < 1)
+    return reportf(TCCL_ERR_INVALID, "%s: rows must not be negative, cols and outputs must be positive (got %d, %d, %d)", what, rows, cols, outputs);
+  if (rows > TCCL_TRAINING_MAX_ROWS) return reportf(TCCL_ERR_UNSUPPORTED, "%s: rows=%d, at most %d", what, rows, TCCL_TRAINING_MAX_ROWS);
+  if (cols > 1 << 24 || outputs > 1 << 24) return reportf(TCCL_ERR_UNSUPPORTED, "%s: %d x %d outputs, at most %d of either", what, cols, outputs, 1 << 24);
+  return 0;
+}
+
 int size_of(int dtype) { return dtype == TCCL_F32 ? 4 : dtype == TCCL_F16 || dtype == TCCL_BF16 ? 2 : 0; }
 
 }  // namespace
@@ -99,10 +107,8 @@ int size_of(int dtype) { return dtype == TCCL_F32 ? 4 : dtype == TCCL_F16 || dty
 extern "C" {
 
 int64_t tccl_weight_gradient_workspace(int32_t rows, int32_t cols, int32_t outputs) {
-  if (rows < 0 || cols < 1 || outputs < 1) return reportf(TCCL_ERR_INVALID, "weight_gradient: sizes %d, %d, %d", rows, cols, outputs);
   int cus = 0;
-  const int rc = compute_units(&cus);
-  if (rc) return -1;
+  if (check_sizes("weight_gradient", rows, cols, outputs) || compute_units(&cus)) return -1;
   const Cut c = choose(rows, cols, outputs, cus);
   if (c.splits == 1) return 0;
   const int64_t kn = partial_rows(cols, outputs), nk = partial_rows(outputs, cols);
@@ -112,9 +118,8 @@ int64_t tccl_weight_gradient_workspace(int32_t rows, int32_t cols, int32_t outpu
 int tccl_weight_gradient(const tccl_weight_gradient_desc* d, void* stream) {
   const char* what = "weight_gradient";
   if (!d) return reportf(TCCL_ERR_INVALID, "%s: the descriptor is NULL", what);
-  if (d->rows < 0 || d->cols < 1 || d->outputs < 1)
-    return reportf(TCCL_ERR_INVALID, "%s: rows must not be negative, cols and outputs must be positive (got %d, %d, %d)", what, d->rows, d->cols, d->outputs);
-  if (d->cols > 1 << 24 || d->outputs > 1 << 24) return reportf(TCCL_ERR_UNSUPPORTED, "%s: %d x %d outputs, at most %d of either", what, d->cols, d->outputs, 1 << 24);
+  int rc = check_sizes(what, d->rows, d->cols, d->outputs);
+  if (rc) return rc;
   if (d->dtype != TCCL_F16 && d->dtype != TCCL_BF16) return reportf(TCCL_ERR_UNSUPPORTED, "%s: grad is F16 or BF16", what);
   if (d->out_dtype != d->dtype && d->out_dtype != TCCL_F32) return reportf(TCCL_ERR_UNSUPPORTED, "%s: out is of grad's type or F32", what);
   if (!d->out) return reportf(TCCL_ERR_INVALID, "%s: out is NULL", what);
@@ -132,7 +137,7 @@ int tccl_weight_gradient(const tccl_weight_gradient_desc* d, void* stream) {
     return reportf(TCCL_ERR_INVALID, "%s: out or add has a pitch below its %d columns", what, cols);
   if (((uintptr_t)d->out | (uintptr_t)d->add) % osize) return reportf(TCCL_ERR_INVALID, "%s: out or add is not aligned to its type", what);
   int cus = 0;
-  int rc = compute_units(&cus);
+  rc = compute_units(&cus);
   if (rc) return rc;
   const Cut c = choose(d->rows, d->cols, d->outputs, cus);
   WeightArgs a;

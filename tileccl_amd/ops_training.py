@@ -126,6 +126,8 @@ def _matrix(t: Any, name: str, op: str, *, like: torch.Tensor | None = None, sha
     rows, cols = t.shape
     if cols == 0:
         raise ValueError(f"{op}: {name} has no columns")
+    if rows > _lib.TRAINING_MAX_ROWS:
+        raise ValueError(f"{op}: {name} has {rows} rows, at most {_lib.TRAINING_MAX_ROWS}")
     if cols > 1 and t.stride(1) != 1:
         raise ValueError(f"{op}: {name} must have contiguous rows (stride(1) == 1), got strides {tuple(t.stride())}")
     pitch = t.stride(0) if rows > 1 else cols
@@ -145,6 +147,8 @@ def _held(c: Any, op: str, device: torch.device | None = None) -> None:
         raise ValueError(f"{op}: expected an ActivationCheckpoint, got {type(c).__name__}")
     if c.dtype not in _HELD_TYPES:
         raise ValueError(f"{op}: a checkpoint holds float16 or bfloat16, not {c.dtype}")
+    if not (0 <= c.rows <= _lib.TRAINING_MAX_ROWS and c.columns >= 1):
+        raise ValueError(f"{op}: a checkpoint of {c.rows} x {c.columns}; rows are 0 to {_lib.TRAINING_MAX_ROWS}, columns 1 or more")
     values, scales = ActivationCheckpoint.shapes(c.rows, c.columns)
     for t, shape, name in ((c.values, values, "values"), (c.scales, scales, "scales")):
         if tuple(t.shape) != shape or t.dtype != torch.uint8 or not t.is_contiguous():
