@@ -13,12 +13,44 @@ interface, which makes tensors *views* that never own the memory.
 from __future__ import annotations
 
 import ctypes as C
+import gc
 
 import torch
 
 from tileccl_amd import _lib
 
 DEVICE = "cuda:0"  # every emulated rank lives on the one GPU
+
+_collecting = False  # the garbage collector is at work
+_collected: list[tuple] = []  # (how to free it, handle) of the arenas that it has found
+
+
+def _note_collection(phase: str, info: dict) -> None:
+    global _collecting
+    _collecting = phase == "start"
+
+
+gc.callbacks.append(_note_collection)
+
+
+def free_collected() -> None:
+    """Return the device memory of arenas that the garbage collector has found.
+
+    Freeing waits for the device.  The collector runs wherever an object happens to be made, between the launches of two
+    ranks too, the first of which waits in its kernel for words that the second will write: a wait for the device there
+    holds the second launch back until the first one gives up.  Such arenas are therefore freed where a heap is made, let go or
+    waited for."""
+    if _collecting:
+        return
+    while True:
+        try:
+            free, handle = _collected.pop()
+        except IndexError:  # none left (another thread may have taken the last one)
+            return
+        try:
+            free(None, handle)
+        except Exception:  # interpreter shutdown: the driver reclaims the memory with the process
+            pass
 
 
 class _RawDeviceBytes:
@@ -41,8 +73,8 @@ class Arena:
     Lifetime: every tensor handed out is a view of a slice tensor, and a slice tensor keeps
     the exporter it was built from -- and through it this object -- alive for as long as its
     storage exists.  ``release()`` by the last heap therefore only forgets the slice tensors;
-    the device memory is freed when this object is collected, i.e. once no tensor views it
-    any more.  (The reference's ``cleanup`` likewise only drops its reference to a
+    the device memory is freed when this object goes, i.e. once no tensor views it
+    any more (``free_collected``, where the garbage collector finds it).  (The reference's ``cleanup`` likewise only drops its reference to a
     torch-owned buffer, so tensors allocated earlier stay valid:
     ``/root/reference/tileccl/memory/symmetric_heap.py:1266-1316``.)
     """
@@ -57,6 +89,7 @@ class Arena:
             raise ValueError(f"world_size={world_size} exceeds the supported maximum {_lib.MAX_WORLD}")
         self.slice_bytes = int(slice_bytes)
         self.world_size = int(world_size)
+        free_collected()
         self._handle, self.bases = self._allocate(self.slice_bytes, self.world_size)
         self._slices: list[torch.Tensor] | None = [self._view(b, self.slice_bytes) for b in self.bases]
         self.heap_bases = self._device_bases(self.bases)
@@ -80,7 +113,7 @@ class Arena:
     def _device_bases(self, bases: list[int]) -> torch.Tensor:
         return torch.tensor(bases, dtype=torch.int64, device=DEVICE)
 
-    def _deallocate(self, handle: object) -> None:
+    def _deallocate(self, handle: object) -> None:  # (without the object, if the collector has found it)
         torch.cuda.synchronize()
         _lib.check(_lib.load().tccl_heap_destroy(handle), "tccl_heap_destroy")
 
@@ -106,12 +139,11 @@ class Arena:
         if self._users <= 0:
             self._slices = None
             self.heap_bases = None
+            free_collected()
 
     def __del__(self) -> None:
         handle, self._handle = getattr(self, "_handle", None), None
         if handle is None:
             return
-        try:
-            self._deallocate(handle)
-        except Exception:  # interpreter shutdown: the driver reclaims the memory with the process
-            pass
+        _collected.append((type(self)._deallocate, handle))
+        free_collected()

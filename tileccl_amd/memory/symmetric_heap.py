@@ -22,7 +22,7 @@ import math
 
 import torch
 
-from tileccl_amd.memory.arena import DEVICE, Arena
+from tileccl_amd.memory.arena import DEVICE, Arena, free_collected
 from tileccl_amd.memory.bump import BumpAllocator
 
 logger = logging.getLogger(__name__)
@@ -238,6 +238,7 @@ class SymmetricHeap:
     # ------------------------------------------------------------------ sync / teardown
     def barrier(self) -> None:
         torch.cuda.synchronize()
+        free_collected()
 
     def metadata(self) -> dict[str, object]:
         return {
