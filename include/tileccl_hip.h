@@ -600,6 +600,10 @@ typedef struct tccl_weight_gradient_desc {
   int32_t transposed;
 } tccl_weight_gradient_desc;
 int64_t tccl_weight_gradient_workspace(int32_t rows, int32_t cols, int32_t outputs);
+/* Host view of how a device of `compute_units` cuts such a call: the edge of its tiles (256 or 128), the groups of wavefronts
+ * that share a tile's rows (1 or 2), the splits of the rows over workgroups and the steps of 64 rows in each. */
+int tccl_weight_gradient_cut(int32_t rows, int32_t cols, int32_t outputs, int32_t compute_units, int32_t* edge, int32_t* groups, int32_t* splits,
+                             int32_t* steps_per_split);
 int tccl_weight_gradient(const tccl_weight_gradient_desc* wg, void* stream);
 
 #ifdef __cplusplus

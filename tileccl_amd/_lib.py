@@ -299,6 +299,7 @@ SIGNATURES = {
     "tccl_layer_norm_grad_workspace": (_i64, [_i32, _i32, _i32, _i32]),
     "tccl_layer_norm_grad": (C.c_int, [_P(NormGradDesc), _vp]),
     "tccl_weight_gradient_workspace": (_i64, [_i32, _i32, _i32]),
+    "tccl_weight_gradient_cut": (C.c_int, [_i32, _i32, _i32, _i32, _P(_i32), _P(_i32), _P(_i32), _P(_i32)]),
     "tccl_weight_gradient": (C.c_int, [_P(WeightGradientDesc), _vp]),
     "tccl_mfma_rate_probe": (C.c_int, [_i32, _vp, _i64, _vp, _i64, _vp, _i32, _i32, _vp]),
     "tccl_gemm_reducescatter": (

@@ -115,6 +115,17 @@ int64_t tccl_weight_gradient_workspace(int32_t rows, int32_t cols, int32_t outpu
   return 4 * c.splits * (kn > nk ? kn : nk);
 }
 
+int tccl_weight_gradient_cut(int32_t rows, int32_t cols, int32_t outputs, int32_t compute_units, int32_t* edge, int32_t* groups, int32_t* splits,
+                             int32_t* steps_per_split) {
+  const int rc = check_sizes("weight_gradient_cut", rows, cols, outputs);
+  if (rc) return rc;
+  if (compute_units < 1 || !edge || !groups || !splits || !steps_per_split)
+    return reportf(TCCL_ERR_INVALID, "weight_gradient_cut: %d compute units, or a NULL result", compute_units);
+  const Cut c = choose(rows, cols, outputs, compute_units);
+  *edge = c.kind == kLarge ? 256 : 128, *groups = c.kind == kPairs ? 2 : 1, *splits = c.splits, *steps_per_split = c.steps_per_split;
+  return 0;
+}
+
 int tccl_weight_gradient(const tccl_weight_gradient_desc* d, void* stream) {
   const char* what = "weight_gradient";
   if (!d) return reportf(TCCL_ERR_INVALID, "%s: the descriptor is NULL", what);
