@@ -1,8 +1,8 @@
-"""Guard against register spills inside the K loops of the large-tile kernels, and against loads that read a
-scalar register too soon.
+"""Guard against register spills inside the K loops of the large-tile and weight-gradient kernels, and against loads that
+read a scalar register too soon.
 
-``python -m tileccl_amd.csrc.check_spills`` compiles ``tccl_api.hip`` and ``tccl_kmajor.hip`` to
-assembly (about two minutes) and, for every ``gemm256_kernel`` / ``fused256_kernel``
+``python -m tileccl_amd.csrc.check_spills`` compiles the library's sources to
+assembly (some five minutes) and, for every ``gemm256_kernel`` / ``fused256_kernel`` / ``weight_gradient_kernel``
 instantiation, counts the scratch-memory instructions that lie between the kernel's first and last
 MFMA, i.e. inside its K loops.  A register that the compiler keeps in scratch memory there is
 reloaded through the same queue as the operand loads, so the reload waits for all of them: a
@@ -15,6 +15,10 @@ The count over the whole kernel is printed as well.  In an all-gather kernel the
 the K loops sit on rarely taken paths; in a reduce-scatter kernel (third template argument true)
 they sit in the reduction phases, between loads of the addends, and are marked: 32 of them made
 the 8192 x 4096 x 2048 reduce-scatter 4 % slower.
+
+The layer-norm kernels have no K loop: those that keep vector registers in scratch memory are listed with how many
+(``layer_norm_grad_kernel``'s comment in ``tccl_norm.h`` says which and why), and one that does so and is not of those makes the
+exit status 1.
 
 A vector memory instruction must not read a scalar register within five wait states of the vector
 instruction (v_readlane, v_readfirstlane, a compare) that wrote it: the hardware does not wait.  The compiler
@@ -36,15 +40,28 @@ from tileccl_amd.csrc.build import FLAGS, HERE, SOURCES
 
 
 def kernels(asm: str):
-    """(name, vgprs, scratch instructions in the K loops, scratch instructions in all) per large-tile kernel."""
+    """(name, vgprs, scratch instructions in the K loops, scratch instructions in all) per kernel with a K loop."""
     counts = dict(re.findall(r"\.name:\s+(\S+)\n(?:.*\n)*?\s+\.vgpr_count:\s+(\d+)", asm))
-    for match in re.finditer(r"^(_ZN4tccl1[45](?:gemm|fused)256_kernel\w*):", asm, flags=re.M):
+    for match in re.finditer(r"^(_ZN4tccl(?:1[45](?:gemm|fused)256|22weight_gradient)_kernel\w*):", asm, flags=re.M):
         name = match.group(1)
         body = asm[match.end(): asm.index(".Lfunc_end", match.end())].split("\n")
         mfma = [i for i, line in enumerate(body) if "v_mfma" in line]
         scratch = [i for i, line in enumerate(body) if "scratch_" in line]
         inside = [i for i in scratch if mfma and mfma[0] < i < mfma[-1]]
         yield name, int(counts.get(name, 0)), len(inside), len(scratch)
+
+
+NORM = re.compile(r"_ZN4tccl(?:17layer_norm|22layer_norm_grad)_kernelI(?:f|DF16b?_?)Li(\d+)ELi(\d+)E")
+
+
+def norm_spills(asm: str):
+    """(name, vector registers in scratch memory, whether that is known of such kernels) of the layer-norm kernels that have any."""
+    for name, count in re.findall(r"\.name:\s+(\S+)\n(?:(?!\.name:).*\n)*?\s+\.vgpr_spill_count:\s+(\d+)", asm):
+        match = NORM.match(name)
+        if match and int(count):
+            rows, vectors = map(int, match.groups())
+            known = vectors == 4 or (rows, vectors) == (4, 2) or (rows == 8 and int(count) <= 6)
+            yield name, int(count), known
 
 
 def is_reduce(name: str) -> bool:
@@ -141,6 +158,9 @@ def report(asm: str, allow: int) -> bool:
         if not flag and total and is_reduce(name):
             flag = "  (scratch accesses in a reduce-scatter kernel)"
         print(f"{name}: {vgprs} VGPRs, scratch instructions {inside} in K loops / {total} in all{flag}")
+    for name, count, known in norm_spills(asm):
+        good &= known
+        print(f"{name}: {count} VGPRs in scratch{'' if known else '  <-- not of the forms that have any'}")
     for name, body in bodies(asm):
         early = early_reads(body)
         if early:

@@ -450,7 +450,8 @@ TCCL_D void held_quad(uint32_t left, uint32_t right, float scale, f32x2n (&v)[4]
 }
 
 // ---- forward ---------------------------------------------------------------------------------------
-// blockDim = (64 W, G): G groups of W wavefronts, each with R rows at a time.
+// blockDim = (64 W, G): G groups of W wavefronts, each with R rows at a time.  (kHold: 1 or 2 of the 128 registers are in scratch; four
+// vectors of fp32 with ends of rows to move: 16.)
 template <typename T, int R, int NV, bool kHold, int kRows>
 __global__ __launch_bounds__(1024, 4) void layer_norm_kernel(NormArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -730,6 +731,10 @@ TCCL_D void sum_columns(const NormGradArgs& a, int wg, float* joined) {
 }
 
 // kHeld: s comes from its 8-bit values, R is a row block or half of one.
+// Registers: 16 of a vector's are its column sums, 8 more gamma where it stays.  Forms that need more than they have keep the rest in scratch
+// memory, read back in every turn: beyond 16384 columns (four vectors) 123 registers of fp32, 188 with ends of rows to move, 11 and 81 of 16
+// bits, 85 and 150 from 8 bits; from 8 bits beyond 8192 columns (two vectors) 3 and 30; with ends to move alone, 18 of 16 bits
+// a turn ahead beyond 8192 columns and 6 of eight rows from 8 bits.  (python -m tileccl_amd.csrc.check_spills lists them.)
 // kAhead: workgroups of up to 512 threads, 512 threads of a CU, whose 256 registers hold two turns: a turn's operands are on their way
 // while the turn before is computed (from 8 bits the turns are the halves of a row block, whose codes come with the first).  bf16
 // 4096 x 4096 37.3 -> 33.0 us, 4096 x 16384 119 -> 105, from 8 bits 34.6 -> 29.1 and 1030 x 4096 21.1 -> 14.9; fp32 4096 x 4096
@@ -740,7 +745,7 @@ __global__ __launch_bounds__(kAhead ? 512 : 1024, kAhead ? 2 : 4) void layer_nor
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int Q = R < 4 ? R : 4;          // rows taken together
   constexpr bool kHalves = kHeld && kAhead;  // turns are the halves of a row block, whose codes are loaded with the first
-  constexpr bool kTwice = kHeld && NV > 1;  // four rows are more than 128 registers: read again
+  constexpr bool kTwice = kHeld && NV > 1;  // four rows are more than 128 registers: read again (and some are in scratch all the same)
   constexpr int kQuads = kHeld ? R / 4 : 1;  // rows of codes, four in a word
   constexpr bool kKeep = NV == 1 || kAhead;  // gamma stays in registers (a load of it would be waited for with those of the next turn)
   constexpr int KJ = kTwice ? 1 : NV;
