@@ -507,7 +507,8 @@ int tccl_mfma_rate_probe(int32_t kind, const void* a_like, int64_t a_bytes, cons
  * Activations in 8 bits.  A rows x cols tensor of TCCL_F16 or TCCL_BF16 is held in blocks of TCCL_HELD_ROWS x
  * TCCL_HELD_COLS: with e the smallest whole number, not under -117, with max|x| <= 448 * 2^e over the block's finite
  * values, a value is held as the e4m3 of x / 2^e (exact division, round to nearest even), what is not finite as NaN.
- * The value that is held, q * 2^e, is exact in the tensor's type.  With RB = ceil(rows / 8), CB = ceil(cols / 128):
+ * Where that would be 256 * 2^e with e = 8 (F16) or 120 (BF16), more than the type can hold, it is 240 * 2^e, the value below it.
+ * The value that is held, q * 2^e, is therefore exact in the tensor's type.  With RB = ceil(rows / 8), CB = ceil(cols / 128):
  *   values  uint8[RB][128 * CB][8]     row block, column, row in the block; zeros beyond the tensor; on 16 bytes
  *   scales  uint8[CB][SP]              e + 127 of column block, row block; SP = RB rounded up to 16; bytes from RB on
  *                                      may hold anything

@@ -11,7 +11,9 @@ input) in half their size, and what the backward pass makes of them:
   rows x 128 columns, and back.
 * ``weight_gradient``: ``x.t() @ grad`` of a linear layer whose input is held in 8 bits.
 
-Tensors may lie on a symmetric heap or elsewhere on the device; launches go to torch's current stream.
+Tensors may lie on a symmetric heap or elsewhere on the device; launches go to torch's current stream.  Nothing is recorded for
+autograd: results are detached from inputs that require gradients, and a program calls the backward operators itself (in the
+``backward`` of an ``autograd.Function`` of its own, say).
 """
 
 from __future__ import annotations
