@@ -58,3 +58,14 @@ def test_a_heap_in_a_cycle_lets_go_inside_the_collection(freed):
     assert freed == []
     _FakeArena(16, 1)
     assert freed[0] == ("handle", 4096)
+
+
+def test_a_program_can_free_them_itself(freed):
+    from tileccl_amd.memory import free_collected
+
+    Holder(_FakeArena(1024, 1))
+    gc.collect()
+    assert freed == []
+    free_collected()
+    free_collected()
+    assert freed == [("handle", 1024)]

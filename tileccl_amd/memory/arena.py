@@ -39,7 +39,7 @@ def free_collected() -> None:
     Freeing waits for the device.  The collector runs wherever an object happens to be made, between the launches of two
     ranks too, the first of which waits in its kernel for words that the second will write: a wait for the device there
     holds the second launch back until the first one gives up.  Such arenas are therefore freed where a heap is made, let go or
-    waited for."""
+    waited for; a program that wants their memory for something else, behind a ``gc.collect()`` of its own, calls this."""
     if _collecting:
         return
     while True:
@@ -145,5 +145,8 @@ class Arena:
         handle, self._handle = getattr(self, "_handle", None), None
         if handle is None:
             return
-        _collected.append((type(self)._deallocate, handle))
-        free_collected()
+        try:
+            _collected.append((type(self)._deallocate, handle))
+            free_collected()
+        except Exception:  # interpreter shutdown: this module's names are gone
+            pass
