@@ -607,6 +607,118 @@ int tccl_weight_gradient_cut(int32_t rows, int32_t cols, int32_t outputs, int32_
                              int32_t* steps_per_split);
 int tccl_weight_gradient(const tccl_weight_gradient_desc* wg, void* stream);
 
+/* The same from an input in full: x (rows x cols) of grad's type.  x's and grad's rows start on 16 bytes and are readable in whole
+ * 16-byte vectors, past their last columns too (what lies there has no part in the result); pitches of at most 2^24 elements. */
+typedef struct tccl_weight_gradient_full_desc {
+  const void* x;
+  const void* grad;
+  const void* add;
+  void* out;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t ld_x, ld_grad, ld_add, ld_out;
+  int32_t rows, cols, outputs;
+  int32_t dtype;      /* x, grad: F16 or BF16 */
+  int32_t out_dtype;  /* add, out */
+  int32_t transposed;
+} tccl_weight_gradient_full_desc;
+int64_t tccl_weight_gradient_full_workspace(int32_t rows, int32_t cols, int32_t outputs);
+int tccl_weight_gradient_full(const tccl_weight_gradient_full_desc* wg, void* stream);
+
+/* Gated linear layer: z = x W = [g | u], out = act(g) * u, from a weight (inputs x 2 outputs) whose first half of columns is the
+ * gate's.  Sums and activations are fp32, out and kept (z, rows x 2 outputs; NULL: not wanted) are rounded once.
+ *   weight: kmajor 0: rows of 2 outputs, ld_weight apart; kmajor 1: 2 outputs rows of inputs (the layer holds it transposed).  `up`: elements
+ *   from the gate's part to the other one's (kmajor 0: at least `outputs`; kmajor 1: at least outputs - 1 rows).
+ *   x's and weight's rows start on 16 bytes (`up` is a multiple of 8) and are readable in whole 16-byte vectors; where inputs is no
+ *   multiple of 8, x is 0 up to the next one (and a kmajor weight is).  Pitches of at most 2^22 elements.
+ *   act: TCCL_SILU g / (1 + exp(-g)); TCCL_GELU g Phi(g), Phi the normal distribution; TCCL_GELU_TANH
+ *   g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2; TCCL_RELU max(g, 0).
+ * out and kept have any alignment of their type and share no memory with another operand. */
+enum { TCCL_SILU = 0, TCCL_GELU = 1, TCCL_GELU_TANH = 2, TCCL_RELU = 3 };
+#define TCCL_GATED_MAX_COLS 2097152
+typedef struct tccl_gated_desc {
+  const void* x;
+  const void* weight;
+  void* out;
+  void* kept;
+  int64_t ld_x, ld_weight, up, ld_out, ld_kept;
+  int32_t rows, inputs, outputs;
+  int32_t dtype;      /* F16 or BF16, of everything */
+  int32_t activation;
+  int32_t kmajor;
+} tccl_gated_desc;
+int tccl_gated(const tccl_gated_desc* gated, void* stream);
+
+/* From the gradient of out (rows x outputs) that of z: inner = [grad * u * act'(g) | grad * act(g)] (rows x 2 outputs), act'(0) = 0 for
+ * TCCL_RELU.  z is read from kept, or, kept NULL, computed again from x and weight and not rounded.  With kept, x and weight are not
+ * looked at, and inner may be kept itself.  The gradients of x and weight are products: inner times the weight's transpose, and
+ * tccl_weight_gradient(_full) of x and inner. */
+typedef struct tccl_gated_grad_desc {
+  const void* grad;
+  const void* kept;
+  const void* x;
+  const void* weight;
+  void* inner;
+  int64_t ld_grad, ld_kept, ld_x, ld_weight, up, ld_inner;
+  int32_t rows, inputs, outputs;
+  int32_t dtype;
+  int32_t activation;
+  int32_t kmajor;
+} tccl_gated_grad_desc;
+int tccl_gated_grad(const tccl_gated_grad_desc* gated, void* stream);
+
+/* AdamW over many tensors, in fp32: with g = grad * grad_scale,
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps).
+ * Tensor i has sizes[i] >= 0 elements, one behind another, at params[i] and grads[i] (host arrays of device addresses, read during the
+ * call; any alignment of the type).  Its moments start at the next multiple of TCCL_MOMENT_BLOCK elements of `first` and `second` behind those
+ * of the tensors ahead of it; what lies between two tensors' moments is left as it is.  bits 32: fp32.  bits 8: bytes, with a scale
+ * byte s for each block, 2^(s - 127), in `first_scales` and `second_scales`:
+ *   m: e4m3, s - 127 the smallest whole number, at least -117, with max|m| <= 448 * 2^(s - 127);
+ *   v: code c from 1 to 254 is (1 + ((c - 1) % 8) / 8) * 2^((c - 1) / 8 - 30), 0 is 0, 255 NaN; s - 127 = floor(log2(max v)) in -90 .. 127;
+ *      what is positive has code 1 or more, and code 248 or less where s is 254.
+ * (Maxima of the block's finite values; what is not finite is held as NaN.)  A value the fraction f of a step above the held value
+ * below it is rounded up where f + u >= 1, u in [0, 1) being 16 bits, the lower ones for m, the upper ones for v, of the hash h
+ * of the element's place i in `first` and the step, in 32 bits: h = i ^ (step * 0x9E3779B9 + (i >> 32) * 0xBB67AE85),
+ * h = (h ^ (h >> 16)) * 0x6A09E667, h = (h ^ (h >> 15)) * 0x3C6EF373, h = h ^ (h >> 16).
+ * The update takes m and v before they are rounded.  `master` (params in 16 bits only; NULL: none): fp32 values of the params, laid out as the
+ * moments, which are updated in the params' place and of which the params are then the rounded values.
+ * step_at, lr_at, grad_scale_at: device words that the launch reads in the place of the values (NULL: the values count), for
+ * recorded calls.  Moments and master lie on 16 bytes.  Tensors share no memory. */
+#define TCCL_MOMENT_BLOCK 128
+typedef struct tccl_adamw_desc {
+  void* const* params;
+  const void* const* grads;
+  const int64_t* sizes;
+  void* first;
+  void* second;
+  void* first_scales;
+  void* second_scales;
+  void* master;
+  const int32_t* step_at;
+  const float* lr_at;
+  const float* grad_scale_at;
+  double lr, beta1, beta2, eps, weight_decay, grad_scale;
+  int32_t tensors;
+  int32_t dtype;       /* params: F32, F16 or BF16 */
+  int32_t grad_dtype;  /* that, or F32 */
+  int32_t bits;        /* of a moment: 8 or 32 */
+  int32_t step;        /* from 1 on */
+} tccl_adamw_desc;
+int tccl_adamw(const tccl_adamw_desc* adamw, void* stream);
+
+/* The values that moments in 8 bits stand for, which are exact in BF16: blocks * TCCL_MOMENT_BLOCK of either. */
+typedef struct tccl_adamw_moments_desc {
+  const void* first;
+  const void* second;
+  const void* first_scales;
+  const void* second_scales;
+  void* to_first;
+  void* to_second;
+  int64_t blocks;
+} tccl_adamw_moments_desc;
+int tccl_adamw_moments(const tccl_adamw_moments_desc* moments, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

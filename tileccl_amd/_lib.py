@@ -218,8 +218,113 @@ class WeightGradientDesc(C.Structure):
     ]
 
 
+class WeightGradientFullDesc(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("grad", C.c_void_p),
+        ("add", C.c_void_p),
+        ("out", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+        ("ld_x", C.c_int64),
+        ("ld_grad", C.c_int64),
+        ("ld_add", C.c_int64),
+        ("ld_out", C.c_int64),
+        ("rows", C.c_int32),
+        ("cols", C.c_int32),
+        ("outputs", C.c_int32),
+        ("dtype", C.c_int32),
+        ("out_dtype", C.c_int32),
+        ("transposed", C.c_int32),
+    ]
+
+
+class GatedDesc(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("out", C.c_void_p),
+        ("kept", C.c_void_p),
+        ("ld_x", C.c_int64),
+        ("ld_weight", C.c_int64),
+        ("up", C.c_int64),
+        ("ld_out", C.c_int64),
+        ("ld_kept", C.c_int64),
+        ("rows", C.c_int32),
+        ("inputs", C.c_int32),
+        ("outputs", C.c_int32),
+        ("dtype", C.c_int32),
+        ("activation", C.c_int32),
+        ("kmajor", C.c_int32),
+    ]
+
+
+class GatedGradDesc(C.Structure):
+    _fields_ = [
+        ("grad", C.c_void_p),
+        ("kept", C.c_void_p),
+        ("x", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("inner", C.c_void_p),
+        ("ld_grad", C.c_int64),
+        ("ld_kept", C.c_int64),
+        ("ld_x", C.c_int64),
+        ("ld_weight", C.c_int64),
+        ("up", C.c_int64),
+        ("ld_inner", C.c_int64),
+        ("rows", C.c_int32),
+        ("inputs", C.c_int32),
+        ("outputs", C.c_int32),
+        ("dtype", C.c_int32),
+        ("activation", C.c_int32),
+        ("kmajor", C.c_int32),
+    ]
+
+
+class AdamwDesc(C.Structure):
+    _fields_ = [
+        ("params", C.c_void_p),
+        ("grads", C.c_void_p),
+        ("sizes", C.c_void_p),
+        ("first", C.c_void_p),
+        ("second", C.c_void_p),
+        ("first_scales", C.c_void_p),
+        ("second_scales", C.c_void_p),
+        ("master", C.c_void_p),
+        ("step_at", C.c_void_p),
+        ("lr_at", C.c_void_p),
+        ("grad_scale_at", C.c_void_p),
+        ("lr", C.c_double),
+        ("beta1", C.c_double),
+        ("beta2", C.c_double),
+        ("eps", C.c_double),
+        ("weight_decay", C.c_double),
+        ("grad_scale", C.c_double),
+        ("tensors", C.c_int32),
+        ("dtype", C.c_int32),
+        ("grad_dtype", C.c_int32),
+        ("bits", C.c_int32),
+        ("step", C.c_int32),
+    ]
+
+
+class AdamwMomentsDesc(C.Structure):
+    _fields_ = [
+        ("first", C.c_void_p),
+        ("second", C.c_void_p),
+        ("first_scales", C.c_void_p),
+        ("second_scales", C.c_void_p),
+        ("to_first", C.c_void_p),
+        ("to_second", C.c_void_p),
+        ("blocks", C.c_int64),
+    ]
+
+
 HELD_ROWS, HELD_COLS, NORM_MAX_COLS = 8, 128, 32768  # TCCL_HELD_ROWS, TCCL_HELD_COLS, TCCL_NORM_MAX_COLS
 TRAINING_MAX_ROWS = 2147418111  # TCCL_TRAINING_MAX_ROWS
+GATED_MAX_COLS = 2097152  # TCCL_GATED_MAX_COLS
+MOMENT_BLOCK = 128  # TCCL_MOMENT_BLOCK
+SILU, GELU, GELU_TANH, RELU = 0, 1, 2, 3
 STATIC_MAX_TILES, STATIC_MAX_GROUPS = 16384, 64
 
 
@@ -301,6 +406,12 @@ SIGNATURES = {
     "tccl_weight_gradient_workspace": (_i64, [_i32, _i32, _i32]),
     "tccl_weight_gradient_cut": (C.c_int, [_i32, _i32, _i32, _i32, _P(_i32), _P(_i32), _P(_i32), _P(_i32)]),
     "tccl_weight_gradient": (C.c_int, [_P(WeightGradientDesc), _vp]),
+    "tccl_weight_gradient_full_workspace": (_i64, [_i32, _i32, _i32]),
+    "tccl_weight_gradient_full": (C.c_int, [_P(WeightGradientFullDesc), _vp]),
+    "tccl_gated": (C.c_int, [_P(GatedDesc), _vp]),
+    "tccl_gated_grad": (C.c_int, [_P(GatedGradDesc), _vp]),
+    "tccl_adamw": (C.c_int, [_P(AdamwDesc), _vp]),
+    "tccl_adamw_moments": (C.c_int, [_P(AdamwMomentsDesc), _vp]),
     "tccl_mfma_rate_probe": (C.c_int, [_i32, _vp, _i64, _vp, _i64, _vp, _i32, _i32, _vp]),
     "tccl_gemm_reducescatter": (
         C.c_int,

@@ -13,9 +13,12 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <cstring>
 #include <exception>
+#include <utility>
+#include <vector>
 
 #include "../../include/tileccl_hip.h"
 #include "tccl_host_ops.h"
@@ -33,6 +36,14 @@ int (*entry_hold)(const tccl_held_desc*, void*);
 int (*entry_restore)(const tccl_held_desc*, void*);
 int (*entry_weight)(const tccl_weight_gradient_desc*, void*);
 int64_t (*entry_weight_workspace)(int32_t, int32_t, int32_t);
+// What bind_layers() is given.
+PyObject* gated_result;
+int (*entry_weight_full)(const tccl_weight_gradient_full_desc*, void*);
+int64_t (*entry_weight_full_workspace)(int32_t, int32_t, int32_t);
+int (*entry_gated)(const tccl_gated_desc*, void*);
+int (*entry_gated_grad)(const tccl_gated_grad_desc*, void*);
+int (*entry_adamw)(const tccl_adamw_desc*, void*);
+int (*entry_moments)(const tccl_adamw_moments_desc*, void*);
 
 template <typename Body>
 PyObject* guarded(Body body) {
@@ -419,6 +430,332 @@ PyObject* weight_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
+// ---- the gated layer, weight gradients from an input in full, AdamW ---------------------------------
+
+bool on_device0(const at::Tensor& t) { return t.is_cuda() && t.device().index() == 0; }  // where the ranks live
+
+bool sixteen_bits(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
+
+// Rows as the product kernels read them: on 16 bytes, in whole vectors.
+bool vectored(const Matrix& m) { return !((uintptr_t)m.at % 16) && !(m.cols % 8) && (m.rows <= 1 || !(m.pitch % 8)) && m.pitch <= 1 << 22; }
+
+// A weight (inputs x 2 outputs) as its memory lies: by rows, or (k-major) as 2 outputs rows of inputs.
+struct GatedWeight {
+  const at::Tensor* t = nullptr;
+  char* at = nullptr;
+  int64_t inputs = 0, outputs = 0, pitch = 0, up = 0;
+  bool kmajor = false;
+
+  bool open(PyObject* o) {
+    if (!THPVariable_Check(o)) return false;
+    t = &THPVariable_Unpack(o);
+    if (!on_device0(*t) || t->layout() != at::kStrided || t->dim() != 2) return false;
+    inputs = t->size(0), outputs = t->size(1) / 2;
+    if (inputs < 1 || outputs < 1 || t->size(1) % 2 || inputs > TCCL_GATED_MAX_COLS || outputs > TCCL_GATED_MAX_COLS || !sixteen_bits(t->scalar_type())) return false;
+    at = (char*)t->data_ptr();
+    if (t->stride(1) == 1 && (inputs == 1 || t->stride(0) >= 2 * outputs)) {
+      pitch = inputs > 1 ? t->stride(0) : 2 * outputs;
+      up = outputs;
+      return true;
+    }
+    kmajor = true;
+    pitch = t->stride(1), up = outputs * pitch;
+    return (inputs == 1 || t->stride(0) == 1) && pitch >= inputs;
+  }
+  // What the kernels read without a copy.
+  bool vectored() const {
+    return !((uintptr_t)at % 16) && !(pitch % 8) && pitch <= 1 << 22 && (kmajor ? inputs % 8 == 0 : outputs % 8 == 0);
+  }
+  bool clear_of(const Matrix& m) const {
+    const char* end = at + ((kmajor ? 2 * outputs - 1 : inputs - 1) * pitch + (kmajor ? inputs : 2 * outputs)) * 2;
+    return !(at < m.end() && m.at < end);
+  }
+};
+
+// gated_linear(x, weight, activation, keep, out)
+PyObject* gated_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 5) return none();
+  return guarded([&]() -> PyObject* {
+    Matrix x, out;
+    GatedWeight w;
+    if (!x.open(args[0]) || !on_device0(*x.t) || !w.open(args[1])) return none();
+    const at::ScalarType type = x.t->scalar_type();
+    const at::Device device = x.t->device();
+    if (type != w.t->scalar_type() || x.cols != w.inputs || (x.rows && (!vectored(x) || !w.vectored()))) return none();
+    tccl_gated_desc d;
+    memset(&d, 0, sizeof d);
+    d.activation = (int32_t)PyLong_AsLong(args[2]);
+    const int keep = PyObject_IsTrue(args[3]);
+    if (PyErr_Occurred()) return nullptr;
+    at::Tensor made, kept;
+    if (args[4] != Py_None) {
+      if (!out.open(args[4]) || out.rows != x.rows || out.cols != w.outputs || out.t->scalar_type() != type || out.t->device() != device || !out.elsewhere(x) || !w.clear_of(out))
+        return none();
+      d.out = out.at, d.ld_out = out.pitch;
+    } else {
+      made = empty({x.rows, w.outputs}, type, device);
+      d.out = made.data_ptr(), d.ld_out = w.outputs;
+    }
+    if (keep) {
+      kept = empty({x.rows, 2 * w.outputs}, type, device);
+      d.kept = kept.data_ptr(), d.ld_kept = 2 * w.outputs;
+    }
+    d.x = x.at, d.weight = w.at, d.ld_x = x.pitch, d.ld_weight = w.pitch, d.up = w.up;
+    d.rows = (int32_t)x.rows, d.inputs = (int32_t)w.inputs, d.outputs = (int32_t)w.outputs;
+    d.dtype = code_of(type), d.kmajor = w.kmajor;
+    void* stream;
+    if (!stream_now(stream)) return nullptr;
+    if (failed(entry_gated(&d, stream), "tccl_gated")) return nullptr;
+    PyObject* result = args[4];
+    if (out.t)
+      Py_INCREF(result);
+    else
+      result = THPVariable_Wrap(made);
+    PyObject* fields[2] = {result, optional(kept)};
+    return named(gated_result, fields, 2);
+  });
+}
+
+// gated_gradient(grad, kept, x, weight, activation, out): of the projections.  With kept, x is None and weight is not read.
+PyObject* gated_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 6) return none();
+  return guarded([&]() -> PyObject* {
+    Matrix grad, kept, x, out;
+    GatedWeight w;
+    if (!grad.open(args[0]) || !on_device0(*grad.t) || !w.open(args[3])) return none();
+    const at::ScalarType type = grad.t->scalar_type();
+    const at::Device device = grad.t->device();
+    if (!sixteen_bits(type) || w.t->scalar_type() != type || grad.cols != w.outputs) return none();
+    const bool computed = args[1] == Py_None;
+    if (computed) {
+      if (!x.open(args[2]) || x.t->scalar_type() != type || x.t->device() != device || x.cols != w.inputs || x.rows != grad.rows || (x.rows && (!vectored(x) || !w.vectored()))) return none();
+    } else if (!kept.open(args[1]) || kept.rows != grad.rows || kept.cols != 2 * w.outputs || kept.t->scalar_type() != type || kept.t->device() != device) {
+      return none();
+    }
+    tccl_gated_grad_desc d;
+    memset(&d, 0, sizeof d);
+    d.activation = (int32_t)PyLong_AsLong(args[4]);
+    if (PyErr_Occurred()) return nullptr;
+    at::Tensor made;
+    if (args[5] != Py_None) {
+      if (!out.open(args[5]) || out.rows != grad.rows || out.cols != 2 * w.outputs || out.t->scalar_type() != type || out.t->device() != device || !out.elsewhere(grad) ||
+          !out.apart(kept) || (x.t && !out.elsewhere(x)) || !w.clear_of(out))
+        return none();
+      d.inner = out.at, d.ld_inner = out.pitch;
+    } else {
+      made = empty({grad.rows, 2 * w.outputs}, type, device);
+      d.inner = made.data_ptr(), d.ld_inner = 2 * w.outputs;
+    }
+    d.grad = grad.at, d.ld_grad = grad.pitch;
+    if (computed)
+      d.x = x.at, d.ld_x = x.pitch, d.weight = w.at, d.ld_weight = w.pitch, d.up = w.up;
+    else
+      d.kept = kept.at, d.ld_kept = kept.pitch;
+    d.rows = (int32_t)grad.rows, d.inputs = (int32_t)w.inputs, d.outputs = (int32_t)w.outputs;
+    d.dtype = code_of(type), d.kmajor = w.kmajor;
+    void* stream;
+    if (!stream_now(stream)) return nullptr;
+    if (failed(entry_gated_grad(&d, stream), "tccl_gated_grad")) return nullptr;
+    if (made.defined()) return THPVariable_Wrap(made);
+    Py_INCREF(args[5]);
+    return args[5];
+  });
+}
+
+// weight_gradient_full(x, grad, cols, outputs, transposed, out_dtype, add, out): cols and outputs as `outputs` of weight_gradient, of x
+// and of grad.
+PyObject* weight_gradient_full(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 8) return none();
+  return guarded([&]() -> PyObject* {
+    Matrix x, grad, add, out;
+    if (!x.open(args[0]) || !on_device0(*x.t) || !grad.open(args[1])) return none();
+    const at::ScalarType type = grad.t->scalar_type();
+    const at::Device device = grad.t->device();
+    if (!sixteen_bits(type) || x.t->scalar_type() != type || x.t->device() != device || x.rows != grad.rows) return none();
+    for (const Matrix* m : {&x, &grad})
+      if (m->cols > 1 << 24 || (m->rows && (m->cols % 8 || (m->rows > 1 && (m->pitch % 8 || m->pitch > 1 << 24)) || (uintptr_t)m->at % 16))) return none();
+    const int64_t inputs = args[2] == Py_None ? x.cols : PyLong_AsLongLong(args[2]), outputs = args[3] == Py_None ? grad.cols : PyLong_AsLongLong(args[3]);
+    const int transposed = PyObject_IsTrue(args[4]);
+    if (PyErr_Occurred()) return nullptr;
+    if (inputs < 1 || inputs > x.cols || outputs < 1 || outputs > grad.cols) return none();
+    if (args[5] != f32 && args[5] != (type == at::kHalf ? f16 : bf16)) return none();
+    const at::ScalarType result = args[5] == f32 ? at::kFloat : type;
+    const int64_t rows = transposed ? outputs : inputs, cols = transposed ? inputs : outputs;
+    tccl_weight_gradient_full_desc d;
+    memset(&d, 0, sizeof d);
+    if (args[6] != Py_None) {
+      if (!add.open(args[6]) || add.rows != rows || add.cols != cols || add.t->scalar_type() != result || add.t->device() != device) return none();
+      d.add = add.at, d.ld_add = add.pitch;
+    }
+    at::Tensor made;
+    if (args[7] != Py_None) {
+      if (!out.open(args[7]) || out.rows != rows || out.cols != cols || out.t->scalar_type() != result || out.t->device() != device || !out.apart(add) || !out.elsewhere(grad) || !out.elsewhere(x))
+        return none();
+      d.out = out.at, d.ld_out = out.pitch;
+    } else {
+      made = empty({rows, cols}, result, device);
+      d.out = made.data_ptr(), d.ld_out = cols;
+    }
+    d.x = x.at, d.ld_x = x.pitch, d.grad = grad.at, d.ld_grad = grad.pitch;
+    d.rows = (int32_t)grad.rows, d.cols = (int32_t)inputs, d.outputs = (int32_t)outputs;
+    d.dtype = code_of(type), d.out_dtype = code_of(result), d.transposed = transposed;
+    d.workspace_bytes = entry_weight_full_workspace(d.rows, d.cols, d.outputs);
+    if (d.workspace_bytes < 0) return failed((int)TCCL_ERR_INVALID, "tccl_weight_gradient_full"), nullptr;
+    at::Tensor workspace;
+    if (d.workspace_bytes) {
+      workspace = empty({d.workspace_bytes}, at::kByte, device);
+      d.workspace = workspace.data_ptr();
+    }
+    void* stream;
+    if (!stream_now(stream)) return nullptr;
+    if (failed(entry_weight_full(&d, stream), "tccl_weight_gradient_full")) return nullptr;
+    if (made.defined()) return THPVariable_Wrap(made);
+    Py_INCREF(args[7]);
+    return args[7];
+  });
+}
+
+bool flat_of(PyObject* o, at::ScalarType type, int64_t least, const at::Tensor*& t) {
+  if (!THPVariable_Check(o)) return false;
+  t = &THPVariable_Unpack(o);
+  return on_device0(*t) && t->layout() == at::kStrided && t->dim() == 1 && t->scalar_type() == type && t->numel() >= least && (t->numel() <= 1 || t->stride(0) == 1) &&
+         !((uintptr_t)t->data_ptr() % 16 && type != at::kByte);
+}
+
+// A number, or a device tensor of one element that holds it.
+bool number_or_word(PyObject* o, at::ScalarType type, const void*& at) {
+  if (!THPVariable_Check(o)) return true;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  at = t.data_ptr();
+  return on_device0(t) && t.scalar_type() == type && t.numel() == 1 && !t.is_neg() && !((uintptr_t)at % 4);
+}
+
+typedef std::pair<const char*, const char*> Span;
+
+// adamw_step(params, grads, (first, second, first_scales, second_scales, master, sizes), step, lr, beta1, beta2, eps, weight_decay, grad_scale):
+// True, or None for arguments that it does not take.  params and grads are tuples.
+PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 10) return none();
+  return guarded([&]() -> PyObject* {
+    if (!PyTuple_Check(args[0]) || !PyTuple_Check(args[1]) || !PyTuple_Check(args[2]) || PyTuple_GET_SIZE(args[2]) != 6) return none();
+    const Py_ssize_t n = PyTuple_GET_SIZE(args[0]);
+    PyObject* state[6];
+    for (int i = 0; i < 6; ++i) state[i] = PyTuple_GET_ITEM(args[2], i);
+    if (PyTuple_GET_SIZE(args[1]) != n || !PyTuple_Check(state[5]) || PyTuple_GET_SIZE(state[5]) != n || n > INT32_MAX) return none();
+    tccl_adamw_desc d;
+    memset(&d, 0, sizeof d);
+    std::vector<void*> params(n), grads(n);
+    std::vector<int64_t> sizes(n);
+    std::vector<const at::Tensor*> tensors(n);
+    std::vector<Span> written, read;
+    int64_t blocks = 0;
+    at::ScalarType type = at::kFloat, grad_type = at::kFloat;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      PyObject *po = PyTuple_GET_ITEM(args[0], i), *go = PyTuple_GET_ITEM(args[1], i);
+      if (!THPVariable_Check(po) || !THPVariable_Check(go)) return none();
+      const at::Tensor &p = THPVariable_Unpack(po), &g = THPVariable_Unpack(go);
+      if (!i) type = p.scalar_type(), grad_type = g.scalar_type();
+      if (!on_device0(p) || !on_device0(g) || p.scalar_type() != type || g.scalar_type() != grad_type || !p.sizes().equals(g.sizes()) || !p.is_contiguous() || !g.is_contiguous() || g.is_neg() ||
+          p.is_neg())
+        return none();
+      sizes[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(state[5], i));
+      if (PyErr_Occurred()) return nullptr;
+      if (sizes[i] != p.numel()) return none();
+      params[i] = p.data_ptr(), grads[i] = g.data_ptr(), tensors[i] = &p;
+      blocks += (sizes[i] + TCCL_MOMENT_BLOCK - 1) / TCCL_MOMENT_BLOCK;
+      if (sizes[i]) {
+        written.emplace_back((const char*)p.data_ptr(), (const char*)p.data_ptr() + p.nbytes());
+        read.emplace_back((const char*)g.data_ptr(), (const char*)g.data_ptr() + g.nbytes());
+      }
+    }
+    d.dtype = code_of(type), d.grad_dtype = code_of(grad_type);
+    if (d.dtype < 0 || d.grad_dtype < 0 || (grad_type != type && grad_type != at::kFloat)) return none();
+    d.bits = state[2] == Py_None ? 32 : 8;
+    const at::ScalarType moment = d.bits == 8 ? at::kByte : at::kFloat;
+    const at::Tensor* flat[5] = {};
+    for (int i = 0; i < 5; ++i) {
+      if (i == 4 ? state[4] == Py_None : i >= 2 && d.bits == 32) {
+        if (state[i] != Py_None) return none();
+        continue;
+      }
+      const bool scales = i == 2 || i == 3;
+      if (!flat_of(state[i], i == 4 ? at::kFloat : scales ? at::kByte : moment, scales ? blocks : blocks * TCCL_MOMENT_BLOCK, flat[i])) return none();
+      if (!scales && (uintptr_t)flat[i]->data_ptr() % 16) return none();
+      if (flat[i]->numel()) written.emplace_back((const char*)flat[i]->data_ptr(), (const char*)flat[i]->data_ptr() + flat[i]->nbytes());
+    }
+    if (flat[4] && type == at::kFloat) return none();
+    // Nothing that is written shares memory with anything else.
+    std::sort(written.begin(), written.end());
+    for (size_t i = 1; i < written.size(); ++i)
+      if (written[i].first < written[i - 1].second) return none();
+    for (const Span& g : read) {
+      auto after = std::lower_bound(written.begin(), written.end(), Span(g.second, nullptr));
+      if (after != written.begin() && (after - 1)->second > g.first) return none();
+    }
+    const void *step_at = nullptr, *lr_at = nullptr, *scale_at = nullptr;
+    if (!number_or_word(args[3], at::kInt, step_at) || !number_or_word(args[4], at::kFloat, lr_at) || !number_or_word(args[9], at::kFloat, scale_at)) return none();
+    d.step_at = (const int32_t*)step_at, d.lr_at = (const float*)lr_at, d.grad_scale_at = (const float*)scale_at;
+    const long long step = step_at ? 1 : PyLong_AsLongLong(args[3]);
+    if (!lr_at) d.lr = PyFloat_AsDouble(args[4]);
+    if (!scale_at) d.grad_scale = PyFloat_AsDouble(args[9]);
+    d.beta1 = PyFloat_AsDouble(args[5]), d.beta2 = PyFloat_AsDouble(args[6]), d.eps = PyFloat_AsDouble(args[7]), d.weight_decay = PyFloat_AsDouble(args[8]);
+    if (PyErr_Occurred()) return nullptr;
+    if (step < 1 || step > INT32_MAX) return none();
+    d.step = (int32_t)step;
+    d.params = params.data(), d.grads = grads.data(), d.sizes = sizes.data(), d.tensors = (int32_t)n;
+    d.first = flat[0]->data_ptr(), d.second = flat[1]->data_ptr();
+    if (flat[2]) d.first_scales = flat[2]->data_ptr(), d.second_scales = flat[3]->data_ptr();
+    if (flat[4]) d.master = flat[4]->data_ptr();
+    void* stream;
+    if (!stream_now(stream)) return nullptr;
+    if (failed(entry_adamw(&d, stream), "tccl_adamw")) return nullptr;
+    for (const at::Tensor* t : tensors)
+      if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();  // what autograd has saved of them is no longer there
+    Py_RETURN_TRUE;
+  });
+}
+
+// adamw_moments(first, second, first_scales, second_scales)
+PyObject* adamw_moments(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 4) return none();
+  return guarded([&]() -> PyObject* {
+    const at::Tensor *first, *second, *fs, *ss;
+    if (!flat_of(args[0], at::kByte, 0, first)) return none();
+    const int64_t n = first->numel(), blocks = n / TCCL_MOMENT_BLOCK;
+    if (n % TCCL_MOMENT_BLOCK || !flat_of(args[1], at::kByte, n, second) || second->numel() != n || !flat_of(args[2], at::kByte, blocks, fs) || !flat_of(args[3], at::kByte, blocks, ss) ||
+        ((uintptr_t)first->data_ptr() | (uintptr_t)second->data_ptr()) % 16)
+      return none();
+    const at::Tensor m = empty({n}, at::kBFloat16, first->device()), v = empty({n}, at::kBFloat16, first->device());
+    const tccl_adamw_moments_desc d = {first->data_ptr(), second->data_ptr(), fs->data_ptr(), ss->data_ptr(), m.data_ptr(), v.data_ptr(), blocks};
+    void* stream;
+    if (!stream_now(stream)) return nullptr;
+    if (failed(entry_moments(&d, stream), "tccl_adamw_moments")) return nullptr;
+    Owned a, b;
+    a.o = THPVariable_Wrap(m), b.o = THPVariable_Wrap(v);
+    return a.o && b.o ? PyTuple_Pack(2, a.o, b.o) : nullptr;
+  });
+}
+
+// bind_layers(GatedLinearResult, entries): the entry points in the order below.
+PyObject* bind_layers(PyObject*, PyObject* args) {
+  PyObject* result;
+  unsigned long long e[6];
+  if (!PyArg_ParseTuple(args, "O(KKKKKK)", &result, e, e + 1, e + 2, e + 3, e + 4, e + 5)) return nullptr;
+  if (!PyType_Check(result) || !PyType_IsSubtype((PyTypeObject*)result, &PyTuple_Type)) {
+    PyErr_SetString(PyExc_TypeError, "results are named tuples");
+    return nullptr;
+  }
+  Py_INCREF(result);
+  Py_XSETREF(gated_result, result);
+  entry_weight_full = (decltype(entry_weight_full))(uintptr_t)e[0];
+  entry_weight_full_workspace = (decltype(entry_weight_full_workspace))(uintptr_t)e[1];
+  entry_gated = (decltype(entry_gated))(uintptr_t)e[2];
+  entry_gated_grad = (decltype(entry_gated_grad))(uintptr_t)e[3];
+  entry_adamw = (decltype(entry_adamw))(uintptr_t)e[4];
+  entry_moments = (decltype(entry_moments))(uintptr_t)e[5];
+  Py_RETURN_NONE;
+}
+
 // bind_operators(stream, report, (LayerNormResult, LayerNormGradients, ActivationCheckpoint), (float16, bfloat16, float32), entries):
 // entries are the addresses of the entry points, in the order below.
 PyObject* bind_operators(PyObject*, PyObject* args) {
@@ -455,6 +792,12 @@ PyMethodDef methods[] = {{"bind_operators", bind_operators, METH_VARARGS, nullpt
                          {"checkpoint_activation", FAST(checkpoint_activation)},
                          {"restore_activation", FAST(restore_activation)},
                          {"weight_gradient", FAST(weight_gradient)},
+                         {"bind_layers", bind_layers, METH_VARARGS, nullptr},
+                         {"gated_linear", FAST(gated_linear)},
+                         {"gated_gradient", FAST(gated_gradient)},
+                         {"weight_gradient_full", FAST(weight_gradient_full)},
+                         {"adamw_step", FAST(adamw_step)},
+                         {"adamw_moments", FAST(adamw_moments)},
                          {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace

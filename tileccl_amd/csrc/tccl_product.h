@@ -1,0 +1,273 @@
+// Products of two 16-bit matrices on MFMA tiles, for gfx950, by how each operand lies in memory: the common part of the gated
+// layer's projections (tccl_gated.h) and of the weight gradient from an input in full (tccl_weight_full.hip).
+//
+//     P[m][n] = sum over k of A(m, k) * B(n, k)
+//
+// An operand lies by rows (element (i, k) at i * ld + k: k is contiguous) or deep (at k * ld + i: i is).  Rows go through LDS as
+// 128 bytes of 64 k each and are read with ds_read_b128; deep operands as 64 k rows, read through the transposing
+// ds_read_b64_tr_b16 (within 16 lanes, lane i supplies 4 neighbours of k row i / 4, lane j receives 4 k of column j).  A paired B
+// is two matrices that lie `up` bytes apart: of every 64 columns of the tile 32 are the first one's and 32 the same
+// columns of the second, so that a lane that has an element of one product has that of the other, too.
+//
+// global --buffer_load_dwordx4 ... lds--> LDS: lane l's 16 bytes land at base + 16 l, so the swizzles that keep reads off each
+// other's banks are applied by choosing what a lane fetches:
+//   rows:  chunk c (8 k) of row r in slot c ^ ((r >> 1) & 7)
+//   deep:  chunk c (8 columns) of k row k in slot c ^ 4 (k & 3) ^ 2 ((k >> 3) & 1); with k rows of 128 bytes
+//          c ^ 2 ((k >> 1) & 1) ^ 4 ((k >> 3) & 1)
+// What lies past an operand's window reads as zero; chunks of rows at k >= K are sent there.
+#pragma once
+
+#include "tccl_gemm.h"
+
+namespace tccl {
+
+struct ProductArgs {
+  const char *a, *b;
+  int64_t lda, ldb;  // elements
+  int64_t up;        // paired: bytes from the first matrix of B to the second
+  int M, N, K;       // N: columns of either matrix of a paired B
+};
+
+#if defined(__HIPCC__)
+
+// kTile x kTile outputs by 2 x kTile / 64 wavefronts, each kTile / 2 x 64.
+template <typename T, int kTile, bool kADeep, bool kBDeep, bool kPaired>
+struct Product {
+  typedef typename Mfma<T>::Vec Vec;
+  typedef __attribute__((address_space(3))) void LdsVoid;
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4 LdsQuad;
+  typedef uint32_t Words4 __attribute__((ext_vector_type(4)));
+  static constexpr int kWavesN = kTile / 64, kWaves = 2 * kWavesN;
+  static constexpr int kStepK = 64;
+  static constexpr int kOperand = kTile * 128;  // bytes of an operand in a stage
+  static constexpr int kStage = 2 * kOperand, kLds = 2 * kStage;
+  static constexpr int kBlocksM = kTile / 32, kBlocksN = 4;  // 16 x 16 blocks of a wavefront
+  static constexpr int kTileN = kPaired ? kTile / 2 : kTile;  // columns of either matrix
+  static constexpr int kPitchA = 2 * kTile, kPitchB = 2 * kTileN;  // bytes of a deep operand's k row in a stage
+
+  const ProductArgs& p;
+  char* lds;
+  const int lane, wave, wm, wn;
+
+  TCCL_D Product(const ProductArgs& args, char* mem)
+      : p(args), lds(mem), lane((int)(threadIdx.x & 63)), wave(__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6))), wm(wave / kWavesN), wn(wave % kWavesN) {}
+
+  // ---- global -> LDS ------------------------------------------------------------------------------
+  // A step's operand is fetched in two halves of two pieces (1 KiB, one load) per wavefront.  Rows: half h of a 256 tile's A is rows
+  // 64 h .. + 63 of each 128, of the others rows 32 h .. + 31 of each 64 (of a paired B: matrix h).  Deep: k rows 32 h .. + 31
+  // (of a paired B: piece i from matrix i).
+  static constexpr int row_of(int wave, int h, int i, bool a) {
+    return kTile == 256 && a ? (wave >> 2) * 128 + h * 64 + (wave & 3) * 16 + 8 * i : (wave >> 1) * 64 + h * 32 + (wave & 1) * 16 + 8 * i;
+  }
+  template <int kPitch>
+  static TCCL_D int deep_swizzle(int k) {
+    return kPitch == 128 ? 2 * ((k >> 1) & 1) ^ 4 * ((k >> 3) & 1) : 4 * (k & 3) ^ 2 * ((k >> 3) & 1);
+  }
+  struct Side {
+    const char* at;     // of the tile and of the step that is loaded next
+    int64_t left;       // bytes from there to the end of what may be read
+    int64_t step;       // bytes of a step
+    uint32_t off[2][2];  // this lane's offsets
+  };
+  struct Source {
+    Side a, b;
+    int kt;
+  };
+
+  // Rows: `rows` of them are left from the tile's first on, K elements each.
+  template <bool kA>
+  TCCL_D void by_rows(Side& s, const char* at, int64_t ld, int rows) const {
+    const int kw = (p.K + 7) / 8 * 8;
+    s.at = at;
+    s.left = ((int64_t)(rows - 1) * ld + kw) * 2;
+    s.step = kStepK * 2;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = row_of(wave, h, i, kA) + (lane >> 3), kc = (lane & 7) ^ ((row >> 1) & 7);
+        const int real = kA || !kPaired ? row : row / 64 * 32 + row % 32;
+        s.off[h][i] = (uint32_t)(real * ld * 2 + kc * 16);
+      }
+  }
+  // Deep: `cols` columns are left from the tile's first on.  (Whole vectors are there.)
+  template <bool kA>
+  TCCL_D void by_depth(Side& s, const char* at, int64_t ld, int cols) const {
+    constexpr int kPitch = kA ? kPitchA : kPitchB, kRows = 1024 / kPitch;  // k rows of a piece
+    s.at = at;
+    s.left = ((int64_t)(p.K - 1) * ld + (cols + 7) / 8 * 8) * 2 + (kA || !kPaired ? 0 : p.up);
+    s.step = kStepK * ld * 2;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int k = 32 * h + (kPaired && !kA ? wave : 2 * wave + i) * kRows + lane / (kPitch / 16);
+        const int c = lane % (kPitch / 16) ^ deep_swizzle<kPitch>(k);
+        s.off[h][i] = (uint32_t)(k * ld * 2 + c * 16 + (kPaired && !kA && i ? p.up : 0));
+      }
+  }
+  TCCL_D Source source(int m0, int n0, int first) const {
+    Source s;
+    if constexpr (kADeep)
+      by_depth<true>(s.a, p.a + (int64_t)m0 * 2, p.lda, p.M - m0);
+    else
+      by_rows<true>(s.a, p.a + (int64_t)m0 * p.lda * 2, p.lda, p.M - m0);
+    if constexpr (kBDeep)
+      by_depth<false>(s.b, p.b + (int64_t)n0 * 2, p.ldb, p.N - n0);
+    else
+      by_rows<false>(s.b, p.b + (int64_t)n0 * p.ldb * 2, p.ldb, p.N - n0);
+    for (Side* side : {&s.a, &s.b}) {
+      side->at += first * side->step;
+      side->left -= first * side->step;
+    }
+    s.kt = first;
+    return s;
+  }
+  static TCCL_D Words4 window(const char* at, int64_t bytes) {
+    const uint64_t a = (uint64_t)(uintptr_t)at;
+    Words4 d;
+    d[0] = __builtin_amdgcn_readfirstlane((uint32_t)a);
+    d[1] = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xffffu);
+    d[2] = __builtin_amdgcn_readfirstlane(bytes > 0xfffffff0ll ? 0xfffffff0u : bytes < 0 ? 0u : (uint32_t)bytes);
+    d[3] = 0x00020000u;
+    return d;
+  }
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  // Two loads of 16 bytes per lane, global -> LDS.  Written out because the compiler makes every later read of an LDS array wait for
+  // all loads into it.  M0 wants an instruction between its write and the load; a scalar register that a vector instruction has
+  // written wants five wait states before a vector memory instruction reads it, which the block spends itself.
+  static TCCL_D void copy_pair(char* to0, char* to1, Words4 from, uint32_t off0, uint32_t off1) {
+    const uint32_t first = (uint32_t)(uintptr_t)(LdsVoid*)to0, second = (uint32_t)(uintptr_t)(LdsVoid*)to1;
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %2, %4, 0 offen lds\n\t"
+        "s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %4, 0 offen lds" ::"s"(first), "s"(second), "v"(off0), "v"(off1), "s"(from)
+        : "memory", "m0");
+  }
+#pragma clang diagnostic pop
+  static constexpr uint32_t kDead = 0xfffffff0u;  // past the end of every window
+  // Half h of A, of B of the source's step into `stage`.
+  TCCL_D void issue_a(char* stage, const Source& s, int h) const {
+    char* to0 = stage + (kADeep ? (32 * h + 2 * wave * (1024 / kPitchA)) * kPitchA : row_of(wave, h, 0, true) * 128);
+    copy_pair(to0, to0 + 1024, window(s.a.at, s.a.left), s.a.off[h][0], s.a.off[h][1]);
+  }
+  TCCL_D void issue_b(char* stage, const Source& s, int h) const {
+    char* to = stage + kOperand;
+    if constexpr (kBDeep && kPaired) {
+      to += (32 * h + wave * (1024 / kPitchB)) * kPitchB;
+      copy_pair(to, to + kOperand / 2, window(s.b.at, s.b.left), s.b.off[h][0], s.b.off[h][1]);
+    } else if constexpr (kBDeep) {
+      to += (32 * h + 2 * wave * (1024 / kPitchB)) * kPitchB;
+      copy_pair(to, to + 1024, window(s.b.at, s.b.left), s.b.off[h][0], s.b.off[h][1]);
+    } else {
+      to += row_of(wave, h, 0, false) * 128;
+      copy_pair(to, to + 1024, window(s.b.at + (kPaired && h ? p.up : 0), s.b.left), s.b.off[h][0], s.b.off[h][1]);
+    }
+  }
+  // Ahead of the loads of the source's step (steps come in ascending order): chunks at k >= K are dead from here on.
+  TCCL_D void mask(Source& s) const {
+    if ((kADeep && kBDeep) || (s.kt + 1) * kStepK <= p.K) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int kc = (lane & 7) ^ ((4 * i + (lane >> 4)) & 7);
+      if (s.kt * kStepK + 8 * kc >= p.K)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (!kADeep) s.a.off[h][i] = kDead;
+          if (!kBDeep) s.b.off[h][i] = kDead;
+        }
+    }
+  }
+  // Steps past the last one read zeros: nothing is left there (rows: all chunks are dead).
+  TCCL_D void advance(Source& s) const {
+    s.a.at += s.a.step, s.a.left -= s.a.step;
+    s.b.at += s.b.step, s.b.left -= s.b.step;
+    ++s.kt;
+  }
+
+  // ---- LDS -> operands ----------------------------------------------------------------------------
+  template <int kPitch>
+  TCCL_D Vec turned(const char* base, int chunk, int kh) const {
+    const int i = lane & 15, g = lane >> 4, t = i >> 2, cq = i & 3;
+    const char* q = base + (32 * kh + 8 * g + t) * kPitch + ((chunk + (cq >> 1)) ^ deep_swizzle<kPitch>(8 * g + t)) * 16 + (cq & 1) * 8;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad*)q);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad*)(q + 4 * kPitch));
+    return __builtin_bit_cast(Vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  TCCL_D Vec by_row(const char* base, int row, int kh) const {
+    const int i = lane & 15;
+    return *(const Vec*)(base + (row + i) * 128 + (((4 * kh + (lane >> 4)) ^ ((i >> 1) & 7)) << 4));
+  }
+  // Block `rb` of 16 rows, of 16 columns of the wavefront's, k block kh (32 k).
+  TCCL_D Vec operand_a(const char* stage, int kh, int rb) const {
+    const int row = wm * (kTile / 2) + 16 * rb;
+    if constexpr (kADeep)
+      return turned<kPitchA>(stage, row / 8, kh);
+    else
+      return by_row(stage, row, kh);
+  }
+  TCCL_D Vec operand_b(const char* stage, int kh, int cb) const {
+    if constexpr (kBDeep && kPaired)
+      return turned<kPitchB>(stage + kOperand + (cb >> 1) * (kOperand / 2), wn * 4 + 2 * (cb & 1), kh);
+    else if constexpr (kBDeep)
+      return turned<kPitchB>(stage + kOperand, wn * 8 + 2 * cb, kh);
+    else
+      return by_row(stage + kOperand, wn * 64 + 16 * cb, kh);
+  }
+
+  typedef f32x4 Sums[kBlocksM][kBlocksN];
+  static TCCL_D void clear(Sums& acc) {
+#pragma unroll
+    for (int i = 0; i < kBlocksM; ++i)
+#pragma unroll
+      for (int j = 0; j < kBlocksN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  }
+  static TCCL_D void barrier() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+  }
+
+  // Lane l has row l % 16 of a block and columns 4 (l / 16) .. + 3 of it.  Steps first .. first + steps - 1; behind them nothing is under
+  // way and everybody has left the stages.
+  TCCL_D void run(Sums& acc, int m0, int n0, int first, int steps) const {
+    Source s = source(m0, n0, first);
+    mask(s);
+    auto load = [&](char* stage) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        issue_a(stage, s, h);
+        issue_b(stage, s, h);
+      }
+      advance(s);
+      mask(s);
+    };
+    load(lds);
+    for (int t = 0; t < steps; ++t) {
+      const char* cur = lds + (t & 1) * kStage;
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      barrier();
+      if (t + 1 < steps) load(lds + ((t + 1) & 1) * kStage);
+#pragma unroll
+      for (int kh = 0; kh < 2; ++kh) {
+        Vec a[kBlocksM], b[kBlocksN];
+#pragma unroll
+        for (int j = 0; j < kBlocksN; ++j) b[j] = operand_b(cur, kh, j);
+#pragma unroll
+        for (int i = 0; i < kBlocksM; ++i) a[i] = operand_a(cur, kh, i);
+#pragma unroll
+        for (int i = 0; i < kBlocksM; ++i)
+#pragma unroll
+          for (int j = 0; j < kBlocksN; ++j) acc[i][j] = Mfma<T>::run16(b[j], a[i], acc[i][j]);
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    barrier();
+  }
+};
+
+#endif  // __HIPCC__
+
+}  // namespace tccl

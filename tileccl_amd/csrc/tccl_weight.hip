@@ -1,4 +1,4 @@
-// Weight gradients from activations in 8 bits: argument checks, launch shapes and the entry points.
+// Weight gradients, from activations in 8 bits and in full: argument checks, launch shapes and the entry points.
 #include <hip/hip_runtime.h>
 #include <initializer_list>
 
@@ -7,6 +7,7 @@
 #pragma GCC visibility pop
 #include "tccl_host.h"
 #include "tccl_weight.h"
+#include "tccl_weight_full.h"
 
 namespace {
 
@@ -102,9 +103,94 @@ int check_sizes(const char* what, int rows, int cols, int outputs) {
 
 int size_of(int dtype) { return dtype == TCCL_F32 ? 4 : dtype == TCCL_F16 || dtype == TCCL_BF16 ? 2 : 0; }
 
+// ---- from an input in full ----
+
+Cut full_cut_of(int splits, int rows, int cols, int outputs) { return cut_of(kSmall, splits, rows, cols, outputs); }
+
+Cut choose_full(int rows, int cols, int outputs, int cus) {
+  const Cut whole = full_cut_of(1, rows, cols, outputs);
+  const int64_t tiles = (int64_t)whole.tiles_h * whole.tiles_n;
+  int splits = 1;
+  while (tiles * splits < cus && splits < 32 && whole.steps >= 8 * splits) splits *= 2;
+  return full_cut_of(splits, rows, cols, outputs);
+}
+
+template <typename T, typename OutT>
+int launch_full(const WeightFullArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL((weight_full_kernel<T, OutT, 128>), dim3((unsigned)(a.xcds * a.per_xcd)), dim3(256), 0, stream, a);
+  const int rc = launched("weight_gradient_full");
+  if (rc || a.splits == 1) return rc;
+  WeightSumArgs s;
+  s.rows = a.p.M, s.cols = a.p.N, s.partial = a.partial, s.add = a.add, s.out = a.out;
+  s.ld_partial = a.ld_partial, s.ld_add = a.ld_add, s.ld_out = a.ld_out, s.slice = s.rows * a.ld_partial, s.splits = a.splits;
+  const int64_t wgs = ((int64_t)s.rows * ((s.cols + 3) / 4) + 255) / 256;
+  hipLaunchKernelGGL((weight_sum_kernel<OutT>), dim3((unsigned)(wgs < 4096 ? wgs : 4096)), dim3(256), 0, stream, s);
+  return launched("weight_gradient_full");
+}
+
+int check_full_operand(const char* what, const char* name, const void* at, int64_t ld, int rows, int cols) {
+  if (!at) return reportf(TCCL_ERR_INVALID, "%s: %s is NULL", what, name);
+  if (rows > 1 && ld < cols) return reportf(TCCL_ERR_INVALID, "%s: %s has a pitch of %lld elements for %d columns", what, name, (long long)ld, cols);
+  if (((uintptr_t)at & 15) || (rows > 1 && (ld % 8 || ld < (cols + 7) / 8 * 8)))
+    return reportf(TCCL_ERR_UNSUPPORTED, "%s: %s's rows must lie on 16 bytes and be readable in whole 16-byte vectors (%d columns, pitch %lld)", what, name, cols, (long long)ld);
+  if (ld > 1 << 24) return reportf(TCCL_ERR_UNSUPPORTED, "%s: %s's pitch of %lld elements, at most %d", what, name, (long long)ld, 1 << 24);
+  return 0;
+}
+
 }  // namespace
 
 extern "C" {
+
+int64_t tccl_weight_gradient_full_workspace(int32_t rows, int32_t cols, int32_t outputs) {
+  int cus = 0;
+  if (check_sizes("weight_gradient_full", rows, cols, outputs) || compute_units(&cus)) return -1;
+  const Cut c = choose_full(rows, cols, outputs, cus);
+  if (c.splits == 1) return 0;
+  const int64_t kn = partial_rows(cols, outputs), nk = partial_rows(outputs, cols);
+  return 4 * c.splits * (kn > nk ? kn : nk);
+}
+
+int tccl_weight_gradient_full(const tccl_weight_gradient_full_desc* d, void* stream) {
+  const char* what = "weight_gradient_full";
+  if (!d) return reportf(TCCL_ERR_INVALID, "%s: the descriptor is NULL", what);
+  int rc = check_sizes(what, d->rows, d->cols, d->outputs);
+  if (rc) return rc;
+  if (d->dtype != TCCL_F16 && d->dtype != TCCL_BF16) return reportf(TCCL_ERR_UNSUPPORTED, "%s: x and grad are F16 or BF16", what);
+  if (d->out_dtype != d->dtype && d->out_dtype != TCCL_F32) return reportf(TCCL_ERR_UNSUPPORTED, "%s: out is of grad's type or F32", what);
+  if (!d->out) return reportf(TCCL_ERR_INVALID, "%s: out is NULL", what);
+  if (d->rows) {
+    rc = check_full_operand(what, "x", d->x, d->ld_x, d->rows, d->cols);
+    if (!rc) rc = check_full_operand(what, "grad", d->grad, d->ld_grad, d->rows, d->outputs);
+    if (rc) return rc;
+  }
+  const int rows = d->transposed ? d->outputs : d->cols, cols = d->transposed ? d->cols : d->outputs, osize = size_of(d->out_dtype);
+  if (rows > 1 && (d->ld_out < cols || (d->add && d->ld_add < cols)))
+    return reportf(TCCL_ERR_INVALID, "%s: out or add has a pitch below its %d columns", what, cols);
+  if (((uintptr_t)d->out | (uintptr_t)d->add) % osize) return reportf(TCCL_ERR_INVALID, "%s: out or add is not aligned to its type", what);
+  int cus = 0;
+  rc = compute_units(&cus);
+  if (rc) return rc;
+  const Cut c = choose_full(d->rows, d->cols, d->outputs, cus);
+  if ((int64_t)c.tiles_h * c.tiles_n * c.splits > 1 << 22) return reportf(TCCL_ERR_UNSUPPORTED, "%s: %d x %d tiles of the result", what, c.tiles_h, c.tiles_n);
+  WeightFullArgs a = {};
+  const int64_t ld_x = d->rows > 1 ? d->ld_x : (d->cols + 7) / 8 * 8, ld_grad = d->rows > 1 ? d->ld_grad : (d->outputs + 7) / 8 * 8;
+  a.p.a = (const char*)(d->transposed ? d->grad : d->x), a.p.lda = d->transposed ? ld_grad : ld_x;
+  a.p.b = (const char*)(d->transposed ? d->x : d->grad), a.p.ldb = d->transposed ? ld_x : ld_grad;
+  a.p.M = rows, a.p.N = cols, a.p.K = d->rows;
+  a.add = (const char*)d->add, a.out = (char*)d->out, a.partial = (float*)d->workspace;
+  a.ld_add = d->ld_add, a.ld_out = d->ld_out, a.ld_partial = partial_pitch(cols);
+  a.tiles_m = d->transposed ? c.tiles_n : c.tiles_h, a.tiles_n = d->transposed ? c.tiles_h : c.tiles_n, a.band = 4;
+  a.steps = c.steps, a.splits = c.splits, a.steps_per_split = c.steps_per_split;
+  a.xcds = cus % 8 ? 1 : 8, a.per_xcd = (c.tiles_h * c.tiles_n * c.splits + a.xcds - 1) / a.xcds;
+  if (c.splits > 1) {
+    const int64_t need = 4 * c.splits * partial_rows(rows, cols);
+    if (!d->workspace || ((uintptr_t)d->workspace & 15) || d->workspace_bytes < need)
+      return reportf(TCCL_ERR_INVALID, "%s: the workspace has %lld bytes, %lld on 16 are needed", what, (long long)d->workspace_bytes, (long long)need);
+  }
+  const hipStream_t st = (hipStream_t)stream;
+  if (d->dtype == TCCL_BF16) return d->out_dtype == TCCL_F32 ? launch_full<__bf16, float>(a, st) : launch_full<__bf16, __bf16>(a, st);
+  return d->out_dtype == TCCL_F32 ? launch_full<_Float16, float>(a, st) : launch_full<_Float16, _Float16>(a, st);
+}
 
 int64_t tccl_weight_gradient_workspace(int32_t rows, int32_t cols, int32_t outputs) {
   int cus = 0;

@@ -61,6 +61,13 @@ __all__ = [
     "checkpoint_activation",
     "restore_activation",
     "weight_gradient",
+    "GatedLinearResult",
+    "GatedLinearGradients",
+    "gated_linear",
+    "gated_linear_backward",
+    "AdamWState",
+    "adamw_step",
+    "adamw_moments",
 ]
 
 from tileccl_amd.ops_collective import gemm_allgather, gemm_reducescatter  # noqa: E402  (re-exported)
@@ -74,6 +81,8 @@ from tileccl_amd.ops_training import (  # noqa: E402  (re-exported)
     restore_activation,
     weight_gradient,
 )
+from tileccl_amd.ops_gated import GatedLinearGradients, GatedLinearResult, gated_linear, gated_linear_backward  # noqa: E402  (re-exported)
+from tileccl_amd.ops_adamw import AdamWState, adamw_moments, adamw_step  # noqa: E402  (re-exported)
 from tileccl_amd.ops_plans import (  # noqa: E402  (re-exported)
     AllGatherGemmReduceScatterContract,
     AllGatherGemmReduceScatterPlan,

@@ -9,7 +9,7 @@ input) in half their size, and what the backward pass makes of them:
   or ``x + residual``; the gradients of ``s``, ``weight`` and ``bias``.
 * ``checkpoint_activation`` / ``restore_activation``: a 16-bit tensor to e4m3 with one power-of-two scale per block of 8
   rows x 128 columns, and back.
-* ``weight_gradient``: ``x.t() @ grad`` of a linear layer whose input is held in 8 bits.
+* ``weight_gradient``: ``x.t() @ grad`` of a linear layer whose input is held in 8 bits, or is there in full.
 
 Tensors may lie on a symmetric heap or elsewhere on the device; launches go to torch's current stream.  Nothing is recorded for
 autograd: results are detached from inputs that require gradients, and a program calls the backward operators itself (in the
@@ -99,6 +99,11 @@ def _bind() -> Any:
         host.bind_operators(_launch._raw_stream or (lambda _device: _launch.stream_ptr()), _lib.check,
                             (LayerNormResult, LayerNormGradients, ActivationCheckpoint), _TYPES,
                             tuple(C.cast(e, C.c_void_p).value for e in entries))
+        from tileccl_amd.ops_gated import GatedLinearResult
+
+        entries = (lib.tccl_weight_gradient_full, lib.tccl_weight_gradient_full_workspace, lib.tccl_gated, lib.tccl_gated_grad, lib.tccl_adamw,
+                   lib.tccl_adamw_moments)
+        host.bind_layers(GatedLinearResult, tuple(C.cast(e, C.c_void_p).value for e in entries))
         _native = host
     return _native
 
@@ -327,7 +332,7 @@ def restore_activation(held: ActivationCheckpoint, *, out: torch.Tensor | None =
 
 
 def weight_gradient(
-    x: ActivationCheckpoint,
+    x: "ActivationCheckpoint | torch.Tensor",
     grad: torch.Tensor,
     *,
     layout: str = "kn",
@@ -335,8 +340,8 @@ def weight_gradient(
     add: torch.Tensor | None = None,
     out: torch.Tensor | None = None,
 ) -> torch.Tensor:
-    """``x.t() @ grad``: the gradient of a linear layer's weight from the layer's input ``x``, held in 8 bits, and the
-    gradient of its output, of the type that ``x`` was held from.
+    """``x.t() @ grad``: the gradient of a linear layer's weight from the layer's input ``x``, held in 8 bits or in full (float16 or
+    bfloat16), and the gradient of its output, of the type of ``x``, or the one that it was held from.
 
     ``layout``: ``"kn"`` (inputs, outputs), as the GEMMs here take a row-major B; ``"nk"`` (outputs, inputs), as a linear
     layer holds it.  Sums are float32, rounded once to ``out_dtype`` (float32 or ``grad``'s type; that of ``out`` or
@@ -349,7 +354,11 @@ def weight_gradient(
         out_dtype = out.dtype
     elif add is not None:
         out_dtype = add.dtype
-    result = (_native or _bind()).weight_gradient(x, grad, None, layout == "nk", out_dtype, add, out)
+    native = _native or _bind()
+    if isinstance(x, torch.Tensor):
+        result = native.weight_gradient_full(x, grad, None, None, layout == "nk", out_dtype, add, out)
+        return _weight_gradient_full(x, grad, layout, out_dtype, add, out) if result is None else result
+    result = native.weight_gradient(x, grad, None, layout == "nk", out_dtype, add, out)
     if result is not None:
         return result
     op = "weight_gradient"
@@ -377,6 +386,45 @@ def weight_gradient(
         # The kernel reads 16-byte vectors: a gradient without them is copied first, as the GEMMs' operands are.
         (packed,) = _launch._pack([(grad, rows, width, "weight_gradient")])
         result = _native.weight_gradient(x, packed, outputs, layout == "nk", out_dtype, add, out)
+    if result is None:
+        _unexplained(op)
+    return result
+
+
+def _weight_gradient_full(x, grad, layout, out_dtype, add, out) -> torch.Tensor:
+    """The call with operands that are no rows of whole vectors, or an error."""
+    op = "weight_gradient"
+    _matrix(grad, "grad", op)
+    _matrix(x, "x", op)
+    for t, name in ((x, "x"), (grad, "grad")):
+        if t.dtype not in _HELD_TYPES:
+            raise ValueError(f"{op}: {name} must be float16 or bfloat16, got {t.dtype}")
+        if t.device.index != 0:
+            raise ValueError(f"{op}: {name} must reside on cuda:0, where the ranks live, got {t.device}")
+        if t.shape[1] > 1 << 24:
+            raise ValueError(f"{op}: {name} has {t.shape[1]} columns, at most {1 << 24}")
+    rows, outputs = grad.shape
+    if grad.dtype != x.dtype or rows != x.shape[0]:
+        raise ValueError(f"{op}: x is {x.dtype} with {x.shape[0]} rows, grad is {grad.dtype} with {rows}")
+    if out_dtype not in (torch.float32, grad.dtype):
+        raise ValueError(f"{op}: the result must be float32 or {grad.dtype}, got {out_dtype}")
+    inputs = x.shape[1]
+    shape = (inputs, outputs) if layout == "kn" else (outputs, inputs)
+    for t, name in ((add, "add"), (out, "out")):
+        if t is not None:
+            _matrix(t, name, op, shape=shape, dtype=out_dtype)
+            if t.device != grad.device:
+                raise ValueError(f"{op}: {name} must reside on {grad.device}, got {t.device}")
+    if out is not None:
+        _apart(out, "out", op, add)
+        for t, name in ((grad, "grad"), (x, "x")):
+            lo, hi = _span(out)
+            if lo < _span(t)[1] and _span(t)[0] < hi:
+                raise ValueError(f"{op}: out overlaps {name}")
+    if rows:
+        jobs = [(t, rows, -(-t.shape[1] // 8) * 8, f"weight_gradient {name}") for t, name in ((x, "x"), (grad, "grad"))]
+        x, grad = _launch._pack(jobs)
+    result = _native.weight_gradient_full(x, grad, inputs, outputs, layout == "nk", out_dtype, add, out)
     if result is None:
         _unexplained(op)
     return result
