@@ -203,3 +203,20 @@ def test_graph_and_stream(rows, layout):
         torch.cuda.synchronize()
         now = both()
         assert all(torch.equal(a, b) for a, b in zip(recorded, now)), replay
+
+
+# Beyond what small tiles take in one round of the device: 256 x 128 tiles, with parts of one at every edge.
+LARGE = [(2100, 72, 2056, BF16, "kn", "silu"), (2056, 200, 2100, BF16, "nk", "gelu"), (4096, 64, 1024, F16, "kn", "gelu_tanh"), (2049, 328, 2048, F16, "nk", "silu")]
+
+
+@pytest.mark.parametrize("rows, inputs, outputs, dtype, layout, act", LARGE)
+def test_large_tiles(rows, inputs, outputs, dtype, layout, act):
+    x, dh = rand((rows, inputs), 31, dtype), rand((rows, outputs), 32, dtype, 0.1)
+    w, wd = weight_of(inputs, outputs, dtype, layout, 33)
+    r = ops.gated_linear(x.cuda(), wd, activation=act, keep=True)
+    check_forward(r, x, w, act, True)
+    assert torch.equal(ops.gated_linear(x.cuda(), wd, activation=act).out, r.out)
+    g, u, s = ref.projections(x, w)
+    d = ops.gated_linear_backward(dh.cuda(), None, x.cuda(), wd, activation=act, inputs=False, weights=False)
+    want, bound = inner_bounds(dh, g, u, inputs * SUM * s[:, :outputs], inputs * SUM * s[:, outputs:], dtype, act)
+    within(d.inner, want, bound, "inner")

@@ -32,6 +32,17 @@ def test_weight_gradient(tokens, inputs, outputs, dtype, out_dtype, layout, add)
     within(got, want, rounded(want, (tokens + 8) * SUM * top, out_dtype), "dweight")
 
 
+@pytest.mark.parametrize("tokens", [1, 64, 70, 128, 200, 449])
+@pytest.mark.parametrize("inputs, outputs, layout", [(4200, 2056, "kn"), (2056, 4200, "nk"), (4096, 2304, "nk")])
+def test_large_tiles(tokens, inputs, outputs, layout):
+    x, dy = rand((tokens, inputs), 21, BF16), rand((tokens, outputs), 22, BF16)
+    got = ops.weight_gradient(x.cuda(), dy.cuda(), layout=layout)
+    want, top = x.double().t() @ dy.double(), x.double().abs().t() @ dy.double().abs()
+    if layout == "nk":
+        want, top = want.t(), top.t()
+    within(got, want, rounded(want, tokens * SUM * top, F32), "dweight")
+
+
 def test_pitches_and_places():
     tokens, inputs, outputs = 150, 72, 200
     x, dy = rand((tokens, inputs), 4, BF16), rand((tokens, outputs), 5, BF16)

@@ -60,23 +60,29 @@ int set_product(const char* what, const Sizes& s, const void* x, int64_t ld_x, c
   return 0;
 }
 
-constexpr int kTileOf = 128;
+template <typename T, int kTile, bool kBackward>
+int launch_tile(const char* what, GatedArgs& a, bool kmajor, int cus, hipStream_t stream) {
+  a.tiles_m = (a.p.M + kTile - 1) / kTile, a.tiles_n = (a.p.N + kTile / 2 - 1) / (kTile / 2);
+  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
+  if (tiles > 1 << 22) return reportf(TCCL_ERR_UNSUPPORTED, "%s: %lld tiles of the result", what, (long long)tiles);
+  a.xcds = cus % 8 ? 1 : 8, a.per_xcd = (int)((tiles + a.xcds - 1) / a.xcds), a.band = 4;
+  const dim3 wgs((unsigned)(a.xcds * a.per_xcd));
+  if (kmajor)
+    hipLaunchKernelGGL((gated_kernel<T, kTile, false, kBackward>), wgs, dim3(2 * kTile), 0, stream, a);
+  else
+    hipLaunchKernelGGL((gated_kernel<T, kTile, true, kBackward>), wgs, dim3(2 * kTile), 0, stream, a);
+  return launched(what);
+}
 
 template <typename T, bool kBackward>
 int launch(const char* what, GatedArgs& a, bool kmajor, hipStream_t stream) {
   int cus = 0;
   const int rc = compute_units(&cus);
   if (rc) return rc;
-  a.tiles_m = (a.p.M + kTileOf - 1) / kTileOf, a.tiles_n = (a.p.N + kTileOf / 2 - 1) / (kTileOf / 2);
-  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
-  if (tiles > 1 << 22) return reportf(TCCL_ERR_UNSUPPORTED, "%s: %lld tiles of the result", what, (long long)tiles);
-  a.xcds = cus % 8 ? 1 : 8, a.per_xcd = (int)((tiles + a.xcds - 1) / a.xcds), a.band = 4;
-  const dim3 wgs((unsigned)(a.xcds * a.per_xcd));
-  if (kmajor)
-    hipLaunchKernelGGL((gated_kernel<T, kTileOf, false, kBackward>), wgs, dim3(2 * kTileOf), 0, stream, a);
-  else
-    hipLaunchKernelGGL((gated_kernel<T, kTileOf, true, kBackward>), wgs, dim3(2 * kTileOf), 0, stream, a);
-  return launched(what);
+  // Tiles in rounds of what the device takes at a time: a step of 64 takes a large tile about 1.5 us, two small ones on a CU 1.0.
+  const int64_t large = (int64_t)((a.p.M + 255) / 256) * ((a.p.N + 127) / 128), small = (int64_t)((a.p.M + 127) / 128) * ((a.p.N + 63) / 64);
+  const double us_large = (double)((large + cus - 1) / cus) * 1.5, us_small = (double)((small + 2 * cus - 1) / (2 * cus)) * 1.0;
+  return us_large <= us_small ? launch_tile<T, 256, kBackward>(what, a, kmajor, cus, stream) : launch_tile<T, 128, kBackward>(what, a, kmajor, cus, stream);
 }
 
 }  // namespace

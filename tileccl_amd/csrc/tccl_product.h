@@ -69,10 +69,10 @@ struct Product {
     int64_t left;       // bytes from there to the end of what may be read
     int64_t step;       // bytes of a step
     uint32_t off[2][2];  // this lane's offsets
+    int kt;              // the step
   };
   struct Source {
     Side a, b;
-    int kt;
   };
 
   // Rows: `rows` of them are left from the tile's first on, K elements each.
@@ -120,8 +120,10 @@ struct Product {
     for (Side* side : {&s.a, &s.b}) {
       side->at += first * side->step;
       side->left -= first * side->step;
+      side->kt = first;
     }
-    s.kt = first;
+    mask<kADeep>(s.a);
+    mask<kBDeep>(s.b);
     return s;
   }
   static TCCL_D Words4 window(const char* at, int64_t bytes) {
@@ -147,12 +149,13 @@ struct Product {
   }
 #pragma clang diagnostic pop
   static constexpr uint32_t kDead = 0xfffffff0u;  // past the end of every window
-  // Half h of A, of B of the source's step into `stage`.
-  TCCL_D void issue_a(char* stage, const Source& s, int h) const {
+  // Half h of A, of B of the source's step into `stage`; behind half 1 the source is the next step's.
+  TCCL_D void issue_a(char* stage, Source& s, int h) const {
     char* to0 = stage + (kADeep ? (32 * h + 2 * wave * (1024 / kPitchA)) * kPitchA : row_of(wave, h, 0, true) * 128);
     copy_pair(to0, to0 + 1024, window(s.a.at, s.a.left), s.a.off[h][0], s.a.off[h][1]);
+    if (h) advance<kADeep>(s.a);
   }
-  TCCL_D void issue_b(char* stage, const Source& s, int h) const {
+  TCCL_D void issue_b(char* stage, Source& s, int h) const {
     char* to = stage + kOperand;
     if constexpr (kBDeep && kPaired) {
       to += (32 * h + wave * (1024 / kPitchB)) * kPitchB;
@@ -164,26 +167,24 @@ struct Product {
       to += row_of(wave, h, 0, false) * 128;
       copy_pair(to, to + 1024, window(s.b.at + (kPaired && h ? p.up : 0), s.b.left), s.b.off[h][0], s.b.off[h][1]);
     }
+    if (h) advance<kBDeep>(s.b);
   }
-  // Ahead of the loads of the source's step (steps come in ascending order): chunks at k >= K are dead from here on.
-  TCCL_D void mask(Source& s) const {
-    if ((kADeep && kBDeep) || (s.kt + 1) * kStepK <= p.K) return;
+  // Rows, ahead of a step's loads: chunks at k >= K are dead from here on.
+  template <bool kDeep>
+  TCCL_D void mask(Side& s) const {
+    if (kDeep || (s.kt + 1) * kStepK <= p.K) return;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int kc = (lane & 7) ^ ((4 * i + (lane >> 4)) & 7);
-      if (s.kt * kStepK + 8 * kc >= p.K)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (!kADeep) s.a.off[h][i] = kDead;
-          if (!kBDeep) s.b.off[h][i] = kDead;
-        }
+      if (s.kt * kStepK + 8 * kc >= p.K) s.off[0][i] = s.off[1][i] = kDead;
     }
   }
-  // Steps past the last one read zeros: nothing is left there (rows: all chunks are dead).
-  TCCL_D void advance(Source& s) const {
-    s.a.at += s.a.step, s.a.left -= s.a.step;
-    s.b.at += s.b.step, s.b.left -= s.b.step;
+  // Steps past the last one read zeros: deep, nothing is left there; rows, all chunks are dead.
+  template <bool kDeep>
+  TCCL_D void advance(Side& s) const {
+    s.at += s.step, s.left -= s.step;
     ++s.kt;
+    mask<kDeep>(s);
   }
 
   // ---- LDS -> operands ----------------------------------------------------------------------------
@@ -230,37 +231,137 @@ struct Product {
     asm volatile("" ::: "memory");
   }
 
+  template <int kLeft>
+  static TCCL_D void wait_loads() {  // until at most kLeft of this wavefront's loads are under way
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLeft) : "memory");
+  }
+
+  // The 256 tile.  A step is four phases; in each a wavefront first moves data (two loads, LDS reads) and then multiplies (16 MFMAs,
+  // 256 clocks), with a barrier behind either, and wavefronts 4 .. 7 run one such slot behind wavefronts 0 .. 3: of a SIMD's two
+  // wavefronts one multiplies while the other moves data.  Either stage is refilled in quarters, as soon as both sides have read one
+  // (its last phase, and a phase more), and the waits on loads are counted.
+  struct Running {
+    Vec a[4], b[2][4];
+  };
+  TCCL_D void multiply(Sums& acc, const Running& f, int first, int kh) const {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[first + i][j] = Mfma<T>::run16(f.b[kh][j], f.a[i], acc[first + i][j]);
+    __builtin_amdgcn_s_setprio(0);
+    barrier();
+  }
+  TCCL_D void read_a(Running& f, const char* stage, int kh, int first) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.a[i] = operand_a(stage, kh, first + i);
+  }
+  TCCL_D void read_b(Running& f, const char* stage, int kh) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f.b[kh][j] = operand_b(stage, kh, j);
+  }
+  // A by rows: phases are upper rows of the wavefront with k block 0, 1, lower rows with 0, 1.
+  //                last read in phase    refilled, with step t + 2, in
+  //   B, halves    1                     3, and 0 of the next step
+  //   A, upper     1                     1 of the next step
+  //   A, lower     3                     2 of the next step
+  // Both deep: k block 0 with upper rows, lower, k block 1 with lower, upper.  Halves are k blocks.
+  //   B, block 0   0                     2
+  //   A, block 0   1                     3
+  //   B, block 1   2                     0 of the next step
+  //   A, block 1   3                     1 of the next step
+  TCCL_D void phases(char* cur, char* nxt, Source& s, Sums& acc, Running& f) const {
+    if constexpr (kADeep) {
+      issue_b(nxt, s, 1);
+      read_b(f, cur, 0);
+      read_a(f, cur, 0, 0);
+      multiply(acc, f, 0, 0);
+      issue_a(nxt, s, 1);
+      read_a(f, cur, 0, 4);
+      wait_loads<8>();  // block 1 of this step; behind it: block 0 of the next, which is not waited for, and block 1 of the next
+      multiply(acc, f, 4, 0);
+      issue_b(cur, s, 0);
+      read_b(f, cur, 1);
+      read_a(f, cur, 1, 4);
+      multiply(acc, f, 4, 1);
+      issue_a(cur, s, 0);
+      read_a(f, cur, 1, 0);
+      wait_loads<8>();  // block 0 of the next step
+      multiply(acc, f, 0, 1);
+    } else {
+      issue_b(nxt, s, 1);
+      read_b(f, cur, 0);
+      read_a(f, cur, 0, 0);
+      multiply(acc, f, 0, 0);
+      issue_a(nxt, s, 0);
+      read_b(f, cur, 1);
+      read_a(f, cur, 1, 0);
+      wait_loads<6>();  // lower rows of this step
+      multiply(acc, f, 0, 1);
+      issue_a(nxt, s, 1);
+      read_a(f, cur, 0, 4);
+      multiply(acc, f, 4, 0);
+      issue_b(cur, s, 0);
+      read_a(f, cur, 1, 4);
+      wait_loads<4>();  // B and upper rows of the next step
+      multiply(acc, f, 4, 1);
+    }
+  }
+
   // Lane l has row l % 16 of a block and columns 4 (l / 16) .. + 3 of it.  Steps first .. first + steps - 1; behind them nothing is under
   // way and everybody has left the stages.
   TCCL_D void run(Sums& acc, int m0, int n0, int first, int steps) const {
     Source s = source(m0, n0, first);
-    mask(s);
-    auto load = [&](char* stage) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        issue_a(stage, s, h);
-        issue_b(stage, s, h);
+    if constexpr (kTile == 256) {
+      char* next = lds + kStage;
+      issue_b(lds, s, 0);
+      if constexpr (kADeep) {
+        issue_a(lds, s, 0);
+        issue_b(lds, s, 1);
+        issue_a(lds, s, 1);
+        issue_b(next, s, 0);
+        issue_a(next, s, 0);
+        wait_loads<8>();
+      } else {
+        issue_b(lds, s, 1);
+        issue_a(lds, s, 0);
+        issue_a(lds, s, 1);
+        issue_b(next, s, 0);
+        wait_loads<4>();
       }
-      advance(s);
-      mask(s);
-    };
-    load(lds);
-    for (int t = 0; t < steps; ++t) {
-      const char* cur = lds + (t & 1) * kStage;
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       barrier();
-      if (t + 1 < steps) load(lds + ((t + 1) & 1) * kStage);
+      Running f;
+      if (wave >= 4) barrier();  // one slot behind
+      for (int t = 0; t < steps; ++t) phases(lds + (t & 1) * kStage, lds + ((t + 1) & 1) * kStage, s, acc, f);
+      if (wave < 4) barrier();
+    } else {
+      auto load = [&](char* stage) {
+        issue_a(stage, s, 0);
+        issue_b(stage, s, 0);
+        issue_a(stage, s, 1);
+        issue_b(stage, s, 1);
+      };
+      load(lds);
+      for (int t = 0; t < steps; ++t) {
+        const char* cur = lds + (t & 1) * kStage;
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        barrier();
+        if (t + 1 < steps) load(lds + ((t + 1) & 1) * kStage);
 #pragma unroll
-      for (int kh = 0; kh < 2; ++kh) {
-        Vec a[kBlocksM], b[kBlocksN];
+        for (int kh = 0; kh < 2; ++kh) {
+          Vec a[kBlocksM], b[kBlocksN];
 #pragma unroll
-        for (int j = 0; j < kBlocksN; ++j) b[j] = operand_b(cur, kh, j);
+          for (int j = 0; j < kBlocksN; ++j) b[j] = operand_b(cur, kh, j);
 #pragma unroll
-        for (int i = 0; i < kBlocksM; ++i) a[i] = operand_a(cur, kh, i);
+          for (int i = 0; i < kBlocksM; ++i) a[i] = operand_a(cur, kh, i);
 #pragma unroll
-        for (int i = 0; i < kBlocksM; ++i)
+          for (int i = 0; i < kBlocksM; ++i)
 #pragma unroll
-          for (int j = 0; j < kBlocksN; ++j) acc[i][j] = Mfma<T>::run16(b[j], a[i], acc[i][j]);
+            for (int j = 0; j < kBlocksN; ++j) acc[i][j] = Mfma<T>::run16(b[j], a[i], acc[i][j]);
+        }
       }
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");

@@ -105,19 +105,30 @@ int size_of(int dtype) { return dtype == TCCL_F32 ? 4 : dtype == TCCL_F16 || dty
 
 // ---- from an input in full ----
 
-Cut full_cut_of(int splits, int rows, int cols, int outputs) { return cut_of(kSmall, splits, rows, cols, outputs); }
-
 Cut choose_full(int rows, int cols, int outputs, int cus) {
-  const Cut whole = full_cut_of(1, rows, cols, outputs);
-  const int64_t tiles = (int64_t)whole.tiles_h * whole.tiles_n;
-  int splits = 1;
-  while (tiles * splits < cus && splits < 32 && whole.steps >= 8 * splits) splits *= 2;
-  return full_cut_of(splits, rows, cols, outputs);
+  Cut best = {};
+  double least = 0;
+  for (const Kind kind : {kLarge, kSmall})
+    for (const int splits : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+      if (splits > 1 && (rows + 63) / 64 < 2 * splits) break;
+      const Cut c = cut_of(kind, splits, rows, cols, outputs);
+      const int64_t wgs = (int64_t)c.tiles_h * c.tiles_n * c.splits;
+      const double out_mb = 4e-6 * cols * outputs;
+      double us = 5.0 + out_mb / 5.0;
+      us += kind == kLarge ? (wgs + cus - 1) / cus * 1.5 * c.steps_per_split : (wgs + 2 * cus - 1) / (2 * cus) * 1.0 * c.steps_per_split;
+      if (c.splits > 1) us += 3.5 + 2.0 * c.splits * out_mb / 5.0;
+      if (!best.tiles_h || us < least) best = c, least = us;
+    }
+  return best;
 }
 
 template <typename T, typename OutT>
-int launch_full(const WeightFullArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL((weight_full_kernel<T, OutT, 128>), dim3((unsigned)(a.xcds * a.per_xcd)), dim3(256), 0, stream, a);
+int launch_full(const WeightFullArgs& a, bool large, hipStream_t stream) {
+  const dim3 grid((unsigned)(a.xcds * a.per_xcd));
+  if (large)
+    hipLaunchKernelGGL((weight_full_kernel<T, OutT, 256>), grid, dim3(512), 0, stream, a);
+  else
+    hipLaunchKernelGGL((weight_full_kernel<T, OutT, 128>), grid, dim3(256), 0, stream, a);
   const int rc = launched("weight_gradient_full");
   if (rc || a.splits == 1) return rc;
   WeightSumArgs s;
@@ -188,8 +199,9 @@ int tccl_weight_gradient_full(const tccl_weight_gradient_full_desc* d, void* str
       return reportf(TCCL_ERR_INVALID, "%s: the workspace has %lld bytes, %lld on 16 are needed", what, (long long)d->workspace_bytes, (long long)need);
   }
   const hipStream_t st = (hipStream_t)stream;
-  if (d->dtype == TCCL_BF16) return d->out_dtype == TCCL_F32 ? launch_full<__bf16, float>(a, st) : launch_full<__bf16, __bf16>(a, st);
-  return d->out_dtype == TCCL_F32 ? launch_full<_Float16, float>(a, st) : launch_full<_Float16, _Float16>(a, st);
+  const bool large = c.kind == kLarge;
+  if (d->dtype == TCCL_BF16) return d->out_dtype == TCCL_F32 ? launch_full<__bf16, float>(a, large, st) : launch_full<__bf16, __bf16>(a, large, st);
+  return d->out_dtype == TCCL_F32 ? launch_full<_Float16, float>(a, large, st) : launch_full<_Float16, _Float16>(a, large, st);
 }
 
 int64_t tccl_weight_gradient_workspace(int32_t rows, int32_t cols, int32_t outputs) {
