@@ -38,6 +38,9 @@ FORWARD = [
     (33, 200, 64, F16, "kn", "gelu"), (64, 64, 136, BF16, "nk", "silu"), (65, 1000, 64, BF16, "kn", "silu"), (127, 256, 200, F16, "nk", "gelu_tanh"),
     (129, 72, 72, BF16, "kn", "gelu"), (128, 192, 128, F16, "nk", "silu"), (256, 640, 136, BF16, "nk", "silu"), (300, 328, 264, BF16, "kn", "relu"),
     (511, 64, 520, F16, "kn", "silu"), (520, 520, 392, BF16, "nk", "gelu"), (1024, 128, 1024, F16, "nk", "silu"), (1100, 200, 1288, BF16, "kn", "silu"),
+    # few rows of many outputs
+    (3, 72, 8232, BF16, "kn", "silu"), (16, 1000, 8200, BF16, "nk", "gelu"), (20, 136, 8192, F16, "nk", "silu"), (31, 520, 8200, F16, "kn", "relu"),
+    (40, 64, 8200, BF16, "kn", "gelu_tanh"), (64, 584, 8192, BF16, "nk", "silu"),
     # nothing divides: copies
     (5, 7, 3, BF16, "kn", "silu"), (70, 65, 129, F16, "nk", "gelu"), (257, 1001, 67, BF16, "kn", "gelu_tanh"), (100, 96, 101, F16, "kn", "silu"),
 ]

@@ -105,7 +105,7 @@ template <typename T, int kTile, bool kBDeep, bool kBackward>
 struct Gated : Product<T, kTile, false, kBDeep, true> {
   typedef Product<T, kTile, false, kBDeep, true> Base;
   typedef T Quad __attribute__((ext_vector_type(4)));
-  static constexpr int kWidth = kTile / 2, kThreads = Base::kWaves * 64;
+  static constexpr int kWidth = kTile / 2, kThreads = 512;
   static constexpr int kChunks = kWidth / 8, kMatrix = kTile * kWidth * 2;  // chunks of a row, bytes of a matrix
   const GatedArgs& g;
   TCCL_D Gated(const GatedArgs& args, char* mem) : Base(args.p, mem), g(args) {}
@@ -113,7 +113,7 @@ struct Gated : Product<T, kTile, false, kBDeep, true> {
   static TCCL_D char* place(char* matrix, int row, int chunk) { return matrix + row * (kWidth * 2) + ((chunk ^ (row & (kChunks < 16 ? kChunks - 1 : 15))) << 4); }
   // This lane's four columns of block column j (0, 1) of block row i.
   TCCL_D char* mine(char* matrix, int i, int j) const {
-    const int row = this->wm * (kTile / 2) + 16 * i + (this->lane & 15), col = this->wn * 32 + 16 * j + 4 * (this->lane >> 4);
+    const int row = this->out_row(i), col = this->wn * 32 + 16 * j + 4 * (this->lane >> 4);
     return place(matrix, row, col >> 3) + (col & 4) * 2;
   }
   static TCCL_D Quad rounded(f32x4 v) { return (Quad){(T)v[0], (T)v[1], (T)v[2], (T)v[3]}; }
@@ -145,7 +145,7 @@ struct Gated : Product<T, kTile, false, kBDeep, true> {
       enter(first, g.grad, g.ld_grad, m0, n0, cols);
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < Base::kBlocksM; ++i)
+      for (int i = 0; i < Base::kRows; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const Quad dh = *(const Quad*)mine(first, i, j);
@@ -166,7 +166,7 @@ struct Gated : Product<T, kTile, false, kBDeep, true> {
     } else {
       if (g.kept) {
 #pragma unroll
-        for (int i = 0; i < Base::kBlocksM; ++i)
+        for (int i = 0; i < Base::kRows; ++i)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             *(Quad*)mine(first, i, j) = rounded(acc[i][j]);
@@ -178,7 +178,7 @@ struct Gated : Product<T, kTile, false, kBDeep, true> {
         __syncthreads();
       }
 #pragma unroll
-      for (int i = 0; i < Base::kBlocksM; ++i)
+      for (int i = 0; i < Base::kRows; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           f32x4 h;
@@ -196,7 +196,7 @@ struct Gated : Product<T, kTile, false, kBDeep, true> {
 };
 
 template <typename T, int kTile, bool kBDeep, bool kBackward>
-__global__ __launch_bounds__(2 * kTile, 2) void gated_kernel(GatedArgs a) {
+__global__ __launch_bounds__(512, 2) void gated_kernel(GatedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef Gated<T, kTile, kBDeep, kBackward> Tile;
   __shared__ __attribute__((aligned(1024))) char gated_lds[Tile::kLds];
@@ -205,6 +205,192 @@ __global__ __launch_bounds__(2 * kTile, 2) void gated_kernel(GatedArgs a) {
   if (id >= a.tiles_m * a.tiles_n) return;
   const TileCoord at = tile_coords(id, a.tiles_m, a.tiles_n, a.band);
   Tile(a, gated_lds).tile(at.m * kTile, at.n * (kTile / 2));
+#endif
+}
+
+// Few rows.  The weight is read once and nothing hides its latency but other loads, so a workgroup produces 16 kMB rows x
+// 8 kNB outputs (kNB / 2 blocks of 16 columns of either matrix) and its wavefronts share K: each takes every kWaves-th block of 64, requests
+// several ahead, turns one from load order to operand order through LDS of its own and adds it up by itself; there is no
+// barrier until the sums meet at the end.
+//
+// Loads have neighbouring lanes on neighbouring addresses.  x and a k-major weight: rows of 128 bytes, chunk c of row r in slot
+// c ^ ((r >> 1) & 7).  A weight by rows: of each k row 16 kNB bytes of either matrix, next to each other in LDS; its 32-byte units are permuted
+// (unit()) so that the rows that a transposing read touches at a time lie in different banks.
+template <typename T, int kMB, int kNB, int kWaves, bool kBDeep>
+struct GatedRows {
+  typedef typename Mfma<T>::Vec Vec;
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4 LdsQuad;
+  static constexpr int kBudget = (kNB == 8 ? 160 : 128) / ((kMB + kNB) * 8), kDepth = kBudget > 4 ? 4 : kBudget;  // blocks under way, within the registers there are
+  static constexpr int kWaveBytes = (kMB + kNB) * 2048, kSums = kMB * kNB * 256;              // sums of a wavefront
+  static constexpr int kLds = kWaves * kWaveBytes > (kWaves + 1) * kSums * 4 ? kWaves * kWaveBytes : (kWaves + 1) * kSums * 4;
+  static constexpr int kRowBytes = 32 * kNB, kRowLanes = kRowBytes / 16, kRowsPerLoad = 64 / kRowLanes;  // a k row of a weight by rows
+  static constexpr uint32_t kOutside = 0xffffff00u;
+  struct Block {
+    u32x4 x[2 * kMB], w[2 * kNB];
+  };
+
+  const GatedArgs& g;
+  char* lds;
+  const int lane, wave;
+  __amdgpu_buffer_rsrc_t rx, rw, ru;
+  uint32_t off_x, off_w, pitch_x, pitch_w;
+
+  TCCL_D GatedRows(const GatedArgs& args, char* mem) : g(args), lds(mem), lane((int)(threadIdx.x & 63)), wave(__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6))) {}
+  static TCCL_D __amdgpu_buffer_rsrc_t window(const char* at, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, bytes > 0xfffffff0ll ? 0xfffffff0u : (uint32_t)bytes, 0x00020000);
+  }
+
+  TCCL_D void load(Block& v, int kb) const {
+    const int k = g.p.K - kb * 64;  // what is left from this block on
+    const bool past = 8 * (lane & 7) >= k;
+#pragma unroll
+    for (int h = 0; h < 2 * kMB; ++h) v.x[h] = __builtin_amdgcn_raw_buffer_load_b128(rx, past ? kOutside : off_x + (uint32_t)(8 * h) * pitch_x + (uint32_t)kb * 128u, 0, 0);
+    if constexpr (kBDeep) {
+#pragma unroll
+      for (int h = 0; h < 2 * kNB; ++h) {
+        const bool none = off_w == kOutside || h * kRowsPerLoad + lane / kRowLanes >= k;
+        v.w[h] = __builtin_amdgcn_raw_buffer_load_b128(rw, none ? kOutside : off_w + (uint32_t)(kb * 64 + h * kRowsPerLoad) * pitch_w, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2 * kNB; ++h) {
+        const uint32_t o = off_w + (uint32_t)(8 * (h % kNB)) * pitch_w + (uint32_t)kb * 128u;
+        v.w[h] = __builtin_amdgcn_raw_buffer_load_b128(h < kNB ? rw : ru, past ? kOutside : o, 0, kStreaming);
+      }
+    }
+  }
+  static TCCL_D int unit(int u, int k) { return u ^ (kNB == 8 ? 2 * (k & 3) : kNB == 4 ? k & 2 : 0) ^ ((k >> 3) & 1); }
+  // A wavefront's LDS operations execute in the order issued; the fences keep the compiler to it.
+  TCCL_D void stage(const Block& v) const {
+    asm volatile("" ::: "memory");
+    char* at = lds + wave * kWaveBytes;
+#pragma unroll
+    for (int h = 0; h < 2 * kMB; ++h) {
+      const int r = 8 * h + (lane >> 3);
+      *(u32x4*)(at + r * 128 + (((lane & 7) ^ ((r >> 1) & 7)) << 4)) = v.x[h];
+    }
+    at += kMB * 2048;
+#pragma unroll
+    for (int h = 0; h < 2 * kNB; ++h) {
+      if constexpr (kBDeep) {
+        const int k = h * kRowsPerLoad + lane / kRowLanes, c = lane % kRowLanes;
+        *(u32x4*)(at + k * kRowBytes + (unit(c >> 1, k) << 5) + ((c & 1) << 4)) = v.w[h];
+      } else {
+        const int r = 8 * h + (lane >> 3);
+        *(u32x4*)(at + r * 128 + (((lane & 7) ^ ((r >> 1) & 7)) << 4)) = v.w[h];
+      }
+    }
+    asm volatile("" ::: "memory");
+  }
+  TCCL_D Vec by_row(int block, int kh) const {
+    const int i = lane & 15;
+    return *(const Vec*)(lds + wave * kWaveBytes + block * 2048 + i * 128 + (((4 * kh + (lane >> 4)) ^ ((i >> 1) & 7)) << 4));
+  }
+  TCCL_D Vec turned(int j, int kh) const {
+    const int i = lane & 15, t = i >> 2, cq = i & 3;
+    s16x4 half[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int k = 32 * kh + 8 * (lane >> 4) + 4 * q + t;
+      const char* p = lds + wave * kWaveBytes + kMB * 2048 + k * kRowBytes + (unit(j, k) << 5) + cq * 8;
+      half[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad*)p);
+    }
+    return __builtin_bit_cast(Vec, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  TCCL_D void multiply(f32x4 (&acc)[kMB][kNB]) const {
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh) {
+      Vec x[kMB], w[kNB];
+#pragma unroll
+      for (int j = 0; j < kNB; ++j) w[j] = kBDeep ? turned(j, kh) : by_row(kMB + j, kh);
+#pragma unroll
+      for (int i = 0; i < kMB; ++i) x[i] = by_row(i, kh);
+#pragma unroll
+      for (int i = 0; i < kMB; ++i)
+#pragma unroll
+        for (int j = 0; j < kNB; ++j) acc[i][j] = Mfma<T>::run16(w[j], x[i], acc[i][j]);
+    }
+  }
+
+  TCCL_D void tile(int m0, int n0) {
+    const ProductArgs& p = g.p;
+    const int left = p.N - n0;
+    pitch_x = (uint32_t)(p.lda * 2), pitch_w = (uint32_t)(p.ldb * 2);
+    rx = window(p.a + (int64_t)m0 * p.lda * 2, ((int64_t)(p.M - m0 - 1) * p.lda + (p.K + 7) / 8 * 8) * 2);
+    off_x = (uint32_t)(lane >> 3) * pitch_x + (uint32_t)(lane & 7) * 16u;
+    if constexpr (kBDeep) {
+      rw = window(p.b + (int64_t)n0 * 2, ((int64_t)(p.K - 1) * p.ldb + (left + 7) / 8 * 8) * 2 + p.up);
+      const int c = lane % kRowLanes;
+      off_w = 8 * (c % kNB) < left ? (uint32_t)(lane / kRowLanes) * pitch_w + (uint32_t)((c % kNB) * 16 + (c < kNB ? 0 : p.up)) : kOutside;
+    } else {
+      const int64_t bytes = ((int64_t)(left - 1) * p.ldb + (p.K + 7) / 8 * 8) * 2;
+      rw = window(p.b + (int64_t)n0 * p.ldb * 2, bytes);
+      ru = window(p.b + (int64_t)n0 * p.ldb * 2 + p.up, bytes);
+      off_w = (uint32_t)(lane >> 3) * pitch_w + (uint32_t)(lane & 7) * 16u;
+    }
+    f32x4 acc[kMB][kNB];
+#pragma unroll
+    for (int i = 0; i < kMB; ++i)
+#pragma unroll
+      for (int j = 0; j < kNB; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    const int blocks = (p.K + 63) / 64;
+    Block v[kDepth];
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d)
+      if (wave + d * kWaves < blocks) load(v[d], wave + d * kWaves);
+    for (int kb = wave; kb < blocks;) {
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d) {
+        if (kb < blocks) {
+          stage(v[d]);
+          if (kb + kDepth * kWaves < blocks) load(v[d], kb + kDepth * kWaves);  // the block is in LDS: its registers are free
+          multiply(acc);
+          kb += kWaves;
+        }
+      }
+    }
+    __syncthreads();
+    float* sums = (float*)lds;  // [wavefront][block][lane][4], then their sums
+#pragma unroll
+    for (int i = 0; i < kMB; ++i)
+#pragma unroll
+      for (int j = 0; j < kNB; ++j) *(f32x4*)(sums + wave * kSums + ((i * kNB + j) * 64 + lane) * 4) = acc[i][j];
+    __syncthreads();
+    float* total = sums + kWaves * kSums;
+    for (int u = (int)threadIdx.x; u < kSums; u += kWaves * 64) {
+      float s = sums[u];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) s += sums[w * kSums + u];
+      total[u] = s;
+    }
+    __syncthreads();
+    // Neighbouring threads take neighbouring columns of a row.
+    constexpr int kOut = 8 * kNB;
+    for (int u = (int)threadIdx.x; u < 16 * kMB * kOut; u += kWaves * 64) {
+      const int row = u / kOut, col = u % kOut;
+      if (m0 + row >= p.M || col >= left) continue;
+      const float* at = total + ((row / 16 * kNB + col / 16) * 64 + (col % 16 / 4) * 16 + row % 16) * 4 + col % 4;
+      const float z = at[0], y = at[kNB / 2 * 256];
+      float none;
+      ((T*)g.out)[(int64_t)(m0 + row) * g.ld_out + n0 + col] = to_out<T>(activated<false>(z, g.activation, none) * y);
+      if (g.kept) {
+        T* kept = (T*)g.kept + (int64_t)(m0 + row) * g.ld_kept + n0 + col;
+        kept[0] = to_out<T>(z), kept[p.N] = to_out<T>(y);
+      }
+    }
+  }
+};
+
+template <typename T, int kMB, int kNB, int kWaves, bool kBDeep>
+__global__ __launch_bounds__(kWaves * 64, kMB == 1 && kNB == 2 ? 4 : 2) void gated_rows_kernel(GatedArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef GatedRows<T, kMB, kNB, kWaves, kBDeep> Tile;
+  __shared__ __attribute__((aligned(1024))) char rows_lds[Tile::kLds];
+  // An XCD's workgroups have neighbouring columns: of a weight by rows they share lines.
+  const int id = (int)blockIdx.x % a.xcds * a.per_xcd + (int)blockIdx.x / a.xcds;
+  if (id >= a.tiles_m * a.tiles_n) return;
+  Tile(a, rows_lds).tile(id % a.tiles_m * (16 * kMB), id / a.tiles_m * (8 * kNB));
 #endif
 }
 

@@ -68,10 +68,46 @@ int launch_tile(const char* what, GatedArgs& a, bool kmajor, int cus, hipStream_
   a.xcds = cus % 8 ? 1 : 8, a.per_xcd = (int)((tiles + a.xcds - 1) / a.xcds), a.band = 4;
   const dim3 wgs((unsigned)(a.xcds * a.per_xcd));
   if (kmajor)
-    hipLaunchKernelGGL((gated_kernel<T, kTile, false, kBackward>), wgs, dim3(2 * kTile), 0, stream, a);
+    hipLaunchKernelGGL((gated_kernel<T, kTile, false, kBackward>), wgs, dim3(512), 0, stream, a);
   else
-    hipLaunchKernelGGL((gated_kernel<T, kTile, true, kBackward>), wgs, dim3(2 * kTile), 0, stream, a);
+    hipLaunchKernelGGL((gated_kernel<T, kTile, true, kBackward>), wgs, dim3(512), 0, stream, a);
   return launched(what);
+}
+
+template <typename T, int kMB, int kNB>
+int launch_rows(const char* what, GatedArgs& a, bool kmajor, int cus, hipStream_t stream) {
+  constexpr int kWaves = 8;
+  a.tiles_m = (a.p.M + 16 * kMB - 1) / (16 * kMB), a.tiles_n = (a.p.N + 8 * kNB - 1) / (8 * kNB);
+  a.xcds = cus % 8 ? 1 : 8, a.per_xcd = (a.tiles_m * a.tiles_n + a.xcds - 1) / a.xcds;
+  const dim3 wgs((unsigned)(a.xcds * a.per_xcd)), threads(64 * kWaves);
+  if (kmajor)
+    hipLaunchKernelGGL((gated_rows_kernel<T, kMB, kNB, kWaves, false>), wgs, threads, 0, stream, a);
+  else
+    hipLaunchKernelGGL((gated_rows_kernel<T, kMB, kNB, kWaves, true>), wgs, threads, 0, stream, a);
+  return launched(what);
+}
+
+// The kernel for few rows addresses a weight by rows from its first row on, in 32 bits.
+bool within_reach(const ProductArgs& p, bool kmajor) { return kmajor || ((int64_t)p.K * p.ldb + p.N) * 2 < 0xfffffff0ll; }
+
+// The kernels: 256 and 128 tiles, and those for few rows, 16 blocks_m x 8 blocks_n outputs a workgroup.
+struct Choice {
+  int tile;  // 0: for few rows
+  int blocks_m, blocks_n;
+};
+
+Choice choose(const ProductArgs& p, bool kmajor, bool backward, int cus) {
+  Choice c = {0, 0, 0};
+  if (!backward && p.M <= 64 && within_reach(p, kmajor)) {
+    c.blocks_m = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
+    c.blocks_n = !kmajor && c.blocks_m < 4 ? 8 : p.N / 32 >= cus ? 4 : 2;
+    return c;
+  }
+  // Tiles in rounds of what the device takes at a time: a step of 64 takes a large tile about 1.5 us, two small ones on a CU 1.0.
+  const int64_t large = (int64_t)((p.M + 255) / 256) * ((p.N + 127) / 128), small = (int64_t)((p.M + 127) / 128) * ((p.N + 63) / 64);
+  const double us_large = (double)((large + cus - 1) / cus) * 1.5, us_small = (double)((small + 2 * cus - 1) / (2 * cus)) * 1.0;
+  c.tile = us_large <= us_small ? 256 : 128;
+  return c;
 }
 
 template <typename T, bool kBackward>
@@ -79,10 +115,19 @@ int launch(const char* what, GatedArgs& a, bool kmajor, hipStream_t stream) {
   int cus = 0;
   const int rc = compute_units(&cus);
   if (rc) return rc;
-  // Tiles in rounds of what the device takes at a time: a step of 64 takes a large tile about 1.5 us, two small ones on a CU 1.0.
-  const int64_t large = (int64_t)((a.p.M + 255) / 256) * ((a.p.N + 127) / 128), small = (int64_t)((a.p.M + 127) / 128) * ((a.p.N + 63) / 64);
-  const double us_large = (double)((large + cus - 1) / cus) * 1.5, us_small = (double)((small + 2 * cus - 1) / (2 * cus)) * 1.0;
-  return us_large <= us_small ? launch_tile<T, 256, kBackward>(what, a, kmajor, cus, stream) : launch_tile<T, 128, kBackward>(what, a, kmajor, cus, stream);
+  const Choice c = choose(a.p, kmajor, kBackward, cus);
+  if constexpr (!kBackward)
+    if (!c.tile) switch (10 * c.blocks_m + c.blocks_n) {
+        case 12: return launch_rows<T, 1, 2>(what, a, kmajor, cus, stream);
+        case 14: return launch_rows<T, 1, 4>(what, a, kmajor, cus, stream);
+        case 18: return launch_rows<T, 1, 8>(what, a, kmajor, cus, stream);
+        case 22: return launch_rows<T, 2, 2>(what, a, kmajor, cus, stream);
+        case 24: return launch_rows<T, 2, 4>(what, a, kmajor, cus, stream);
+        case 28: return launch_rows<T, 2, 8>(what, a, kmajor, cus, stream);
+        case 42: return launch_rows<T, 4, 2>(what, a, kmajor, cus, stream);
+        default: return launch_rows<T, 4, 4>(what, a, kmajor, cus, stream);
+      }
+  return c.tile == 256 ? launch_tile<T, 256, kBackward>(what, a, kmajor, cus, stream) : launch_tile<T, 128, kBackward>(what, a, kmajor, cus, stream);
 }
 
 }  // namespace

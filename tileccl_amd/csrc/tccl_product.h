@@ -30,7 +30,9 @@ struct ProductArgs {
 
 #if defined(__HIPCC__)
 
-// kTile x kTile outputs by 2 x kTile / 64 wavefronts, each kTile / 2 x 64.
+// kTile x kTile outputs by 2 x kTile / 64 wavefronts, each kTile / 2 x 64.  A 128 tile has two such groups, each of which takes half of the
+// steps with stages of its own and ends up with half of the rows of blocks: half the steps one behind the other where tiles are few,
+// and no more tiles under way than CUs where they are many.
 template <typename T, int kTile, bool kADeep, bool kBDeep, bool kPaired>
 struct Product {
   typedef typename Mfma<T>::Vec Vec;
@@ -38,20 +40,26 @@ struct Product {
   typedef short s16x4 __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) s16x4 LdsQuad;
   typedef uint32_t Words4 __attribute__((ext_vector_type(4)));
-  static constexpr int kWavesN = kTile / 64, kWaves = 2 * kWavesN;
+  static constexpr int kWavesN = kTile / 64, kWaves = 2 * kWavesN, kGroups = 8 / kWaves;  // kWaves: of a group
   static constexpr int kStepK = 64;
   static constexpr int kOperand = kTile * 128;  // bytes of an operand in a stage
-  static constexpr int kStage = 2 * kOperand, kLds = 2 * kStage;
+  static constexpr int kStage = 2 * kOperand, kLds = kGroups * 2 * kStage;
   static constexpr int kBlocksM = kTile / 32, kBlocksN = 4;  // 16 x 16 blocks of a wavefront
+  static constexpr int kRows = kBlocksM / kGroups;           // rows of blocks that it ends up with
   static constexpr int kTileN = kPaired ? kTile / 2 : kTile;  // columns of either matrix
   static constexpr int kPitchA = 2 * kTile, kPitchB = 2 * kTileN;  // bytes of a deep operand's k row in a stage
 
   const ProductArgs& p;
-  char* lds;
-  const int lane, wave, wm, wn;
+  char *lds, *mine;  // of the workgroup, of the group
+  const int lane, group, wave, wm, wn;
 
   TCCL_D Product(const ProductArgs& args, char* mem)
-      : p(args), lds(mem), lane((int)(threadIdx.x & 63)), wave(__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6))), wm(wave / kWavesN), wn(wave % kWavesN) {}
+      : p(args), lds(mem), lane((int)(threadIdx.x & 63)), group(kGroups > 1 ? __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) / kWaves : 0),
+        wave(__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) % kWaves), wm(wave / kWavesN), wn(wave % kWavesN) {
+    mine = mem + group * 2 * kStage;
+  }
+  // Row of the tile, of this lane in row i of the blocks that the wavefront ends up with.
+  TCCL_D int out_row(int i) const { return wm * (kTile / 2) + 16 * (group * kRows + i) + (lane & 15); }
 
   // ---- global -> LDS ------------------------------------------------------------------------------
   // A step's operand is fetched in two halves of two pieces (1 KiB, one load) per wavefront.  Rows: half h of a 256 tile's A is rows
@@ -311,8 +319,8 @@ struct Product {
     }
   }
 
-  // Lane l has row l % 16 of a block and columns 4 (l / 16) .. + 3 of it.  Steps first .. first + steps - 1; behind them nothing is under
-  // way and everybody has left the stages.
+  // acc[0 .. kRows - 1] at the end: lane l has row out_row() and columns 4 (l / 16) .. + 3 of a block.  Steps first .. first + steps - 1; behind
+  // them nothing is under way and everybody has left the LDS.
   TCCL_D void run(Sums& acc, int m0, int n0, int first, int steps) const {
     Source s = source(m0, n0, first);
     if constexpr (kTile == 256) {
@@ -338,34 +346,58 @@ struct Product {
       for (int t = 0; t < steps; ++t) phases(lds + (t & 1) * kStage, lds + ((t + 1) & 1) * kStage, s, acc, f);
       if (wave < 4) barrier();
     } else {
+      const int turns = (steps + 1) / 2, own = group ? steps - turns : turns;
+      if (group) s = source(m0, n0, first + turns);
       auto load = [&](char* stage) {
         issue_a(stage, s, 0);
         issue_b(stage, s, 0);
         issue_a(stage, s, 1);
         issue_b(stage, s, 1);
       };
-      load(lds);
-      for (int t = 0; t < steps; ++t) {
-        const char* cur = lds + (t & 1) * kStage;
+      load(mine);
+      for (int t = 0; t < turns; ++t) {
+        const char* cur = mine + (t & 1) * kStage;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         barrier();
-        if (t + 1 < steps) load(lds + ((t + 1) & 1) * kStage);
+        if (t + 1 < turns) load(mine + ((t + 1) & 1) * kStage);
+        if (t < own) {
 #pragma unroll
-        for (int kh = 0; kh < 2; ++kh) {
-          Vec a[kBlocksM], b[kBlocksN];
+          for (int kh = 0; kh < 2; ++kh) {
+            Vec a[kBlocksM], b[kBlocksN];
 #pragma unroll
-          for (int j = 0; j < kBlocksN; ++j) b[j] = operand_b(cur, kh, j);
+            for (int j = 0; j < kBlocksN; ++j) b[j] = operand_b(cur, kh, j);
 #pragma unroll
-          for (int i = 0; i < kBlocksM; ++i) a[i] = operand_a(cur, kh, i);
+            for (int i = 0; i < kBlocksM; ++i) a[i] = operand_a(cur, kh, i);
 #pragma unroll
-          for (int i = 0; i < kBlocksM; ++i)
+            for (int i = 0; i < kBlocksM; ++i)
 #pragma unroll
-            for (int j = 0; j < kBlocksN; ++j) acc[i][j] = Mfma<T>::run16(b[j], a[i], acc[i][j]);
+              for (int j = 0; j < kBlocksN; ++j) acc[i][j] = Mfma<T>::run16(b[j], a[i], acc[i][j]);
+          }
         }
       }
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     barrier();
+    if constexpr (kGroups > 1) join(acc);
+  }
+
+  // Each group gives the other half of its rows of blocks away and ends up with the other half in acc[0 .. kRows - 1], group 0 with the first.
+  TCCL_D void join(Sums& acc) const {
+    constexpr int kHalf = kRows * kBlocksN;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+      for (int j = 0; j < kBlocksN; ++j)
+        *(f32x4*)(lds + (((group * kWaves + wave) * kHalf + i * kBlocksN + j) * 64 + lane) * 16) = group ? acc[i][j] : acc[kRows + i][j];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+      for (int j = 0; j < kBlocksN; ++j) {
+        const f32x4 other = *(const f32x4*)(lds + ((((1 - group) * kWaves + wave) * kHalf + i * kBlocksN + j) * 64 + lane) * 16);
+        acc[i][j] = group ? other + acc[kRows + i][j] : acc[i][j] + other;  // (group 0's half of the steps first)
+      }
+    __syncthreads();
   }
 };
 

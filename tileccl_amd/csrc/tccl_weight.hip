@@ -128,7 +128,7 @@ int launch_full(const WeightFullArgs& a, bool large, hipStream_t stream) {
   if (large)
     hipLaunchKernelGGL((weight_full_kernel<T, OutT, 256>), grid, dim3(512), 0, stream, a);
   else
-    hipLaunchKernelGGL((weight_full_kernel<T, OutT, 128>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((weight_full_kernel<T, OutT, 128>), grid, dim3(512), 0, stream, a);
   const int rc = launched("weight_gradient_full");
   if (rc || a.splits == 1) return rc;
   WeightSumArgs s;

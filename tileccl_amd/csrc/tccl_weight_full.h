@@ -23,7 +23,7 @@ struct WeightFullArgs {
 #if defined(__HIPCC__)
 
 template <typename T, typename OutT, int kTile>
-__global__ __launch_bounds__(2 * kTile, 2) void weight_full_kernel(WeightFullArgs a) {
+__global__ __launch_bounds__(512, 2) void weight_full_kernel(WeightFullArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef Product<T, kTile, true, true, false> Tile;
   __shared__ __attribute__((aligned(1024))) char full_lds[Tile::kLds];
@@ -38,12 +38,12 @@ __global__ __launch_bounds__(2 * kTile, 2) void weight_full_kernel(WeightFullArg
   typename Tile::Sums acc;
   Tile::clear(acc);
   if (steps > 0) t.run(acc, m0, n0, first, steps);  // (no tokens: a result of zeros, or of what is added)
-  const int i16 = t.lane & 15, g = t.lane >> 4;
+  const int g = t.lane >> 4;
 #pragma unroll
-  for (int i = 0; i < Tile::kBlocksM; ++i)
+  for (int i = 0; i < Tile::kRows; ++i)
 #pragma unroll
     for (int j = 0; j < Tile::kBlocksN; ++j) {
-      const int row = m0 + t.wm * (kTile / 2) + 16 * i + i16, col = n0 + t.wn * 64 + 16 * j + 4 * g;
+      const int row = m0 + t.out_row(i), col = n0 + t.wn * 64 + 16 * j + 4 * g;
       if (row < a.p.M && col < a.p.N) {
         if (a.splits > 1) {
           put4<float>(acc[i][j], (char*)(a.partial + (int64_t)split * a.p.M * a.ld_partial), row * a.ld_partial + col, a.p.N - col);
