@@ -607,8 +607,9 @@ int tccl_weight_gradient_cut(int32_t rows, int32_t cols, int32_t outputs, int32_
                              int32_t* steps_per_split);
 int tccl_weight_gradient(const tccl_weight_gradient_desc* wg, void* stream);
 
-/* The same from an input in full: x (rows x cols) of grad's type.  x's and grad's rows start on 16 bytes and are readable in whole
- * 16-byte vectors, past their last columns too (what lies there has no part in the result); pitches of at most 2^24 elements. */
+/* The same from an input in full: x (rows x cols) of grad's type; pitches of at most 2^24 elements.  An operand whose rows do not start on 16
+ * bytes is copied into the workspace first: device memory of tccl_weight_gradient_full_workspace() bytes on 16 bytes, which is what this
+ * very call takes (0: none; < 0: an error). */
 typedef struct tccl_weight_gradient_full_desc {
   const void* x;
   const void* grad;
@@ -622,18 +623,21 @@ typedef struct tccl_weight_gradient_full_desc {
   int32_t out_dtype;  /* add, out */
   int32_t transposed;
 } tccl_weight_gradient_full_desc;
-int64_t tccl_weight_gradient_full_workspace(int32_t rows, int32_t cols, int32_t outputs);
+int64_t tccl_weight_gradient_full_workspace(const tccl_weight_gradient_full_desc* wg);
+/* Host view, as tccl_weight_gradient_cut: two groups of wavefronts share a tile of 128, none one of 256. */
+int tccl_weight_gradient_full_cut(int32_t rows, int32_t cols, int32_t outputs, int32_t compute_units, int32_t* edge, int32_t* splits, int32_t* steps_per_split);
 int tccl_weight_gradient_full(const tccl_weight_gradient_full_desc* wg, void* stream);
 
 /* Gated linear layer: z = x W = [g | u], out = act(g) * u, from a weight (inputs x 2 outputs) whose first half of columns is the
  * gate's.  Sums and activations are fp32, out and kept (z, rows x 2 outputs; NULL: not wanted) are rounded once.
  *   weight: kmajor 0: rows of 2 outputs, ld_weight apart; kmajor 1: 2 outputs rows of inputs (the layer holds it transposed).  `up`: elements
  *   from the gate's part to the other one's (kmajor 0: at least `outputs`; kmajor 1: at least outputs - 1 rows).
- *   x's and weight's rows start on 16 bytes (`up` is a multiple of 8) and are readable in whole 16-byte vectors; where inputs is no
- *   multiple of 8, x is 0 up to the next one (and a kmajor weight is).  Pitches of at most 2^22 elements.
  *   act: TCCL_SILU g / (1 + exp(-g)); TCCL_GELU g Phi(g), Phi the normal distribution; TCCL_GELU_TANH
  *   g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2; TCCL_RELU max(g, 0).
- * out and kept have any alignment of their type and share no memory with another operand. */
+ * Operands have any alignment of their type; out and kept share no memory with another operand.  `workspace`: device memory on 16 bytes of
+ * tccl_gated_workspace() bytes, which is what this very call takes (0: none; < 0: an error): sums of inputs that are split over workgroups, and
+ * copies of x and of a weight whose rows do not start on 16 bytes, whose `up` is no multiple of 8, or, where the inputs lie next to
+ * each other in it, whose inputs are not (a caller with few rows holds its weight in rows that need none). */
 enum { TCCL_SILU = 0, TCCL_GELU = 1, TCCL_GELU_TANH = 2, TCCL_RELU = 3 };
 #define TCCL_GATED_MAX_COLS 2097152
 typedef struct tccl_gated_desc {
@@ -641,12 +645,19 @@ typedef struct tccl_gated_desc {
   const void* weight;
   void* out;
   void* kept;
+  void* workspace;
+  int64_t workspace_bytes;
   int64_t ld_x, ld_weight, up, ld_out, ld_kept;
   int32_t rows, inputs, outputs;
   int32_t dtype;      /* F16 or BF16, of everything */
   int32_t activation;
   int32_t kmajor;
 } tccl_gated_desc;
+int64_t tccl_gated_workspace(const tccl_gated_desc* gated);
+/* Host view of how a device of `compute_units` cuts such a call (backward: tccl_gated_grad without kept): tiles of 256 or 128 (rows and
+ * columns of z; 0: the kernels for few rows), the rows and outputs of a workgroup's part, the splits of the inputs over workgroups. */
+int tccl_gated_cut(int32_t rows, int32_t inputs, int32_t outputs, int32_t kmajor, int32_t backward, int32_t compute_units, int32_t* tile, int32_t* tile_rows,
+                   int32_t* tile_outputs, int32_t* splits);
 int tccl_gated(const tccl_gated_desc* gated, void* stream);
 
 /* From the gradient of out (rows x outputs) that of z: inner = [grad * u * act'(g) | grad * act(g)] (rows x 2 outputs), act'(0) = 0 for
@@ -659,12 +670,15 @@ typedef struct tccl_gated_grad_desc {
   const void* x;
   const void* weight;
   void* inner;
+  void* workspace;         /* kept NULL: of tccl_gated_grad_workspace() bytes, as tccl_gated's */
+  int64_t workspace_bytes;
   int64_t ld_grad, ld_kept, ld_x, ld_weight, up, ld_inner;
   int32_t rows, inputs, outputs;
   int32_t dtype;
   int32_t activation;
   int32_t kmajor;
 } tccl_gated_grad_desc;
+int64_t tccl_gated_grad_workspace(const tccl_gated_grad_desc* gated);
 int tccl_gated_grad(const tccl_gated_grad_desc* gated, void* stream);
 
 /* AdamW over many tensors, in fp32: with g = grad * grad_scale,

@@ -94,15 +94,18 @@ def test_bad_gated_descriptors(lib):
     refused(forward(out=0x3001), "not aligned to its type")
     refused(forward(ld_out=100), "out has a pitch of 100 elements for 128 columns")
     refused(forward(kept=0x9000, ld_kept=255), "kept has a pitch of 255 elements for 256 columns")
-    refused(forward(x=0x1008), "on 16 bytes", un)
-    refused(forward(ld_x=68), "whole 16-byte vectors", un)
+    refused(forward(x=0x1001), "x is not aligned to its type")
     refused(forward(ld_x=8), "x has a pitch of 8")
-    refused(forward(ld_x=(1 << 22) + 8), f"at most {1 << 22}", un)
-    refused(forward(up=132), "lies 132 elements behind", un)
-    refused(forward(up=64), "lies 64 elements behind", un)
-    refused(forward(up=136), "lies 136 elements behind", un)  # past the row's pitch
-    refused(forward(kmajor=1, ld_weight=64, up=127 * 64), "lies 8128 elements behind", un)
+    refused(forward(up=64), "lies 64 elements behind")
+    refused(forward(up=136), "lies 136 elements behind")  # past the row's pitch
+    refused(forward(kmajor=1, ld_weight=64, up=127 * 64), "lies 8128 elements behind")
     refused(forward(kmajor=1, ld_weight=56, up=128 * 64), "pitch of 56")
+    for entry, desc in ((lib.tccl_gated_workspace, _lib.GatedDesc), (lib.tccl_gated_grad_workspace, _lib.GatedGradDesc),
+                        (lib.tccl_weight_gradient_full_workspace, _lib.WeightGradientFullDesc)):
+        assert entry(None) == -1 and "the descriptor is NULL" in _lib.last_error()
+        assert entry(C.byref(desc(rows=4, outputs=8))) == -1 and "must be positive" in _lib.last_error()
+    assert lib.tccl_gated_workspace(C.byref(_lib.GatedDesc(inputs=8, outputs=8, dtype=_lib.F16))) == 0  # no rows
+    assert lib.tccl_gated_grad_workspace(C.byref(_lib.GatedGradDesc(kept=0x1000, rows=8, inputs=8, outputs=8, dtype=_lib.F16))) == 0
     refused(backward(grad=None), "grad is NULL")
     refused(backward(inner=None), "inner is NULL")
     refused(backward(ld_kept=128), "kept has a pitch of 128")
@@ -122,13 +125,12 @@ def test_bad_weight_gradient_descriptors(lib):
     refused(call(out_dtype=_lib.F16), "grad's type or F32", un)
     refused(call(out=None), "out is NULL")
     refused(call(x=None), "x is NULL")
-    refused(call(ld_x=132), "whole 16-byte vectors", un)
+    refused(call(ld_x=(1 << 24) + 8), f"at most {1 << 24}", un)
     refused(call(ld_grad=56), "grad has a pitch of 56")
-    refused(call(grad=0x3004), "on 16 bytes", un)
+    refused(call(grad=0x3001), "grad is not aligned to its type")
     refused(call(ld_out=63), "pitch below its 64 columns")
     refused(call(transposed=1), "pitch below its 128 columns")
     refused(call(out=0x4002), "not aligned to its type")
-    assert lib.tccl_weight_gradient_full_workspace(8, 0, 8) == -1 and lib.tccl_weight_gradient_full_workspace(_lib.TRAINING_MAX_ROWS + 1, 8, 8) == -1
 
 
 def test_bad_adamw_descriptors(lib):
@@ -171,6 +173,29 @@ def test_bad_adamw_descriptors(lib):
     refused(moments(first_scales=None), "must be non-NULL")
     refused(moments(to_second=0x6004), "on 16 bytes", un)
     assert moments(blocks=0) == 0
+
+
+def gated_cut(lib, rows, inputs, outputs, kmajor=0, backward=0, cus=256):
+    got = [C.c_int32() for _ in range(4)]
+    assert lib.tccl_gated_cut(rows, inputs, outputs, kmajor, backward, cus, *map(C.byref, got)) == 0
+    return tuple(g.value for g in got)
+
+
+def test_how_calls_are_cut(lib):
+    """What the GPU tests' shapes are for, on 256 compute units: (tile, rows, outputs of a part, splits)."""
+    assert gated_cut(lib, 1, 4096, 8192, 1) == (0, 16, 32, 1) and gated_cut(lib, 13, 4096, 4096) == (0, 16, 64, 4)
+    assert gated_cut(lib, 20, 4096, 4096) == (0, 32, 64, 4) and gated_cut(lib, 40, 4096, 1024) == (0, 32, 64, 8)
+    assert gated_cut(lib, 40, 512, 512) == (0, 64, 16, 1) and gated_cut(lib, 64, 584, 8192, 1) == (0, 64, 32, 1)
+    assert gated_cut(lib, 8192, 4096, 8192, 1) == (256, 256, 128, 1) and gated_cut(lib, 1003, 1001, 1035)[0] == 128
+    assert gated_cut(lib, 1, 4096, 8192, 1, backward=1)[0] == 128  # no kernel for few rows there
+    for rows, inputs, outputs, layout in ((2100, 72, 2056, 0), (2056, 200, 2100, 1), (4096, 64, 1024, 0), (2049, 328, 2048, 1)):
+        assert gated_cut(lib, rows, inputs, outputs, layout)[0] in (128, 256)
+    got = [C.c_int32() for _ in range(3)]
+    for shape, want in (((128, 4200, 2056), 256), ((1000, 1000, 3088), 128)):
+        assert lib.tccl_weight_gradient_full_cut(*shape, 256, *map(C.byref, got)) == 0 and got[0].value == want
+    assert lib.tccl_weight_gradient_full_cut(16384, 1024, 512, 256, *map(C.byref, got)) == 0 and got[1].value == 8
+    refused(lib.tccl_gated_cut(8, 8, 8, 0, 0, 0, *[C.byref(C.c_int32()) for _ in range(4)]), "0 compute units")
+    refused(lib.tccl_weight_gradient_full_cut(8, 8, 8, 256, None, None, None), "NULL result")
 
 
 @pytest.mark.skipif(shutil.which("gcc") is None, reason="needs gcc")

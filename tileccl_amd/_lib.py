@@ -245,6 +245,8 @@ class GatedDesc(C.Structure):
         ("weight", C.c_void_p),
         ("out", C.c_void_p),
         ("kept", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
         ("ld_x", C.c_int64),
         ("ld_weight", C.c_int64),
         ("up", C.c_int64),
@@ -266,6 +268,8 @@ class GatedGradDesc(C.Structure):
         ("x", C.c_void_p),
         ("weight", C.c_void_p),
         ("inner", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
         ("ld_grad", C.c_int64),
         ("ld_kept", C.c_int64),
         ("ld_x", C.c_int64),
@@ -406,9 +410,13 @@ SIGNATURES = {
     "tccl_weight_gradient_workspace": (_i64, [_i32, _i32, _i32]),
     "tccl_weight_gradient_cut": (C.c_int, [_i32, _i32, _i32, _i32, _P(_i32), _P(_i32), _P(_i32), _P(_i32)]),
     "tccl_weight_gradient": (C.c_int, [_P(WeightGradientDesc), _vp]),
-    "tccl_weight_gradient_full_workspace": (_i64, [_i32, _i32, _i32]),
+    "tccl_weight_gradient_full_workspace": (_i64, [_P(WeightGradientFullDesc)]),
     "tccl_weight_gradient_full": (C.c_int, [_P(WeightGradientFullDesc), _vp]),
+    "tccl_weight_gradient_full_cut": (C.c_int, [_i32, _i32, _i32, _i32, _P(_i32), _P(_i32), _P(_i32)]),
+    "tccl_gated_workspace": (_i64, [_P(GatedDesc)]),
+    "tccl_gated_cut": (C.c_int, [_i32, _i32, _i32, _i32, _i32, _i32, _P(_i32), _P(_i32), _P(_i32), _P(_i32)]),
     "tccl_gated": (C.c_int, [_P(GatedDesc), _vp]),
+    "tccl_gated_grad_workspace": (_i64, [_P(GatedGradDesc)]),
     "tccl_gated_grad": (C.c_int, [_P(GatedGradDesc), _vp]),
     "tccl_adamw": (C.c_int, [_P(AdamwDesc), _vp]),
     "tccl_adamw_moments": (C.c_int, [_P(AdamwMomentsDesc), _vp]),

@@ -24,7 +24,7 @@ HOST_OUT = HERE.parent / "_host.so"
 HOST_SOURCES = [HERE / "tccl_host.cpp", HERE / "tccl_host_ops.cpp"]
 SOURCES = [HERE / "tccl_api.hip", HERE / "tccl_kmajor.hip", HERE / "tccl_stream.hip", HERE / "tccl_norm.hip", HERE / "tccl_weight.hip", HERE / "tccl_gated.hip", HERE / "tccl_adamw.hip"]
 HEADERS = [HERE / "tccl_device.h", HERE / "tccl_gemm.h", HERE / "tccl_gemm256.h", HERE / "tccl_kernels256.h", HERE / "tccl_comm.h", HERE / "tccl_bulk.h", HERE / "tccl_stream.h",
-           HERE / "tccl_staged.h", HERE / "tccl_probe.h", HERE / "tccl_host.h", HERE / "tccl_norm.h", HERE / "tccl_weight.h", HERE / "tccl_weight_full.h", HERE / "tccl_product.h", HERE / "tccl_gated.h", HERE / "tccl_adamw.h",
+           HERE / "tccl_staged.h", HERE / "tccl_probe.h", HERE / "tccl_host.h", HERE / "tccl_norm.h", HERE / "tccl_weight.h", HERE / "tccl_weight_full.h", HERE / "tccl_product.h", HERE / "tccl_copy.h", HERE / "tccl_gated.h", HERE / "tccl_adamw.h",
            HERE.parent.parent / "include" / "tileccl_hip.h"]
 
 FLAGS = [

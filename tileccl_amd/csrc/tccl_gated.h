@@ -22,6 +22,9 @@ struct GatedArgs {
   int activation;
   int tiles_m, tiles_n, band;
   int xcds, per_xcd;    // dies with an L2 of their own; tiles of one
+  // Few rows, K split over workgroups: blocks of 64 k in each split, and where their sums go: [split][row][2 N].
+  int splits, blocks_per_split;
+  float* partial;
 };
 
 struct GatedGradArgs {
@@ -68,35 +71,6 @@ TCCL_D float activated(float g, int activation, float& slope) {
   if (kSlope) slope = s + b * s * (1.f - s) * c * (1.f + 3.f * k * b * b);
   return g * s;
 }
-
-// Eight neighbouring elements of a row that may start anywhere; `left` (1 ..) of them exist.
-template <typename T>
-struct Eight {
-  typedef T Vec __attribute__((ext_vector_type(8)));
-  typedef T Anywhere __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-  typedef const Anywhere __attribute__((address_space(1))) From;
-  typedef Anywhere __attribute__((address_space(1))) To;
-  static TCCL_D Vec get(const char* base, int64_t at, int left) {
-    Vec v = {};
-    if (left >= 8) {
-      v = *(From*)((const T*)base + at);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < left) v[e] = ((const T*)base)[at + e];
-    }
-    return v;
-  }
-  static TCCL_D void put(char* base, int64_t at, int left, Vec v) {
-    if (left >= 8) {
-      *(To*)((T*)base + at) = v;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < left) ((T*)base)[at + e] = v[e];
-    }
-  }
-};
 
 // Results leave through LDS, whose rows are then stored whole: out of the accumulators a lane would store 8 bytes of 16 rows each.
 // Chunk c (8 elements) of row r of a kWidth wide matrix lies in slot c ^ (r % 16), or r % 8 where a row has 8 chunks: 16 rows that are
@@ -221,7 +195,7 @@ struct GatedRows {
   typedef typename Mfma<T>::Vec Vec;
   typedef short s16x4 __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) s16x4 LdsQuad;
-  static constexpr int kBudget = (kNB == 8 ? 160 : 128) / ((kMB + kNB) * 8), kDepth = kBudget > 4 ? 4 : kBudget;  // blocks under way, within the registers there are
+  static constexpr int kBudget = (kMB + kNB == 9 ? 160 : 128) / ((kMB + kNB) * 8), kDepth = kBudget > 4 ? 4 : kBudget;  // blocks under way, within the registers there are
   static constexpr int kWaveBytes = (kMB + kNB) * 2048, kSums = kMB * kNB * 256;              // sums of a wavefront
   static constexpr int kLds = kWaves * kWaveBytes > (kWaves + 1) * kSums * 4 ? kWaves * kWaveBytes : (kWaves + 1) * kSums * 4;
   static constexpr int kRowBytes = 32 * kNB, kRowLanes = kRowBytes / 16, kRowsPerLoad = 64 / kRowLanes;  // a k row of a weight by rows
@@ -250,7 +224,7 @@ struct GatedRows {
 #pragma unroll
       for (int h = 0; h < 2 * kNB; ++h) {
         const bool none = off_w == kOutside || h * kRowsPerLoad + lane / kRowLanes >= k;
-        v.w[h] = __builtin_amdgcn_raw_buffer_load_b128(rw, none ? kOutside : off_w + (uint32_t)(kb * 64 + h * kRowsPerLoad) * pitch_w, 0, 0);
+        v.w[h] = __builtin_amdgcn_raw_buffer_load_b128(rw, none ? kOutside : off_w + (uint32_t)(kb * 64 + h * kRowsPerLoad) * pitch_w, 0, kNB == 8 ? kStreaming : 0);
       }
     } else {
 #pragma unroll
@@ -313,7 +287,7 @@ struct GatedRows {
     }
   }
 
-  TCCL_D void tile(int m0, int n0) {
+  TCCL_D void tile(int m0, int n0, int split) {
     const ProductArgs& p = g.p;
     const int left = p.N - n0;
     pitch_x = (uint32_t)(p.lda * 2), pitch_w = (uint32_t)(p.ldb * 2);
@@ -334,12 +308,12 @@ struct GatedRows {
     for (int i = 0; i < kMB; ++i)
 #pragma unroll
       for (int j = 0; j < kNB; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    const int blocks = (p.K + 63) / 64;
+    const int first = split * g.blocks_per_split, all = (p.K + 63) / 64, blocks = first + g.blocks_per_split < all ? first + g.blocks_per_split : all;
     Block v[kDepth];
 #pragma unroll
     for (int d = 0; d < kDepth; ++d)
-      if (wave + d * kWaves < blocks) load(v[d], wave + d * kWaves);
-    for (int kb = wave; kb < blocks;) {
+      if (first + wave + d * kWaves < blocks) load(v[d], first + wave + d * kWaves);
+    for (int kb = first + wave; kb < blocks;) {
 #pragma unroll
       for (int d = 0; d < kDepth; ++d) {
         if (kb < blocks) {
@@ -372,6 +346,11 @@ struct GatedRows {
       if (m0 + row >= p.M || col >= left) continue;
       const float* at = total + ((row / 16 * kNB + col / 16) * 64 + (col % 16 / 4) * 16 + row % 16) * 4 + col % 4;
       const float z = at[0], y = at[kNB / 2 * 256];
+      if (g.splits > 1) {
+        float* to = g.partial + ((int64_t)split * p.M + m0 + row) * (2 * (int64_t)p.N) + n0 + col;
+        to[0] = z, to[p.N] = y;
+        continue;
+      }
       float none;
       ((T*)g.out)[(int64_t)(m0 + row) * g.ld_out + n0 + col] = to_out<T>(activated<false>(z, g.activation, none) * y);
       if (g.kept) {
@@ -387,10 +366,32 @@ __global__ __launch_bounds__(kWaves * 64, kMB == 1 && kNB == 2 ? 4 : 2) void gat
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef GatedRows<T, kMB, kNB, kWaves, kBDeep> Tile;
   __shared__ __attribute__((aligned(1024))) char rows_lds[Tile::kLds];
-  // An XCD's workgroups have neighbouring columns: of a weight by rows they share lines.
-  const int id = (int)blockIdx.x % a.xcds * a.per_xcd + (int)blockIdx.x / a.xcds;
-  if (id >= a.tiles_m * a.tiles_n) return;
-  Tile(a, rows_lds).tile(id % a.tiles_m * (16 * kMB), id / a.tiles_m * (8 * kNB));
+  // An XCD's workgroups have neighbouring columns of a split: of a weight by rows they share lines, and together read stretches of its rows
+  // that lie in all of the L2's channels (rows a power of two apart start in the same one).
+  const int id = (int)blockIdx.x % a.xcds * a.per_xcd + (int)blockIdx.x / a.xcds, tiles = a.tiles_m * a.tiles_n;
+  if (id >= tiles * a.splits) return;
+  const int split = id / tiles, t = id - split * tiles;
+  Tile(a, rows_lds).tile(t % a.tiles_m * (16 * kMB), t / a.tiles_m * (8 * kNB), split);
+#endif
+}
+
+// What the splits have summed, ascending, and from it what the layer gives.
+template <typename T>
+__global__ __launch_bounds__(256) void gated_join_kernel(GatedArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const int64_t n = a.p.N, slice = a.p.M * 2 * n;
+  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < a.p.M * n; u += (int64_t)gridDim.x * 256) {
+    const int64_t row = u / n, col = u - row * n;
+    const float* at = a.partial + row * 2 * n + col;
+    float z = at[0], y = at[n];
+    for (int split = 1; split < a.splits; ++split) z += at[split * slice], y += at[split * slice + n];
+    float none;
+    ((T*)a.out)[row * a.ld_out + col] = to_out<T>(activated<false>(z, a.activation, none) * y);
+    if (a.kept) {
+      T* kept = (T*)a.kept + row * a.ld_kept + col;
+      kept[0] = to_out<T>(z), kept[n] = to_out<T>(y);
+    }
+  }
 #endif
 }
 

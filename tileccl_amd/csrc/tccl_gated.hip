@@ -4,12 +4,14 @@
 #pragma GCC visibility push(default)
 #include "../../include/tileccl_hip.h"
 #pragma GCC visibility pop
+#include "tccl_copy.h"
 #include "tccl_gated.h"
-#include "tccl_host.h"
 
 namespace {
 
 using namespace tccl;
+
+constexpr int64_t kMostPitch = 1 << 22;  // of an operand that is read in place: a tile's offsets have 32 bits
 
 // What the forward and the backward descriptor have in common.
 struct Sizes {
@@ -26,8 +28,6 @@ int check_sizes(const char* what, const Sizes& s) {
   return 0;
 }
 
-int vectors(int n) { return (n + 7) / 8 * 8; }
-
 // A matrix that the elementwise parts touch: any alignment of its type, rows that do not overlap.
 int check_matrix(const char* what, const char* name, const void* at, int64_t ld, int rows, int cols) {
   if (!at) return reportf(TCCL_ERR_INVALID, "%s: %s is NULL", what, name);
@@ -35,29 +35,109 @@ int check_matrix(const char* what, const char* name, const void* at, int64_t ld,
   if (rows > 1 && ld < cols) return reportf(TCCL_ERR_INVALID, "%s: %s has a pitch of %lld elements for %d columns", what, name, (long long)ld, cols);
   return 0;
 }
-// An operand of the product: rows in whole 16-byte vectors, offsets within a tile in 32 bits.
-int check_operand(const char* what, const char* name, const void* at, int64_t ld, int64_t rows, int cols) {
-  if (!at) return reportf(TCCL_ERR_INVALID, "%s: %s is NULL", what, name);
-  if (rows > 1 && ld < cols) return reportf(TCCL_ERR_INVALID, "%s: %s has a pitch of %lld elements for %d columns", what, name, (long long)ld, cols);
-  if (((uintptr_t)at & 15) || (rows > 1 && (ld % 8 || ld < vectors(cols))))
-    return reportf(TCCL_ERR_UNSUPPORTED, "%s: %s's rows must lie on 16 bytes and be readable in whole 16-byte vectors (%d columns, pitch %lld)", what, name, cols, (long long)ld);
-  if (ld > 1 << 22) return reportf(TCCL_ERR_UNSUPPORTED, "%s: %s's pitch of %lld elements, at most %d", what, name, (long long)ld, 1 << 22);
+// x and weight of a product of s.rows > 0 rows, from copies where the kernels cannot read them in place: rows that do not start on 16 bytes, inputs or
+// halves of a weight that end within a vector.
+int set_product(const char* what, const Sizes& s, const void* x, int64_t ld_x, const void* weight, int64_t ld_weight, int64_t up, int kmajor, ProductArgs& p, Copies& copies) {
+  const int64_t weight_rows = kmajor ? s.outputs : s.inputs;
+  int rc = check_matrix(what, "x", x, ld_x, s.rows, s.inputs);
+  if (!rc) rc = check_matrix(what, "weight", weight, ld_weight, (int)weight_rows, kmajor ? s.inputs : s.outputs);
+  if (rc) return rc;
+  if (kmajor ? up < (s.outputs - 1) * ld_weight + s.inputs : up < s.outputs || (s.inputs > 1 && ld_weight < up + s.outputs))
+    return reportf(TCCL_ERR_INVALID, "%s: the second projection's weight lies %lld elements behind the first's (pitch %lld)", what, (long long)up, (long long)ld_weight);
+  const int64_t whole = vectors(s.inputs), width = vectors(s.outputs);
+  p.M = s.rows, p.N = s.outputs, p.K = s.inputs;
+  p.a = (const char*)x, p.lda = s.rows > 1 ? ld_x : whole;
+  if (!on_vectors(x, ld_x, s.rows) || s.inputs % 8 || ld_x > kMostPitch) p.a = copies.add(p.a, ld_x, s.rows, s.inputs, whole), p.lda = whole;
+  p.b = (const char*)weight, p.ldb = weight_rows > 1 ? ld_weight : kmajor ? whole : up + width;
+  if (kmajor && (!on_vectors(weight, ld_weight, 2) || s.inputs % 8 || up % 8 || ld_weight > kMostPitch)) {
+    p.b = copies.add((const char*)weight, ld_weight, s.outputs, s.inputs, whole);
+    const char* second = copies.add((const char*)weight + up * 2, ld_weight, s.outputs, s.inputs, whole);
+    up = (second - p.b) / 2, p.ldb = whole;
+  } else if (!kmajor && (!on_vectors(weight, ld_weight, weight_rows) || up % 8 || ld_weight > kMostPitch)) {
+    p.b = copies.add((const char*)weight, p.ldb, s.inputs, s.outputs, 2 * width);
+    copies.add((const char*)weight + up * 2, p.ldb, s.inputs, s.outputs, 2 * width, width);
+    up = width, p.ldb = 2 * width;
+  }
+  p.up = up * 2;
   return 0;
 }
 
-// x and weight of a product of s.rows > 0 rows.
-int set_product(const char* what, const Sizes& s, const void* x, int64_t ld_x, const void* weight, int64_t ld_weight, int64_t up, int kmajor, ProductArgs& p) {
-  int rc = check_operand(what, "x", x, ld_x, s.rows, s.inputs);
-  if (!rc) rc = kmajor ? check_operand(what, "weight", weight, ld_weight, s.outputs, s.inputs) : check_operand(what, "weight", weight, ld_weight, s.inputs, s.outputs);
-  if (rc) return rc;
-  if (up % 8 || (kmajor ? up < (s.outputs - 1) * ld_weight + s.inputs : up < s.outputs || (s.inputs > 1 && ld_weight < up + vectors(s.outputs))))
-    return reportf(TCCL_ERR_UNSUPPORTED, "%s: the second projection's weight lies %lld elements behind the first's (pitch %lld)", what, (long long)up, (long long)ld_weight);
-  p.a = (const char*)x, p.b = (const char*)weight;
-  p.lda = s.rows > 1 ? ld_x : vectors(s.inputs);
-  p.ldb = (kmajor ? s.outputs : s.inputs) > 1 ? ld_weight : kmajor ? vectors(s.inputs) : up + vectors(s.outputs);
-  p.up = up * 2;
-  p.M = s.rows, p.N = s.outputs, p.K = s.inputs;
-  return 0;
+// The kernels: 256 and 128 tiles, and those for few rows, 16 blocks_m x 8 blocks_n outputs a workgroup.
+struct Choice {
+  int tile;  // 0: for few rows
+  int blocks_m, blocks_n, splits;
+};
+constexpr int kRowsWaves = 8;
+
+// The kernel for few rows addresses a weight by rows from its first row on, in 32 bits.
+bool within_reach(int64_t inputs, int64_t outputs, int64_t ld_weight, bool kmajor) { return kmajor || (inputs * ld_weight + outputs) * 2 < 0xfffffff0ll; }
+
+// Microseconds of a product by tiles: see choose().
+double tiles_take(int tile, int64_t tiles, int steps, int cus) {
+  const double rounds = (double)((tiles + cus - 1) / cus), busy = tiles < cus ? (double)tiles / cus : 1.0;
+  return tile == 256 ? 6.0 + steps * rounds * (rounds > 1 ? 1.5 : 1.12 + 0.48 * busy) : 6.5 + (steps + 1) / 2 * rounds * (rounds > 1 ? 1.0 : 0.78 + 0.15 * busy);
+}
+
+Choice choose(int rows, int inputs, int outputs, bool kmajor, bool few, int cus) {
+  Choice c = {0, 0, 0, 1};
+  const int blocks = (inputs + 63) / 64;
+  if (few && rows <= 64) {
+    // A k-major weight is read in whole lines whatever the tile: as many workgroups as there are CUs, and a wider tile beyond that.  One by rows
+    // in tiles of whole lines, its inputs split until every CU has one; with few inputs, or rows that take two such tiles without a split, narrow
+    // tiles are level or better (64 k of either: 512 x 512 5.4 and 7.1 us, 40 x 4096 x 4160 30 and 32).
+    if (!kmajor && blocks >= 16) {
+      c.blocks_m = rows <= 16 ? 1 : 2, c.blocks_n = 8;
+      const int64_t tiles = (int64_t)((outputs + 63) / 64) * (rows <= 32 ? 1 : 2);
+      while (tiles * c.splits * 2 <= cus && blocks >= 2 * c.splits * kRowsWaves && c.splits < 16) c.splits *= 2;
+      if (rows <= 32 || (c.splits > 1 && blocks >= 64)) return c;
+      c.splits = 1;
+    }
+    c.blocks_m = !kmajor ? 4 : rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    c.blocks_n = outputs / 32 >= cus ? 4 : 2;
+    return c;
+  }
+  const int64_t large = (int64_t)((rows + 255) / 256) * ((outputs + 127) / 128), small = (int64_t)((rows + 127) / 128) * ((outputs + 63) / 64);
+  c.tile = 256;
+  double least = tiles_take(256, large, blocks, cus);
+  const double other = tiles_take(128, small, blocks, cus);
+  if (other < least) c.tile = 128, least = other;
+  if (few)
+    for (const int n : {2, 4}) {
+      const int64_t rounds = ((int64_t)((rows + 63) / 64) * ((outputs + 8 * n - 1) / (8 * n)) + cus - 1) / cus;
+      const double us = 4.0 + rounds * (n == 2 ? 1.6 + 1.45 * inputs / 512 : 2.2 + 2.3 * inputs / 512);
+      if (us < least) c.tile = 0, c.blocks_m = 4, c.blocks_n = n, least = us;
+    }
+  return c;
+}
+
+int64_t partial_floats(const Choice& c, int64_t rows, int64_t outputs) { return c.splits > 1 ? c.splits * rows * 2 * outputs : 0; }
+
+template <typename T, int kMB, int kNB, bool kBDeep>
+void launch_rows(GatedArgs& a, const Choice& c, int cus, hipStream_t stream) {
+  a.tiles_m = (a.p.M + 16 * kMB - 1) / (16 * kMB), a.tiles_n = (a.p.N + 8 * kNB - 1) / (8 * kNB);
+  a.xcds = cus % 8 ? 1 : 8, a.per_xcd = (a.tiles_m * a.tiles_n * c.splits + a.xcds - 1) / a.xcds;
+  hipLaunchKernelGGL((gated_rows_kernel<T, kMB, kNB, kRowsWaves, kBDeep>), dim3((unsigned)(a.xcds * a.per_xcd)), dim3(64 * kRowsWaves), 0, stream, a);
+}
+template <typename T>
+int launch_few(const char* what, GatedArgs& a, const Choice& c, bool kmajor, int cus, hipStream_t stream) {
+  const int blocks = (a.p.K + 63) / 64;
+  a.blocks_per_split = (blocks + c.splits - 1) / c.splits;
+  a.splits = c.splits;  // (a split may be left with nothing: it sums zeros)
+  switch (10 * c.blocks_m + c.blocks_n) {
+    case 18: launch_rows<T, 1, 8, true>(a, c, cus, stream); break;
+    case 28: launch_rows<T, 2, 8, true>(a, c, cus, stream); break;
+    case 12: launch_rows<T, 1, 2, false>(a, c, cus, stream); break;
+    case 14: launch_rows<T, 1, 4, false>(a, c, cus, stream); break;
+    case 22: launch_rows<T, 2, 2, false>(a, c, cus, stream); break;
+    case 24: launch_rows<T, 2, 4, false>(a, c, cus, stream); break;
+    case 42: kmajor ? launch_rows<T, 4, 2, false>(a, c, cus, stream) : launch_rows<T, 4, 2, true>(a, c, cus, stream); break;
+    default: kmajor ? launch_rows<T, 4, 4, false>(a, c, cus, stream) : launch_rows<T, 4, 4, true>(a, c, cus, stream); break;
+  }
+  const int rc = launched(what);
+  if (rc || c.splits == 1) return rc;
+  const int64_t wgs = ((int64_t)a.p.M * a.p.N + 255) / 256;
+  hipLaunchKernelGGL((gated_join_kernel<T>), dim3((unsigned)(wgs < 2048 ? wgs : 2048)), dim3(256), 0, stream, a);
+  return launched(what);
 }
 
 template <typename T, int kTile, bool kBackward>
@@ -74,65 +154,57 @@ int launch_tile(const char* what, GatedArgs& a, bool kmajor, int cus, hipStream_
   return launched(what);
 }
 
-template <typename T, int kMB, int kNB>
-int launch_rows(const char* what, GatedArgs& a, bool kmajor, int cus, hipStream_t stream) {
-  constexpr int kWaves = 8;
-  a.tiles_m = (a.p.M + 16 * kMB - 1) / (16 * kMB), a.tiles_n = (a.p.N + 8 * kNB - 1) / (8 * kNB);
-  a.xcds = cus % 8 ? 1 : 8, a.per_xcd = (a.tiles_m * a.tiles_n + a.xcds - 1) / a.xcds;
-  const dim3 wgs((unsigned)(a.xcds * a.per_xcd)), threads(64 * kWaves);
-  if (kmajor)
-    hipLaunchKernelGGL((gated_rows_kernel<T, kMB, kNB, kWaves, false>), wgs, threads, 0, stream, a);
-  else
-    hipLaunchKernelGGL((gated_rows_kernel<T, kMB, kNB, kWaves, true>), wgs, threads, 0, stream, a);
-  return launched(what);
-}
-
-// The kernel for few rows addresses a weight by rows from its first row on, in 32 bits.
-bool within_reach(const ProductArgs& p, bool kmajor) { return kmajor || ((int64_t)p.K * p.ldb + p.N) * 2 < 0xfffffff0ll; }
-
-// The kernels: 256 and 128 tiles, and those for few rows, 16 blocks_m x 8 blocks_n outputs a workgroup.
-struct Choice {
-  int tile;  // 0: for few rows
-  int blocks_m, blocks_n;
-};
-
-Choice choose(const ProductArgs& p, bool kmajor, bool backward, int cus) {
-  Choice c = {0, 0, 0};
-  if (!backward && p.M <= 64 && within_reach(p, kmajor)) {
-    c.blocks_m = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
-    c.blocks_n = !kmajor && c.blocks_m < 4 ? 8 : p.N / 32 >= cus ? 4 : 2;
-    return c;
-  }
-  // Tiles in rounds of what the device takes at a time: a step of 64 takes a large tile about 1.5 us, two small ones on a CU 1.0.
-  const int64_t large = (int64_t)((p.M + 255) / 256) * ((p.N + 127) / 128), small = (int64_t)((p.M + 127) / 128) * ((p.N + 63) / 64);
-  const double us_large = (double)((large + cus - 1) / cus) * 1.5, us_small = (double)((small + 2 * cus - 1) / (2 * cus)) * 1.0;
-  c.tile = us_large <= us_small ? 256 : 128;
-  return c;
-}
-
 template <typename T, bool kBackward>
-int launch(const char* what, GatedArgs& a, bool kmajor, hipStream_t stream) {
-  int cus = 0;
-  const int rc = compute_units(&cus);
-  if (rc) return rc;
-  const Choice c = choose(a.p, kmajor, kBackward, cus);
+int launch(const char* what, GatedArgs& a, const Choice& c, bool kmajor, int cus, hipStream_t stream) {
   if constexpr (!kBackward)
-    if (!c.tile) switch (10 * c.blocks_m + c.blocks_n) {
-        case 12: return launch_rows<T, 1, 2>(what, a, kmajor, cus, stream);
-        case 14: return launch_rows<T, 1, 4>(what, a, kmajor, cus, stream);
-        case 18: return launch_rows<T, 1, 8>(what, a, kmajor, cus, stream);
-        case 22: return launch_rows<T, 2, 2>(what, a, kmajor, cus, stream);
-        case 24: return launch_rows<T, 2, 4>(what, a, kmajor, cus, stream);
-        case 28: return launch_rows<T, 2, 8>(what, a, kmajor, cus, stream);
-        case 42: return launch_rows<T, 4, 2>(what, a, kmajor, cus, stream);
-        default: return launch_rows<T, 4, 4>(what, a, kmajor, cus, stream);
-      }
+    if (!c.tile) return launch_few<T>(what, a, c, kmajor, cus, stream);
   return c.tile == 256 ? launch_tile<T, 256, kBackward>(what, a, kmajor, cus, stream) : launch_tile<T, 128, kBackward>(what, a, kmajor, cus, stream);
 }
+
+// A product that is ready to be launched, and what it wants of the workspace: copies, then the sums of splits.
+struct Prepared {
+  GatedArgs a = {};
+  Choice c = {};
+  Copies copies;
+  int64_t bytes = 0;
+  int cus = 0;
+  explicit Prepared(void* workspace) : copies(workspace) {}
+
+  template <typename Desc>
+  int of(const char* what, const Sizes& s, const Desc* d, bool backward) {
+    int rc = set_product(what, s, d->x, d->ld_x, d->weight, d->ld_weight, d->up, d->kmajor, a.p, copies);
+    if (!rc) rc = compute_units(&cus);
+    if (rc) return rc;
+    c = choose(s.rows, s.inputs, s.outputs, d->kmajor, !backward && within_reach(s.inputs, s.outputs, a.p.ldb, d->kmajor), cus);
+    a.partial = (float*)(copies.at + copies.bytes);
+    bytes = copies.bytes + 4 * partial_floats(c, s.rows, s.outputs);
+    a.activation = s.activation;
+    return 0;
+  }
+  int enough(const char* what, const void* workspace, int64_t given) const {
+    if (!bytes || (workspace && !((uintptr_t)workspace & 15) && given >= bytes)) return 0;
+    return reportf(TCCL_ERR_INVALID, "%s: the workspace has %lld bytes, %lld on 16 are needed", what, (long long)given, (long long)bytes);
+  }
+  template <bool kBackward>
+  int send(const char* what, int dtype, bool kmajor, hipStream_t stream) {
+    const int rc = dtype == TCCL_BF16 ? copies.launch<__bf16>(what, stream) : copies.launch<_Float16>(what, stream);
+    if (rc) return rc;
+    return dtype == TCCL_BF16 ? launch<__bf16, kBackward>(what, a, c, kmajor, cus, stream) : launch<_Float16, kBackward>(what, a, c, kmajor, cus, stream);
+  }
+};
 
 }  // namespace
 
 extern "C" {
+
+int64_t tccl_gated_workspace(const tccl_gated_desc* d) {
+  const char* what = "gated_workspace";
+  if (!d) return reportf(TCCL_ERR_INVALID, "%s: the descriptor is NULL", what), -1;
+  const Sizes s = {d->rows, d->inputs, d->outputs, d->dtype, d->activation};
+  Prepared p(nullptr);
+  if (check_sizes(what, s) || (s.rows && p.of(what, s, d, false))) return -1;
+  return p.bytes;
+}
 
 int tccl_gated(const tccl_gated_desc* d, void* stream) {
   const char* what = "gated";
@@ -140,13 +212,34 @@ int tccl_gated(const tccl_gated_desc* d, void* stream) {
   const Sizes s = {d->rows, d->inputs, d->outputs, d->dtype, d->activation};
   int rc = check_sizes(what, s);
   if (rc || !s.rows) return rc;
-  GatedArgs a = {};
-  rc = set_product(what, s, d->x, d->ld_x, d->weight, d->ld_weight, d->up, d->kmajor, a.p);
-  if (!rc) rc = check_matrix(what, "out", d->out, d->ld_out, s.rows, s.outputs);
+  rc = check_matrix(what, "out", d->out, d->ld_out, s.rows, s.outputs);
   if (!rc && d->kept) rc = check_matrix(what, "kept", d->kept, d->ld_kept, s.rows, 2 * s.outputs);
+  Prepared p(d->workspace);
+  if (!rc) rc = p.of(what, s, d, false);
+  if (!rc) rc = p.enough(what, d->workspace, d->workspace_bytes);
   if (rc) return rc;
-  a.out = (char*)d->out, a.ld_out = d->ld_out, a.kept = (char*)d->kept, a.ld_kept = d->ld_kept, a.activation = d->activation;
-  return d->dtype == TCCL_BF16 ? launch<__bf16, false>(what, a, d->kmajor, (hipStream_t)stream) : launch<_Float16, false>(what, a, d->kmajor, (hipStream_t)stream);
+  p.a.out = (char*)d->out, p.a.ld_out = d->ld_out, p.a.kept = (char*)d->kept, p.a.ld_kept = d->ld_kept;
+  return p.send<false>(what, d->dtype, d->kmajor, (hipStream_t)stream);
+}
+
+int tccl_gated_cut(int32_t rows, int32_t inputs, int32_t outputs, int32_t kmajor, int32_t backward, int32_t compute_units, int32_t* tile, int32_t* tile_rows, int32_t* tile_outputs,
+                   int32_t* splits) {
+  const int rc = check_sizes("gated_cut", Sizes{rows, inputs, outputs, TCCL_BF16, TCCL_SILU});
+  if (rc) return rc;
+  if (compute_units < 1 || !tile || !tile_rows || !tile_outputs || !splits) return reportf(TCCL_ERR_INVALID, "gated_cut: %d compute units, or a NULL result", compute_units);
+  const Choice c = choose(rows, inputs, outputs, kmajor != 0, !backward, compute_units);
+  *tile = c.tile, *splits = c.splits;
+  *tile_rows = c.tile ? c.tile : 16 * c.blocks_m, *tile_outputs = c.tile ? c.tile / 2 : 8 * c.blocks_n;
+  return 0;
+}
+
+int64_t tccl_gated_grad_workspace(const tccl_gated_grad_desc* d) {
+  const char* what = "gated_grad_workspace";
+  if (!d) return reportf(TCCL_ERR_INVALID, "%s: the descriptor is NULL", what), -1;
+  const Sizes s = {d->rows, d->inputs, d->outputs, d->dtype, d->activation};
+  Prepared p(nullptr);
+  if (check_sizes(what, s) || (s.rows && !d->kept && p.of(what, s, d, true))) return -1;
+  return p.bytes;
 }
 
 int tccl_gated_grad(const tccl_gated_grad_desc* d, void* stream) {
@@ -160,11 +253,12 @@ int tccl_gated_grad(const tccl_gated_grad_desc* d, void* stream) {
   if (rc) return rc;
   const hipStream_t st = (hipStream_t)stream;
   if (!d->kept) {
-    GatedArgs a = {};
-    rc = set_product(what, s, d->x, d->ld_x, d->weight, d->ld_weight, d->up, d->kmajor, a.p);
+    Prepared p(d->workspace);
+    rc = p.of(what, s, d, true);
+    if (!rc) rc = p.enough(what, d->workspace, d->workspace_bytes);
     if (rc) return rc;
-    a.grad = (const char*)d->grad, a.ld_grad = d->ld_grad, a.inner = (char*)d->inner, a.ld_inner = d->ld_inner, a.activation = d->activation;
-    return d->dtype == TCCL_BF16 ? launch<__bf16, true>(what, a, d->kmajor, st) : launch<_Float16, true>(what, a, d->kmajor, st);
+    p.a.grad = (const char*)d->grad, p.a.ld_grad = d->ld_grad, p.a.inner = (char*)d->inner, p.a.ld_inner = d->ld_inner;
+    return p.send<true>(what, d->dtype, d->kmajor, st);
   }
   rc = check_matrix(what, "kept", d->kept, d->ld_kept, s.rows, 2 * s.outputs);
   if (rc) return rc;

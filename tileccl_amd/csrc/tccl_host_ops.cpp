@@ -39,8 +39,10 @@ int64_t (*entry_weight_workspace)(int32_t, int32_t, int32_t);
 // What bind_layers() is given.
 PyObject* gated_result;
 int (*entry_weight_full)(const tccl_weight_gradient_full_desc*, void*);
-int64_t (*entry_weight_full_workspace)(int32_t, int32_t, int32_t);
+int64_t (*entry_weight_full_workspace)(const tccl_weight_gradient_full_desc*);
 int (*entry_gated)(const tccl_gated_desc*, void*);
+int64_t (*entry_gated_workspace)(const tccl_gated_desc*);
+int64_t (*entry_gated_grad_workspace)(const tccl_gated_grad_desc*);
 int (*entry_gated_grad)(const tccl_gated_grad_desc*, void*);
 int (*entry_adamw)(const tccl_adamw_desc*, void*);
 int (*entry_moments)(const tccl_adamw_moments_desc*, void*);
@@ -436,8 +438,17 @@ bool on_device0(const at::Tensor& t) { return t.is_cuda() && t.device().index() 
 
 bool sixteen_bits(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
 
-// Rows as the product kernels read them: on 16 bytes, in whole vectors.
-bool vectored(const Matrix& m) { return !((uintptr_t)m.at % 16) && !(m.cols % 8) && (m.rows <= 1 || !(m.pitch % 8)) && m.pitch <= 1 << 22; }
+// The workspace that a call asks for; false: an error is set.
+template <typename Desc>
+bool with_workspace(Desc& d, int64_t (*entry)(const Desc*), const char* what, const at::Device& device, at::Tensor& workspace) {
+  d.workspace_bytes = entry(&d);
+  if (d.workspace_bytes < 0) return failed((int)TCCL_ERR_INVALID, what), false;
+  if (d.workspace_bytes) {
+    workspace = empty({d.workspace_bytes}, at::kByte, device);
+    d.workspace = workspace.data_ptr();
+  }
+  return true;
+}
 
 // A weight (inputs x 2 outputs) as its memory lies: by rows, or (k-major) as 2 outputs rows of inputs.
 struct GatedWeight {
@@ -462,10 +473,6 @@ struct GatedWeight {
     pitch = t->stride(1), up = outputs * pitch;
     return (inputs == 1 || t->stride(0) == 1) && pitch >= inputs;
   }
-  // What the kernels read without a copy.
-  bool vectored() const {
-    return !((uintptr_t)at % 16) && !(pitch % 8) && pitch <= 1 << 22 && (kmajor ? inputs % 8 == 0 : outputs % 8 == 0);
-  }
   bool clear_of(const Matrix& m) const {
     const char* end = at + ((kmajor ? 2 * outputs - 1 : inputs - 1) * pitch + (kmajor ? inputs : 2 * outputs)) * 2;
     return !(at < m.end() && m.at < end);
@@ -481,7 +488,7 @@ PyObject* gated_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!x.open(args[0]) || !on_device0(*x.t) || !w.open(args[1])) return none();
     const at::ScalarType type = x.t->scalar_type();
     const at::Device device = x.t->device();
-    if (type != w.t->scalar_type() || x.cols != w.inputs || (x.rows && (!vectored(x) || !w.vectored()))) return none();
+    if (type != w.t->scalar_type() || x.cols != w.inputs) return none();
     tccl_gated_desc d;
     memset(&d, 0, sizeof d);
     d.activation = (int32_t)PyLong_AsLong(args[2]);
@@ -503,6 +510,8 @@ PyObject* gated_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     d.x = x.at, d.weight = w.at, d.ld_x = x.pitch, d.ld_weight = w.pitch, d.up = w.up;
     d.rows = (int32_t)x.rows, d.inputs = (int32_t)w.inputs, d.outputs = (int32_t)w.outputs;
     d.dtype = code_of(type), d.kmajor = w.kmajor;
+    at::Tensor workspace;
+    if (!with_workspace(d, entry_gated_workspace, "tccl_gated", device, workspace)) return nullptr;
     void* stream;
     if (!stream_now(stream)) return nullptr;
     if (failed(entry_gated(&d, stream), "tccl_gated")) return nullptr;
@@ -528,7 +537,7 @@ PyObject* gated_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!sixteen_bits(type) || w.t->scalar_type() != type || grad.cols != w.outputs) return none();
     const bool computed = args[1] == Py_None;
     if (computed) {
-      if (!x.open(args[2]) || x.t->scalar_type() != type || x.t->device() != device || x.cols != w.inputs || x.rows != grad.rows || (x.rows && (!vectored(x) || !w.vectored()))) return none();
+      if (!x.open(args[2]) || x.t->scalar_type() != type || x.t->device() != device || x.cols != w.inputs || x.rows != grad.rows) return none();
     } else if (!kept.open(args[1]) || kept.rows != grad.rows || kept.cols != 2 * w.outputs || kept.t->scalar_type() != type || kept.t->device() != device) {
       return none();
     }
@@ -553,6 +562,8 @@ PyObject* gated_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       d.kept = kept.at, d.ld_kept = kept.pitch;
     d.rows = (int32_t)grad.rows, d.inputs = (int32_t)w.inputs, d.outputs = (int32_t)w.outputs;
     d.dtype = code_of(type), d.kmajor = w.kmajor;
+    at::Tensor workspace;
+    if (!with_workspace(d, entry_gated_grad_workspace, "tccl_gated_grad", device, workspace)) return nullptr;
     void* stream;
     if (!stream_now(stream)) return nullptr;
     if (failed(entry_gated_grad(&d, stream), "tccl_gated_grad")) return nullptr;
@@ -562,34 +573,31 @@ PyObject* gated_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
-// weight_gradient_full(x, grad, cols, outputs, transposed, out_dtype, add, out): cols and outputs as `outputs` of weight_gradient, of x
-// and of grad.
+// weight_gradient_full(x, grad, transposed, out_dtype, add, out)
 PyObject* weight_gradient_full(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  if (nargs != 8) return none();
+  if (nargs != 6) return none();
   return guarded([&]() -> PyObject* {
     Matrix x, grad, add, out;
     if (!x.open(args[0]) || !on_device0(*x.t) || !grad.open(args[1])) return none();
     const at::ScalarType type = grad.t->scalar_type();
     const at::Device device = grad.t->device();
     if (!sixteen_bits(type) || x.t->scalar_type() != type || x.t->device() != device || x.rows != grad.rows) return none();
-    for (const Matrix* m : {&x, &grad})
-      if (m->cols > 1 << 24 || (m->rows && (m->cols % 8 || (m->rows > 1 && (m->pitch % 8 || m->pitch > 1 << 24)) || (uintptr_t)m->at % 16))) return none();
-    const int64_t inputs = args[2] == Py_None ? x.cols : PyLong_AsLongLong(args[2]), outputs = args[3] == Py_None ? grad.cols : PyLong_AsLongLong(args[3]);
-    const int transposed = PyObject_IsTrue(args[4]);
+    if (x.cols > 1 << 24 || grad.cols > 1 << 24 || x.pitch > 1 << 24 || grad.pitch > 1 << 24) return none();
+    const int64_t inputs = x.cols, outputs = grad.cols;
+    const int transposed = PyObject_IsTrue(args[2]);
     if (PyErr_Occurred()) return nullptr;
-    if (inputs < 1 || inputs > x.cols || outputs < 1 || outputs > grad.cols) return none();
-    if (args[5] != f32 && args[5] != (type == at::kHalf ? f16 : bf16)) return none();
-    const at::ScalarType result = args[5] == f32 ? at::kFloat : type;
+    if (args[3] != f32 && args[3] != (type == at::kHalf ? f16 : bf16)) return none();
+    const at::ScalarType result = args[3] == f32 ? at::kFloat : type;
     const int64_t rows = transposed ? outputs : inputs, cols = transposed ? inputs : outputs;
     tccl_weight_gradient_full_desc d;
     memset(&d, 0, sizeof d);
-    if (args[6] != Py_None) {
-      if (!add.open(args[6]) || add.rows != rows || add.cols != cols || add.t->scalar_type() != result || add.t->device() != device) return none();
+    if (args[4] != Py_None) {
+      if (!add.open(args[4]) || add.rows != rows || add.cols != cols || add.t->scalar_type() != result || add.t->device() != device) return none();
       d.add = add.at, d.ld_add = add.pitch;
     }
     at::Tensor made;
-    if (args[7] != Py_None) {
-      if (!out.open(args[7]) || out.rows != rows || out.cols != cols || out.t->scalar_type() != result || out.t->device() != device || !out.apart(add) || !out.elsewhere(grad) || !out.elsewhere(x))
+    if (args[5] != Py_None) {
+      if (!out.open(args[5]) || out.rows != rows || out.cols != cols || out.t->scalar_type() != result || out.t->device() != device || !out.apart(add) || !out.elsewhere(grad) || !out.elsewhere(x))
         return none();
       d.out = out.at, d.ld_out = out.pitch;
     } else {
@@ -599,19 +607,14 @@ PyObject* weight_gradient_full(PyObject*, PyObject* const* args, Py_ssize_t narg
     d.x = x.at, d.ld_x = x.pitch, d.grad = grad.at, d.ld_grad = grad.pitch;
     d.rows = (int32_t)grad.rows, d.cols = (int32_t)inputs, d.outputs = (int32_t)outputs;
     d.dtype = code_of(type), d.out_dtype = code_of(result), d.transposed = transposed;
-    d.workspace_bytes = entry_weight_full_workspace(d.rows, d.cols, d.outputs);
-    if (d.workspace_bytes < 0) return failed((int)TCCL_ERR_INVALID, "tccl_weight_gradient_full"), nullptr;
     at::Tensor workspace;
-    if (d.workspace_bytes) {
-      workspace = empty({d.workspace_bytes}, at::kByte, device);
-      d.workspace = workspace.data_ptr();
-    }
+    if (!with_workspace(d, entry_weight_full_workspace, "tccl_weight_gradient_full", device, workspace)) return nullptr;
     void* stream;
     if (!stream_now(stream)) return nullptr;
     if (failed(entry_weight_full(&d, stream), "tccl_weight_gradient_full")) return nullptr;
     if (made.defined()) return THPVariable_Wrap(made);
-    Py_INCREF(args[7]);
-    return args[7];
+    Py_INCREF(args[5]);
+    return args[5];
   });
 }
 
@@ -739,8 +742,8 @@ PyObject* adamw_moments(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // bind_layers(GatedLinearResult, entries): the entry points in the order below.
 PyObject* bind_layers(PyObject*, PyObject* args) {
   PyObject* result;
-  unsigned long long e[6];
-  if (!PyArg_ParseTuple(args, "O(KKKKKK)", &result, e, e + 1, e + 2, e + 3, e + 4, e + 5)) return nullptr;
+  unsigned long long e[8];
+  if (!PyArg_ParseTuple(args, "O(KKKKKKKK)", &result, e, e + 1, e + 2, e + 3, e + 4, e + 5, e + 6, e + 7)) return nullptr;
   if (!PyType_Check(result) || !PyType_IsSubtype((PyTypeObject*)result, &PyTuple_Type)) {
     PyErr_SetString(PyExc_TypeError, "results are named tuples");
     return nullptr;
@@ -753,6 +756,8 @@ PyObject* bind_layers(PyObject*, PyObject* args) {
   entry_gated_grad = (decltype(entry_gated_grad))(uintptr_t)e[3];
   entry_adamw = (decltype(entry_adamw))(uintptr_t)e[4];
   entry_moments = (decltype(entry_moments))(uintptr_t)e[5];
+  entry_gated_workspace = (decltype(entry_gated_workspace))(uintptr_t)e[6];
+  entry_gated_grad_workspace = (decltype(entry_gated_grad_workspace))(uintptr_t)e[7];
   Py_RETURN_NONE;
 }
 

@@ -28,13 +28,53 @@ struct ProductArgs {
   int M, N, K;       // N: columns of either matrix of a paired B
 };
 
+// Up to three copies in one launch: operands whose rows start anywhere, into rows of whole 16-byte vectors, zero behind their columns.
+struct CopyArgs {
+  const char* from[3];
+  char* to[3];
+  int64_t ld_from[3], ld_to[3];  // elements
+  int64_t chunks[3];             // vectors of all copies up to and with this one
+  int cols[3], per_row[3];       // columns; vectors of a row
+  int n;
+};
+
 #if defined(__HIPCC__)
+
+// Eight neighbouring elements of a row that may start anywhere; `left` (1 ..) of them exist.
+template <typename T>
+struct Eight {
+  typedef T Vec __attribute__((ext_vector_type(8)));
+  typedef T Anywhere __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  typedef const Anywhere __attribute__((address_space(1))) From;
+  typedef Anywhere __attribute__((address_space(1))) To;
+  static TCCL_D Vec get(const char* base, int64_t at, int left) {
+    Vec v = {};
+    if (left >= 8) {
+      v = *(From*)((const T*)base + at);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < left) v[e] = ((const T*)base)[at + e];
+    }
+    return v;
+  }
+  static TCCL_D void put(char* base, int64_t at, int left, Vec v) {
+    if (left >= 8) {
+      *(To*)((T*)base + at) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < left) ((T*)base)[at + e] = v[e];
+    }
+  }
+};
 
 // kTile x kTile outputs by 2 x kTile / 64 wavefronts, each kTile / 2 x 64.  A 128 tile has two such groups, each of which takes half of the
 // steps with stages of its own and ends up with half of the rows of blocks: half the steps one behind the other where tiles are few,
 // and no more tiles under way than CUs where they are many.
 template <typename T, int kTile, bool kADeep, bool kBDeep, bool kPaired>
 struct Product {
+
   typedef typename Mfma<T>::Vec Vec;
   typedef __attribute__((address_space(3))) void LdsVoid;
   typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -125,14 +165,16 @@ struct Product {
       by_depth<false>(s.b, p.b + (int64_t)n0 * 2, p.ldb, p.N - n0);
     else
       by_rows<false>(s.b, p.b + (int64_t)n0 * p.ldb * 2, p.ldb, p.N - n0);
-    for (Side* side : {&s.a, &s.b}) {
-      side->at += first * side->step;
-      side->left -= first * side->step;
-      side->kt = first;
-    }
-    mask<kADeep>(s.a);
-    mask<kBDeep>(s.b);
+    start<kADeep>(s.a, first);
+    start<kBDeep>(s.b, first);
     return s;
+  }
+  template <bool kDeep>
+  TCCL_D void start(Side& s, int first) const {
+    s.at += first * s.step;
+    s.left -= first * s.step;
+    s.kt = first;
+    mask<kDeep>(s);
   }
   static TCCL_D Words4 window(const char* at, int64_t bytes) {
     const uint64_t a = (uint64_t)(uintptr_t)at;
@@ -267,16 +309,17 @@ struct Product {
 #pragma unroll
     for (int i = 0; i < 4; ++i) f.a[i] = operand_a(stage, kh, first + i);
   }
-  TCCL_D void read_b(Running& f, const char* stage, int kh) const {
+  TCCL_D void read_b(Running& f, const char* stage, int kh, int from = 0, int to = 4) const {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f.b[kh][j] = operand_b(stage, kh, j);
+    for (int j = from; j < to; ++j) f.b[kh][j] = operand_b(stage, kh, j);
   }
   // A by rows: phases are upper rows of the wavefront with k block 0, 1, lower rows with 0, 1.
   //                last read in phase    refilled, with step t + 2, in
   //   B, halves    1                     3, and 0 of the next step
   //   A, upper     1                     1 of the next step
   //   A, lower     3                     2 of the next step
-  // Both deep: k block 0 with upper rows, lower, k block 1 with lower, upper.  Halves are k blocks.
+  // Both deep: k block 0 with upper rows, lower, k block 1 with lower, upper.  Halves are k blocks.  Twelve of the
+  // transposing reads in each phase: half of a block of B is read in the phase ahead of its own.
   //   B, block 0   0                     2
   //   A, block 0   1                     3
   //   B, block 1   2                     0 of the next step
@@ -284,20 +327,24 @@ struct Product {
   TCCL_D void phases(char* cur, char* nxt, Source& s, Sums& acc, Running& f) const {
     if constexpr (kADeep) {
       issue_b(nxt, s, 1);
-      read_b(f, cur, 0);
+      read_b(f, cur, 0, 2, 4);
       read_a(f, cur, 0, 0);
+      wait_loads<8>();  // B, block 1 of this step
       multiply(acc, f, 0, 0);
       issue_a(nxt, s, 1);
       read_a(f, cur, 0, 4);
-      wait_loads<8>();  // block 1 of this step; behind it: block 0 of the next, which is not waited for, and block 1 of the next
+      read_b(f, cur, 1, 0, 2);
+      wait_loads<8>();  // A, block 1
       multiply(acc, f, 4, 0);
       issue_b(cur, s, 0);
-      read_b(f, cur, 1);
+      read_b(f, cur, 1, 2, 4);
       read_a(f, cur, 1, 4);
+      wait_loads<8>();  // B, block 0 of the next step
       multiply(acc, f, 4, 1);
       issue_a(cur, s, 0);
       read_a(f, cur, 1, 0);
-      wait_loads<8>();  // block 0 of the next step
+      read_b(f, nxt, 0, 0, 2);
+      wait_loads<8>();  // A, block 0
       multiply(acc, f, 0, 1);
     } else {
       issue_b(nxt, s, 1);
@@ -319,10 +366,29 @@ struct Product {
     }
   }
 
+  // The multiplying slot of a 128 tile.
+  TCCL_D void whole_step(Sums& acc, const char* cur) const {
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh) {
+      Vec a[kBlocksM], b[kBlocksN];
+#pragma unroll
+      for (int j = 0; j < kBlocksN; ++j) b[j] = operand_b(cur, kh, j);
+#pragma unroll
+      for (int i = 0; i < kBlocksM; ++i) a[i] = operand_a(cur, kh, i);
+#pragma unroll
+      for (int i = 0; i < kBlocksM; ++i)
+#pragma unroll
+        for (int j = 0; j < kBlocksN; ++j) acc[i][j] = Mfma<T>::run16(b[j], a[i], acc[i][j]);
+    }
+    __builtin_amdgcn_s_setprio(0);
+  }
+
   // acc[0 .. kRows - 1] at the end: lane l has row out_row() and columns 4 (l / 16) .. + 3 of a block.  Steps first .. first + steps - 1; behind
   // them nothing is under way and everybody has left the LDS.
   TCCL_D void run(Sums& acc, int m0, int n0, int first, int steps) const {
-    Source s = source(m0, n0, first);
+    const int turns = kGroups > 1 ? (steps + 1) / 2 : steps, own = group ? steps - turns : turns;
+    Source s = source(m0, n0, first + (group ? turns : 0));
     if constexpr (kTile == 256) {
       char* next = lds + kStage;
       issue_b(lds, s, 0);
@@ -342,12 +408,11 @@ struct Product {
       }
       barrier();
       Running f;
+      if constexpr (kADeep) read_b(f, lds, 0, 0, 2);
       if (wave >= 4) barrier();  // one slot behind
       for (int t = 0; t < steps; ++t) phases(lds + (t & 1) * kStage, lds + ((t + 1) & 1) * kStage, s, acc, f);
       if (wave < 4) barrier();
     } else {
-      const int turns = (steps + 1) / 2, own = group ? steps - turns : turns;
-      if (group) s = source(m0, n0, first + turns);
       auto load = [&](char* stage) {
         issue_a(stage, s, 0);
         issue_b(stage, s, 0);
@@ -355,26 +420,21 @@ struct Product {
         issue_b(stage, s, 1);
       };
       load(mine);
+      if (group) barrier();  // one slot behind
       for (int t = 0; t < turns; ++t) {
         const char* cur = mine + (t & 1) * kStage;
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        barrier();
-        if (t + 1 < turns) load(mine + ((t + 1) & 1) * kStage);
-        if (t < own) {
-#pragma unroll
-          for (int kh = 0; kh < 2; ++kh) {
-            Vec a[kBlocksM], b[kBlocksN];
-#pragma unroll
-            for (int j = 0; j < kBlocksN; ++j) b[j] = operand_b(cur, kh, j);
-#pragma unroll
-            for (int i = 0; i < kBlocksM; ++i) a[i] = operand_a(cur, kh, i);
-#pragma unroll
-            for (int i = 0; i < kBlocksM; ++i)
-#pragma unroll
-              for (int j = 0; j < kBlocksN; ++j) acc[i][j] = Mfma<T>::run16(b[j], a[i], acc[i][j]);
-          }
+        if (t + 1 < turns) {
+          load(mine + ((t + 1) & 1) * kStage);
+          wait_loads<8>();
+        } else {
+          wait_loads<0>();
         }
+        barrier();
+        if (t < own) whole_step(acc, cur);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        barrier();
       }
+      if (!group) barrier();
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     barrier();
@@ -387,19 +447,36 @@ struct Product {
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
 #pragma unroll
-      for (int j = 0; j < kBlocksN; ++j)
-        *(f32x4*)(lds + (((group * kWaves + wave) * kHalf + i * kBlocksN + j) * 64 + lane) * 16) = group ? acc[i][j] : acc[kRows + i][j];
+      for (int j = 0; j < kBlocksN; ++j) {
+        const f32x4 first = acc[i][j], second = acc[kRows + i][j];  // (values: a choice between places would need them in memory)
+        *(f32x4*)(lds + (((group * kWaves + wave) * kHalf + i * kBlocksN + j) * 64 + lane) * 16) = group ? first : second;
+      }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
 #pragma unroll
       for (int j = 0; j < kBlocksN; ++j) {
         const f32x4 other = *(const f32x4*)(lds + ((((1 - group) * kWaves + wave) * kHalf + i * kBlocksN + j) * 64 + lane) * 16);
-        acc[i][j] = group ? other + acc[kRows + i][j] : acc[i][j] + other;  // (group 0's half of the steps first)
+        const f32x4 first = acc[i][j] + other, second = other + acc[kRows + i][j];  // group 0's half of the steps first
+        acc[i][j] = group ? second : first;
       }
     __syncthreads();
   }
 };
+
+// A thread takes a vector: 16 bytes from anywhere, 16 bytes to a boundary.
+template <typename T>
+__global__ __launch_bounds__(256) void copy_rows_kernel(CopyArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < a.chunks[a.n - 1]; u += (int64_t)gridDim.x * 256) {
+    int which = 0;
+    while (u >= a.chunks[which]) ++which;
+    const int64_t at = which ? u - a.chunks[which - 1] : u, row = at / a.per_row[which];
+    const int col = (int)(at - row * a.per_row[which]) * 8;
+    *(typename Eight<T>::Vec*)(a.to[which] + (row * a.ld_to[which] + col) * 2) = Eight<T>::get(a.from[which], row * a.ld_from[which] + col, a.cols[which] - col);
+  }
+#endif
+}
 
 #endif  // __HIPCC__
 

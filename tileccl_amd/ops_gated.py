@@ -22,7 +22,7 @@ from typing import Any, NamedTuple, NoReturn
 import torch
 
 from tileccl_amd import _launch, _lib, ops_training
-from tileccl_amd.ops_training import ActivationCheckpoint, _apart, _held, _matrix, _span, _unexplained, weight_gradient
+from tileccl_amd.ops_training import ActivationCheckpoint, _apart, _matrix, _span, _unexplained, weight_gradient
 
 __all__ = ["GatedLinearResult", "GatedLinearGradients", "gated_linear", "gated_linear_backward"]
 
@@ -86,15 +86,6 @@ def _elsewhere(out: torch.Tensor, op: str, **others: "tuple[int, int]") -> None:
             raise ValueError(f"{op}: out overlaps {name}")
 
 
-def _in_vectors(x: torch.Tensor, w: torch.Tensor, op: str) -> tuple[torch.Tensor, torch.Tensor]:
-    """Copies of both that the kernels can read: rows of whole 16-byte vectors, zero behind the inputs.  (The weight's rows then
-    are its columns: that way its two halves may have any size.)"""
-    inputs = x.shape[1]
-    width = -(-inputs // 8) * 8
-    px, pw = _launch._pack([(x, x.shape[0], width, op + " x"), (w.t(), w.shape[1], width, op + " weight")])
-    return px, pw.t()
-
-
 def gated_linear(x: torch.Tensor, weight: torch.Tensor, *, activation: str = "silu", keep: bool = False, out: torch.Tensor | None = None) -> GatedLinearResult:
     """``act(x @ weight[:, :F]) * (x @ weight[:, F:])`` for ``x`` (rows, inputs) and ``weight`` (inputs, 2 * F), float16 or bfloat16.
 
@@ -103,21 +94,18 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, *, activation: str = "si
     ``keep``: also hand back ``x @ weight`` in ``x``'s type (rows, 2 * F), which ``gated_linear_backward`` takes.  Sums,
     activation and product are float32, rounded once.  ``out`` lies across no operand.
 
-    Rows that are no whole 16-byte vectors (inputs, F or a pitch no multiple of 8) are copied first, the weight among them: a program
-    that calls often holds such a weight in rows that are.
+    Rows that are no whole 16-byte vectors (inputs, F or a pitch no multiple of 8) are copied first, the weight's among them: a program
+    that calls with few rows holds its weight in rows that are.
     """
     code = _activation(activation, "gated_linear")
     native = ops_training._native or ops_training._bind()
     result = native.gated_linear(x, weight, code, keep, out)
     if result is None:
-        _check_gated_linear(x, weight, out)
-        result = native.gated_linear(*_in_vectors(x, weight, "gated_linear"), code, keep, out)
-        if result is None:
-            _unexplained("gated_linear")
+        _refuse_gated_linear(x, weight, out)
     return result
 
 
-def _check_gated_linear(x, weight, out) -> None:
+def _refuse_gated_linear(x, weight, out) -> NoReturn:
     op = "gated_linear"
     _weight(weight, op)
     _matrix(x, "x", op, dtype=weight.dtype)
@@ -128,6 +116,7 @@ def _check_gated_linear(x, weight, out) -> None:
         _matrix(out, "out", op, shape=(x.shape[0], weight.shape[1] // 2), dtype=x.dtype)
         _device0(out, "out", op)
         _elsewhere(out, op, x=_span(x), weight=_weight_span(weight))
+    _unexplained(op)
 
 
 def gated_linear_backward(
@@ -158,11 +147,7 @@ def gated_linear_backward(
     native = ops_training._native or ops_training._bind()
     inner = native.gated_gradient(grad, kept, x if kept is None else None, weight, code, out)
     if inner is None:
-        _check_backward(grad, kept, x, weight, out)
-        packed = _in_vectors(x, weight, op) if kept is None else (None, weight)
-        inner = native.gated_gradient(grad, kept, *packed, code, out)
-        if inner is None:
-            _unexplained(op)
+        _refuse_backward(grad, kept, x, weight, out)
     dx = dw = None
     if weights:
         by_rows = _by_rows(weight)
@@ -175,7 +160,7 @@ def gated_linear_backward(
     return GatedLinearGradients(inner, dx, dw)
 
 
-def _check_backward(grad, kept, x, weight, out) -> None:
+def _refuse_backward(grad, kept, x, weight, out) -> NoReturn:
     op = "gated_linear_backward"
     _weight(weight, op)
     outputs = weight.shape[1] // 2
@@ -197,6 +182,7 @@ def _check_backward(grad, kept, x, weight, out) -> None:
         _device0(out, "out", op)
         _elsewhere(out, op, grad=_span(grad), weight=_weight_span(weight), **({"x": _span(x)} if kept is None else {}))
         _apart(out, "out", op, kept)
+    _unexplained(op)
 
 
 def _input_gradient(inner: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:

@@ -102,7 +102,7 @@ def _bind() -> Any:
         from tileccl_amd.ops_gated import GatedLinearResult
 
         entries = (lib.tccl_weight_gradient_full, lib.tccl_weight_gradient_full_workspace, lib.tccl_gated, lib.tccl_gated_grad, lib.tccl_adamw,
-                   lib.tccl_adamw_moments)
+                   lib.tccl_adamw_moments, lib.tccl_gated_workspace, lib.tccl_gated_grad_workspace)
         host.bind_layers(GatedLinearResult, tuple(C.cast(e, C.c_void_p).value for e in entries))
         _native = host
     return _native
@@ -356,8 +356,10 @@ def weight_gradient(
         out_dtype = add.dtype
     native = _native or _bind()
     if isinstance(x, torch.Tensor):
-        result = native.weight_gradient_full(x, grad, None, None, layout == "nk", out_dtype, add, out)
-        return _weight_gradient_full(x, grad, layout, out_dtype, add, out) if result is None else result
+        result = native.weight_gradient_full(x, grad, layout == "nk", out_dtype, add, out)
+        if result is None:
+            _refuse_weight_gradient(x, grad, layout, out_dtype, add, out)
+        return result
     result = native.weight_gradient(x, grad, None, layout == "nk", out_dtype, add, out)
     if result is not None:
         return result
@@ -391,8 +393,7 @@ def weight_gradient(
     return result
 
 
-def _weight_gradient_full(x, grad, layout, out_dtype, add, out) -> torch.Tensor:
-    """The call with operands that are no rows of whole vectors, or an error."""
+def _refuse_weight_gradient(x, grad, layout, out_dtype, add, out) -> NoReturn:
     op = "weight_gradient"
     _matrix(grad, "grad", op)
     _matrix(x, "x", op)
@@ -401,8 +402,8 @@ def _weight_gradient_full(x, grad, layout, out_dtype, add, out) -> torch.Tensor:
             raise ValueError(f"{op}: {name} must be float16 or bfloat16, got {t.dtype}")
         if t.device.index != 0:
             raise ValueError(f"{op}: {name} must reside on cuda:0, where the ranks live, got {t.device}")
-        if t.shape[1] > 1 << 24:
-            raise ValueError(f"{op}: {name} has {t.shape[1]} columns, at most {1 << 24}")
+        if max(t.shape[1], t.stride(0)) > 1 << 24:
+            raise ValueError(f"{op}: {name} has {t.shape[1]} columns (pitch {t.stride(0)}), at most {1 << 24}")
     rows, outputs = grad.shape
     if grad.dtype != x.dtype or rows != x.shape[0]:
         raise ValueError(f"{op}: x is {x.dtype} with {x.shape[0]} rows, grad is {grad.dtype} with {rows}")
@@ -421,10 +422,4 @@ def _weight_gradient_full(x, grad, layout, out_dtype, add, out) -> torch.Tensor:
             lo, hi = _span(out)
             if lo < _span(t)[1] and _span(t)[0] < hi:
                 raise ValueError(f"{op}: out overlaps {name}")
-    if rows:
-        jobs = [(t, rows, -(-t.shape[1] // 8) * 8, f"weight_gradient {name}") for t, name in ((x, "x"), (grad, "grad"))]
-        x, grad = _launch._pack(jobs)
-    result = _native.weight_gradient_full(x, grad, inputs, outputs, layout == "nk", out_dtype, add, out)
-    if result is None:
-        _unexplained(op)
-    return result
+    _unexplained(op)
