@@ -45,18 +45,18 @@ TCCL_D float logistic(float x) { return __builtin_amdgcn_rcpf(1.f + exp_of(-x));
 // t Q(t) with t = 1 / (1 + y / 2), Q of degree 8 fitted to it over y in [0, 12] (largest relative error 4.4e-8, 4e-7 as it is computed).
 // gelu_tanh is g s(2 c (g + k g^3)), s the logistic function: (1 + tanh z) / 2 = s(2 z).  Beyond |g| = 64 s is 0 or 1 and its derivative 0;
 // the bound keeps g^3 finite.
-template <bool kSlope>
-TCCL_D float activated(float g, int activation, float& slope) {
-  if (activation == kSilu) {
+template <int kAct, bool kSlope>
+TCCL_D float activated(float g, float& slope) {
+  if (kAct == kSilu) {
     const float s = logistic(g);
     if (kSlope) slope = s * (1.f + g * (1.f - s));
     return g * s;
   }
-  if (activation == kRelu) {
+  if (kAct == kRelu) {
     if (kSlope) slope = g > 0.f ? 1.f : 0.f;
     return g > 0.f ? g : g == g ? 0.f : g;
   }
-  if (activation == kGelu) {
+  if (kAct == kGelu) {
     const float a = fabsf(g), e = exp_of(-0.5f * a * a), t = __builtin_amdgcn_rcpf(1.f + 0.353553390593273762f * a);
     constexpr float q[] = {0.282084465f, 0.282409579f, 0.242853642f, 0.203678414f, -0.028971795f, 0.281474948f, -0.4901793f, 0.286013812f, -0.0593638085f};
     float s = q[8];
@@ -70,6 +70,22 @@ TCCL_D float activated(float g, int activation, float& slope) {
   const float b = fminf(fmaxf(g, -64.f), 64.f), s = logistic(c * b * (1.f + k * b * b));
   if (kSlope) slope = s + b * s * (1.f - s) * c * (1.f + 3.f * k * b * b);
   return g * s;
+}
+
+template <int kAct>
+TCCL_D float activated(float g) {
+  float none;
+  return activated<kAct, false>(g, none);
+}
+// One choice for all elements that `body` takes, not one for each.
+template <typename Body>
+TCCL_D void with_activation(int activation, Body body) {
+  switch (activation) {
+    case kSilu: return body(std::integral_constant<int, kSilu>{});
+    case kGelu: return body(std::integral_constant<int, kGelu>{});
+    case kGeluTanh: return body(std::integral_constant<int, kGeluTanh>{});
+    default: return body(std::integral_constant<int, kRelu>{});
+  }
 }
 
 // Results leave through LDS, whose rows are then stored whole: out of the accumulators a lane would store 8 bytes of 16 rows each.
@@ -118,22 +134,24 @@ struct Gated : Product<T, kTile, false, kBDeep, true> {
     if constexpr (kBackward) {
       enter(first, g.grad, g.ld_grad, m0, n0, cols);
       __syncthreads();
+      with_activation(g.activation, [&](auto act) {
 #pragma unroll
-      for (int i = 0; i < Base::kRows; ++i)
+        for (int i = 0; i < Base::kRows; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const Quad dh = *(const Quad*)mine(first, i, j);
-          f32x4 dg, du;
+          for (int j = 0; j < 2; ++j) {
+            const Quad dh = *(const Quad*)mine(first, i, j);
+            f32x4 dg, du;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float slope;
-            const float a = activated<true>(acc[i][j][e], g.activation, slope), d = (float)dh[e];
-            dg[e] = d * acc[i][j + 2][e] * slope;
-            du[e] = d * a;
+            for (int e = 0; e < 4; ++e) {
+              float slope;
+              const float a = activated<decltype(act)::value, true>(acc[i][j][e], slope), d = (float)dh[e];
+              dg[e] = d * acc[i][j + 2][e] * slope;
+              du[e] = d * a;
+            }
+            *(Quad*)mine(first, i, j) = rounded(dg);  // in dh's place: nobody else reads it
+            *(Quad*)mine(second, i, j) = rounded(du);
           }
-          *(Quad*)mine(first, i, j) = rounded(dg);  // in dh's place: nobody else reads it
-          *(Quad*)mine(second, i, j) = rounded(du);
-        }
+      });
       __syncthreads();
       leave(first, g.inner, g.ld_inner, m0, n0, cols);
       leave(second, g.inner, g.ld_inner, m0, (int64_t)n0 + this->p.N, cols);
@@ -151,18 +169,17 @@ struct Gated : Product<T, kTile, false, kBDeep, true> {
         leave(second, g.kept, g.ld_kept, m0, (int64_t)n0 + this->p.N, cols);
         __syncthreads();
       }
+      with_activation(g.activation, [&](auto act) {
 #pragma unroll
-      for (int i = 0; i < Base::kRows; ++i)
+        for (int i = 0; i < Base::kRows; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          f32x4 h;
+          for (int j = 0; j < 2; ++j) {
+            f32x4 h;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float none;
-            h[e] = activated<false>(acc[i][j][e], g.activation, none) * acc[i][j + 2][e];
+            for (int e = 0; e < 4; ++e) h[e] = activated<decltype(act)::value>(acc[i][j][e]) * acc[i][j + 2][e];
+            *(Quad*)mine(first, i, j) = rounded(h);
           }
-          *(Quad*)mine(first, i, j) = rounded(h);
-        }
+      });
       __syncthreads();
       leave(first, g.out, g.ld_out, m0, n0, cols);
     }
@@ -340,24 +357,25 @@ struct GatedRows {
     }
     __syncthreads();
     // Neighbouring threads take neighbouring columns of a row.
-    constexpr int kOut = 8 * kNB;
-    for (int u = (int)threadIdx.x; u < 16 * kMB * kOut; u += kWaves * 64) {
-      const int row = u / kOut, col = u % kOut;
-      if (m0 + row >= p.M || col >= left) continue;
-      const float* at = total + ((row / 16 * kNB + col / 16) * 64 + (col % 16 / 4) * 16 + row % 16) * 4 + col % 4;
-      const float z = at[0], y = at[kNB / 2 * 256];
-      if (g.splits > 1) {
-        float* to = g.partial + ((int64_t)split * p.M + m0 + row) * (2 * (int64_t)p.N) + n0 + col;
-        to[0] = z, to[p.N] = y;
-        continue;
+    with_activation(g.activation, [&](auto act) {
+      constexpr int kOut = 8 * kNB;
+      for (int u = (int)threadIdx.x; u < 16 * kMB * kOut; u += kWaves * 64) {
+        const int row = u / kOut, col = u % kOut;
+        if (m0 + row >= p.M || col >= left) continue;
+        const float* at = total + ((row / 16 * kNB + col / 16) * 64 + (col % 16 / 4) * 16 + row % 16) * 4 + col % 4;
+        const float z = at[0], y = at[kNB / 2 * 256];
+        if (g.splits > 1) {
+          float* to = g.partial + ((int64_t)split * p.M + m0 + row) * (2 * (int64_t)p.N) + n0 + col;
+          to[0] = z, to[p.N] = y;
+          continue;
+        }
+        ((T*)g.out)[(int64_t)(m0 + row) * g.ld_out + n0 + col] = to_out<T>(activated<decltype(act)::value>(z) * y);
+        if (g.kept) {
+          T* kept = (T*)g.kept + (int64_t)(m0 + row) * g.ld_kept + n0 + col;
+          kept[0] = to_out<T>(z), kept[p.N] = to_out<T>(y);
+        }
       }
-      float none;
-      ((T*)g.out)[(int64_t)(m0 + row) * g.ld_out + n0 + col] = to_out<T>(activated<false>(z, g.activation, none) * y);
-      if (g.kept) {
-        T* kept = (T*)g.kept + (int64_t)(m0 + row) * g.ld_kept + n0 + col;
-        kept[0] = to_out<T>(z), kept[p.N] = to_out<T>(y);
-      }
-    }
+    });
   }
 };
 
@@ -380,18 +398,19 @@ template <typename T>
 __global__ __launch_bounds__(256) void gated_join_kernel(GatedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   const int64_t n = a.p.N, slice = a.p.M * 2 * n;
-  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < a.p.M * n; u += (int64_t)gridDim.x * 256) {
-    const int64_t row = u / n, col = u - row * n;
-    const float* at = a.partial + row * 2 * n + col;
-    float z = at[0], y = at[n];
-    for (int split = 1; split < a.splits; ++split) z += at[split * slice], y += at[split * slice + n];
-    float none;
-    ((T*)a.out)[row * a.ld_out + col] = to_out<T>(activated<false>(z, a.activation, none) * y);
-    if (a.kept) {
-      T* kept = (T*)a.kept + row * a.ld_kept + col;
-      kept[0] = to_out<T>(z), kept[n] = to_out<T>(y);
+  with_activation(a.activation, [&](auto act) {
+    for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < a.p.M * n; u += (int64_t)gridDim.x * 256) {
+      const int64_t row = u / n, col = u - row * n;
+      const float* at = a.partial + row * 2 * n + col;
+      float z = at[0], y = at[n];
+      for (int split = 1; split < a.splits; ++split) z += at[split * slice], y += at[split * slice + n];
+      ((T*)a.out)[row * a.ld_out + col] = to_out<T>(activated<decltype(act)::value>(z) * y);
+      if (a.kept) {
+        T* kept = (T*)a.kept + row * a.ld_kept + col;
+        kept[0] = to_out<T>(z), kept[n] = to_out<T>(y);
+      }
     }
-  }
+  });
 #endif
 }
 
@@ -401,22 +420,24 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(GatedGradArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   const int chunks = (a.cols + 7) / 8;
   const int64_t all = (int64_t)a.rows * chunks;
-  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < all; at += (int64_t)gridDim.x * 256) {
-    const int64_t row = at / chunks;
-    const int col = (int)(at - row * chunks) * 8, left = a.cols - col;
-    const typename Eight<T>::Vec dh = Eight<T>::get(a.grad, row * a.ld_grad + col, left), g = Eight<T>::get(a.kept, row * a.ld_kept + col, left),
-                                 u = Eight<T>::get(a.kept, row * a.ld_kept + a.cols + col, left);
-    typename Eight<T>::Vec dg, du;
+  with_activation(a.activation, [&](auto act) {
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < all; at += (int64_t)gridDim.x * 256) {
+      const int64_t row = quotient(at, chunks);
+      const int col = (int)(at - row * chunks) * 8, left = a.cols - col;
+      const typename Eight<T>::Vec dh = Eight<T>::get(a.grad, row * a.ld_grad + col, left), g = Eight<T>::get(a.kept, row * a.ld_kept + col, left),
+                                   u = Eight<T>::get(a.kept, row * a.ld_kept + a.cols + col, left);
+      typename Eight<T>::Vec dg, du;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float slope;
-      const float act = activated<true>((float)g[e], a.activation, slope), d = (float)dh[e];
-      dg[e] = (T)(d * (float)u[e] * slope);
-      du[e] = (T)(d * act);
+      for (int e = 0; e < 8; ++e) {
+        float slope;
+        const float activation = activated<decltype(act)::value, true>((float)g[e], slope), d = (float)dh[e];
+        dg[e] = (T)(d * (float)u[e] * slope);
+        du[e] = (T)(d * activation);
+      }
+      Eight<T>::put(a.inner, row * a.ld_inner + col, left, dg);
+      Eight<T>::put(a.inner, row * a.ld_inner + a.cols + col, left, du);
     }
-    Eight<T>::put(a.inner, row * a.ld_inner + col, left, dg);
-    Eight<T>::put(a.inner, row * a.ld_inner + a.cols + col, left, du);
-  }
+  });
 #endif
 }
 

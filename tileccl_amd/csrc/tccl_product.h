@@ -464,6 +464,9 @@ struct Product {
   }
 };
 
+// A quotient in 32 bits where that is enough (a 64-bit one is a hundred instructions).
+TCCL_D int64_t quotient(int64_t at, int by) { return at >> 32 ? at / by : (int64_t)((uint32_t)at / (uint32_t)by); }
+
 // A thread takes a vector: 16 bytes from anywhere, 16 bytes to a boundary.
 template <typename T>
 __global__ __launch_bounds__(256) void copy_rows_kernel(CopyArgs a) {
@@ -471,7 +474,7 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(CopyArgs a) {
   for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < a.chunks[a.n - 1]; u += (int64_t)gridDim.x * 256) {
     int which = 0;
     while (u >= a.chunks[which]) ++which;
-    const int64_t at = which ? u - a.chunks[which - 1] : u, row = at / a.per_row[which];
+    const int64_t at = which ? u - a.chunks[which - 1] : u, row = quotient(at, a.per_row[which]);
     const int col = (int)(at - row * a.per_row[which]) * 8;
     *(typename Eight<T>::Vec*)(a.to[which] + (row * a.ld_to[which] + col) * 2) = Eight<T>::get(a.from[which], row * a.ld_from[which] + col, a.cols[which] - col);
   }
