@@ -695,7 +695,7 @@ int tccl_gated_grad(const tccl_gated_grad_desc* gated, void* stream);
  * below it is rounded up where f + u >= 1, u in [0, 1) being 16 bits, the lower ones for m, the upper ones for v, of the hash h
  * of the element's place i in `first` and the step, in 32 bits: h = i ^ (step * 0x9E3779B9 + (i >> 32) * 0xBB67AE85),
  * h = (h ^ (h >> 16)) * 0x6A09E667, h = (h ^ (h >> 15)) * 0x3C6EF373, h = h ^ (h >> 16).
- * The update takes m and v before they are rounded.  `master` (params in 16 bits only; NULL: none): fp32 values of the params, laid out as the
+ * The update takes m and v before they are rounded, and under its root a v below 2^-126 as 0.  `master` (params in 16 bits only; NULL: none): fp32 values of the params, laid out as the
  * moments, which are updated in the params' place and of which the params are then the rounded values.
  * step_at, lr_at, grad_scale_at: device words that the launch reads in the place of the values (NULL: the values count), for
  * recorded calls.  Moments and master lie on 16 bytes.  Tensors share no memory. */

@@ -1,7 +1,7 @@
 // AdamW over many tensors at once, for gfx950:
 //     g = grad * grad_scale,   m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2,
 //     p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
-// in fp32, on p or, where there is one, on its copy in fp32 ("master"), which then leaves rounded as p.
+// in fp32 (under the root a v below 2^-126 counts as 0), on p or, where there is one, on its copy in fp32 ("master"), which then leaves rounded as p.
 //
 // The moments lie in flat memory, one tensor behind another from a multiple of kMomentBlock elements on.  In 8 bits a block of
 // them shares a scale 2^e, a byte e + 127:
@@ -68,62 +68,64 @@ TCCL_D uint32_t noise(uint32_t place, uint32_t key) {
 }
 
 // The largest of 16 neighbouring lanes' values, which hold a block.
-TCCL_D float max16(float v) {
-  auto turn = [](float x, auto by) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(by)::value, 0xf, 0xf, true));
-  };
-  v = fmaxf(v, turn(v, std::integral_constant<int, 0x128>{}));  // row_ror: 8, 4, 2, 1
-  v = fmaxf(v, turn(v, std::integral_constant<int, 0x124>{}));
-  v = fmaxf(v, turn(v, std::integral_constant<int, 0x122>{}));
-  return fmaxf(v, turn(v, std::integral_constant<int, 0x121>{}));
+TCCL_D uint32_t max16(uint32_t v) {
+  auto turn = [](uint32_t x, auto by) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(by)::value, 0xf, 0xf, true); };
+  auto most = [](uint32_t x, uint32_t y) { return x > y ? x : y; };
+  v = most(v, turn(v, std::integral_constant<int, 0x128>{}));  // row_ror: 8, 4, 2, 1
+  v = most(v, turn(v, std::integral_constant<int, 0x124>{}));
+  v = most(v, turn(v, std::integral_constant<int, 0x122>{}));
+  return most(v, turn(v, std::integral_constant<int, 0x121>{}));
 }
-TCCL_D bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+// Magnitudes are compared by their bits, among which what is not finite stands above all others.
+constexpr uint32_t kNotFinite = 0x7f800000u;
+TCCL_D uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-TCCL_D uint32_t first_scale(float top) {
-  const uint32_t bits = __float_as_uint(top);
-  const int e = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u);
+TCCL_D uint32_t first_scale(uint32_t top) {
+  const int e = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u);
   return (uint32_t)(e > 10 ? e : 10);
 }
-TCCL_D uint32_t second_scale(float top) {
-  const int e = (int)(__float_as_uint(top) >> 23);
-  return (uint32_t)(e > 37 ? e : 37);
+TCCL_D uint32_t second_scale(uint32_t top) { return top >> 23 > 37u ? top >> 23 : 37u; }
+// Byte e of `into` becomes the code of m / 2^e, of finite values.  The conversion adds its random number below the last bit that stays,
+// denormal or not; of the 32 bits that it takes the upper 20 count here, and 16 of them are random (4M values and random numbers of every magnitude
+// gave the codes of the definition).
+template <int kByte>
+TCCL_D uint32_t first_code(float m, float inverse, uint32_t random, uint32_t into) {
+  return (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(m * inverse, (int)(random << 16), (int)into, kByte);
 }
-// `up`: 20 random bits, added below the last bit that stays.  Below 2^-6 e4m3 has steps of 2^-9: with 2^-6 added the value's
-// own bits have them, too.
-TCCL_D uint32_t first_code(float m, uint32_t scale, uint32_t up) {
-  const float y = fabsf(m) * __uint_as_float((254u - scale) << 23);
-  const bool small = y < 0.015625f;
-  const uint32_t t = __float_as_uint(small ? y + 0.015625f : y) + up;
-  const uint32_t code = (t >> 20) - (small ? 968u : 960u);
-  return finite(m) ? code | ((__float_as_uint(m) >> 24) & 0x80u) : 0x7fu;
-}
-TCCL_D uint32_t second_code(float v, uint32_t scale, uint32_t up) {
+TCCL_D uint32_t second_code(float v, uint32_t scale, uint32_t random) {
   const float y = __builtin_amdgcn_ldexpf(v, 127 - (int)scale);
-  int code = (int)((__float_as_uint(y) + up) >> 20) - 775;
-  const int last = scale == 254u ? 248 : 254;  // 2 * 2^127 is no fp32
-  code = code < 1 ? 1 : code > last ? last : code;
-  return !finite(v) ? 255u : v > 0.f ? (uint32_t)code : 0u;
+  const int code = (int)((__float_as_uint(y) + ((random >> 12) & 0xffff0u)) >> 20) - 775;
+  return v > 0.f ? (uint32_t)(code > 1 ? code : 1) : 0u;
 }
-TCCL_D float second_value(uint32_t code, float scale) {
-  const float y = __uint_as_float((code + 775u) << 20) * scale;
-  return code == 0u ? 0.f : code == 255u ? __builtin_nanf("") : y;
-}
-// Codes 4 w .. + 3 of eight.
+// The values of four codes.
 TCCL_D void first_values(uint32_t codes, float scale, float* m) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
   m[0] = lo[0] * scale, m[1] = lo[1] * scale, m[2] = hi[0] * scale, m[3] = hi[1] * scale;
 }
+TCCL_D void second_values(uint32_t codes, float scale, float* v) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t code = (codes >> (8 * e)) & 255u;
+    v[e] = code ? __uint_as_float((code + 775u) << 20) * scale : 0.f;
+  }
+  if ((~codes - 0x01010101u) & codes & 0x80808080u)  // a byte of ~codes may be 0: one of 255 is NaN
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (((codes >> (8 * e)) & 255u) == 255u) v[e] = __builtin_nanf("");
+}
 
-// kN elements from `at` on as fp32, and back; `left` of them exist.  Non-temporal: nothing is looked at again before the next step.
+// kN elements from `at` on as fp32, and back; `left` of them exist.  Non-temporal, as nothing is looked at again before the next step, but where a
+// wavefront's access has gaps, which the next one fills.
 template <typename T, int kN>
 struct AdamVector {
+  static constexpr bool kGaps = sizeof(T) * kN > 16;
   typedef T Anywhere __attribute__((ext_vector_type(kN), aligned(sizeof(T))));
   typedef const Anywhere __attribute__((address_space(1))) From;
   typedef Anywhere __attribute__((address_space(1))) To;
   static TCCL_D void get(const char* base, int64_t at, int left, float (&v)[kN]) {
     if (left >= kN) {
-      const Anywhere x = __builtin_nontemporal_load((From*)((const T*)base + at));
+      const Anywhere x = kGaps ? *(From*)((const T*)base + at) : __builtin_nontemporal_load((From*)((const T*)base + at));
 #pragma unroll
       for (int e = 0; e < kN; ++e) v[e] = (float)x[e];
     } else {
@@ -136,7 +138,10 @@ struct AdamVector {
       Anywhere x;
 #pragma unroll
       for (int e = 0; e < kN; ++e) x[e] = to_out<T>(v[e]);
-      __builtin_nontemporal_store(x, (To*)((T*)base + at));
+      if (kGaps)
+        *(To*)((T*)base + at) = x;
+      else
+        __builtin_nontemporal_store(x, (To*)((T*)base + at));
     } else {
 #pragma unroll
       for (int e = 0; e < kN; ++e)
@@ -197,11 +202,12 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamArgs a) {
           const float sm = __uint_as_float((uint32_t)a.first_scales[block] << 23), sv = __uint_as_float((uint32_t)a.second_scales[block] << 23);
           first_values(cm[0], sm, m[k]);
           first_values(cm[1], sm, m[k] + 4);
+          second_values(cv[0], sv, v[k]);
+          second_values(cv[1], sv, v[k] + 4);
+          if (left[k] < kN)
 #pragma unroll
-          for (int e = 0; e < kN; ++e) {
-            v[k][e] = second_value((cv[e >> 2] >> (8 * (e & 3))) & 255u, sv);
-            if (e >= left[k]) m[k][e] = v[k][e] = 0.f;
-          }
+            for (int e = 0; e < kN; ++e)
+              if (e >= left[k]) m[k][e] = v[k][e] = 0.f;
         }
       } else {
         AdamVector<float, kN>::get(a.first, place, left[k], m[k]);
@@ -216,7 +222,7 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamArgs a) {
         const float d = g[k][e] * scale;
         m[k][e] = a.beta1 * m[k][e] + a.left1 * d;
         v[k][e] = a.beta2 * v[k][e] + a.left2 * (d * d);
-        p[k][e] = p[k][e] * keep - rate * m[k][e] * __builtin_amdgcn_rcpf(sqrtf(v[k][e]) * root + a.eps);
+        p[k][e] = p[k][e] * keep - rate * m[k][e] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[k][e]) * root + a.eps);
       }
       if constexpr (kMaster) AdamVector<float, kN>::put((char*)a.master, place, left[k], p[k]);
       AdamVector<P, kN>::put(t.param, at, left[k], p[k]);
@@ -225,21 +231,52 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamArgs a) {
         AdamVector<float, kN>::put(a.second, place, left[k], v[k]);
       } else {
         // A block's 16 lanes are here together: those past the end have nothing and take part in the block's maximum.
-        float top_m = 0.f, top_v = 0.f;
+        uint32_t top_m = 0, top_v = 0;
 #pragma unroll
         for (int e = 0; e < kN; ++e) {
-          if (finite(m[k][e])) top_m = fmaxf(top_m, fabsf(m[k][e]));
-          if (finite(v[k][e])) top_v = fmaxf(top_v, v[k][e]);
+          const uint32_t bm = magnitude(m[k][e]), bv = magnitude(v[k][e]);
+          top_m = bm > top_m ? bm : top_m, top_v = bv > top_v ? bv : top_v;
         }
-        const uint32_t sm = first_scale(max16(top_m)), sv = second_scale(max16(top_v));
-        if (left[k]) {
-          const uint32_t key = noise_key(step, (uint32_t)(place >> 32));
-          u32x2 cm = {0, 0}, cv = {0, 0};
+        top_m = max16(top_m), top_v = max16(top_v);
+        // Blocks with something that is not finite, or with a v that may be rounded up to 2^128.
+        const bool odd = top_m >= kNotFinite || top_v >= 254u << 23;
+        if (odd) {
+          top_m = top_v = 0;
 #pragma unroll
           for (int e = 0; e < kN; ++e) {
-            const uint32_t r = noise((uint32_t)place + e, key);
-            cm[e >> 2] |= first_code(m[k][e], sm, (r & 0xffffu) << 4) << (8 * (e & 3));
-            cv[e >> 2] |= second_code(v[k][e], sv, (r >> 16) << 4) << (8 * (e & 3));
+            const uint32_t bm = magnitude(m[k][e]), bv = magnitude(v[k][e]);
+            if (bm < kNotFinite && bm > top_m) top_m = bm;
+            if (bv < kNotFinite && bv > top_v) top_v = bv;
+          }
+          top_m = max16(top_m), top_v = max16(top_v);
+        }
+        const uint32_t sm = first_scale(top_m), sv = second_scale(top_v);
+        if (left[k]) {
+          const float inverse = __uint_as_float((254u - sm) << 23);
+          const uint32_t key = noise_key(step, (uint32_t)(place >> 32));
+          uint32_t random[kN];
+#pragma unroll
+          for (int e = 0; e < kN; ++e) random[e] = noise((uint32_t)place + e, key);
+          u32x2 cm, cv;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            cm[w] = first_code<3>(m[k][4 * w + 3], inverse, random[4 * w + 3],
+                                  first_code<2>(m[k][4 * w + 2], inverse, random[4 * w + 2],
+                                                first_code<1>(m[k][4 * w + 1], inverse, random[4 * w + 1], first_code<0>(m[k][4 * w], inverse, random[4 * w], 0u))));
+            cv[w] = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) cv[w] |= second_code(v[k][4 * w + e], sv, random[4 * w + e]) << (8 * e);
+          }
+          if (odd) {
+#pragma unroll
+            for (int e = 0; e < kN; ++e) {
+              const uint32_t shift = 8 * (e & 3), byte = 255u << shift, code = (cv[e >> 2] >> shift) & 255u;
+              if (magnitude(m[k][e]) >= kNotFinite) cm[e >> 2] = (cm[e >> 2] & ~byte) | 0x7fu << shift;
+              if (magnitude(v[k][e]) >= kNotFinite)
+                cv[e >> 2] |= byte;
+              else if (sv == 254u && code > 248u)  // 2 * 2^127 is no fp32
+                cv[e >> 2] = (cv[e >> 2] & ~byte) | 248u << shift;
+            }
           }
           if (left[k] >= kN) {
             __builtin_nontemporal_store(cm, (u32x2*)(a.first + place));
@@ -270,13 +307,13 @@ __global__ __launch_bounds__(256) void moments_kernel(MomentArgs a) {
   typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
   for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < a.blocks * (kMomentBlock / 8); u += (int64_t)gridDim.x * 256) {
     const int64_t block = u / (kMomentBlock / 8);
-    const u32x2 cm = *(const u32x2*)(a.first + 8 * u), cv = *(const u32x2*)(a.second + 8 * u);
+    const u32x2 cm = __builtin_nontemporal_load((const u32x2*)(a.first + 8 * u)), cv = __builtin_nontemporal_load((const u32x2*)(a.second + 8 * u));
     const float sm = __uint_as_float((uint32_t)a.first_scales[block] << 23), sv = __uint_as_float((uint32_t)a.second_scales[block] << 23);
     float m[8], v[8];
     first_values(cm[0], sm, m);
     first_values(cm[1], sm, m + 4);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = second_value((cv[e >> 2] >> (8 * (e & 3))) & 255u, sv);
+    second_values(cv[0], sv, v);
+    second_values(cv[1], sv, v + 4);
     AdamVector<__bf16, 8>::put(a.to_first, 8 * u, 8, m);
     AdamVector<__bf16, 8>::put(a.to_second, 8 * u, 8, v);
   }
