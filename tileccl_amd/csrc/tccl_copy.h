@@ -21,22 +21,23 @@ struct Copies {
   // rows x cols from `from` on, into rows of `ld_to` elements, `to_col` elements further on in the memory of the last copy or (0) in new memory.
   const char* add(const char* from, int64_t ld_from, int64_t rows, int cols, int64_t ld_to, int64_t to_col = 0) {
     if (!to_col) last = bytes, bytes += (rows * ld_to * 2 + 255) / 256 * 256;
-    const int i = a.n++;
-    a.from[i] = from, a.ld_from[i] = ld_from, a.ld_to[i] = ld_to, a.cols[i] = cols, a.per_row[i] = (int)(vectors(cols) / 8);
-    a.to[i] = at + last + to_col * 2;
-    a.chunks[i] = (i ? a.chunks[i - 1] : 0) + rows * a.per_row[i];
+    CopyJob& j = a.job[a.n++];
+    j.from = from, j.to = at + last + to_col * 2, j.ld_from = ld_from, j.ld_to = ld_to;
+    j.cols = cols, j.per_row = (int)(vectors(cols) / 8), j.chunks = rows * j.per_row;
+    const int64_t wgs = (j.chunks + 255) / 256;
+    j.first_wg = all, j.wgs = (int)(wgs < 8192 ? wgs : 8192), all += j.wgs;
     return at + last;
   }
   template <typename T>
   int launch(const char* what, hipStream_t stream) const {
     if (!a.n) return 0;
-    const int64_t wgs = (a.chunks[a.n - 1] + 255) / 256;
-    hipLaunchKernelGGL((copy_rows_kernel<T>), dim3((unsigned)(wgs < 16384 ? wgs : 16384)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((copy_rows_kernel<T>), dim3((unsigned)all), dim3(256), 0, stream, a);
     return launched(what);
   }
 
  private:
   int64_t last = 0;
+  int all = 0;  // workgroups
 };
 
 }  // namespace tccl

@@ -29,12 +29,16 @@ struct ProductArgs {
 };
 
 // Up to three copies in one launch: operands whose rows start anywhere, into rows of whole 16-byte vectors, zero behind their columns.
+struct CopyJob {
+  const char* from;
+  char* to;
+  int64_t ld_from, ld_to;  // elements
+  int64_t chunks;          // vectors in all
+  int cols, per_row;       // columns; vectors of a row
+  int first_wg, wgs;       // workgroups that take them
+};
 struct CopyArgs {
-  const char* from[3];
-  char* to[3];
-  int64_t ld_from[3], ld_to[3];  // elements
-  int64_t chunks[3];             // vectors of all copies up to and with this one
-  int cols[3], per_row[3];       // columns; vectors of a row
+  CopyJob job[3];
   int n;
 };
 
@@ -467,16 +471,17 @@ struct Product {
 // A quotient in 32 bits where that is enough (a 64-bit one is a hundred instructions).
 TCCL_D int64_t quotient(int64_t at, int by) { return at >> 32 ? at / by : (int64_t)((uint32_t)at / (uint32_t)by); }
 
-// A thread takes a vector: 16 bytes from anywhere, 16 bytes to a boundary.
+// A thread takes a vector: 16 bytes from anywhere, 16 bytes to a boundary.  (A workgroup is one job's: read lane by lane, a job's numbers were a
+// chain of trips to memory.)
 template <typename T>
 __global__ __launch_bounds__(256) void copy_rows_kernel(CopyArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < a.chunks[a.n - 1]; u += (int64_t)gridDim.x * 256) {
-    int which = 0;
-    while (u >= a.chunks[which]) ++which;
-    const int64_t at = which ? u - a.chunks[which - 1] : u, row = quotient(at, a.per_row[which]);
-    const int col = (int)(at - row * a.per_row[which]) * 8;
-    *(typename Eight<T>::Vec*)(a.to[which] + (row * a.ld_to[which] + col) * 2) = Eight<T>::get(a.from[which], row * a.ld_from[which] + col, a.cols[which] - col);
+  const int which = (a.n > 1 && (int)blockIdx.x >= a.job[1].first_wg) + (a.n > 2 && (int)blockIdx.x >= a.job[2].first_wg);
+  const CopyJob j = a.job[which];
+  for (int64_t u = (int64_t)((int)blockIdx.x - j.first_wg) * 256 + threadIdx.x; u < j.chunks; u += (int64_t)j.wgs * 256) {
+    const int64_t row = quotient(u, j.per_row);
+    const int col = (int)(u - row * j.per_row) * 8;
+    *(typename Eight<T>::Vec*)(j.to + (row * j.ld_to + col) * 2) = Eight<T>::get(j.from, row * j.ld_from + col, j.cols - col);
   }
 #endif
 }
