@@ -41,6 +41,15 @@ def test_large_tiles(tokens, inputs, outputs, layout):
     if layout == "nk":
         want, top = want.t(), top.t()
     within(got, want, rounded(want, tokens * SUM * top, F32), "dweight")
+    # on top of another, into it, and with rows that are no vectors
+    shape = tuple(got.shape)
+    for pitch, offset in ((shape[1], 0), (shape[1] + 4, 4), (shape[1] + 1, 1)):
+        memory = torch.zeros(shape[0] * pitch + offset, device="cuda")
+        more = memory[offset:].as_strided(shape, (pitch, 1))
+        more.copy_(rand(shape, 23))
+        first = more.cpu().double()
+        assert ops.weight_gradient(x.cuda(), dy.cuda(), layout=layout, add=more, out=more) is more
+        within(more, want + first, rounded(want + first, (tokens + 1) * SUM * (top + first.abs()), F32), "dweight on top of another")
 
 
 def test_pitches_and_places():

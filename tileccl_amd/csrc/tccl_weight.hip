@@ -229,6 +229,7 @@ int tccl_weight_gradient_full(const tccl_weight_gradient_full_desc* d, void* str
   a.tiles_m = d->transposed ? c.tiles_n : c.tiles_h, a.tiles_n = d->transposed ? c.tiles_h : c.tiles_n, a.band = 4;
   a.steps = c.steps, a.splits = c.splits, a.steps_per_split = c.steps_per_split;
   a.xcds = cus % 8 ? 1 : 8, a.per_xcd = (c.tiles_h * c.tiles_n * c.splits + a.xcds - 1) / a.xcds;
+  a.staged = d->add && c.splits == 1 && d->out_dtype == TCCL_F32 && !((uintptr_t)d->add & 15) && d->ld_add % 4 == 0 && d->ld_add <= 1 << 22;
   const hipStream_t st = (hipStream_t)stream;
   rc = d->dtype == TCCL_BF16 ? copies.launch<__bf16>(what, st) : copies.launch<_Float16>(what, st);
   if (rc) return rc;

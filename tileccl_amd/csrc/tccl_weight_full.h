@@ -17,10 +17,53 @@ struct WeightFullArgs {
   int64_t ld_add, ld_out, ld_partial;
   int tiles_m, tiles_n, band;
   int steps, splits, steps_per_split;
+  int staged;             // `add` is fp32 with rows on 16 bytes and within reach: add_staged()
   int xcds, per_xcd;
 };
 
 #if defined(__HIPCC__)
+
+// A whole 256 x 256 tile of fp32 on top of `add`, whose rows come through LDS in two rounds of 128 (1 KiB each, one load), round 1 while round
+// 0 is added and stored: rows of the wavefronts' blocks of either half.  16-byte chunk c of row k lies in slot c ^ (k % 16).
+// (Block by block a wavefront would read 64 bytes of 16 rows at a time.)
+template <typename Tile>
+TCCL_D void add_staged(const WeightFullArgs& a, const Tile& t, typename Tile::Sums& acc, int m0, int n0) {
+  const int i16 = t.lane & 15, g = t.lane >> 4;
+  const auto from = Tile::window(a.add + ((int64_t)m0 * a.ld_add + n0) * 4, 0xfffffff0ll);
+  auto fetch = [&](int r) {
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      uint32_t off[2];
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        const int k = 16 * t.wave + 2 * p + o, row = k / 64 * 128 + r * 64 + k % 64;
+        off[o] = (uint32_t)(row * a.ld_add * 4) + (uint32_t)((t.lane ^ (k & 15)) * 16);
+      }
+      char* to = t.lds + (16 * t.wave + 2 * p) * 1024;
+      Tile::copy_pair(to, to + 1024, from, off[0], off[1]);
+    }
+  };
+  fetch(0);
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    f32x4 more[4][4];
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    Tile::barrier();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) more[i][j] = *(const f32x4*)(t.lds + (t.wm * 64 + 16 * i + i16) * 1024 + (((t.wn * 16 + 4 * j + g) ^ i16) * 16));
+    if (r == 0) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      Tile::barrier();
+      fetch(1);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) put4<float>(acc[4 * r + i][j] + more[i][j], a.out, (int64_t)(m0 + t.out_row(4 * r + i)) * a.ld_out + n0 + t.wn * 64 + 16 * j + 4 * g, 4);
+  }
+}
 
 template <typename T, typename OutT, int kTile>
 __global__ __launch_bounds__(512, 2) void weight_full_kernel(WeightFullArgs a) {
@@ -39,11 +82,14 @@ __global__ __launch_bounds__(512, 2) void weight_full_kernel(WeightFullArgs a) {
   Tile::clear(acc);
   if (steps > 0) t.run(acc, m0, n0, first, steps);  // (no tokens: a result of zeros, or of what is added)
   const int g = t.lane >> 4;
+  if constexpr (kTile == 256 && sizeof(OutT) == 4)
+    if (a.staged && m0 + kTile <= a.p.M && n0 + kTile <= a.p.N) return add_staged(a, t, acc, m0, n0);
 #pragma unroll
   for (int i = 0; i < Tile::kRows; ++i)
 #pragma unroll
     for (int j = 0; j < Tile::kBlocksN; ++j) {
-      const int row = m0 + t.out_row(i), col = n0 + t.wn * 64 + 16 * j + 4 * g;
+      const int64_t row = m0 + t.out_row(i);
+      const int col = n0 + t.wn * 64 + 16 * j + 4 * g;
       if (row < a.p.M && col < a.p.N) {
         if (a.splits > 1) {
           put4<float>(acc[i][j], (char*)(a.partial + (int64_t)split * a.p.M * a.ld_partial), row * a.ld_partial + col, a.p.N - col);
