@@ -208,6 +208,34 @@ def test_graph_and_stream(rows, layout):
         assert all(torch.equal(a, b) for a, b in zip(recorded, now)), replay
 
 
+# Inputs that are split over workgroups, in every kind of tile; 4104 and 2120 leave the last split a part of its blocks, 7175 no whole vector.
+SPLIT = [
+    (3, 4104, 40, BF16, "kn", "silu"), (1, 4104, 2056, F16, "kn", "gelu"), (20, 4104, 1032, BF16, "kn", "gelu_tanh"), (40, 4104, 1032, F16, "kn", "silu"),
+    (61, 2120, 136, BF16, "kn", "relu"), (112, 7175, 104, BF16, "kn", "gelu"), (260, 4104, 264, BF16, "kn", "silu"), (130, 4104, 2056, F16, "kn", "silu"),
+    (2, 4104, 8, F16, "nk", "silu"), (16, 4104, 1032, BF16, "nk", "gelu_tanh"), (25, 2120, 72, BF16, "nk", "silu"), (30, 4104, 1032, F16, "nk", "gelu"),
+    (50, 2120, 101, BF16, "nk", "silu"), (64, 4104, 1032, BF16, "nk", "silu"), (260, 4104, 264, F16, "nk", "gelu"), (500, 4104, 1040, BF16, "nk", "silu"),
+    (500, 4104, 516, F16, "nk", "gelu_tanh"), (500, 4104, 516, BF16, "kn", "silu"),
+]
+
+
+@pytest.mark.parametrize("rows, inputs, outputs, dtype, layout, act", SPLIT)
+def test_inputs_split_over_workgroups(rows, inputs, outputs, dtype, layout, act):
+    x, dh = rand((rows, inputs), 41, dtype), rand((rows, outputs), 42, dtype, 0.1)
+    w, wd = weight_of(inputs, outputs, dtype, layout, 43)
+    memory = torch.full((rows + 2, 2 * outputs + 3), 7.0, dtype=dtype, device="cuda")
+    r = ops.gated_linear(x.cuda(), wd, activation=act, keep=True)
+    check_forward(r, x, w, act, True)
+    r = ops.gated_linear(x.cuda(), wd, activation=act, out=memory[1:-1, 1 : outputs + 1])
+    check_forward(r, x, w, act, False)
+    act = "silu" if act == "relu" else act
+    g, u, s = ref.projections(x, w)
+    want, bound = inner_bounds(dh, g, u, inputs * SUM * s[:, :outputs], inputs * SUM * s[:, outputs:], dtype, act)
+    d = ops.gated_linear_backward(placed(dh, outputs + 5, 1), None, x.cuda(), wd, activation=act, inputs=False, weights=False, out=memory[1:-1, 1:-2])
+    within(d.inner, want, bound, "inner")
+    memory[1:-1, 1:-2].fill_(7.0)
+    assert bool((memory == 7.0).all()), "bytes around a result were written"
+
+
 # Beyond what small tiles take in one round of the device: 256 x 128 tiles, with parts of one at every edge.
 LARGE = [(2100, 72, 2056, BF16, "kn", "silu"), (2056, 200, 2100, BF16, "nk", "gelu"), (4096, 64, 1024, F16, "kn", "gelu_tanh"), (2049, 328, 2048, F16, "nk", "silu")]
 

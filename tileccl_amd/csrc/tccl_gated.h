@@ -22,7 +22,7 @@ struct GatedArgs {
   int activation;
   int tiles_m, tiles_n, band;
   int xcds, per_xcd;    // dies with an L2 of their own; tiles of one
-  // Few rows, K split over workgroups: blocks of 64 k in each split, and where their sums go: [split][row][2 N].
+  // K split over workgroups: blocks of 64 k in each split, and where their sums go: [split][row][2 N] (NULL: nowhere, a workgroup has them all).
   int splits, blocks_per_split;
   float* partial;
 };
@@ -125,10 +125,27 @@ struct Gated : Product<T, kTile, false, kBDeep, true> {
     }
   }
 
-  TCCL_D void tile(int m0, int n0) {
+  // A split's sums, for gated_join_kernel.
+  TCCL_D void hand_on(const typename Base::Sums& acc, int m0, int n0, int split) const {
+    const int64_t n = this->p.N;
+#pragma unroll
+    for (int i = 0; i < Base::kRows; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t row = m0 + this->out_row(i);
+        const int col = n0 + this->wn * 32 + 16 * (j & 1) + 4 * (this->lane >> 4);
+        if (row < this->p.M && col < n) put4<float>(acc[i][j], (char*)g.partial, (split * (int64_t)this->p.M + row) * (2 * n) + (j < 2 ? 0 : n) + col, (int)n - col);
+      }
+  }
+
+  TCCL_D void tile(int m0, int n0, int split) {
     typename Base::Sums acc;
     Base::clear(acc);
-    Base::run(acc, m0, n0, 0, (this->p.K + Base::kStepK - 1) / Base::kStepK);
+    const int begin = split * g.blocks_per_split, all = (this->p.K + Base::kStepK - 1) / Base::kStepK;
+    const int steps = all - begin < g.blocks_per_split ? all - begin : g.blocks_per_split;
+    if (steps > 0) Base::run(acc, m0, n0, begin, steps);
+    if constexpr (kTile == 128)
+      if (g.partial) return hand_on(acc, m0, n0, split);
     char *first = this->lds, *second = this->lds + kMatrix;
     const int cols = this->p.N - n0;
     if constexpr (kBackward) {
@@ -192,10 +209,11 @@ __global__ __launch_bounds__(512, 2) void gated_kernel(GatedArgs a) {
   typedef Gated<T, kTile, kBDeep, kBackward> Tile;
   __shared__ __attribute__((aligned(1024))) char gated_lds[Tile::kLds];
   // Workgroups go to the XCDs in turn; each XCD takes a run of neighbouring tiles, which share their operands in its L2.
-  const int id = (int)blockIdx.x % a.xcds * a.per_xcd + (int)blockIdx.x / a.xcds;
-  if (id >= a.tiles_m * a.tiles_n) return;
-  const TileCoord at = tile_coords(id, a.tiles_m, a.tiles_n, a.band);
-  Tile(a, gated_lds).tile(at.m * kTile, at.n * (kTile / 2));
+  const int id = (int)blockIdx.x % a.xcds * a.per_xcd + (int)blockIdx.x / a.xcds, tiles = a.tiles_m * a.tiles_n;
+  if (id >= tiles * a.splits) return;
+  const int split = id / tiles;
+  const TileCoord at = tile_coords(id - split * tiles, a.tiles_m, a.tiles_n, a.band);
+  Tile(a, gated_lds).tile(at.m * kTile, at.n * (kTile / 2), split);
 #endif
 }
 
@@ -364,7 +382,7 @@ struct GatedRows {
         if (m0 + row >= p.M || col >= left) continue;
         const float* at = total + ((row / 16 * kNB + col / 16) * 64 + (col % 16 / 4) * 16 + row % 16) * 4 + col % 4;
         const float z = at[0], y = at[kNB / 2 * 256];
-        if (g.splits > 1) {
+        if (g.partial) {
           float* to = g.partial + ((int64_t)split * p.M + m0 + row) * (2 * (int64_t)p.N) + n0 + col;
           to[0] = z, to[p.N] = y;
           continue;
@@ -393,21 +411,29 @@ __global__ __launch_bounds__(kWaves * 64, kMB == 1 && kNB == 2 ? 4 : 2) void gat
 #endif
 }
 
-// What the splits have summed, ascending, and from it what the layer gives.
-template <typename T>
+// What the splits have summed, ascending, and from it what the layer or its gradient gives.
+template <typename T, bool kBackward>
 __global__ __launch_bounds__(256) void gated_join_kernel(GatedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  const int64_t n = a.p.N, slice = a.p.M * 2 * n;
+  const int n = a.p.N;
+  const int64_t all = (int64_t)a.p.M * n;
   with_activation(a.activation, [&](auto act) {
-    for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < a.p.M * n; u += (int64_t)gridDim.x * 256) {
-      const int64_t row = u / n, col = u - row * n;
+    for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < all; u += (int64_t)gridDim.x * 256) {
+      const int64_t row = quotient(u, n), col = u - row * n;
       const float* at = a.partial + row * 2 * n + col;
       float z = at[0], y = at[n];
-      for (int split = 1; split < a.splits; ++split) z += at[split * slice], y += at[split * slice + n];
-      ((T*)a.out)[row * a.ld_out + col] = to_out<T>(activated<decltype(act)::value>(z) * y);
-      if (a.kept) {
-        T* kept = (T*)a.kept + row * a.ld_kept + col;
-        kept[0] = to_out<T>(z), kept[n] = to_out<T>(y);
+      for (int split = 1; split < a.splits; ++split) z += at[split * 2 * all], y += at[split * 2 * all + n];
+      if constexpr (kBackward) {
+        float slope;
+        const float activation = activated<decltype(act)::value, true>(z, slope), d = (float)((const T*)a.grad)[row * a.ld_grad + col];
+        T* inner = (T*)a.inner + row * a.ld_inner + col;
+        inner[0] = to_out<T>(d * y * slope), inner[n] = to_out<T>(d * activation);
+      } else {
+        ((T*)a.out)[row * a.ld_out + col] = to_out<T>(activated<decltype(act)::value>(z) * y);
+        if (a.kept) {
+          T* kept = (T*)a.kept + row * a.ld_kept + col;
+          kept[0] = to_out<T>(z), kept[n] = to_out<T>(y);
+        }
       }
     }
   });

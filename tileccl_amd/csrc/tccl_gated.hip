@@ -77,40 +77,48 @@ double tiles_take(int tile, int64_t tiles, int steps, int cus) {
   const double rounds = (double)((tiles + cus - 1) / cus), busy = tiles < cus ? (double)tiles / cus : 1.0;
   return tile == 256 ? 6.0 + steps * rounds * (rounds > 1 ? 1.5 : 1.12 + 0.48 * busy) : 6.5 + (steps + 1) / 2 * rounds * (rounds > 1 ? 1.0 : 0.78 + 0.15 * busy);
 }
+// ... by the kernels for few rows, of `wgs` workgroups with `turns` times 512 k each.  Narrow tiles of a weight by rows read it in pieces of 32 or 64
+// bytes, at a rate of their own.
+double rows_take(int blocks_m, int blocks_n, int64_t wgs, double turns, bool kmajor, double weight_bytes, int cus) {
+  const double rounds = (double)((wgs + cus - 1) / cus);
+  const double us = blocks_n == 2 ? 4.0 + rounds * (1.6 + 1.45 * turns) : blocks_n == 4 ? 4.0 + rounds * (2.2 + 2.3 * turns) : 6.5 + rounds * (blocks_m == 1 ? 3.3 : 3.8) * turns;
+  const double reads = kmajor ? 0.0 : 4.0 + weight_bytes / (blocks_n == 2 ? 2.7e6 : blocks_n == 4 ? 4.2e6 : 6e6);
+  return us > reads ? us : reads;
+}
+// ... of joining splits: a launch, and 16 bytes written and read for an output and split.
+double join_takes(int splits, int64_t rows, int64_t outputs) { return 4.0 + splits * rows * outputs * 16 / 8e6; }
 
-Choice choose(int rows, int inputs, int outputs, bool kmajor, bool few, int cus) {
-  Choice c = {0, 0, 0, 1};
+// The variant whose estimate is least.  The figures are fitted to calls of 1 .. 4000 rows, 104 .. 8192 outputs, 512 .. 8192 inputs, whose best
+// variant the choice reaches within a tenth, mostly.  Inputs are split over workgroups where these would leave CUs without work
+// (112 x 7168 x 104 in 128 tiles 46 us, split in 8 14.6, in narrow tiles split in 8 11).
+Choice choose(int rows, int inputs, int outputs, bool kmajor, bool few, bool backward, int cus) {
+  Choice best = {0, 0, 0, 1};
   const int blocks = (inputs + 63) / 64;
-  if (few && rows <= 64) {
-    // A k-major weight is read in whole lines whatever the tile: as many workgroups as there are CUs, and a wider tile beyond that.  One by rows
-    // in tiles of whole lines, its inputs split until every CU has one; with few inputs, or rows that take two such tiles without a split, narrow
-    // tiles are level or better (64 k of either: 512 x 512 5.4 and 7.1 us, 40 x 4096 x 4160 30 and 32).
-    if (!kmajor && blocks >= 16) {
-      c.blocks_m = rows <= 16 ? 1 : 2, c.blocks_n = 8;
-      const int64_t tiles = (int64_t)((outputs + 63) / 64) * (rows <= 32 ? 1 : 2);
-      while (tiles * c.splits * 2 <= cus && blocks >= 2 * c.splits * kRowsWaves && c.splits < 16) c.splits *= 2;
-      if (rows <= 32 || (c.splits > 1 && blocks >= 64)) return c;
-      c.splits = 1;
-    }
-    c.blocks_m = !kmajor ? 4 : rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    c.blocks_n = outputs / 32 >= cus ? 4 : 2;
-    return c;
+  double least = 1e30;
+  auto consider = [&](const Choice& c, double us) {
+    if (c.splits > 1 || (backward && !c.tile)) us += join_takes(c.splits, rows, outputs);
+    if (us < least) best = c, least = us;
+  };
+  auto consider_rows = [&](int m, int n) {
+    const int64_t tiles = (int64_t)((rows + 16 * m - 1) / (16 * m)) * ((outputs + 8 * n - 1) / (8 * n));
+    for (int splits = 1; splits <= 16 && (splits == 1 || (tiles * splits <= cus && blocks >= splits * kRowsWaves)); splits *= 2)
+      consider({0, m, n, splits}, rows_take(m, n, tiles * splits, inputs / (512.0 * splits), kmajor, 4.0 * inputs * outputs, cus));
+  };
+  if (few) {
+    // A k-major weight is read in whole lines whatever the tile.  One by rows is in tiles that are 64 outputs wide only, which many workgroups
+    // gain from: 1 x 4096 x 4160 20 us split in 2, 26.5 in tiles of 32 outputs; 30 x 4096 x 1024 15.0 split in 8, 12.8 in tiles of 16 split in 4.
+    const int m = kmajor && rows <= 16 ? 1 : kmajor && rows <= 32 ? 2 : 4;
+    if (!kmajor && rows <= 64) consider_rows(rows <= 16 ? 1 : 2, 8);
+    consider_rows(m, 2);
+    consider_rows(m, 4);
+    if (rows <= 64) return best;
   }
   const int64_t large = (int64_t)((rows + 255) / 256) * ((outputs + 127) / 128), small = (int64_t)((rows + 127) / 128) * ((outputs + 63) / 64);
-  c.tile = 256;
-  double least = tiles_take(256, large, blocks, cus);
-  const double other = tiles_take(128, small, blocks, cus);
-  if (other < least) c.tile = 128, least = other;
-  if (few)
-    for (const int n : {2, 4}) {
-      const int64_t rounds = ((int64_t)((rows + 63) / 64) * ((outputs + 8 * n - 1) / (8 * n)) + cus - 1) / cus;
-      const double us = 4.0 + rounds * (n == 2 ? 1.6 + 1.45 * inputs / 512 : 2.2 + 2.3 * inputs / 512);
-      if (us < least) c.tile = 0, c.blocks_m = 4, c.blocks_n = n, least = us;
-    }
-  return c;
+  consider({256, 0, 0, 1}, tiles_take(256, large, blocks, cus));
+  for (int splits = 1; splits <= 16 && (splits == 1 || (small * splits <= cus && blocks >= 4 * splits)); splits *= 2)
+    consider({128, 0, 0, splits}, tiles_take(128, small * splits, (blocks + splits - 1) / splits, cus) + (splits > 1));
+  return best;
 }
-
-int64_t partial_floats(const Choice& c, int64_t rows, int64_t outputs) { return c.splits > 1 ? c.splits * rows * 2 * outputs : 0; }
 
 template <typename T, int kMB, int kNB, bool kBDeep>
 void launch_rows(GatedArgs& a, const Choice& c, int cus, hipStream_t stream) {
@@ -120,9 +128,6 @@ void launch_rows(GatedArgs& a, const Choice& c, int cus, hipStream_t stream) {
 }
 template <typename T>
 int launch_few(const char* what, GatedArgs& a, const Choice& c, bool kmajor, int cus, hipStream_t stream) {
-  const int blocks = (a.p.K + 63) / 64;
-  a.blocks_per_split = (blocks + c.splits - 1) / c.splits;
-  a.splits = c.splits;  // (a split may be left with nothing: it sums zeros)
   switch (10 * c.blocks_m + c.blocks_n) {
     case 18: launch_rows<T, 1, 8, true>(a, c, cus, stream); break;
     case 28: launch_rows<T, 2, 8, true>(a, c, cus, stream); break;
@@ -133,10 +138,6 @@ int launch_few(const char* what, GatedArgs& a, const Choice& c, bool kmajor, int
     case 42: kmajor ? launch_rows<T, 4, 2, false>(a, c, cus, stream) : launch_rows<T, 4, 2, true>(a, c, cus, stream); break;
     default: kmajor ? launch_rows<T, 4, 4, false>(a, c, cus, stream) : launch_rows<T, 4, 4, true>(a, c, cus, stream); break;
   }
-  const int rc = launched(what);
-  if (rc || c.splits == 1) return rc;
-  const int64_t wgs = ((int64_t)a.p.M * a.p.N + 255) / 256;
-  hipLaunchKernelGGL((gated_join_kernel<T>), dim3((unsigned)(wgs < 2048 ? wgs : 2048)), dim3(256), 0, stream, a);
   return launched(what);
 }
 
@@ -145,7 +146,7 @@ int launch_tile(const char* what, GatedArgs& a, bool kmajor, int cus, hipStream_
   a.tiles_m = (a.p.M + kTile - 1) / kTile, a.tiles_n = (a.p.N + kTile / 2 - 1) / (kTile / 2);
   const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
   if (tiles > 1 << 22) return reportf(TCCL_ERR_UNSUPPORTED, "%s: %lld tiles of the result", what, (long long)tiles);
-  a.xcds = cus % 8 ? 1 : 8, a.per_xcd = (int)((tiles + a.xcds - 1) / a.xcds), a.band = 4;
+  a.xcds = cus % 8 ? 1 : 8, a.per_xcd = (int)((tiles * a.splits + a.xcds - 1) / a.xcds), a.band = 4;
   const dim3 wgs((unsigned)(a.xcds * a.per_xcd));
   if (kmajor)
     hipLaunchKernelGGL((gated_kernel<T, kTile, false, kBackward>), wgs, dim3(512), 0, stream, a);
@@ -156,9 +157,14 @@ int launch_tile(const char* what, GatedArgs& a, bool kmajor, int cus, hipStream_
 
 template <typename T, bool kBackward>
 int launch(const char* what, GatedArgs& a, const Choice& c, bool kmajor, int cus, hipStream_t stream) {
-  if constexpr (!kBackward)
-    if (!c.tile) return launch_few<T>(what, a, c, kmajor, cus, stream);
-  return c.tile == 256 ? launch_tile<T, 256, kBackward>(what, a, kmajor, cus, stream) : launch_tile<T, 128, kBackward>(what, a, kmajor, cus, stream);
+  a.splits = c.splits, a.blocks_per_split = ((a.p.K + 63) / 64 + c.splits - 1) / c.splits;  // (a split may be left with nothing: it sums zeros)
+  const int rc = !c.tile           ? launch_few<T>(what, a, c, kmajor, cus, stream)
+                 : c.tile == 256 ? launch_tile<T, 256, kBackward>(what, a, kmajor, cus, stream)
+                                 : launch_tile<T, 128, kBackward>(what, a, kmajor, cus, stream);
+  if (rc || !a.partial) return rc;
+  const int64_t wgs = ((int64_t)a.p.M * a.p.N + 255) / 256;
+  hipLaunchKernelGGL((gated_join_kernel<T, kBackward>), dim3((unsigned)(wgs < 2048 ? wgs : 2048)), dim3(256), 0, stream, a);
+  return launched(what);
 }
 
 // A product that is ready to be launched, and what it wants of the workspace: copies, then the sums of splits.
@@ -175,9 +181,12 @@ struct Prepared {
     int rc = set_product(what, s, d->x, d->ld_x, d->weight, d->ld_weight, d->up, d->kmajor, a.p, copies);
     if (!rc) rc = compute_units(&cus);
     if (rc) return rc;
-    c = choose(s.rows, s.inputs, s.outputs, d->kmajor, !backward && within_reach(s.inputs, s.outputs, a.p.ldb, d->kmajor), cus);
-    a.partial = (float*)(copies.at + copies.bytes);
-    bytes = copies.bytes + 4 * partial_floats(c, s.rows, s.outputs);
+    c = choose(s.rows, s.inputs, s.outputs, d->kmajor, within_reach(s.inputs, s.outputs, a.p.ldb, d->kmajor), backward, cus);
+    bytes = copies.bytes;
+    if (c.splits > 1 || (backward && !c.tile)) {  // (the kernels for few rows have no gradient of their own)
+      a.partial = (float*)(copies.at + copies.bytes);
+      bytes += 4ll * c.splits * s.rows * 2 * s.outputs;
+    }
     a.activation = s.activation;
     return 0;
   }
@@ -227,7 +236,7 @@ int tccl_gated_cut(int32_t rows, int32_t inputs, int32_t outputs, int32_t kmajor
   const int rc = check_sizes("gated_cut", Sizes{rows, inputs, outputs, TCCL_BF16, TCCL_SILU});
   if (rc) return rc;
   if (compute_units < 1 || !tile || !tile_rows || !tile_outputs || !splits) return reportf(TCCL_ERR_INVALID, "gated_cut: %d compute units, or a NULL result", compute_units);
-  const Choice c = choose(rows, inputs, outputs, kmajor != 0, !backward, compute_units);
+  const Choice c = choose(rows, inputs, outputs, kmajor != 0, true, backward != 0, compute_units);
   *tile = c.tile, *splits = c.splits;
   *tile_rows = c.tile ? c.tile : 16 * c.blocks_m, *tile_outputs = c.tile ? c.tile / 2 : 8 * c.blocks_n;
   return 0;

@@ -4,7 +4,6 @@
 // operands exchanged.  Where tiles are few the tokens are split over workgroups, whose sums weight_sum_kernel adds up.
 #pragma once
 
-#include "tccl_product.h"
 #include "tccl_weight.h"
 
 namespace tccl {
