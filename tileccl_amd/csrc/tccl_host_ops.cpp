@@ -44,6 +44,7 @@ int (*entry_gated)(const tccl_gated_desc*, void*);
 int64_t (*entry_gated_workspace)(const tccl_gated_desc*);
 int64_t (*entry_gated_grad_workspace)(const tccl_gated_grad_desc*);
 int (*entry_gated_grad)(const tccl_gated_grad_desc*, void*);
+int (*entry_gemm)(const tccl_gemm_desc*, void*);
 int (*entry_adamw)(const tccl_adamw_desc*, void*);
 int (*entry_moments)(const tccl_adamw_moments_desc*, void*);
 
@@ -573,6 +574,33 @@ PyObject* gated_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
+// input_gradient(inner, weight): inner @ weight.t(), or None where an operand does not lie in whole 16-byte vectors.
+PyObject* input_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 2) return none();
+  return guarded([&]() -> PyObject* {
+    Matrix inner;
+    GatedWeight w;
+    if (!inner.open(args[0]) || !on_device0(*inner.t) || !w.open(args[1])) return none();
+    const at::ScalarType type = inner.t->scalar_type();
+    if (w.t->scalar_type() != type || inner.cols != 2 * w.outputs) return none();
+    if (w.inputs % 8 || inner.cols % 8 || inner.pitch % 8 || w.pitch % 8 || ((uintptr_t)inner.at | (uintptr_t)w.at) % 16) return none();
+    const at::Tensor made = empty({inner.rows, w.inputs}, type, inner.t->device());
+    if (!inner.rows) return THPVariable_Wrap(made);
+    tccl_gemm_desc d;
+    memset(&d, 0, sizeof d);
+    d.A = inner.at, d.B = w.at, d.C = made.data_ptr();
+    d.M = (int32_t)inner.rows, d.N = (int32_t)w.inputs, d.K = (int32_t)inner.cols;
+    d.lda = inner.pitch, d.ldb = w.pitch, d.ldc = w.inputs;
+    d.in_dtype = d.out_dtype = code_of(type);
+    d.alpha = 1.f, d.block_m = d.block_n = 128, d.group_m = 8;
+    d.flags = w.kmajor ? 0 : TCCL_GEMM_B_KMAJOR;  // of weight.t(): its columns are the weight's rows
+    void* stream;
+    if (!stream_now(stream)) return nullptr;
+    if (failed(entry_gemm(&d, stream), "tccl_gemm")) return nullptr;
+    return THPVariable_Wrap(made);
+  });
+}
+
 // weight_gradient_full(x, grad, transposed, out_dtype, add, out)
 PyObject* weight_gradient_full(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 6) return none();
@@ -742,8 +770,8 @@ PyObject* adamw_moments(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // bind_layers(GatedLinearResult, entries): the entry points in the order below.
 PyObject* bind_layers(PyObject*, PyObject* args) {
   PyObject* result;
-  unsigned long long e[8];
-  if (!PyArg_ParseTuple(args, "O(KKKKKKKK)", &result, e, e + 1, e + 2, e + 3, e + 4, e + 5, e + 6, e + 7)) return nullptr;
+  unsigned long long e[9];
+  if (!PyArg_ParseTuple(args, "O(KKKKKKKKK)", &result, e, e + 1, e + 2, e + 3, e + 4, e + 5, e + 6, e + 7, e + 8)) return nullptr;
   if (!PyType_Check(result) || !PyType_IsSubtype((PyTypeObject*)result, &PyTuple_Type)) {
     PyErr_SetString(PyExc_TypeError, "results are named tuples");
     return nullptr;
@@ -758,6 +786,7 @@ PyObject* bind_layers(PyObject*, PyObject* args) {
   entry_moments = (decltype(entry_moments))(uintptr_t)e[5];
   entry_gated_workspace = (decltype(entry_gated_workspace))(uintptr_t)e[6];
   entry_gated_grad_workspace = (decltype(entry_gated_grad_workspace))(uintptr_t)e[7];
+  entry_gemm = (decltype(entry_gemm))(uintptr_t)e[8];
   Py_RETURN_NONE;
 }
 
@@ -800,6 +829,7 @@ PyMethodDef methods[] = {{"bind_operators", bind_operators, METH_VARARGS, nullpt
                          {"bind_layers", bind_layers, METH_VARARGS, nullptr},
                          {"gated_linear", FAST(gated_linear)},
                          {"gated_gradient", FAST(gated_gradient)},
+                         {"input_gradient", FAST(input_gradient)},
                          {"weight_gradient_full", FAST(weight_gradient_full)},
                          {"adamw_step", FAST(adamw_step)},
                          {"adamw_moments", FAST(adamw_moments)},

@@ -156,7 +156,9 @@ def gated_linear_backward(
         dw = weight_gradient(x, inner, layout="kn" if by_rows else "nk", out_dtype=out_dtype, add=add if add is None or by_rows else add.t())
         dw = dw if by_rows else dw.t()
     if inputs:
-        dx = _input_gradient(inner, weight)
+        dx = native.input_gradient(inner, weight)
+        if dx is None:
+            dx = _input_gradient(inner, weight)
     return GatedLinearGradients(inner, dx, dw)
 
 
@@ -186,7 +188,7 @@ def _refuse_backward(grad, kept, x, weight, out) -> NoReturn:
 
 
 def _input_gradient(inner: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
-    """``inner @ weight.t()``: a plain GEMM of the library's."""
+    """``inner @ weight.t()`` of operands that are no whole 16-byte vectors: the library's GEMM of copies."""
     rows, n = inner.shape[0], weight.shape[0]
     width = -(-n // 8) * 8  # the GEMM stores whole vectors
     out = torch.empty((rows, width), dtype=inner.dtype, device=inner.device)
