@@ -177,6 +177,30 @@ def test_values_at_the_ends(act):
     within(r.out, want, rounded(want, 2.0**-19 * (g.abs() + 1), BF16), "out")
 
 
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("rows", [8, 300])
+def test_gradients_at_the_ends(act, rows):
+    """Projections as they were kept and computed again: large ones, zeros and NaN, whose gradients are NaN (relu's of the gate: 0)."""
+    inputs, outputs = 8, 16
+    ends = torch.tensor([0.0, 1e-3, 20.0, -20.0, 1e4, -1e4, 3e8, float("nan")])
+    x = torch.zeros(rows, inputs)
+    x[:8, 0], x[:, 1] = ends, 1.0
+    w = torch.zeros(inputs, 2 * outputs)
+    w[0, :outputs], w[1, outputs:] = 1.0, 2.0
+    x, w, dh = x.to(BF16), w.to(BF16), torch.ones(rows, outputs, dtype=BF16)
+    g, u = x.double() @ w.double()[:, :outputs], torch.full((rows, outputs), 2.0, dtype=torch.float64)
+    g[7] = float("nan")
+    kept = torch.cat([g, u], dim=1).to(BF16)
+    exact, error = ref.gated_gradient(dh, g, u, act), 2.0**-18 * (g.nan_to_num(0.0).abs() + 1)
+    bound = rounded(exact, torch.cat([error, error], dim=1), BF16)
+    for z in (kept, None):
+        inner = ops.gated_linear_backward(dh.cuda(), None if z is None else z.cuda(), x.cuda(), w.cuda(), activation=act, inputs=False, weights=False).inner.cpu()
+        within(inner[:7], exact[:7], bound[:7], "inner")
+        assert bool(torch.isnan(inner[7, outputs:]).all()), "du = dh act(NaN)"
+        # (computed again, u of that row is 0 * NaN + 2, too: relu's dg is NaN * 0)
+        assert bool(torch.isnan(inner[7, :outputs]).all()) or (act == "relu" and z is not None), "dg = dh u act'(NaN)"
+
+
 @pytest.mark.parametrize("rows, layout", [(3, "nk"), (200, "kn"), (600, "nk")])
 def test_graph_and_stream(rows, layout):
     """Recorded calls give the eager result at every replay, beside eager calls of their own; so does another stream."""

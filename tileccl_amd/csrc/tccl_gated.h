@@ -44,7 +44,7 @@ TCCL_D float logistic(float x) { return __builtin_amdgcn_rcpf(1.f + exp_of(-x));
 // gelu is g Phi(g).  Phi(-a) = erfcx(a / sqrt 2) exp(-a^2 / 2) / 2 keeps its relative accuracy where Phi is small: erfcx(y) is
 // t Q(t) with t = 1 / (1 + y / 2), Q of degree 8 fitted to it over y in [0, 12] (largest relative error 4.4e-8, 4e-7 as it is computed).
 // gelu_tanh is g s(2 c (g + k g^3)), s the logistic function: (1 + tanh z) / 2 = s(2 z).  Beyond |g| = 64 s is 0 or 1 and its derivative 0;
-// the bound keeps g^3 finite.
+// the bound keeps g^3 finite (and a NaN what it is).
 template <int kAct, bool kSlope>
 TCCL_D float activated(float g, float& slope) {
   if (kAct == kSilu) {
@@ -67,7 +67,7 @@ TCCL_D float activated(float g, float& slope) {
     return g * phi;
   }
   constexpr float c = 1.59576912160573071f, k = 0.044715f;  // 2 sqrt(2 / pi)
-  const float b = fminf(fmaxf(g, -64.f), 64.f), s = logistic(c * b * (1.f + k * b * b));
+  const float b = g < -64.f ? -64.f : g > 64.f ? 64.f : g, s = logistic(c * b * (1.f + k * b * b));
   if (kSlope) slope = s + b * s * (1.f - s) * c * (1.f + 3.f * k * b * b);
   return g * s;
 }
