@@ -631,7 +631,8 @@ int tccl_weight_gradient_full(const tccl_weight_gradient_full_desc* wg, void* st
 /* Gated linear layer: z = x W = [g | u], out = act(g) * u, from a weight (inputs x 2 outputs) whose first half of columns is the
  * gate's.  Sums and activations are fp32, out and kept (z, rows x 2 outputs; NULL: not wanted) are rounded once.
  *   weight: kmajor 0: rows of 2 outputs, ld_weight apart; kmajor 1: 2 outputs rows of inputs (the layer holds it transposed).  `up`: elements
- *   from the gate's part to the other one's (kmajor 0: at least `outputs`; kmajor 1: at least outputs - 1 rows).
+ *   from the gate's part to the other one's (kmajor 0: at least `outputs`, in the same row, all of whose elements can be read; kmajor 1: at least
+ *   outputs - 1 rows).
  *   act: TCCL_SILU g / (1 + exp(-g)); TCCL_GELU g Phi(g), Phi the normal distribution; TCCL_GELU_TANH
  *   g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2; TCCL_RELU max(g, 0).
  * Operands have any alignment of their type; out and kept share no memory with another operand.  `workspace`: device memory on 16 bytes of

@@ -1,11 +1,13 @@
 """The gated linear layer and its gradients on the GPU against their definitions in 64 bits (bounds: layer_bounds.py)."""
 
+import ctypes
+
 import pytest
 import torch
 
 from oracle import layers as ref
 from tests.layer_bounds import BF16, F16, F32, SUM, gated_bounds, half, inner_bounds, placed, rand, rounded, within
-from tileccl_amd import ops
+from tileccl_amd import _lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -175,6 +177,27 @@ def test_values_at_the_ends(act):
     want = want * 2.0
     want[9], want[10] = float("nan"), float("nan")
     within(r.out, want, rounded(want, 2.0**-19 * (g.abs() + 1), BF16), "out")
+
+
+@pytest.mark.parametrize("rows", [2, 200])
+@pytest.mark.parametrize("up", [8, (1 << 22) + 8, 1 << 23])
+def test_halves_far_from_each_other(lib, rows, up):
+    """One row of a weight by rows, whose second half lies further on than a pitch may be: a copy, the C entry asks for room for it."""
+    outputs = 8
+    x, memory = rand((rows, 1), 51, BF16), torch.full((up + outputs,), float("nan"), dtype=BF16, device="cuda")
+    w = rand((1, 2 * outputs), 52, BF16)
+    memory[:outputs], memory[up:] = w[0, :outputs].cuda(), w[0, outputs:].cuda()
+    xd, out = x.cuda(), torch.empty(rows, outputs, dtype=BF16, device="cuda")
+    d = _lib.GatedDesc(x=xd.data_ptr(), weight=memory.data_ptr(), out=out.data_ptr(), ld_x=1, ld_weight=2 * outputs, up=up, ld_out=outputs, rows=rows, inputs=1,
+                       outputs=outputs, dtype=_lib.BF16)
+    d.workspace_bytes = lib.tccl_gated_workspace(ctypes.byref(d))
+    assert d.workspace_bytes >= 256 * (1 + (up > 1 << 22))  # of x, and of the weight
+    workspace = torch.empty(d.workspace_bytes, dtype=torch.uint8, device="cuda")
+    d.workspace = workspace.data_ptr()
+    assert lib.tccl_gated(ctypes.byref(d), torch.cuda.current_stream().cuda_stream) == 0
+    g, u, s = ref.projections(x, w)
+    want, bound = gated_bounds(g, u, s, 1, BF16, "silu")
+    within(out, want, bound, "out")
 
 
 @pytest.mark.parametrize("act", ACTS)

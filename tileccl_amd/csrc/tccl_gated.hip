@@ -53,7 +53,7 @@ int set_product(const char* what, const Sizes& s, const void* x, int64_t ld_x, c
     p.b = copies.add((const char*)weight, ld_weight, s.outputs, s.inputs, whole);
     const char* second = copies.add((const char*)weight + up * 2, ld_weight, s.outputs, s.inputs, whole);
     up = (second - p.b) / 2, p.ldb = whole;
-  } else if (!kmajor && (!on_vectors(weight, ld_weight, weight_rows) || up % 8 || ld_weight > kMostPitch)) {
+  } else if (!kmajor && (!on_vectors(weight, ld_weight, weight_rows) || up % 8 || p.ldb > kMostPitch)) {
     p.b = copies.add((const char*)weight, p.ldb, s.inputs, s.outputs, 2 * width);
     copies.add((const char*)weight + up * 2, p.ldb, s.inputs, s.outputs, 2 * width, width);
     up = width, p.ldb = 2 * width;
