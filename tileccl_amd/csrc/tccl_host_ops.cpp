@@ -719,12 +719,14 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     std::sort(written.begin(), written.end());
     for (size_t i = 1; i < written.size(); ++i)
       if (written[i].first < written[i - 1].second) return none();
+    const void *step_at = nullptr, *lr_at = nullptr, *scale_at = nullptr;
+    if (!number_or_word(args[3], at::kInt, step_at) || !number_or_word(args[4], at::kFloat, lr_at) || !number_or_word(args[9], at::kFloat, scale_at)) return none();
+    for (const void* word : {step_at, lr_at, scale_at})
+      if (word) read.emplace_back((const char*)word, (const char*)word + 4);
     for (const Span& g : read) {
       auto after = std::lower_bound(written.begin(), written.end(), Span(g.second, nullptr));
       if (after != written.begin() && (after - 1)->second > g.first) return none();
     }
-    const void *step_at = nullptr, *lr_at = nullptr, *scale_at = nullptr;
-    if (!number_or_word(args[3], at::kInt, step_at) || !number_or_word(args[4], at::kFloat, lr_at) || !number_or_word(args[9], at::kFloat, scale_at)) return none();
     d.step_at = (const int32_t*)step_at, d.lr_at = (const float*)lr_at, d.grad_scale_at = (const float*)scale_at;
     const long long step = step_at ? 1 : PyLong_AsLongLong(args[3]);
     if (!lr_at) d.lr = PyFloat_AsDouble(args[4]);

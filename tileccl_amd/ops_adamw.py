@@ -99,10 +99,12 @@ def adamw_step(
     """
     native = ops_training._native or ops_training._bind()
     params, grads = tuple(params), tuple(grads)
+    if not isinstance(betas, (tuple, list)) or len(betas) != 2:
+        raise ValueError(f"adamw_step: betas are two numbers, got {betas!r}")
+    b1, b2 = betas
     try:
-        b1, b2 = betas
         done = native.adamw_step(params, grads, tuple(state), step, lr, b1, b2, eps, weight_decay, grad_scale)
-    except TypeError as e:
+    except (TypeError, OverflowError) as e:
         raise ValueError(f"adamw_step: {e}") from e
     if done is None:
         _refuse_adamw_step(params, grads, state, step, lr, grad_scale)
@@ -167,6 +169,9 @@ def _refuse_adamw_step(params, grads, state, step, lr, grad_scale) -> NoReturn:
         for a, b, other in written[i + 1 :] + read:
             if a < hi and lo < b:
                 raise ValueError(f"{op}: {name} and {other} share memory")
+        for t, word in ((step, "step"), (lr, "lr"), (grad_scale, "grad_scale")):
+            if isinstance(t, torch.Tensor) and lo - 4 < t.data_ptr() < hi:
+                raise ValueError(f"{op}: {word} shares memory with {name}")
     _unexplained(op)
 
 

@@ -145,14 +145,14 @@ def gated_linear_backward(
     op = "gated_linear_backward"
     code = _activation(activation, op)
     native = ops_training._native or ops_training._bind()
+    if weights:  # ahead of a result that may lie in kept's place
+        _check_weight_gradient(grad, x, weight, add, op)
     inner = native.gated_gradient(grad, kept, x if kept is None else None, weight, code, out)
     if inner is None:
         _refuse_backward(grad, kept, x, weight, out)
     dx = dw = None
     if weights:
         by_rows = _by_rows(weight)
-        if add is not None and add.shape != weight.shape:
-            raise ValueError(f"{op}: add must have shape {tuple(weight.shape)}, got {tuple(add.shape)}")
         dw = weight_gradient(x, inner, layout="kn" if by_rows else "nk", out_dtype=out_dtype, add=add if add is None or by_rows else add.t())
         dw = dw if by_rows else dw.t()
     if inputs:
@@ -160,6 +160,22 @@ def gated_linear_backward(
         if dx is None:
             dx = _input_gradient(inner, weight)
     return GatedLinearGradients(inner, dx, dw)
+
+
+def _check_weight_gradient(grad, x, weight, add, op) -> None:
+    if isinstance(x, ActivationCheckpoint):
+        rows, columns = x.rows, x.columns
+    elif isinstance(x, torch.Tensor) and x.ndim == 2:
+        rows, columns = x.shape
+    else:
+        raise ValueError(f"{op}: the weight's gradient wants x, a 2-D tensor or its checkpoint, got {type(x).__name__}")
+    if isinstance(weight, torch.Tensor) and isinstance(grad, torch.Tensor) and weight.ndim == grad.ndim == 2:  # (else refused with their names)
+        if columns != weight.shape[0]:
+            raise ValueError(f"{op}: x has {columns} columns, weight {weight.shape[0]} rows")
+        if rows != grad.shape[0]:
+            raise ValueError(f"{op}: x has {rows} rows, grad {grad.shape[0]}")
+        if add is not None and add.shape != weight.shape:
+            raise ValueError(f"{op}: add must have shape {tuple(weight.shape)}, got {tuple(add.shape)}")
 
 
 def _refuse_backward(grad, kept, x, weight, out) -> NoReturn:
