@@ -45,6 +45,7 @@ int64_t (*entry_gated_workspace)(const tccl_gated_desc*);
 int64_t (*entry_gated_grad_workspace)(const tccl_gated_grad_desc*);
 int (*entry_gated_grad)(const tccl_gated_grad_desc*, void*);
 int (*entry_gemm)(const tccl_gemm_desc*, void*);
+int (*entry_pack)(const tccl_pack_desc*, int32_t, int32_t, void*);
 int (*entry_adamw)(const tccl_adamw_desc*, void*);
 int (*entry_moments)(const tccl_adamw_moments_desc*, void*);
 
@@ -574,7 +575,8 @@ PyObject* gated_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
-// input_gradient(inner, weight): inner @ weight.t(), or None where an operand does not lie in whole 16-byte vectors.
+// input_gradient(inner, weight): inner @ weight.t(), by the library's GEMM, which reads and writes whole 16-byte vectors: an operand that does not lie in
+// these is copied first, both in one launch, and a result whose rows do not has the columns that it wants of wider rows.
 PyObject* input_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 2) return none();
   return guarded([&]() -> PyObject* {
@@ -583,21 +585,40 @@ PyObject* input_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!inner.open(args[0]) || !on_device0(*inner.t) || !w.open(args[1])) return none();
     const at::ScalarType type = inner.t->scalar_type();
     if (w.t->scalar_type() != type || inner.cols != 2 * w.outputs) return none();
-    if (w.inputs % 8 || inner.cols % 8 || inner.pitch % 8 || w.pitch % 8 || ((uintptr_t)inner.at | (uintptr_t)w.at) % 16) return none();
-    const at::Tensor made = empty({inner.rows, w.inputs}, type, inner.t->device());
-    if (!inner.rows) return THPVariable_Wrap(made);
+    const int64_t N = w.inputs, K = inner.cols, width = (N + 7) / 8 * 8, depth = (K + 7) / 8 * 8;
+    const at::Tensor made = empty({inner.rows, width}, type, inner.t->device());
+    const at::Tensor result = width == N ? made : made.narrow(1, 0, N);
+    if (!inner.rows) return THPVariable_Wrap(result);
+    void* stream;
+    if (!stream_now(stream)) return nullptr;
     tccl_gemm_desc d;
     memset(&d, 0, sizeof d);
     d.A = inner.at, d.B = w.at, d.C = made.data_ptr();
-    d.M = (int32_t)inner.rows, d.N = (int32_t)w.inputs, d.K = (int32_t)inner.cols;
-    d.lda = inner.pitch, d.ldb = w.pitch, d.ldc = w.inputs;
+    d.M = (int32_t)inner.rows, d.N = (int32_t)width, d.K = (int32_t)depth;
+    d.lda = inner.pitch, d.ldb = w.pitch, d.ldc = width;
     d.in_dtype = d.out_dtype = code_of(type);
     d.alpha = 1.f, d.block_m = d.block_n = 128, d.group_m = 8;
     d.flags = w.kmajor ? 0 : TCCL_GEMM_B_KMAJOR;  // of weight.t(): its columns are the weight's rows
-    void* stream;
-    if (!stream_now(stream)) return nullptr;
+    tccl_pack_desc jobs[2];
+    int n = 0;
+    at::Tensor a, b;
+    auto copied = [&](at::Tensor& to, const char* from, int64_t pitch, int64_t rows, int64_t cols, int64_t to_rows, int64_t to_cols) {
+      const int64_t to_pitch = (to_cols + 31) / 32 * 32;  // rows on 64 bytes, as the GEMM fetches them
+      to = empty({to_rows, to_pitch}, type, inner.t->device());
+      jobs[n++] = {from, to.data_ptr(), pitch, 1, to_pitch, (int32_t)rows, (int32_t)cols, (int32_t)to_rows, (int32_t)to_cols};
+      return to_pitch;
+    };
+    if (K != depth || inner.pitch % 8 || (uintptr_t)inner.at % 16) d.lda = copied(a, inner.at, inner.pitch, inner.rows, K, inner.rows, depth), d.A = a.data_ptr();
+    if (N != width || K != depth || w.pitch % 8 || (uintptr_t)w.at % 16) {
+      if (w.kmajor)
+        d.ldb = copied(b, w.at, w.pitch, K, N, depth, width);
+      else
+        d.ldb = copied(b, w.at, w.pitch, N, K, width, depth);
+      d.B = b.data_ptr();
+    }
+    if (n && failed(entry_pack(jobs, n, 2, stream), "tccl_pack_matrices")) return nullptr;
     if (failed(entry_gemm(&d, stream), "tccl_gemm")) return nullptr;
-    return THPVariable_Wrap(made);
+    return THPVariable_Wrap(result);
   });
 }
 
@@ -772,8 +793,8 @@ PyObject* adamw_moments(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // bind_layers(GatedLinearResult, entries): the entry points in the order below.
 PyObject* bind_layers(PyObject*, PyObject* args) {
   PyObject* result;
-  unsigned long long e[9];
-  if (!PyArg_ParseTuple(args, "O(KKKKKKKKK)", &result, e, e + 1, e + 2, e + 3, e + 4, e + 5, e + 6, e + 7, e + 8)) return nullptr;
+  unsigned long long e[10];
+  if (!PyArg_ParseTuple(args, "O(KKKKKKKKKK)", &result, e, e + 1, e + 2, e + 3, e + 4, e + 5, e + 6, e + 7, e + 8, e + 9)) return nullptr;
   if (!PyType_Check(result) || !PyType_IsSubtype((PyTypeObject*)result, &PyTuple_Type)) {
     PyErr_SetString(PyExc_TypeError, "results are named tuples");
     return nullptr;
@@ -789,6 +810,7 @@ PyObject* bind_layers(PyObject*, PyObject* args) {
   entry_gated_workspace = (decltype(entry_gated_workspace))(uintptr_t)e[6];
   entry_gated_grad_workspace = (decltype(entry_gated_grad_workspace))(uintptr_t)e[7];
   entry_gemm = (decltype(entry_gemm))(uintptr_t)e[8];
+  entry_pack = (decltype(entry_pack))(uintptr_t)e[9];
   Py_RETURN_NONE;
 }
 

@@ -16,12 +16,11 @@ as in ``ops_training``.
 
 from __future__ import annotations
 
-import ctypes as C
 from typing import Any, NamedTuple, NoReturn
 
 import torch
 
-from tileccl_amd import _launch, _lib, ops_training
+from tileccl_amd import _lib, ops_training
 from tileccl_amd.ops_training import ActivationCheckpoint, _apart, _matrix, _span, _unexplained, weight_gradient
 
 __all__ = ["GatedLinearResult", "GatedLinearGradients", "gated_linear", "gated_linear_backward"]
@@ -158,7 +157,7 @@ def gated_linear_backward(
     if inputs:
         dx = native.input_gradient(inner, weight)
         if dx is None:
-            dx = _input_gradient(inner, weight)
+            _unexplained(op)
     return GatedLinearGradients(inner, dx, dw)
 
 
@@ -201,17 +200,3 @@ def _refuse_backward(grad, kept, x, weight, out) -> NoReturn:
         _elsewhere(out, op, grad=_span(grad), weight=_weight_span(weight), **({"x": _span(x)} if kept is None else {}))
         _apart(out, "out", op, kept)
     _unexplained(op)
-
-
-def _input_gradient(inner: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
-    """``inner @ weight.t()`` of operands that are no whole 16-byte vectors: the library's GEMM of copies."""
-    rows, n = inner.shape[0], weight.shape[0]
-    width = -(-n // 8) * 8  # the GEMM stores whole vectors
-    out = torch.empty((rows, width), dtype=inner.dtype, device=inner.device)
-    if rows:
-        B = weight.t()
-        if width != n:
-            (B,) = _launch._pack([(B, B.shape[0], width, "gated_linear_backward weight")])
-        desc = _launch.gemm_desc(inner, B, out)
-        _lib.check(_lib.load().tccl_gemm(C.byref(desc), _launch.stream_ptr()), "tccl_gemm")
-    return out if width == n else out[:, :n]
