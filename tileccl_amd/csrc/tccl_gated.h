@@ -203,6 +203,10 @@ struct Gated : Product<T, kTile, false, kBDeep, true> {
   }
 };
 
+// 8192 x 4096 x 8192 bf16, k-major: 800 us, 1.38 PFLOP/s, the matrix pipes busy 67 % of a clock that the load holds at 1.9 GHz (the vendor
+// library's product alone 794).  4096 x 4096 x 4096 by rows with z kept 214 us, 1.28 PFLOP/s.  128 tiles are bound by what comes from L2 to a
+// CU, 64 KiB for 4.2 MFLOP at 67 KB a microsecond: 1003 x 1001 x 1035 16 us.  Of a short sum the epilogue is the larger part, bound by the vector
+// instructions of the activation (silu 13 a value, gelu 25, 30 with its derivative): 12628 x 208 x 808, gelu, 33 us, backward 47, memory 10.
 template <typename T, int kTile, bool kBDeep, bool kBackward>
 __global__ __launch_bounds__(512, 2) void gated_kernel(GatedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -225,6 +229,9 @@ __global__ __launch_bounds__(512, 2) void gated_kernel(GatedArgs a) {
 // Loads have neighbouring lanes on neighbouring addresses.  x and a k-major weight: rows of 128 bytes, chunk c of row r in slot
 // c ^ ((r >> 1) & 7).  A weight by rows: of each k row 16 kNB bytes of either matrix, next to each other in LDS; its 32-byte units are permuted
 // (unit()) so that the rows that a transposing read touches at a time lie in different banks.
+//
+// Bound by memory: 1 x 4096 x 8192 bf16, k-major, 23.3 us, 5.8 TB/s; 13 x 4096 x 4096 fp16 by rows 14.8 us, 4.5 TB/s (rows that are a power of two
+// apart lie in few of the L2's channels at a time), and 3 to 4 for the join; in tiles of 32 outputs, that is 64 bytes of a row, 26.
 template <typename T, int kMB, int kNB, int kWaves, bool kBDeep>
 struct GatedRows {
   typedef typename Mfma<T>::Vec Vec;
@@ -411,7 +418,8 @@ __global__ __launch_bounds__(kWaves * 64, kMB == 1 && kNB == 2 ? 4 : 2) void gat
 #endif
 }
 
-// What the splits have summed, ascending, and from it what the layer or its gradient gives.
+// What the splits have summed, ascending, and from it what the layer or its gradient gives.  The sums are still in the caches: 13 x 4096 outputs
+// from four splits 2.9 us, most of it the launch.
 template <typename T, bool kBackward>
 __global__ __launch_bounds__(256) void gated_join_kernel(GatedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -440,7 +448,7 @@ __global__ __launch_bounds__(256) void gated_join_kernel(GatedArgs a) {
 #endif
 }
 
-// dg and du from z as it was kept.  Every value is read once; inner may be kept itself.
+// dg and du from z as it was kept.  Every value is read once; inner may be kept itself.  Bound by memory: 4096 x 4096 bf16 28 us, 6.0 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void gated_grad_kernel(GatedGradArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
