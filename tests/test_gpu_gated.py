@@ -97,6 +97,32 @@ def test_backward(rows, inputs, outputs, dtype, layout, act, keep):
     within(d.weight, dw, (rows + 1) * SUM * (x.double().abs().t() @ inner.abs()), "dweight")
 
 
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("rows, inputs, outputs", [(1, 24, 8), (30, 136, 72), (200, 65, 36), (530, 264, 201)])
+def test_backward_pitches_and_places(rows, inputs, outputs, layout):
+    """Every operand and inner in rows apart from each other, anywhere, NaN around them: whole vectors, then none."""
+    x, dh = rand((rows, inputs), 44, BF16), rand((rows, outputs), 45, BF16, 0.1)
+    for pad, offset in ((8, 8), (0, 1), (5, 3)):
+        w, wd = weight_of(inputs, outputs, BF16, layout, 46, pad, offset)
+        g, u, s = ref.projections(x, w)
+        kept = torch.cat([g, u], dim=1).to(BF16)
+        for z in (None, placed(kept, 2 * outputs + pad, offset)):
+            memory = torch.full((rows * (2 * outputs + pad) + offset + 9,), 7.0, dtype=BF16, device="cuda")
+            out = memory[offset:].as_strided((rows, 2 * outputs), (2 * outputs + pad, 1))
+            d = ops.gated_linear_backward(placed(dh, outputs + pad, offset), z, placed(x, inputs + pad, offset), wd, out=out)
+            assert d.inner is out
+            e = inputs * SUM * s if z is None else torch.zeros_like(s)
+            a, b = (g, u) if z is None else (kept[:, :outputs], kept[:, outputs:])
+            want, bound = inner_bounds(dh, a, b, e[:, :outputs], e[:, outputs:], BF16, "silu")
+            within(out, want, bound, "inner")
+            inner = out.cpu().double()
+            dx = inner @ w.double().t()
+            within(d.x, dx, rounded(dx, 2 * outputs * SUM * (inner.abs() @ w.double().abs().t()), BF16), "dx")
+            within(d.weight, x.double().t() @ inner, (rows + 16) * SUM * (x.double().abs().t() @ inner.abs()), "dweight")
+            out.fill_(7.0)
+            assert bool((memory == 7.0).all()), "bytes around inner were written"
+
+
 def test_backward_against_differences():
     """The gradients are those of sum(dh * gated(x, w)): against differences of the 64-bit definition."""
     rows, inputs, outputs = 3, 16, 8
