@@ -23,8 +23,11 @@ namespace tccl {
 
 constexpr int kMomentBlock = 128;
 constexpr int kAdamTensors = 100;   // of a launch: its arguments have to fit 4 KiB
-constexpr int kAdamThreads = 256;
-constexpr int kAdamChunk = 4096;    // elements of a workgroup
+// Threads of a workgroup, and elements of a thread: each has one turn.  Moments in 32 bits: 4 elements, so that each access of a wavefront is 1 KiB in
+// a row.  In 8 bits: 8, 16 lanes a block.  Larger workgroups and several turns are slower (128M weights in 32 bits 618 us; 256 threads 629, 512
+// 648, with two turns 673; 197M in 8 bits, with the values, 773; 128 threads 783, two turns 788).
+constexpr int kAdamThreads = 128, kAdamThreadsHeld = 256;
+constexpr int kAdamChunk = 4 * kAdamThreads, kAdamChunkHeld = 8 * kAdamThreadsHeld;
 
 struct AdamTensor {
   char *param;
@@ -153,7 +156,7 @@ struct AdamVector {
 // Bound by memory: bf16 weights with fp32 copy, gradients and moments, 128M of them, 670 us, 5.7 TB/s with as many writes as reads (a
 // plain copy of 512 MiB 5.3 to 6.1); moments in 8 bits, 197M with bf16 gradients, 570 us, 5.5 TB/s, the vector units half busy.
 template <typename P, typename G, bool kMaster, bool kHeld>
-__global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamArgs a) {
+__global__ __launch_bounds__(kHeld ? kAdamThreadsHeld : kAdamThreads) void adamw_kernel(AdamArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
   // The tensor that this chunk is of: the last one that starts at or before it.
@@ -178,125 +181,112 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamArgs a) {
   }
   const float scale = a.grad_scale_at ? *a.grad_scale_at : a.grad_scale;
 
-  const int64_t begin = (int64_t)(blockIdx.x - t.first_chunk) * kAdamChunk;
-  // Moments in 32 bits: 4 elements a lane, so that each access of a wavefront is 1 KiB in a row (8 a lane in two accesses each: 67M elements
-  // 726 us, 773 non-temporal), two groups of them on their way at a time.  In 8 bits: 8 a lane, 16 lanes a block.
-  constexpr int kN = kHeld ? 8 : 4, kGroups = kHeld ? 1 : 2, kTurn = kAdamThreads * kN;
-  for (int64_t first = begin + (int)threadIdx.x * kN; first < begin + kAdamChunk; first += kTurn * kGroups) {
-    float p[kGroups][kN], g[kGroups][kN], m[kGroups][kN], v[kGroups][kN];
-    int left[kGroups];
+  constexpr int kN = kHeld ? 8 : 4;
+  const int64_t at = (int64_t)(blockIdx.x - t.first_chunk) * (kHeld ? kAdamChunkHeld : kAdamChunk) + (int)threadIdx.x * kN, place = (int64_t)t.block * kMomentBlock + at;
+  const int left = t.n - at < kN ? (t.n - at > 0 ? (int)(t.n - at) : 0) : kN;
+  float p[kN], g[kN], m[kN], v[kN];
+  AdamVector<G, kN>::get(t.grad, at, left, g);
+  if constexpr (kMaster)
+    AdamVector<float, kN>::get((const char*)a.master, place, left, p);
+  else
+    AdamVector<P, kN>::get(t.param, at, left, p);
+  if constexpr (kHeld) {
 #pragma unroll
-    for (int k = 0; k < kGroups; ++k) {
-      const int64_t at = first + k * kTurn, place = (int64_t)t.block * kMomentBlock + at;
-      left[k] = t.n - at < kN ? (t.n - at > 0 ? (int)(t.n - at) : 0) : kN;
-      AdamVector<G, kN>::get(t.grad, at, left[k], g[k]);
-      if constexpr (kMaster)
-        AdamVector<float, kN>::get((const char*)a.master, place, left[k], p[k]);
-      else
-        AdamVector<P, kN>::get(t.param, at, left[k], p[k]);
-      if constexpr (kHeld) {
+    for (int e = 0; e < kN; ++e) m[e] = v[e] = 0.f;
+    if (left) {
+      // (codes of a whole vector are there: a tensor's moments go on to the end of a block)
+      const u32x2 cm = __builtin_nontemporal_load((const u32x2*)(a.first + place)), cv = __builtin_nontemporal_load((const u32x2*)(a.second + place));
+      const int64_t block = place / kMomentBlock;
+      const float sm = __uint_as_float((uint32_t)a.first_scales[block] << 23), sv = __uint_as_float((uint32_t)a.second_scales[block] << 23);
+      first_values(cm[0], sm, m);
+      first_values(cm[1], sm, m + 4);
+      second_values(cv[0], sv, v);
+      second_values(cv[1], sv, v + 4);
+      if (left < kN)
 #pragma unroll
-        for (int e = 0; e < kN; ++e) m[k][e] = v[k][e] = 0.f;
-        if (left[k]) {
-          // (codes of a whole vector are there: a tensor's moments go on to the end of a block)
-          const u32x2 cm = __builtin_nontemporal_load((const u32x2*)(a.first + place)), cv = __builtin_nontemporal_load((const u32x2*)(a.second + place));
-          const int64_t block = place / kMomentBlock;
-          const float sm = __uint_as_float((uint32_t)a.first_scales[block] << 23), sv = __uint_as_float((uint32_t)a.second_scales[block] << 23);
-          first_values(cm[0], sm, m[k]);
-          first_values(cm[1], sm, m[k] + 4);
-          second_values(cv[0], sv, v[k]);
-          second_values(cv[1], sv, v[k] + 4);
-          if (left[k] < kN)
-#pragma unroll
-            for (int e = 0; e < kN; ++e)
-              if (e >= left[k]) m[k][e] = v[k][e] = 0.f;
-        }
-      } else {
-        AdamVector<float, kN>::get(a.first, place, left[k], m[k]);
-        AdamVector<float, kN>::get(a.second, place, left[k], v[k]);
-      }
+        for (int e = 0; e < kN; ++e)
+          if (e >= left) m[e] = v[e] = 0.f;
     }
+  } else {
+    AdamVector<float, kN>::get(a.first, place, left, m);
+    AdamVector<float, kN>::get(a.second, place, left, v);
+  }
 #pragma unroll
-    for (int k = 0; k < kGroups; ++k) {
-      const int64_t at = first + k * kTurn, place = (int64_t)t.block * kMomentBlock + at;
+  for (int e = 0; e < kN; ++e) {
+    const float d = g[e] * scale;
+    m[e] = a.beta1 * m[e] + a.left1 * d;
+    v[e] = a.beta2 * v[e] + a.left2 * (d * d);
+    p[e] = p[e] * keep - rate * m[e] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[e]) * root + a.eps);
+  }
+  if constexpr (kMaster) AdamVector<float, kN>::put((char*)a.master, place, left, p);
+  AdamVector<P, kN>::put(t.param, at, left, p);
+  if constexpr (!kHeld) {
+    AdamVector<float, kN>::put(a.first, place, left, m);
+    AdamVector<float, kN>::put(a.second, place, left, v);
+  } else {
+    // A block's 16 lanes are here together: those past the end have nothing and take part in the block's maximum.
+    uint32_t top_m = 0, top_v = 0;
+#pragma unroll
+    for (int e = 0; e < kN; ++e) {
+      const uint32_t bm = magnitude(m[e]), bv = magnitude(v[e]);
+      top_m = bm > top_m ? bm : top_m, top_v = bv > top_v ? bv : top_v;
+    }
+    top_m = max16(top_m), top_v = max16(top_v);
+    // Blocks with something that is not finite, or with a v that may be rounded up to 2^128.
+    const bool odd = top_m >= kNotFinite || top_v >= 254u << 23;
+    if (odd) {
+      top_m = top_v = 0;
 #pragma unroll
       for (int e = 0; e < kN; ++e) {
-        const float d = g[k][e] * scale;
-        m[k][e] = a.beta1 * m[k][e] + a.left1 * d;
-        v[k][e] = a.beta2 * v[k][e] + a.left2 * (d * d);
-        p[k][e] = p[k][e] * keep - rate * m[k][e] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[k][e]) * root + a.eps);
+        const uint32_t bm = magnitude(m[e]), bv = magnitude(v[e]);
+        if (bm < kNotFinite && bm > top_m) top_m = bm;
+        if (bv < kNotFinite && bv > top_v) top_v = bv;
       }
-      if constexpr (kMaster) AdamVector<float, kN>::put((char*)a.master, place, left[k], p[k]);
-      AdamVector<P, kN>::put(t.param, at, left[k], p[k]);
-      if constexpr (!kHeld) {
-        AdamVector<float, kN>::put(a.first, place, left[k], m[k]);
-        AdamVector<float, kN>::put(a.second, place, left[k], v[k]);
-      } else {
-        // A block's 16 lanes are here together: those past the end have nothing and take part in the block's maximum.
-        uint32_t top_m = 0, top_v = 0;
+      top_m = max16(top_m), top_v = max16(top_v);
+    }
+    const uint32_t sm = first_scale(top_m), sv = second_scale(top_v);
+    if (left) {
+      const float inverse = __uint_as_float((254u - sm) << 23);
+      const uint32_t key = noise_key(step, (uint32_t)(place >> 32));
+      uint32_t random[kN];
+#pragma unroll
+      for (int e = 0; e < kN; ++e) random[e] = noise((uint32_t)place + e, key);
+      u32x2 cm, cv;
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        cm[w] = first_code<3>(m[4 * w + 3], inverse, random[4 * w + 3],
+                              first_code<2>(m[4 * w + 2], inverse, random[4 * w + 2],
+                                            first_code<1>(m[4 * w + 1], inverse, random[4 * w + 1], first_code<0>(m[4 * w], inverse, random[4 * w], 0u))));
+        cv[w] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) cv[w] |= second_code(v[4 * w + e], sv, random[4 * w + e]) << (8 * e);
+      }
+      if (odd) {
 #pragma unroll
         for (int e = 0; e < kN; ++e) {
-          const uint32_t bm = magnitude(m[k][e]), bv = magnitude(v[k][e]);
-          top_m = bm > top_m ? bm : top_m, top_v = bv > top_v ? bv : top_v;
+          const uint32_t shift = 8 * (e & 3), byte = 255u << shift, code = (cv[e >> 2] >> shift) & 255u;
+          if (magnitude(m[e]) >= kNotFinite) cm[e >> 2] = (cm[e >> 2] & ~byte) | 0x7fu << shift;
+          if (magnitude(v[e]) >= kNotFinite)
+            cv[e >> 2] |= byte;
+          else if (sv == 254u && code > 248u)  // 2 * 2^127 is no fp32
+            cv[e >> 2] = (cv[e >> 2] & ~byte) | 248u << shift;
         }
-        top_m = max16(top_m), top_v = max16(top_v);
-        // Blocks with something that is not finite, or with a v that may be rounded up to 2^128.
-        const bool odd = top_m >= kNotFinite || top_v >= 254u << 23;
-        if (odd) {
-          top_m = top_v = 0;
+      }
+      if (left >= kN) {
+        __builtin_nontemporal_store(cm, (u32x2*)(a.first + place));
+        __builtin_nontemporal_store(cv, (u32x2*)(a.second + place));
+      } else {
 #pragma unroll
-          for (int e = 0; e < kN; ++e) {
-            const uint32_t bm = magnitude(m[k][e]), bv = magnitude(v[k][e]);
-            if (bm < kNotFinite && bm > top_m) top_m = bm;
-            if (bv < kNotFinite && bv > top_v) top_v = bv;
+        for (int e = 0; e < kN; ++e)
+          if (e < left) {
+            a.first[place + e] = (char)(cm[e >> 2] >> (8 * (e & 3)));
+            a.second[place + e] = (char)(cv[e >> 2] >> (8 * (e & 3)));
           }
-          top_m = max16(top_m), top_v = max16(top_v);
-        }
-        const uint32_t sm = first_scale(top_m), sv = second_scale(top_v);
-        if (left[k]) {
-          const float inverse = __uint_as_float((254u - sm) << 23);
-          const uint32_t key = noise_key(step, (uint32_t)(place >> 32));
-          uint32_t random[kN];
-#pragma unroll
-          for (int e = 0; e < kN; ++e) random[e] = noise((uint32_t)place + e, key);
-          u32x2 cm, cv;
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            cm[w] = first_code<3>(m[k][4 * w + 3], inverse, random[4 * w + 3],
-                                  first_code<2>(m[k][4 * w + 2], inverse, random[4 * w + 2],
-                                                first_code<1>(m[k][4 * w + 1], inverse, random[4 * w + 1], first_code<0>(m[k][4 * w], inverse, random[4 * w], 0u))));
-            cv[w] = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) cv[w] |= second_code(v[k][4 * w + e], sv, random[4 * w + e]) << (8 * e);
-          }
-          if (odd) {
-#pragma unroll
-            for (int e = 0; e < kN; ++e) {
-              const uint32_t shift = 8 * (e & 3), byte = 255u << shift, code = (cv[e >> 2] >> shift) & 255u;
-              if (magnitude(m[k][e]) >= kNotFinite) cm[e >> 2] = (cm[e >> 2] & ~byte) | 0x7fu << shift;
-              if (magnitude(v[k][e]) >= kNotFinite)
-                cv[e >> 2] |= byte;
-              else if (sv == 254u && code > 248u)  // 2 * 2^127 is no fp32
-                cv[e >> 2] = (cv[e >> 2] & ~byte) | 248u << shift;
-            }
-          }
-          if (left[k] >= kN) {
-            __builtin_nontemporal_store(cm, (u32x2*)(a.first + place));
-            __builtin_nontemporal_store(cv, (u32x2*)(a.second + place));
-          } else {
-#pragma unroll
-            for (int e = 0; e < kN; ++e)
-              if (e < left[k]) {
-                a.first[place + e] = (char)(cm[e >> 2] >> (8 * (e & 3)));
-                a.second[place + e] = (char)(cv[e >> 2] >> (8 * (e & 3)));
-              }
-          }
-          if ((place & (kMomentBlock - 1)) == 0) {
-            const int64_t block = place / kMomentBlock;
-            a.first_scales[block] = (uint8_t)sm;
-            a.second_scales[block] = (uint8_t)sv;
-          }
-        }
+      }
+      if ((place & (kMomentBlock - 1)) == 0) {
+        const int64_t block = place / kMomentBlock;
+        a.first_scales[block] = (uint8_t)sm;
+        a.second_scales[block] = (uint8_t)sv;
       }
     }
   }

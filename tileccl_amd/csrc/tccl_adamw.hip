@@ -15,7 +15,7 @@ using namespace tccl;
 
 template <typename P, typename G>
 void launch(const AdamArgs& a, bool master, bool held, unsigned chunks, hipStream_t stream) {
-  const dim3 grid(chunks), threads(kAdamThreads);
+  const dim3 grid(chunks), threads(held ? kAdamThreadsHeld : kAdamThreads);
   if constexpr (sizeof(P) == 2) {
     if (master) {
       if (held)
@@ -101,6 +101,7 @@ int tccl_adamw(const tccl_adamw_desc* d, void* stream) {
   };
   // A launch counts its threads in 32 bits.
   constexpr uint64_t kMostChunks = 1u << 23;
+  const int chunk = d->bits == 8 ? kAdamChunkHeld : kAdamChunk;
   for (int i = 0; i < d->tensors; ++i) {
     const uint32_t first_block = block;
     block += (uint32_t)((d->sizes[i] + kMomentBlock - 1) / kMomentBlock);
@@ -109,12 +110,12 @@ int tccl_adamw(const tccl_adamw_desc* d, void* stream) {
         rc = send();
         if (rc) return rc;
       }
-      const int64_t room = (int64_t)(kMostChunks - chunks) * kAdamChunk, n = d->sizes[i] - done < room ? d->sizes[i] - done : room;
+      const int64_t room = (int64_t)(kMostChunks - chunks) * chunk, n = d->sizes[i] - done < room ? d->sizes[i] - done : room;
       AdamTensor& t = a.t[a.tensors++];
       t.param = (char*)d->params[i] + done * (d->dtype == TCCL_F32 ? 4 : 2);
       t.grad = (const char*)d->grads[i] + done * (d->grad_dtype == TCCL_F32 ? 4 : 2);
       t.n = n, t.block = first_block + (uint32_t)(done / kMomentBlock), t.first_chunk = (uint32_t)chunks;
-      chunks += (uint64_t)((n + kAdamChunk - 1) / kAdamChunk);
+      chunks += (uint64_t)((n + chunk - 1) / chunk);
       done += n;
     }
   }
