@@ -24,8 +24,8 @@ namespace tccl {
 constexpr int kMomentBlock = 128;
 constexpr int kAdamTensors = 100;   // of a launch: its arguments have to fit 4 KiB
 // Threads of a workgroup, and elements of a thread: each has one turn.  Moments in 32 bits: 4 elements, so that each access of a wavefront is 1 KiB in
-// a row.  In 8 bits: 8, 16 lanes a block.  Larger workgroups and several turns are slower (128M weights in 32 bits 618 us; 256 threads 629, 512
-// 648, with two turns 673; 197M in 8 bits, with the values, 773; 128 threads 783, two turns 788).
+// a row.  In 8 bits: 8, 16 lanes a block (4, 32 lanes, 585 us).  Larger workgroups and several turns are slower (128M weights in 32 bits 617 us; 256 threads
+// 629, 512 648, with two turns 673; 197M in 8 bits 563; 128 threads 572, two turns 575).
 constexpr int kAdamThreads = 128, kAdamThreadsHeld = 256;
 constexpr int kAdamChunk = 4 * kAdamThreads, kAdamChunkHeld = 8 * kAdamThreadsHeld;
 
@@ -153,8 +153,8 @@ struct AdamVector {
   }
 };
 
-// Bound by memory: bf16 weights with fp32 copy, gradients and moments, 128M of them, 670 us, 5.7 TB/s with as many writes as reads (a
-// plain copy of 512 MiB 5.3 to 6.1); moments in 8 bits, 197M with bf16 gradients, 570 us, 5.5 TB/s, the vector units half busy.
+// Bound by memory: bf16 weights with fp32 copy, gradients and moments, 128M of them, 617 us, 6.2 TB/s with as many writes as reads (a
+// plain copy of 512 MiB 5.3 to 6.1); moments in 8 bits, 197M with bf16 gradients, 563 us, 5.6 TB/s, the vector units half busy.
 template <typename P, typename G, bool kMaster, bool kHeld>
 __global__ __launch_bounds__(kHeld ? kAdamThreadsHeld : kAdamThreads) void adamw_kernel(AdamArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -293,7 +293,8 @@ __global__ __launch_bounds__(kHeld ? kAdamThreadsHeld : kAdamThreads) void adamw
 #endif
 }
 
-// The values that 8-bit moments stand for, exact in bf16: q * 2^e with 4 significant bits.  16 lanes a block.  197M 214 us, 5.5 TB/s.
+// The values that 8-bit moments stand for, exact in bf16: q * 2^e with 4 significant bits.  16 lanes a block.  197M 187 us, 6.3 TB/s (in turns
+// of 16384 workgroups 214).
 __global__ __launch_bounds__(256) void moments_kernel(MomentArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));

@@ -131,7 +131,7 @@ int tccl_adamw_moments(const tccl_adamw_moments_desc* d, void* stream) {
   if (((uintptr_t)d->first | (uintptr_t)d->second | (uintptr_t)d->to_first | (uintptr_t)d->to_second) & 15) return reportf(TCCL_ERR_UNSUPPORTED, "%s: moments and results must lie on 16 bytes", what);
   const MomentArgs a = {(const uint8_t*)d->first, (const uint8_t*)d->second, (const uint8_t*)d->first_scales, (const uint8_t*)d->second_scales, (char*)d->to_first, (char*)d->to_second, d->blocks};
   const int64_t wgs = (d->blocks + 15) / 16;
-  hipLaunchKernelGGL(moments_kernel, dim3((unsigned)(wgs < 16384 ? wgs : 16384)), dim3(256), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL(moments_kernel, dim3((unsigned)(wgs < 1 << 23 ? wgs : 1 << 23)), dim3(256), 0, (hipStream_t)stream, a);
   return launched(what);
 }
 

@@ -25,7 +25,7 @@ struct Copies {
     j.from = from, j.to = at + last + to_col * 2, j.ld_from = ld_from, j.ld_to = ld_to;
     j.cols = cols, j.per_row = (int)(vectors(cols) / 8), j.chunks = rows * j.per_row;
     const int64_t wgs = (j.chunks + 255) / 256;
-    j.first_wg = all, j.wgs = (int)(wgs < 8192 ? wgs : 8192), all += j.wgs;
+    j.first_wg = all, j.wgs = (int)(wgs < 1 << 20 ? wgs : 1 << 20), all += j.wgs;
     return at + last;
   }
   template <typename T>

@@ -448,7 +448,8 @@ __global__ __launch_bounds__(256) void gated_join_kernel(GatedArgs a) {
 #endif
 }
 
-// dg and du from z as it was kept.  Every value is read once; inner may be kept itself.  Bound by memory: 4096 x 4096 bf16 28 us, 6.0 TB/s.
+// dg and du from z as it was kept.  Every value is read once; inner may be kept itself.  Bound by memory: 4096 x 4096 bf16 28 us,
+// 6.0 TB/s; 8192 x 8192 116, 5.8 (in turns of 8192 workgroups 124).
 template <typename T>
 __global__ __launch_bounds__(256) void gated_grad_kernel(GatedGradArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)

@@ -163,7 +163,7 @@ int launch(const char* what, GatedArgs& a, const Choice& c, bool kmajor, int cus
                                  : launch_tile<T, 128, kBackward>(what, a, kmajor, cus, stream);
   if (rc || !a.partial) return rc;
   const int64_t wgs = ((int64_t)a.p.M * a.p.N + 255) / 256;
-  hipLaunchKernelGGL((gated_join_kernel<T, kBackward>), dim3((unsigned)(wgs < 2048 ? wgs : 2048)), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((gated_join_kernel<T, kBackward>), dim3((unsigned)(wgs < 1 << 23 ? wgs : 1 << 23)), dim3(256), 0, stream, a);
   return launched(what);
 }
 
@@ -273,7 +273,7 @@ int tccl_gated_grad(const tccl_gated_grad_desc* d, void* stream) {
   if (rc) return rc;
   const GatedGradArgs a = {(const char*)d->grad, (const char*)d->kept, (char*)d->inner, d->ld_grad, d->ld_kept, d->ld_inner, s.rows, s.outputs, s.activation};
   const int64_t wgs = ((int64_t)s.rows * ((s.outputs + 7) / 8) + 255) / 256;
-  const dim3 grid((unsigned)(wgs < 8192 ? wgs : 8192));
+  const dim3 grid((unsigned)(wgs < 1 << 23 ? wgs : 1 << 23));  // (a launch counts its threads in 32 bits)
   if (d->dtype == TCCL_BF16)
     hipLaunchKernelGGL((gated_grad_kernel<__bf16>), grid, dim3(256), 0, st, a);
   else
