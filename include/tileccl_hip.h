@@ -655,9 +655,9 @@ typedef struct tccl_gated_desc {
   int32_t kmajor;
 } tccl_gated_desc;
 int64_t tccl_gated_workspace(const tccl_gated_desc* gated);
-/* Host view of how a device of `compute_units` cuts such a call (backward: tccl_gated_grad without kept): tiles of 256 or 128 (rows and
+/* Host view of how a device of `compute_units` cuts such a call, or a tccl_gated_grad without kept: tiles of 256 or 128 (rows and
  * columns of z; 0: the kernels for few rows), the rows and outputs of a workgroup's part, the splits of the inputs over workgroups. */
-int tccl_gated_cut(int32_t rows, int32_t inputs, int32_t outputs, int32_t kmajor, int32_t backward, int32_t compute_units, int32_t* tile, int32_t* tile_rows,
+int tccl_gated_cut(int32_t rows, int32_t inputs, int32_t outputs, int32_t kmajor, int32_t compute_units, int32_t* tile, int32_t* tile_rows,
                    int32_t* tile_outputs, int32_t* splits);
 int tccl_gated(const tccl_gated_desc* gated, void* stream);
 

@@ -176,9 +176,9 @@ def test_bad_adamw_descriptors(lib):
     assert moments(blocks=0) == 0
 
 
-def gated_cut(lib, rows, inputs, outputs, kmajor=0, backward=0, cus=256):
+def gated_cut(lib, rows, inputs, outputs, kmajor=0, cus=256):
     got = [C.c_int32() for _ in range(4)]
-    assert lib.tccl_gated_cut(rows, inputs, outputs, kmajor, backward, cus, *map(C.byref, got)) == 0
+    assert lib.tccl_gated_cut(rows, inputs, outputs, kmajor, cus, *map(C.byref, got)) == 0
     return tuple(g.value for g in got)
 
 
@@ -188,18 +188,17 @@ def test_how_calls_are_cut(lib):
     assert gated_cut(lib, 20, 4096, 4096) == (0, 32, 64, 4) and gated_cut(lib, 40, 4096, 1024) == (0, 64, 32, 8)
     assert gated_cut(lib, 40, 512, 512) == (0, 64, 16, 1) and gated_cut(lib, 64, 584, 8192, 1) == (0, 64, 32, 1)
     assert gated_cut(lib, 8192, 4096, 8192, 1) == (256, 256, 128, 1) and gated_cut(lib, 1003, 1001, 1035)[0] == 128
-    assert gated_cut(lib, 112, 7168, 104, 1) == (0, 64, 16, 8) and gated_cut(lib, 1000, 4096, 512, 0, 1)[::3] == (128, 4)
-    for backward in (0, 1):
-        for rows, inputs, outputs, _, layout, _ in test_gpu_gated.LARGE:
-            assert gated_cut(lib, rows, inputs, outputs, layout == "nk", backward) == (256, 256, 128, 1)
-        kinds = {(layout, *gated_cut(lib, rows, inputs, outputs, layout == "nk", backward)[:3]) for rows, inputs, outputs, _, layout, _ in test_gpu_gated.SPLIT}
-        assert all(("kn", *k) in kinds for k in ((0, 16, 64), (0, 32, 64), (0, 64, 16), (0, 64, 32), (128, 128, 64)))
-        assert all(("nk", *k) in kinds for k in ((0, 16, 16), (0, 16, 32), (0, 32, 16), (0, 32, 32), (0, 64, 16), (0, 64, 32), (128, 128, 64)))
+    assert gated_cut(lib, 112, 7168, 104, 1) == (0, 64, 16, 8) and gated_cut(lib, 1000, 4096, 512)[::3] == (128, 4)
+    for rows, inputs, outputs, _, layout, _ in test_gpu_gated.LARGE:
+        assert gated_cut(lib, rows, inputs, outputs, layout == "nk") == (256, 256, 128, 1)
+    kinds = {(layout, *gated_cut(lib, rows, inputs, outputs, layout == "nk")[:3]) for rows, inputs, outputs, _, layout, _ in test_gpu_gated.SPLIT}
+    assert all(("kn", *k) in kinds for k in ((0, 16, 64), (0, 32, 64), (0, 64, 16), (0, 64, 32), (128, 128, 64)))
+    assert all(("nk", *k) in kinds for k in ((0, 16, 16), (0, 16, 32), (0, 32, 16), (0, 32, 32), (0, 64, 16), (0, 64, 32), (128, 128, 64)))
     got = [C.c_int32() for _ in range(3)]
     for shape, want in (((128, 4200, 2056), 256), ((1000, 1000, 3088), 128)):
         assert lib.tccl_weight_gradient_full_cut(*shape, 256, *map(C.byref, got)) == 0 and got[0].value == want
     assert lib.tccl_weight_gradient_full_cut(16384, 1024, 512, 256, *map(C.byref, got)) == 0 and got[1].value == 8
-    refused(lib.tccl_gated_cut(8, 8, 8, 0, 0, 0, *[C.byref(C.c_int32()) for _ in range(4)]), "0 compute units")
+    refused(lib.tccl_gated_cut(8, 8, 8, 0, 0, *[C.byref(C.c_int32()) for _ in range(4)]), "0 compute units")
     refused(lib.tccl_weight_gradient_full_cut(8, 8, 8, 256, None, None, None), "NULL result")
 
 

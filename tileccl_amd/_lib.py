@@ -414,7 +414,7 @@ SIGNATURES = {
     "tccl_weight_gradient_full": (C.c_int, [_P(WeightGradientFullDesc), _vp]),
     "tccl_weight_gradient_full_cut": (C.c_int, [_i32, _i32, _i32, _i32, _P(_i32), _P(_i32), _P(_i32)]),
     "tccl_gated_workspace": (_i64, [_P(GatedDesc)]),
-    "tccl_gated_cut": (C.c_int, [_i32, _i32, _i32, _i32, _i32, _i32, _P(_i32), _P(_i32), _P(_i32), _P(_i32)]),
+    "tccl_gated_cut": (C.c_int, [_i32, _i32, _i32, _i32, _i32, _P(_i32), _P(_i32), _P(_i32), _P(_i32)]),
     "tccl_gated": (C.c_int, [_P(GatedDesc), _vp]),
     "tccl_gated_grad_workspace": (_i64, [_P(GatedGradDesc)]),
     "tccl_gated_grad": (C.c_int, [_P(GatedGradDesc), _vp]),

@@ -394,6 +394,13 @@ struct GatedRows {
           to[0] = z, to[p.N] = y;
           continue;
         }
+        if (g.inner) {
+          float slope;
+          const float activation = activated<decltype(act)::value, true>(z, slope), d = (float)((const T*)g.grad)[(int64_t)(m0 + row) * g.ld_grad + n0 + col];
+          T* inner = (T*)g.inner + (int64_t)(m0 + row) * g.ld_inner + n0 + col;
+          inner[0] = to_out<T>(d * y * slope), inner[p.N] = to_out<T>(d * activation);
+          continue;
+        }
         ((T*)g.out)[(int64_t)(m0 + row) * g.ld_out + n0 + col] = to_out<T>(activated<decltype(act)::value>(z) * y);
         if (g.kept) {
           T* kept = (T*)g.kept + (int64_t)(m0 + row) * g.ld_kept + n0 + col;

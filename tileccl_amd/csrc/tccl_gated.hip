@@ -91,12 +91,12 @@ double join_takes(int splits, int64_t rows, int64_t outputs) { return 4.0 + spli
 // The variant whose estimate is least.  The figures are fitted to calls of 1 .. 4000 rows, 104 .. 8192 outputs, 512 .. 8192 inputs, whose best
 // variant the choice reaches within a tenth, mostly.  Inputs are split over workgroups where these would leave CUs without work
 // (112 x 7168 x 104 in 128 tiles 46 us, split in 8 14.6, in narrow tiles split in 8 11).
-Choice choose(int rows, int inputs, int outputs, bool kmajor, bool few, bool backward, int cus) {
+Choice choose(int rows, int inputs, int outputs, bool kmajor, bool few, int cus) {
   Choice best = {0, 0, 0, 1};
   const int blocks = (inputs + 63) / 64;
   double least = 1e30;
   auto consider = [&](const Choice& c, double us) {
-    if (c.splits > 1 || (backward && !c.tile)) us += join_takes(c.splits, rows, outputs);
+    if (c.splits > 1) us += join_takes(c.splits, rows, outputs);
     if (us < least) best = c, least = us;
   };
   auto consider_rows = [&](int m, int n) {
@@ -177,13 +177,13 @@ struct Prepared {
   explicit Prepared(void* workspace) : copies(workspace) {}
 
   template <typename Desc>
-  int of(const char* what, const Sizes& s, const Desc* d, bool backward) {
+  int of(const char* what, const Sizes& s, const Desc* d) {
     int rc = set_product(what, s, d->x, d->ld_x, d->weight, d->ld_weight, d->up, d->kmajor, a.p, copies);
     if (!rc) rc = compute_units(&cus);
     if (rc) return rc;
-    c = choose(s.rows, s.inputs, s.outputs, d->kmajor, within_reach(s.inputs, s.outputs, a.p.ldb, d->kmajor), backward, cus);
+    c = choose(s.rows, s.inputs, s.outputs, d->kmajor, within_reach(s.inputs, s.outputs, a.p.ldb, d->kmajor), cus);
     bytes = copies.bytes;
-    if (c.splits > 1 || (backward && !c.tile)) {  // (the kernels for few rows have no gradient of their own)
+    if (c.splits > 1) {
       a.partial = (float*)(copies.at + copies.bytes);
       bytes += 4ll * c.splits * s.rows * 2 * s.outputs;
     }
@@ -211,7 +211,7 @@ int64_t tccl_gated_workspace(const tccl_gated_desc* d) {
   if (!d) return reportf(TCCL_ERR_INVALID, "%s: the descriptor is NULL", what), -1;
   const Sizes s = {d->rows, d->inputs, d->outputs, d->dtype, d->activation};
   Prepared p(nullptr);
-  if (check_sizes(what, s) || (s.rows && p.of(what, s, d, false))) return -1;
+  if (check_sizes(what, s) || (s.rows && p.of(what, s, d))) return -1;
   return p.bytes;
 }
 
@@ -224,19 +224,19 @@ int tccl_gated(const tccl_gated_desc* d, void* stream) {
   rc = check_matrix(what, "out", d->out, d->ld_out, s.rows, s.outputs);
   if (!rc && d->kept) rc = check_matrix(what, "kept", d->kept, d->ld_kept, s.rows, 2 * s.outputs);
   Prepared p(d->workspace);
-  if (!rc) rc = p.of(what, s, d, false);
+  if (!rc) rc = p.of(what, s, d);
   if (!rc) rc = p.enough(what, d->workspace, d->workspace_bytes);
   if (rc) return rc;
   p.a.out = (char*)d->out, p.a.ld_out = d->ld_out, p.a.kept = (char*)d->kept, p.a.ld_kept = d->ld_kept;
   return p.send<false>(what, d->dtype, d->kmajor, (hipStream_t)stream);
 }
 
-int tccl_gated_cut(int32_t rows, int32_t inputs, int32_t outputs, int32_t kmajor, int32_t backward, int32_t compute_units, int32_t* tile, int32_t* tile_rows, int32_t* tile_outputs,
+int tccl_gated_cut(int32_t rows, int32_t inputs, int32_t outputs, int32_t kmajor, int32_t compute_units, int32_t* tile, int32_t* tile_rows, int32_t* tile_outputs,
                    int32_t* splits) {
   const int rc = check_sizes("gated_cut", Sizes{rows, inputs, outputs, TCCL_BF16, TCCL_SILU});
   if (rc) return rc;
   if (compute_units < 1 || !tile || !tile_rows || !tile_outputs || !splits) return reportf(TCCL_ERR_INVALID, "gated_cut: %d compute units, or a NULL result", compute_units);
-  const Choice c = choose(rows, inputs, outputs, kmajor != 0, true, backward != 0, compute_units);
+  const Choice c = choose(rows, inputs, outputs, kmajor != 0, true, compute_units);
   *tile = c.tile, *splits = c.splits;
   *tile_rows = c.tile ? c.tile : 16 * c.blocks_m, *tile_outputs = c.tile ? c.tile / 2 : 8 * c.blocks_n;
   return 0;
@@ -247,7 +247,7 @@ int64_t tccl_gated_grad_workspace(const tccl_gated_grad_desc* d) {
   if (!d) return reportf(TCCL_ERR_INVALID, "%s: the descriptor is NULL", what), -1;
   const Sizes s = {d->rows, d->inputs, d->outputs, d->dtype, d->activation};
   Prepared p(nullptr);
-  if (check_sizes(what, s) || (s.rows && !d->kept && p.of(what, s, d, true))) return -1;
+  if (check_sizes(what, s) || (s.rows && !d->kept && p.of(what, s, d))) return -1;
   return p.bytes;
 }
 
@@ -263,7 +263,7 @@ int tccl_gated_grad(const tccl_gated_grad_desc* d, void* stream) {
   const hipStream_t st = (hipStream_t)stream;
   if (!d->kept) {
     Prepared p(d->workspace);
-    rc = p.of(what, s, d, true);
+    rc = p.of(what, s, d);
     if (!rc) rc = p.enough(what, d->workspace, d->workspace_bytes);
     if (rc) return rc;
     p.a.grad = (const char*)d->grad, p.a.ld_grad = d->ld_grad, p.a.inner = (char*)d->inner, p.a.ld_inner = d->ld_inner;
