@@ -682,6 +682,25 @@ typedef struct tccl_gated_grad_desc {
 int64_t tccl_gated_grad_workspace(const tccl_gated_grad_desc* gated);
 int tccl_gated_grad(const tccl_gated_grad_desc* gated, void* stream);
 
+/* The gradient of x from that of z: dx (rows x inputs) = inner times the weight's transpose, in tiles that split the sum over workgroups; for few rows and
+ * inputs with many outputs.  `splits` of the host view _cut (compute_units 0: of the current device) is 0 where tccl_gemm is quicker.  The weight is
+ * tccl_gated's, both halves in one matrix: kmajor 0: inputs rows of 2 outputs; kmajor 1: 2 outputs rows of inputs.  Alignments and the workspace
+ * as tccl_gated's; dx shares no memory with an operand. */
+typedef struct tccl_gated_input_grad_desc {
+  const void* inner;
+  const void* weight;
+  void* dx;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t ld_inner, ld_weight, ld_dx;
+  int32_t rows, inputs, outputs;
+  int32_t dtype;
+  int32_t kmajor;
+} tccl_gated_input_grad_desc;
+int64_t tccl_gated_input_grad_workspace(const tccl_gated_input_grad_desc* grad);
+int tccl_gated_input_grad_cut(int32_t rows, int32_t inputs, int32_t outputs, int32_t compute_units, int32_t* splits);
+int tccl_gated_input_grad(const tccl_gated_input_grad_desc* grad, void* stream);
+
 /* AdamW over many tensors, in fp32: with g = grad * grad_scale,
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
  *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps).

@@ -123,6 +123,23 @@ def test_backward_pitches_and_places(rows, inputs, outputs, layout):
             assert bool((memory == 7.0).all()), "bytes around inner were written"
 
 
+# Sums over the projections that are split over workgroups.
+LONG = [(300, 264, 16384 // 2, BF16, "kn"), (1030, 232, 8200, F16, "nk"), (200, 1001, 8195, BF16, "kn"), (700, 703, 4100, F16, "nk"), (1003, 1000, 2100, BF16, "kn")]
+
+
+@pytest.mark.parametrize("rows, inputs, outputs, dtype, layout", LONG)
+def test_input_gradient_from_many_outputs(rows, inputs, outputs, dtype, layout):
+    dh, kept = rand((rows, outputs), 61, dtype, 0.1), rand((rows, 2 * outputs), 62, dtype)
+    w, wd = weight_of(inputs, outputs, dtype, layout, 63, pad=3 * (inputs % 8 > 0), offset=inputs % 8)
+    for pad in (0, 5):
+        d = ops.gated_linear_backward(dh.cuda(), placed(kept, 2 * outputs + pad, pad), None, wd, weights=False,
+                                      out=torch.empty(rows, 2 * outputs + pad, dtype=dtype, device="cuda")[:, : 2 * outputs])
+        inner = d.inner.cpu().double()
+        want = inner @ w.double().t()
+        within(d.x, want, rounded(want, 2 * outputs * SUM * (inner.abs() @ w.double().abs().t()), dtype), "dx")
+        assert d.x.is_contiguous() and torch.equal(d.x, ops.gated_linear_backward(dh.cuda(), kept.cuda(), None, wd, weights=False).x)
+
+
 def test_backward_against_differences():
     """The gradients are those of sum(dh * gated(x, w)): against differences of the 64-bit definition."""
     rows, inputs, outputs = 3, 16, 8

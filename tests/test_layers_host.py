@@ -65,7 +65,7 @@ def refused(rc, text, code=None):
 
 
 def test_bad_gated_descriptors(lib):
-    for entry in (lib.tccl_gated, lib.tccl_gated_grad, lib.tccl_weight_gradient_full, lib.tccl_adamw, lib.tccl_adamw_moments):
+    for entry in (lib.tccl_gated, lib.tccl_gated_grad, lib.tccl_gated_input_grad, lib.tccl_weight_gradient_full, lib.tccl_adamw, lib.tccl_adamw_moments):
         refused(entry(None, None), "the descriptor is NULL")
 
     def forward(**kw):
@@ -107,6 +107,21 @@ def test_bad_gated_descriptors(lib):
         assert entry(C.byref(desc(rows=4, outputs=8))) == -1 and "must be positive" in _lib.last_error()
     assert lib.tccl_gated_workspace(C.byref(_lib.GatedDesc(inputs=8, outputs=8, dtype=_lib.F16))) == 0  # no rows
     assert lib.tccl_gated_grad_workspace(C.byref(_lib.GatedGradDesc(kept=0x1000, rows=8, inputs=8, outputs=8, dtype=_lib.F16))) == 0
+    def input_grad(**kw):
+        d = _lib.GatedInputGradDesc(inner=0x1000, weight=0x2000, dx=0x3000, ld_inner=256, ld_weight=256, ld_dx=64, rows=4, inputs=64, outputs=128, dtype=_lib.F16)
+        for k, v in kw.items():
+            setattr(d, k, v)
+        return lib.tccl_gated_input_grad(C.byref(d), None)
+
+    assert input_grad(rows=0) == 0 and lib.tccl_gated_input_grad_workspace(None) == -1
+    refused(input_grad(rows=-1), "rows must not be negative")
+    refused(input_grad(dtype=_lib.F32), "F16 or BF16", un)
+    refused(input_grad(inner=None), "inner is NULL")
+    refused(input_grad(ld_inner=255), "inner has a pitch of 255 elements for 256 columns")
+    refused(input_grad(ld_weight=200), "weight has a pitch of 200 elements for 256 columns")
+    refused(input_grad(kmajor=1, ld_weight=60), "weight has a pitch of 60 elements for 64 columns")
+    refused(input_grad(dx=0x3001), "dx is not aligned to its type")
+    refused(input_grad(ld_dx=63), "dx has a pitch of 63 elements for 64 columns")
     refused(backward(grad=None), "grad is NULL")
     refused(backward(inner=None), "inner is NULL")
     refused(backward(ld_kept=128), "kept has a pitch of 128")
@@ -194,6 +209,12 @@ def test_how_calls_are_cut(lib):
     kinds = {(layout, *gated_cut(lib, rows, inputs, outputs, layout == "nk")[:3]) for rows, inputs, outputs, _, layout, _ in test_gpu_gated.SPLIT}
     assert all(("kn", *k) in kinds for k in ((0, 16, 64), (0, 32, 64), (0, 64, 16), (0, 64, 32), (128, 128, 64)))
     assert all(("nk", *k) in kinds for k in ((0, 16, 16), (0, 16, 32), (0, 32, 16), (0, 32, 32), (0, 64, 16), (0, 64, 32), (128, 128, 64)))
+    splits = C.c_int32()
+    for rows, inputs, outputs, _, _ in test_gpu_gated.LONG:
+        assert lib.tccl_gated_input_grad_cut(rows, inputs, outputs, 256, C.byref(splits)) == 0 and splits.value >= 2
+    for shape in ((64, 128, 2048), (2048, 2048, 4096), (300, 256, 600), (1, 4096, 4096)):
+        assert lib.tccl_gated_input_grad_cut(*shape, 256, C.byref(splits)) == 0 and splits.value == 0
+    refused(lib.tccl_gated_input_grad_cut(8, 8, 8, 256, None), "NULL result")
     got = [C.c_int32() for _ in range(3)]
     for shape, want in (((128, 4200, 2056), 256), ((1000, 1000, 3088), 128)):
         assert lib.tccl_weight_gradient_full_cut(*shape, 256, *map(C.byref, got)) == 0 and got[0].value == want
@@ -205,6 +226,7 @@ def test_how_calls_are_cut(lib):
 @pytest.mark.skipif(shutil.which("gcc") is None, reason="needs gcc")
 def test_descriptors_as_gcc_sees_them(tmp_path):
     structs = {"tccl_weight_gradient_full_desc": _lib.WeightGradientFullDesc, "tccl_gated_desc": _lib.GatedDesc, "tccl_gated_grad_desc": _lib.GatedGradDesc,
+               "tccl_gated_input_grad_desc": _lib.GatedInputGradDesc,
                "tccl_adamw_desc": _lib.AdamwDesc, "tccl_adamw_moments_desc": _lib.AdamwMomentsDesc}
     body = ""
     for cname, py in structs.items():

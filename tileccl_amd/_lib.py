@@ -285,6 +285,24 @@ class GatedGradDesc(C.Structure):
     ]
 
 
+class GatedInputGradDesc(C.Structure):
+    _fields_ = [
+        ("inner", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("dx", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+        ("ld_inner", C.c_int64),
+        ("ld_weight", C.c_int64),
+        ("ld_dx", C.c_int64),
+        ("rows", C.c_int32),
+        ("inputs", C.c_int32),
+        ("outputs", C.c_int32),
+        ("dtype", C.c_int32),
+        ("kmajor", C.c_int32),
+    ]
+
+
 class AdamwDesc(C.Structure):
     _fields_ = [
         ("params", C.c_void_p),
@@ -418,6 +436,9 @@ SIGNATURES = {
     "tccl_gated": (C.c_int, [_P(GatedDesc), _vp]),
     "tccl_gated_grad_workspace": (_i64, [_P(GatedGradDesc)]),
     "tccl_gated_grad": (C.c_int, [_P(GatedGradDesc), _vp]),
+    "tccl_gated_input_grad_workspace": (_i64, [_P(GatedInputGradDesc)]),
+    "tccl_gated_input_grad_cut": (C.c_int, [_i32, _i32, _i32, _i32, _P(_i32)]),
+    "tccl_gated_input_grad": (C.c_int, [_P(GatedInputGradDesc), _vp]),
     "tccl_adamw": (C.c_int, [_P(AdamwDesc), _vp]),
     "tccl_adamw_moments": (C.c_int, [_P(AdamwMomentsDesc), _vp]),
     "tccl_mfma_rate_probe": (C.c_int, [_i32, _vp, _i64, _vp, _i64, _vp, _i32, _i32, _vp]),

@@ -3,7 +3,7 @@ that read a scalar register too soon.
 
 ``python -m tileccl_amd.csrc.check_spills`` compiles the library's sources to
 assembly (some five minutes) and, for every ``gemm256_kernel`` / ``fused256_kernel`` / ``weight_gradient_kernel`` /
-``weight_full_kernel`` / ``gated_kernel`` / ``gated_rows_kernel`` instantiation, counts the scratch-memory instructions that lie between the kernel's first and last
+``weight_full_kernel`` / ``gated_kernel`` / ``gated_rows_kernel`` / ``input_grad_kernel`` instantiation, counts the scratch-memory instructions that lie between the kernel's first and last
 MFMA, i.e. inside its K loops.  A register that the compiler keeps in scratch memory there is
 reloaded through the same queue as the operand loads, so the reload waits for all of them: a
 handful of such reloads per K step has cost the fused launches more than a third of their time.
@@ -42,7 +42,7 @@ from tileccl_amd.csrc.build import FLAGS, HERE, SOURCES
 def kernels(asm: str):
     """(name, vgprs, scratch instructions in the K loops, scratch instructions in all) per kernel with a K loop."""
     counts = dict(re.findall(r"\.name:\s+(\S+)\n(?:.*\n)*?\s+\.vgpr_count:\s+(\d+)", asm))
-    for match in re.finditer(r"^(_ZN4tccl(?:1[45](?:gemm|fused)256|22weight_gradient|18weight_full|12gated|17gated_rows)_kernel\w*):", asm, flags=re.M):
+    for match in re.finditer(r"^(_ZN4tccl(?:1[45](?:gemm|fused)256|22weight_gradient|18weight_full|12gated|17gated_rows|17input_grad)_kernel\w*):", asm, flags=re.M):
         name = match.group(1)
         body = asm[match.end(): asm.index(".Lfunc_end", match.end())].split("\n")
         mfma = [i for i, line in enumerate(body) if "v_mfma" in line]

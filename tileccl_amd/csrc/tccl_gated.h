@@ -8,6 +8,7 @@
 #pragma once
 
 #include "tccl_product.h"
+#include "tccl_weight.h"
 
 namespace tccl {
 
@@ -25,6 +26,16 @@ struct GatedArgs {
   // K split over workgroups: blocks of 64 k in each split, and where their sums go: [split][row][2 N] (NULL: nowhere, a workgroup has them all).
   int splits, blocks_per_split;
   float* partial;
+};
+
+struct InputGradArgs {
+  ProductArgs p;      // M: tokens, N: inputs, K: both projections
+  char* out;
+  float* partial;     // [split][M][ld_partial], where K is split
+  int64_t ld_out, ld_partial;
+  int tiles_m, tiles_n, band;
+  int splits, blocks_per_split;
+  int xcds, per_xcd;
 };
 
 struct GatedGradArgs {
@@ -422,6 +433,41 @@ __global__ __launch_bounds__(kWaves * 64, kMB == 1 && kNB == 2 ? 4 : 2) void gat
   if (id >= tiles * a.splits) return;
   const int split = id / tiles, t = id - split * tiles;
   Tile(a, rows_lds).tile(t % a.tiles_m * (16 * kMB), t / a.tiles_m * (8 * kNB), split);
+#endif
+}
+
+// dx = inner W', the tiles of Product without pairs: of few outputs and a long sum, where the GEMM's kernels, which do not split K, leave CUs without
+// work.  Sums of splits are added up by weight_sum_kernel.  Bound by
+// what comes from L2 to a CU, as gated_kernel's 128 tiles: 1024 x 2048 from 8192 42 us (the GEMM 62),
+// 4142 x 232 from 7952 32 to 35 (70 to 77), 8192 x 128 from 16384 62 (81 to 95).
+template <typename T, bool kBDeep>
+__global__ __launch_bounds__(512, 2) void input_grad_kernel(InputGradArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef Product<T, 128, false, kBDeep, false> Tile;
+  __shared__ __attribute__((aligned(1024))) char grad_lds[Tile::kLds];
+  const int tiles = a.tiles_m * a.tiles_n, item = (int)blockIdx.x % a.xcds * a.per_xcd + (int)blockIdx.x / a.xcds;
+  if (item >= tiles * a.splits) return;
+  const int split = item / tiles;
+  const TileCoord at = tile_coords(item - split * tiles, a.tiles_m, a.tiles_n, a.band);
+  const int m0 = at.m * 128, n0 = at.n * 128, first = split * a.blocks_per_split, all = (a.p.K + 63) / 64;
+  const int steps = all - first < a.blocks_per_split ? all - first : a.blocks_per_split;
+  Tile t(a.p, grad_lds);
+  typename Tile::Sums acc;
+  Tile::clear(acc);
+  if (steps > 0) t.run(acc, m0, n0, first, steps);
+#pragma unroll
+  for (int i = 0; i < Tile::kRows; ++i)
+#pragma unroll
+    for (int j = 0; j < Tile::kBlocksN; ++j) {
+      const int64_t row = m0 + t.out_row(i);
+      const int col = n0 + t.wn * 64 + 16 * j + 4 * (t.lane >> 4);
+      if (row < a.p.M && col < a.p.N) {
+        if (a.splits > 1)
+          put4<float>(acc[i][j], (char*)(a.partial + (int64_t)split * a.p.M * a.ld_partial), row * a.ld_partial + col, a.p.N - col);
+        else
+          put4<T>(acc[i][j], a.out, row * a.ld_out + col, a.p.N - col);
+      }
+    }
 #endif
 }
 

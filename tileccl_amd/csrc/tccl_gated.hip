@@ -77,6 +77,11 @@ double tiles_take(int tile, int64_t tiles, int steps, int cus) {
   const double rounds = (double)((tiles + cus - 1) / cus), busy = tiles < cus ? (double)tiles / cus : 1.0;
   return tile == 256 ? 6.0 + steps * rounds * (rounds > 1 ? 1.5 : 1.12 + 0.48 * busy) : 6.5 + (steps + 1) / 2 * rounds * (rounds > 1 ? 1.0 : 0.78 + 0.15 * busy);
 }
+// ... by 128 tiles with K split: several rounds of shorter ones may fill the device better, and each starts anew.
+double split_takes(int64_t tiles, int blocks, int splits, int cus) {
+  const double again = (double)((tiles * splits - 1) / cus);
+  return tiles_take(128, tiles * splits, (blocks + splits - 1) / splits, cus) + (splits > 1 ? 1.0 + 3.0 * again : 0.0);
+}
 // ... by the kernels for few rows, of `wgs` workgroups with `turns` times 512 k each.  Narrow tiles of a weight by rows read it in pieces of 32 or 64
 // bytes, at a rate of their own.
 double rows_take(int blocks_m, int blocks_n, int64_t wgs, double turns, bool kmajor, double weight_bytes, int cus) {
@@ -115,8 +120,8 @@ Choice choose(int rows, int inputs, int outputs, bool kmajor, bool few, int cus)
   }
   const int64_t large = (int64_t)((rows + 255) / 256) * ((outputs + 127) / 128), small = (int64_t)((rows + 127) / 128) * ((outputs + 63) / 64);
   consider({256, 0, 0, 1}, tiles_take(256, large, blocks, cus));
-  for (int splits = 1; splits <= 16 && (splits == 1 || (small * splits <= cus && blocks >= 4 * splits)); splits *= 2)
-    consider({128, 0, 0, splits}, tiles_take(128, small * splits, (blocks + splits - 1) / splits, cus) + (splits > 1));
+  for (int splits = 1; splits <= 16 && (splits == 1 || blocks >= 4 * splits); ++splits)
+    consider({128, 0, 0, splits}, split_takes(small, blocks, splits, cus));
   return best;
 }
 
@@ -202,6 +207,73 @@ struct Prepared {
   }
 };
 
+// The gradient of x by these kernels: how often the sum is split, 0 where the library's GEMM is left to make it, which is as quick where tiles
+// are many or the sum is short (37 shapes of both layouts, this and the GEMM: 1000 x 1000 from 6000 24 to 25 us and 31 to 34, from 4096 21 and 19 to 25,
+// from 1200 16 and 10 to 11; 1 x 4096 from 8192 15 and 14 to 19; 300 x 256 from 4096 12.6 and 7.4 to 8.6; 256 x 256 from 16384 16 and 16 to 29).
+int input_grad_splits(int rows, int inputs, int depth, int cus) {
+  const int64_t tiles = (int64_t)((rows + 127) / 128) * ((inputs + 127) / 128);
+  const int blocks = (depth + 63) / 64;
+  if (rows < 64 || tiles * 2 > cus || tiles * blocks < (blocks < 256 ? 4096 : 1024)) return 0;
+  int best = 0;
+  double least = 1e30;
+  for (int splits = 2; splits <= 16 && blocks >= 4 * splits; ++splits) {
+    const double us = split_takes(tiles, blocks, splits, cus) + join_takes(splits, rows, (inputs + 1) / 2);
+    if (us < least) best = splits, least = us;
+  }
+  return best;
+}
+
+int check_input_grad(const char* what, const tccl_gated_input_grad_desc* d) {
+  if (!d) return reportf(TCCL_ERR_INVALID, "%s: the descriptor is NULL", what);
+  int rc = check_sizes(what, Sizes{d->rows, d->inputs, d->outputs, d->dtype, TCCL_SILU});
+  if (rc || !d->rows) return rc;
+  rc = check_matrix(what, "inner", d->inner, d->ld_inner, d->rows, 2 * d->outputs);
+  if (!rc) rc = check_matrix(what, "weight", d->weight, d->ld_weight, d->kmajor ? 2 * d->outputs : d->inputs, d->kmajor ? d->inputs : 2 * d->outputs);
+  return rc;
+}
+// The product's operands (of d->rows > 0 rows), from copies where they do not lie on vectors.
+int set_input_grad(const tccl_gated_input_grad_desc* d, InputGradArgs& a, Copies& copies, int64_t& bytes, int& cus) {
+  const int rc = compute_units(&cus);
+  if (rc) return rc;
+  const int depth = 2 * d->outputs;
+  const int64_t whole = vectors(depth), width = vectors(d->inputs);
+  ProductArgs& p = a.p;
+  p.M = d->rows, p.N = d->inputs, p.K = depth, p.up = 0;
+  p.a = (const char*)d->inner, p.lda = d->rows > 1 ? d->ld_inner : whole;
+  if (!on_vectors(d->inner, d->ld_inner, d->rows) || depth % 8 || p.lda > kMostPitch) p.a = copies.add(p.a, d->ld_inner, d->rows, depth, whole), p.lda = whole;
+  p.b = (const char*)d->weight, p.ldb = d->kmajor || d->inputs > 1 ? d->ld_weight : whole;
+  if (d->kmajor ? !on_vectors(d->weight, d->ld_weight, 2) || p.ldb > kMostPitch : !on_vectors(d->weight, d->ld_weight, d->inputs) || depth % 8 || p.ldb > kMostPitch) {
+    p.b = d->kmajor ? copies.add(p.b, d->ld_weight, depth, d->inputs, width) : copies.add(p.b, d->ld_weight, d->inputs, depth, whole);
+    p.ldb = d->kmajor ? width : whole;
+  }
+  a.splits = input_grad_splits(d->rows, d->inputs, depth, cus);
+  if (!a.splits) a.splits = 1;
+  a.blocks_per_split = ((depth + 63) / 64 + a.splits - 1) / a.splits;
+  a.ld_partial = ((int64_t)d->inputs + 3) / 4 * 4;
+  bytes = copies.bytes + (a.splits > 1 ? 4 * a.splits * d->rows * a.ld_partial : 0);
+  a.partial = (float*)(copies.at + copies.bytes);
+  return 0;
+}
+
+template <typename T>
+int launch_input_grad(const char* what, InputGradArgs& a, bool kmajor, int cus, hipStream_t stream) {
+  a.tiles_m = (a.p.M + 127) / 128, a.tiles_n = (a.p.N + 127) / 128, a.band = 4;
+  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
+  if (tiles > 1 << 22) return reportf(TCCL_ERR_UNSUPPORTED, "%s: %lld tiles of the result", what, (long long)tiles);
+  a.xcds = cus % 8 ? 1 : 8, a.per_xcd = (int)((tiles * a.splits + a.xcds - 1) / a.xcds);
+  const dim3 wgs((unsigned)(a.xcds * a.per_xcd));
+  if (kmajor)
+    hipLaunchKernelGGL((input_grad_kernel<T, true>), wgs, dim3(512), 0, stream, a);
+  else
+    hipLaunchKernelGGL((input_grad_kernel<T, false>), wgs, dim3(512), 0, stream, a);
+  const int rc = launched(what);
+  if (rc || a.splits == 1) return rc;
+  const WeightSumArgs s = {a.partial, nullptr, a.out, a.ld_partial, 0, a.ld_out, a.p.M * a.ld_partial, a.p.M, a.p.N, a.splits};
+  const int64_t sums = ((int64_t)a.p.M * ((a.p.N + 3) / 4) + 255) / 256;
+  hipLaunchKernelGGL((weight_sum_kernel<T>), dim3((unsigned)(sums < 1 << 23 ? sums : 1 << 23)), dim3(256), 0, stream, s);
+  return launched(what);
+}
+
 }  // namespace
 
 extern "C" {
@@ -279,6 +351,47 @@ int tccl_gated_grad(const tccl_gated_grad_desc* d, void* stream) {
   else
     hipLaunchKernelGGL((gated_grad_kernel<_Float16>), grid, dim3(256), 0, st, a);
   return launched(what);
+}
+
+int tccl_gated_input_grad_cut(int32_t rows, int32_t inputs, int32_t outputs, int32_t compute_units, int32_t* splits) {
+  const int rc = check_sizes("gated_input_grad_cut", Sizes{rows, inputs, outputs, TCCL_BF16, TCCL_SILU});
+  if (rc) return rc;
+  if (!splits) return reportf(TCCL_ERR_INVALID, "gated_input_grad_cut: a NULL result");
+  int cus = compute_units;
+  if (cus < 1 && tccl::compute_units(&cus)) return TCCL_ERR_INVALID;
+  *splits = input_grad_splits(rows, inputs, 2 * outputs, cus);
+  return 0;
+}
+
+int64_t tccl_gated_input_grad_workspace(const tccl_gated_input_grad_desc* d) {
+  if (check_input_grad("gated_input_grad_workspace", d)) return -1;
+  if (!d->rows) return 0;
+  Copies copies(nullptr);
+  InputGradArgs a = {};
+  int64_t bytes = 0;
+  int cus = 0;
+  return set_input_grad(d, a, copies, bytes, cus) ? -1 : bytes;
+}
+
+int tccl_gated_input_grad(const tccl_gated_input_grad_desc* d, void* stream) {
+  const char* what = "gated_input_grad";
+  int rc = check_input_grad(what, d);
+  if (rc || !d->rows) return rc;
+  rc = check_matrix(what, "dx", d->dx, d->ld_dx, d->rows, d->inputs);
+  if (rc) return rc;
+  Copies copies(d->workspace);
+  InputGradArgs a = {};
+  int64_t bytes = 0;
+  int cus = 0;
+  rc = set_input_grad(d, a, copies, bytes, cus);
+  if (rc) return rc;
+  if (bytes && (!d->workspace || ((uintptr_t)d->workspace & 15) || d->workspace_bytes < bytes))
+    return reportf(TCCL_ERR_INVALID, "%s: the workspace has %lld bytes, %lld on 16 are needed", what, (long long)d->workspace_bytes, (long long)bytes);
+  a.out = (char*)d->dx, a.ld_out = d->ld_dx;
+  const hipStream_t st = (hipStream_t)stream;
+  rc = d->dtype == TCCL_BF16 ? copies.launch<__bf16>(what, st) : copies.launch<_Float16>(what, st);
+  if (rc) return rc;
+  return d->dtype == TCCL_BF16 ? launch_input_grad<__bf16>(what, a, d->kmajor, cus, st) : launch_input_grad<_Float16>(what, a, d->kmajor, cus, st);
 }
 
 }  // extern "C"

@@ -45,6 +45,9 @@ int64_t (*entry_gated_workspace)(const tccl_gated_desc*);
 int64_t (*entry_gated_grad_workspace)(const tccl_gated_grad_desc*);
 int (*entry_gated_grad)(const tccl_gated_grad_desc*, void*);
 int (*entry_gemm)(const tccl_gemm_desc*, void*);
+int64_t (*entry_input_grad_workspace)(const tccl_gated_input_grad_desc*);
+int (*entry_input_grad_cut)(int32_t, int32_t, int32_t, int32_t, int32_t*);
+int (*entry_input_grad)(const tccl_gated_input_grad_desc*, void*);
 int (*entry_pack)(const tccl_pack_desc*, int32_t, int32_t, void*);
 int (*entry_adamw)(const tccl_adamw_desc*, void*);
 int (*entry_moments)(const tccl_adamw_moments_desc*, void*);
@@ -575,7 +578,7 @@ PyObject* gated_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
-// input_gradient(inner, weight): inner @ weight.t(), by the library's GEMM, which reads and writes whole 16-byte vectors: an operand that does not lie in
+// input_gradient(inner, weight): inner @ weight.t(), by the kernel that splits the sum where it is the quicker one; else by the library's GEMM, which reads and writes whole 16-byte vectors: an operand that does not lie in
 // these is copied first, both in one launch, and a result whose rows do not has the columns that it wants of wider rows.
 PyObject* input_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 2) return none();
@@ -585,6 +588,22 @@ PyObject* input_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!inner.open(args[0]) || !on_device0(*inner.t) || !w.open(args[1])) return none();
     const at::ScalarType type = inner.t->scalar_type();
     if (w.t->scalar_type() != type || inner.cols != 2 * w.outputs) return none();
+    int32_t splits = 0;
+    if (failed(entry_input_grad_cut((int32_t)inner.rows, (int32_t)w.inputs, (int32_t)w.outputs, 0, &splits), "tccl_gated_input_grad_cut")) return nullptr;
+    if (splits) {
+      const at::Tensor dx = empty({inner.rows, w.inputs}, type, inner.t->device());
+      tccl_gated_input_grad_desc g;
+      memset(&g, 0, sizeof g);
+      g.inner = inner.at, g.weight = w.at, g.dx = dx.data_ptr();
+      g.ld_inner = inner.pitch, g.ld_weight = w.pitch, g.ld_dx = w.inputs;
+      g.rows = (int32_t)inner.rows, g.inputs = (int32_t)w.inputs, g.outputs = (int32_t)w.outputs, g.dtype = code_of(type), g.kmajor = w.kmajor;
+      at::Tensor workspace;
+      if (!with_workspace(g, entry_input_grad_workspace, "tccl_gated_input_grad", inner.t->device(), workspace)) return nullptr;
+      void* stream;
+      if (!stream_now(stream)) return nullptr;
+      if (failed(entry_input_grad(&g, stream), "tccl_gated_input_grad")) return nullptr;
+      return THPVariable_Wrap(dx);
+    }
     const int64_t N = w.inputs, K = inner.cols, width = (N + 7) / 8 * 8, depth = (K + 7) / 8 * 8;
     const at::Tensor made = empty({inner.rows, width}, type, inner.t->device());
     const at::Tensor result = width == N ? made : made.narrow(1, 0, N);
@@ -793,8 +812,8 @@ PyObject* adamw_moments(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // bind_layers(GatedLinearResult, entries): the entry points in the order below.
 PyObject* bind_layers(PyObject*, PyObject* args) {
   PyObject* result;
-  unsigned long long e[10];
-  if (!PyArg_ParseTuple(args, "O(KKKKKKKKKK)", &result, e, e + 1, e + 2, e + 3, e + 4, e + 5, e + 6, e + 7, e + 8, e + 9)) return nullptr;
+  unsigned long long e[13];
+  if (!PyArg_ParseTuple(args, "O(KKKKKKKKKKKKK)", &result, e, e + 1, e + 2, e + 3, e + 4, e + 5, e + 6, e + 7, e + 8, e + 9, e + 10, e + 11, e + 12)) return nullptr;
   if (!PyType_Check(result) || !PyType_IsSubtype((PyTypeObject*)result, &PyTuple_Type)) {
     PyErr_SetString(PyExc_TypeError, "results are named tuples");
     return nullptr;
@@ -811,6 +830,9 @@ PyObject* bind_layers(PyObject*, PyObject* args) {
   entry_gated_grad_workspace = (decltype(entry_gated_grad_workspace))(uintptr_t)e[7];
   entry_gemm = (decltype(entry_gemm))(uintptr_t)e[8];
   entry_pack = (decltype(entry_pack))(uintptr_t)e[9];
+  entry_input_grad_workspace = (decltype(entry_input_grad_workspace))(uintptr_t)e[10];
+  entry_input_grad_cut = (decltype(entry_input_grad_cut))(uintptr_t)e[11];
+  entry_input_grad = (decltype(entry_input_grad))(uintptr_t)e[12];
   Py_RETURN_NONE;
 }
 

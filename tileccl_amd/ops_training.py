@@ -103,7 +103,7 @@ def _bind() -> Any:
 
         entries = (lib.tccl_weight_gradient_full, lib.tccl_weight_gradient_full_workspace, lib.tccl_gated, lib.tccl_gated_grad, lib.tccl_adamw,
                    lib.tccl_adamw_moments, lib.tccl_gated_workspace, lib.tccl_gated_grad_workspace, lib.tccl_gemm,
-                   lib.tccl_pack_matrices)
+                   lib.tccl_pack_matrices, lib.tccl_gated_input_grad_workspace, lib.tccl_gated_input_grad_cut, lib.tccl_gated_input_grad)
         host.bind_layers(GatedLinearResult, tuple(C.cast(e, C.c_void_p).value for e in entries))
         _native = host
     return _native
