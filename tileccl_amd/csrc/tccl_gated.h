@@ -214,7 +214,7 @@ struct Gated : Product<T, kTile, false, kBDeep, true> {
   }
 };
 
-// 8192 x 4096 x 8192 bf16, k-major: 800 us, 1.38 PFLOP/s, the matrix pipes busy 67 % of a clock that the load holds at 1.9 GHz (the vendor
+// 8192 x 4096 x 8192 bf16, k-major: 803 us, 1.37 PFLOP/s, the matrix pipes busy 67 % of a clock that the load holds at 1.9 GHz (the vendor
 // library's product alone 794).  4096 x 4096 x 4096 by rows with z kept 214 us, 1.28 PFLOP/s.  128 tiles are bound by what comes from L2 to a
 // CU, 64 KiB for 4.2 MFLOP at 67 KB a microsecond: 1003 x 1001 x 1035 16 us.  Of a short sum the epilogue is the larger part, bound by the vector
 // instructions of the activation (silu 13 a value, gelu 25, 30 with its derivative): 12628 x 208 x 808, gelu, 33 us, backward 47, memory 10.

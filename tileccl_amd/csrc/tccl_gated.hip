@@ -250,7 +250,7 @@ int set_input_grad(const tccl_gated_input_grad_desc* d, InputGradArgs& a, Copies
   if (!a.splits) a.splits = 1;
   a.blocks_per_split = ((depth + 63) / 64 + a.splits - 1) / a.splits;
   a.ld_partial = ((int64_t)d->inputs + 3) / 4 * 4;
-  bytes = copies.bytes + (a.splits > 1 ? 4 * a.splits * d->rows * a.ld_partial : 0);
+  bytes = copies.bytes + (a.splits > 1 ? 4ll * a.splits * d->rows * a.ld_partial : 0);
   a.partial = (float*)(copies.at + copies.bytes);
   return 0;
 }
