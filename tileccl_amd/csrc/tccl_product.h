@@ -1,5 +1,5 @@
 // Products of two 16-bit matrices on MFMA tiles, for gfx950, by how each operand lies in memory: the common part of the gated
-// layer's projections (tccl_gated.h) and of the weight gradient from an input in full (tccl_weight_full.hip).
+// layer's projections (tccl_gated.h) and of the weight gradient from an input in full (tccl_weight_full.h), and of the input gradient.
 //
 //     P[m][n] = sum over k of A(m, k) * B(n, k)
 //
