@@ -252,7 +252,7 @@ struct GatedRows {
   static constexpr int kWaveBytes = (kMB + kNB) * 2048, kSums = kMB * kNB * 256;              // sums of a wavefront
   static constexpr int kLds = kWaves * kWaveBytes > (kWaves + 1) * kSums * 4 ? kWaves * kWaveBytes : (kWaves + 1) * kSums * 4;
   static constexpr int kRowBytes = 32 * kNB, kRowLanes = kRowBytes / 16, kRowsPerLoad = 64 / kRowLanes;  // a k row of a weight by rows
-  static constexpr uint32_t kOutside = 0xffffff00u;
+  static constexpr uint32_t kLongest = 0xfffffff0u, kOutside = kLongest;  // bytes of a window; an offset past the end of every one
   struct Block {
     u32x4 x[2 * kMB], w[2 * kNB];
   };
@@ -265,7 +265,7 @@ struct GatedRows {
 
   TCCL_D GatedRows(const GatedArgs& args, char* mem) : g(args), lds(mem), lane((int)(threadIdx.x & 63)), wave(__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6))) {}
   static TCCL_D __amdgpu_buffer_rsrc_t window(const char* at, int64_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, bytes > 0xfffffff0ll ? 0xfffffff0u : (uint32_t)bytes, 0x00020000);
+    return __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, bytes > (int64_t)kLongest ? kLongest : (uint32_t)bytes, 0x00020000);
   }
 
   TCCL_D void load(Block& v, int kb) const {
