@@ -1,5 +1,6 @@
-"""The gated layer's kernels for few rows where an operand reaches further than 32 bits from a tile's first row: what lies past the inputs reads as zero
-there, too.  NaN between the rows, which has no part, and inputs that end within a step of 64."""
+"""The kernels for few rows, of the gated layer and of the GEMM that makes its input's gradient, where an operand reaches further than 32 bits from a
+tile's first row: what lies past the summed index reads as zero there, too.  NaN between the rows, which has no part, and sums that end within a step of
+64."""
 
 import pytest
 import torch
@@ -48,3 +49,23 @@ def test_rows_of_a_weight_far_apart(rows):
     assert bool(torch.isfinite(want.out).all())
     got = ops.gated_linear(x, apart(ws, 1 << 22).t(), keep=True)
     assert torch.equal(got.out, want.out) and torch.equal(got.kept, want.kept)
+
+
+def test_input_gradient_of_rows_far_apart():
+    rows, inputs, outputs = 1100, 16, 36
+    dh, kept = rand((rows, outputs), 6, F16, 0.1).cuda(), rand((rows, 2 * outputs), 7, F16).cuda()
+    _, w = weight_of(inputs, outputs, F16, "kn", 8)
+    out = apart(torch.zeros(rows, 2 * outputs, dtype=F16), (1 << 21) + 8)
+    want = ops.gated_linear_backward(dh, kept, None, w, weights=False)
+    assert bool(torch.isfinite(want.x).all())
+    got = ops.gated_linear_backward(dh, kept, None, w, weights=False, out=out)
+    assert torch.equal(got.inner, want.inner) and torch.equal(got.x, want.x)
+
+
+def test_input_gradient_of_a_weight_far_apart():
+    rows, inputs, outputs = 5, 600, 36
+    dh, kept = rand((rows, outputs), 9, F16, 0.1).cuda(), rand((rows, 2 * outputs), 10, F16).cuda()
+    ws = rand((inputs, 2 * outputs), 11, F16, 0.1)
+    want = ops.gated_linear_backward(dh, kept, None, ws.cuda(), weights=False)
+    assert bool(torch.isfinite(want.x).all())
+    assert torch.equal(ops.gated_linear_backward(dh, kept, None, apart(ws, 1 << 22), weights=False).x, want.x)

@@ -104,7 +104,8 @@ struct StreamGemm {
   TCCL_D StreamGemm(const StreamArgs& args, char* l)
       : a(args), lds(l), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6))) {}
 
-  static TCCL_D uint32_t clamp_u32(int64_t v) { return v > 0xfffffff0ll ? 0xfffffff0u : (v < 0 ? 0u : (uint32_t)v); }
+  static constexpr uint32_t kLongest = 0xfffffff0u, kOutside = kLongest;  // bytes of a window; past the end of every one: reads as zero
+  static TCCL_D uint32_t clamp_u32(int64_t v) { return v > (int64_t)kLongest ? kLongest : (v < 0 ? 0u : (uint32_t)v); }
 
   // One K block as it is loaded, 16 bytes per lane with neighbouring lanes on neighbouring addresses (a
   // load whose lanes 0..3 lie in four rows takes in a third of the bytes per clock: 34 against 104 KB/us per CU).
@@ -115,7 +116,6 @@ struct StreamGemm {
   };
   static constexpr int kRowBytes = 16 * kNB * kEsz, kRowLanes = kRowBytes / 16;  // of a k row of row-major B in a tile
   static constexpr int kRowsPerLoad = 64 / kRowLanes;
-  static constexpr uint32_t kOutside = 0xffffff00u;  // beyond every buffer: reads as zero
 
   __amdgpu_buffer_rsrc_t ra, rb;
   uint32_t off_a, off_b, pitch_a, pitch_b;  // this lane's offset in K block 0; bytes per row
