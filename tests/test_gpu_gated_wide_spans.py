@@ -69,3 +69,23 @@ def test_input_gradient_of_a_weight_far_apart():
     want = ops.gated_linear_backward(dh, kept, None, ws.cuda(), weights=False)
     assert bool(torch.isfinite(want.x).all())
     assert torch.equal(ops.gated_linear_backward(dh, kept, None, apart(ws, 1 << 22), weights=False).x, want.x)
+
+
+def test_input_gradient_of_many_rows_far_apart():
+    """The GEMM in 128 tiles."""
+    rows, inputs, outputs = 5000, 512, 36
+    dh, kept = rand((rows, outputs), 12, F16, 0.1).cuda(), rand((rows, 2 * outputs), 13, F16).cuda()
+    _, w = weight_of(inputs, outputs, F16, "kn", 14)
+    want = ops.gated_linear_backward(dh, kept, None, w, weights=False)
+    assert bool(torch.isfinite(want.x).all())
+    got = ops.gated_linear_backward(dh, kept, None, w, weights=False, out=apart(torch.zeros(rows, 2 * outputs, dtype=F16), (1 << 20) + 8))
+    assert torch.equal(got.inner, want.inner) and torch.equal(got.x, want.x)
+
+
+def test_input_gradient_of_many_rows_of_a_weight_far_apart():
+    rows, inputs, outputs = 1100, 2000, 36
+    dh, kept = rand((rows, outputs), 15, F16, 0.1).cuda(), rand((rows, 2 * outputs), 16, F16).cuda()
+    ws = rand((inputs, 2 * outputs), 17, F16, 0.1)
+    want = ops.gated_linear_backward(dh, kept, None, ws.cuda(), weights=False)
+    assert bool(torch.isfinite(want.x).all())
+    assert torch.equal(ops.gated_linear_backward(dh, kept, None, apart(ws, 1 << 21), weights=False).x, want.x)

@@ -288,7 +288,8 @@ struct GemmRole {
     asm volatile("" : "+v"(v));
     return v;
   }
-  static TCCL_D uint32_t clamp_u32(int64_t v) { return v > 0xffffffffll ? 0xffffffffu : (v < 0 ? 0u : (uint32_t)v); }
+  static constexpr uint32_t kDead = 0xfffffff0u;  // an offset past the end of every window: reads as zero
+  static TCCL_D uint32_t clamp_u32(int64_t v) { return v > (int64_t)kDead ? kDead : (v < 0 ? 0u : (uint32_t)v); }
 
   // ---- global -> LDS ------------------------------------------------------------------------
   // Per K step a wavefront fetches two 1 KiB pieces of A and kBLoads of B (wide form in brackets):
@@ -355,13 +356,13 @@ struct GemmRole {
   template <bool kAColumns>
   TCCL_D void issue_a(char* stage, const Source& s, int kt, int i) const {
     const bool dead = !kAColumns && kt * kStepK + s.k_lane[i & 1] >= g.K;  // (by columns: those >= K lie past the end of the buffer)
-    const uint32_t oa = dead ? 0xfffffff0u : s.off_a[i] + kt * s.step_a;
+    const uint32_t oa = dead ? kDead : s.off_a[i] + kt * s.step_a;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(s.a, (LdsVoid*)(stage + (kALoads * wave + i) * 1024), 16, oa, 0, 0, 0);
   }
   template <bool kBKMajor>
   TCCL_D void issue_b(char* stage, const Source& s, int kt, int i) const {
     uint32_t ob = s.off_b[i] + kt * s.step_b;  // row-major B: rows >= K lie past the end of the buffer
-    if constexpr (kBKMajor) ob = (kt * kStepK + s.k_lane[i & 1] >= g.K) ? 0xfffffff0u : ob;
+    if constexpr (kBKMajor) ob = (kt * kStepK + s.k_lane[i & 1] >= g.K) ? kDead : ob;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(s.b, (LdsVoid*)(stage + kAStage + (kBLoads * wave + i) * 1024), 16, ob, 0, 0, 0);
   }
   // Load number n of a K step: A 0, B 0, A 1, B 1, then the rest of B.
