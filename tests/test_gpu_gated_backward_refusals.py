@@ -1,0 +1,73 @@
+"""What ``gated_linear_backward`` refuses of a call that wants the weight's gradient: ahead of the first launch, which may write ``inner`` where the
+kept projections are."""
+
+import pytest
+import torch
+
+from tests.layer_bounds import BF16, F16, F32
+from tileccl_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def zeros(*shape, dtype=BF16):
+    return torch.zeros(*shape, dtype=dtype, device="cuda")
+
+
+def held_from(dtype):
+    return ops.checkpoint_activation(zeros(4, 16, dtype=dtype))
+
+
+def off_vectors():
+    """A checkpoint whose values do not start on 16 bytes."""
+    held = held_from(BF16)
+    memory = torch.zeros(held.values.numel() + 8, dtype=torch.uint8, device="cuda")
+    return held._replace(values=memory[8:].view(held.values.shape))
+
+
+REFUSED = {
+    "type of the result": (lambda: dict(out_dtype=F16), "float32 or torch.bfloat16"),
+    "type of what is added": (lambda: dict(add=zeros(16, 16, dtype=F16)), "float32 or torch.bfloat16"),
+    "layout of what is added": (lambda: dict(add=zeros(16, 16, dtype=F32).t()), "add must"),
+    "rows of what is added": (lambda: dict(add=zeros(1, 16, dtype=F32).expand(16, 16)), "add"),
+    "place of what is added": (lambda: dict(add=torch.zeros(16, 16)), "add must reside"),
+    "what is added is no tensor": (lambda: dict(add=[0.0]), "add must be a 2-D tensor"),
+    "type of x": (lambda: dict(x=zeros(4, 16, dtype=F16)), "x must have dtype"),
+    "rows of x": (lambda: dict(x=zeros(16, 4).t()), "x must have contiguous rows"),
+    "place of x": (lambda: dict(x=torch.zeros(4, 16, dtype=BF16)), "x must reside"),
+    "pitch of x": (lambda: dict(x=torch.empty(3 * ((1 << 24) + 8) + 16, dtype=BF16, device="cuda").as_strided((4, 16), ((1 << 24) + 8, 1))), "x has 16 columns .*at most"),
+    "type that x was held from": (lambda: dict(x=held_from(F16)), "the checkpoint is of torch.float16"),
+    "values of x off 16 bytes": (lambda: dict(x=off_vectors()), "16 bytes"),
+}
+
+
+@pytest.mark.parametrize("which", REFUSED)
+def test_kept_outlives_a_refused_call(which):
+    make, text = REFUSED[which]
+    grad, kept, w = zeros(4, 8), torch.ones(4, 16, dtype=BF16, device="cuda"), zeros(16, 16)
+    args = dict(x=zeros(4, 16)) | make()
+    with pytest.raises(ValueError, match="gated_linear_backward: .*" + text):
+        ops.gated_linear_backward(grad, kept, args.pop("x"), w, out=kept, **args)
+    assert bool((kept == 1).all()), "kept was written by a refused call"
+
+
+def test_what_is_added_lies_as_the_weight():
+    grad, kept, x, w = zeros(4, 8), torch.ones(4, 16, dtype=BF16, device="cuda"), zeros(4, 16), zeros(16, 16).t()
+    add = zeros(16, 16, dtype=F32)
+    add[0, 1] = 1.0
+    with pytest.raises(ValueError, match="gated_linear_backward: .*add must"):
+        ops.gated_linear_backward(grad, kept, x, w, out=kept, add=add)
+    assert bool((kept == 1).all())
+    assert torch.equal(ops.gated_linear_backward(grad, kept, x, w, out=kept, add=add.t()).weight, add.t())
+
+
+def test_a_pitch_that_the_weight_gradient_does_not_take():
+    rows, pitch = 4, (1 << 24) + 8
+    kept = torch.zeros(3 * pitch + 16, dtype=BF16, device="cuda").as_strided((rows, 16), (pitch, 1))
+    kept.fill_(1.0)
+    for x in (zeros(rows, 16), held_from(BF16)):
+        with pytest.raises(ValueError, match="out has a pitch"):
+            ops.gated_linear_backward(zeros(rows, 8), kept, x, zeros(16, 16), out=kept)
+    assert bool((kept == 1).all())
+    ops.gated_linear_backward(zeros(rows, 8), kept, None, zeros(16, 16), out=kept, inputs=False, weights=False)
+    assert not bool(kept.any())

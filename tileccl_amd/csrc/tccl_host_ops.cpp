@@ -76,13 +76,14 @@ struct Matrix {
   char* at = nullptr;
   int64_t rows = 0, cols = 0, pitch = 0;
 
-  bool open(PyObject* o) {
+  // turned: the transposed view.
+  bool open(PyObject* o, bool turned = false) {
     if (!THPVariable_Check(o)) return false;
     t = &THPVariable_Unpack(o);
     if (!t->is_cuda() || t->layout() != at::kStrided || t->dim() != 2) return false;
-    rows = t->size(0), cols = t->size(1);
-    if (cols < 1 || rows > TCCL_TRAINING_MAX_ROWS || cols > INT32_MAX || (cols > 1 && t->stride(1) != 1)) return false;
-    pitch = rows > 1 ? t->stride(0) : cols;
+    rows = t->size(turned), cols = t->size(!turned);
+    if (cols < 1 || rows > TCCL_TRAINING_MAX_ROWS || cols > INT32_MAX || (cols > 1 && t->stride(!turned) != 1)) return false;
+    pitch = rows > 1 ? t->stride(turned) : cols;
     at = (char*)t->data_ptr();
     return pitch >= cols;
   }
@@ -441,6 +442,8 @@ PyObject* weight_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 bool on_device0(const at::Tensor& t) { return t.is_cuda() && t.device().index() == 0; }  // where the ranks live
 
+constexpr int64_t kMostPitch = 1 << 24;  // of what weight gradients read
+
 bool sixteen_bits(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
 
 // The workspace that a call asks for; false: an error is set.
@@ -530,12 +533,35 @@ PyObject* gated_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
-// gated_gradient(grad, kept, x, weight, activation, out): of the projections.  With kept, x is None and weight is not read.
+// What weight_gradient() will be given beside `inner` (t NULL: memory of its own): x, a tensor or its checkpoint, the result's type or what is added.
+// All that it refuses is refused ahead of the launch that writes inner, perhaps over what this is made of.
+struct WeightGradientWanted {
+  Matrix x, add;
+  Held held;
+
+  bool takes(PyObject* o, const GatedWeight& w, int64_t rows, at::ScalarType type, const at::Device& device, const Matrix& inner, PyObject* out_dtype, PyObject* added) {
+    const bool on_vectors = inner.cols % 8 == 0 && (inner.rows <= 1 || inner.pitch % 8 == 0) && (uintptr_t)inner.at % 16 == 0;
+    if (THPVariable_Check(o)) {
+      if (!x.open(o) || x.t->scalar_type() != type || x.t->device() != device || x.rows != rows || x.cols != w.inputs || x.pitch > kMostPitch) return false;
+      if (inner.t && inner.pitch > kMostPitch) return false;
+    } else {
+      if (!open_held(o, held) || held.type != type || held.values->device() != device || held.rows != rows || held.cols != w.inputs || (uintptr_t)held.values->data_ptr() % 16) return false;
+      if (inner.t && on_vectors && inner.pitch > kMostPitch) return false;  // (else it is copied)
+    }
+    if (added == Py_None) return out_dtype == f32 || out_dtype == (type == at::kHalf ? f16 : bf16);
+    return add.open(added, w.kmajor) && add.rows == (w.kmajor ? 2 * w.outputs : w.inputs) && add.cols == (w.kmajor ? w.inputs : 2 * w.outputs) &&
+           (add.t->scalar_type() == at::kFloat || add.t->scalar_type() == type) && add.t->device() == device;
+  }
+};
+
+// gated_gradient(grad, kept, x, weight, activation, out, weights, out_dtype, add): of the projections.  With kept, weight is not read.  `weights`: weight_gradient()
+// of x, out_dtype and add follows.
 PyObject* gated_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  if (nargs != 6) return none();
+  if (nargs != 9) return none();
   return guarded([&]() -> PyObject* {
     Matrix grad, kept, x, out;
     GatedWeight w;
+    WeightGradientWanted wanted;
     if (!grad.open(args[0]) || !on_device0(*grad.t) || !w.open(args[3])) return none();
     const at::ScalarType type = grad.t->scalar_type();
     const at::Device device = grad.t->device();
@@ -549,6 +575,7 @@ PyObject* gated_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     tccl_gated_grad_desc d;
     memset(&d, 0, sizeof d);
     d.activation = (int32_t)PyLong_AsLong(args[4]);
+    const int weights = PyObject_IsTrue(args[6]);
     if (PyErr_Occurred()) return nullptr;
     at::Tensor made;
     if (args[5] != Py_None) {
@@ -560,6 +587,7 @@ PyObject* gated_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       made = empty({grad.rows, 2 * w.outputs}, type, device);
       d.inner = made.data_ptr(), d.ld_inner = 2 * w.outputs;
     }
+    if (weights && !wanted.takes(args[2], w, grad.rows, type, device, out, args[7], args[8])) return none();
     d.grad = grad.at, d.ld_grad = grad.pitch;
     if (computed)
       d.x = x.at, d.ld_x = x.pitch, d.weight = w.at, d.ld_weight = w.pitch, d.up = w.up;
@@ -650,7 +678,7 @@ PyObject* weight_gradient_full(PyObject*, PyObject* const* args, Py_ssize_t narg
     const at::ScalarType type = grad.t->scalar_type();
     const at::Device device = grad.t->device();
     if (!sixteen_bits(type) || x.t->scalar_type() != type || x.t->device() != device || x.rows != grad.rows) return none();
-    if (x.cols > 1 << 24 || grad.cols > 1 << 24 || x.pitch > 1 << 24 || grad.pitch > 1 << 24) return none();
+    if (x.cols > kMostPitch || grad.cols > kMostPitch || x.pitch > kMostPitch || grad.pitch > kMostPitch) return none();
     const int64_t inputs = x.cols, outputs = grad.cols;
     const int transposed = PyObject_IsTrue(args[2]);
     if (PyErr_Occurred()) return nullptr;

@@ -21,12 +21,13 @@ from typing import Any, NamedTuple, NoReturn
 import torch
 
 from tileccl_amd import _lib, ops_training
-from tileccl_amd.ops_training import ActivationCheckpoint, _apart, _matrix, _span, _unexplained, weight_gradient
+from tileccl_amd.ops_training import ActivationCheckpoint, _apart, _held, _matrix, _span, _unexplained, weight_gradient
 
 __all__ = ["GatedLinearResult", "GatedLinearGradients", "gated_linear", "gated_linear_backward"]
 
 ACTIVATIONS = {"silu": _lib.SILU, "gelu": _lib.GELU, "gelu_tanh": _lib.GELU_TANH, "relu": _lib.RELU}
 _TYPES = (torch.float16, torch.bfloat16)
+_MOST_PITCH = 1 << 24  # of what weight gradients read
 
 
 class GatedLinearResult(NamedTuple):
@@ -144,11 +145,10 @@ def gated_linear_backward(
     op = "gated_linear_backward"
     code = _activation(activation, op)
     native = ops_training._native or ops_training._bind()
-    if weights:  # ahead of a result that may lie in kept's place
-        _check_weight_gradient(grad, x, weight, add, op)
-    inner = native.gated_gradient(grad, kept, x if kept is None else None, weight, code, out)
+    # What the weight's gradient would refuse is refused here, ahead of a result that may lie in kept's place.
+    inner = native.gated_gradient(grad, kept, x, weight, code, out, weights, out_dtype, add)
     if inner is None:
-        _refuse_backward(grad, kept, x, weight, out)
+        _refuse_backward(grad, kept, x, weight, out, weights, out_dtype, add)
     dx = dw = None
     if weights:
         by_rows = _by_rows(weight)
@@ -161,13 +161,15 @@ def gated_linear_backward(
     return GatedLinearGradients(inner, dx, dw)
 
 
-def _check_weight_gradient(grad, x, weight, add, op) -> None:
+def _refuse_shapes(grad, x, weight, add, op) -> None:
     if isinstance(x, ActivationCheckpoint):
         rows, columns = x.rows, x.columns
     elif isinstance(x, torch.Tensor) and x.ndim == 2:
         rows, columns = x.shape
     else:
         raise ValueError(f"{op}: the weight's gradient wants x, a 2-D tensor or its checkpoint, got {type(x).__name__}")
+    if add is not None and (not isinstance(add, torch.Tensor) or add.ndim != 2):
+        raise ValueError(f"{op}: add must be a 2-D tensor, got {getattr(add, 'ndim', type(add).__name__)}")
     if isinstance(weight, torch.Tensor) and isinstance(grad, torch.Tensor) and weight.ndim == grad.ndim == 2:  # (else refused with their names)
         if columns != weight.shape[0]:
             raise ValueError(f"{op}: x has {columns} columns, weight {weight.shape[0]} rows")
@@ -177,8 +179,38 @@ def _check_weight_gradient(grad, x, weight, add, op) -> None:
             raise ValueError(f"{op}: add must have shape {tuple(weight.shape)}, got {tuple(add.shape)}")
 
 
-def _refuse_backward(grad, kept, x, weight, out) -> NoReturn:
+def _refuse_weight_gradient(grad, x, weight, out, out_dtype, add, op) -> None:
+    """What ``weight_gradient`` would refuse."""
+    if isinstance(x, ActivationCheckpoint):
+        _held(x, op, grad.device)
+        if x.dtype != grad.dtype:
+            raise ValueError(f"{op}: the checkpoint is of {x.dtype}, grad is {grad.dtype}")
+        if x.values.data_ptr() % 16:
+            raise ValueError(f"{op}: the checkpoint's values must lie on 16 bytes")
+    else:
+        pitch = _matrix(x, "x", op, dtype=grad.dtype)
+        _device0(x, "x", op)
+        if pitch > _MOST_PITCH:
+            raise ValueError(f"{op}: x has {x.shape[1]} columns (pitch {pitch}), at most {_MOST_PITCH}")
+    if out is not None and out.shape[0] > 1 and out.stride(0) > _MOST_PITCH:
+        raise ValueError(f"{op}: out has a pitch of {out.stride(0)} elements, at most {_MOST_PITCH} where the weight's gradient is made of it")
+    if add is None:
+        if out_dtype not in (torch.float32, grad.dtype):
+            raise ValueError(f"{op}: the weight's gradient must be float32 or {grad.dtype}, got {out_dtype}")
+        return
+    if add.dtype not in (torch.float32, grad.dtype):
+        raise ValueError(f"{op}: add must be float32 or {grad.dtype}, got {add.dtype}")
+    lies = add if _by_rows(weight) else add.t()
+    if lies.shape[1] > 1 and lies.stride(1) != 1:
+        raise ValueError(f"{op}: add must have contiguous rows where weight has, columns where weight has these, got strides {tuple(add.stride())}")
+    _matrix(lies, "add", op)
+    _device0(add, "add", op)
+
+
+def _refuse_backward(grad, kept, x, weight, out, weights, out_dtype, add) -> NoReturn:
     op = "gated_linear_backward"
+    if weights:
+        _refuse_shapes(grad, x, weight, add, op)
     _weight(weight, op)
     outputs = weight.shape[1] // 2
     _matrix(grad, "grad", op, dtype=weight.dtype)
@@ -199,4 +231,6 @@ def _refuse_backward(grad, kept, x, weight, out) -> NoReturn:
         _device0(out, "out", op)
         _elsewhere(out, op, grad=_span(grad), weight=_weight_span(weight), **({"x": _span(x)} if kept is None else {}))
         _apart(out, "out", op, kept)
+    if weights:
+        _refuse_weight_gradient(grad, x, weight, out, out_dtype, add, op)
     _unexplained(op)
