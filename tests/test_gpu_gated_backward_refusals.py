@@ -71,3 +71,47 @@ def test_a_pitch_that_the_weight_gradient_does_not_take():
     assert bool((kept == 1).all())
     ops.gated_linear_backward(zeros(rows, 8), kept, None, zeros(16, 16), out=kept, inputs=False, weights=False)
     assert not bool(kept.any())
+
+
+def across_x():
+    x = torch.ones(4, 16, dtype=BF16, device="cuda")
+    return dict(x=x, out=x), x
+
+
+def across_values():
+    held = held_from(BF16)
+    return dict(x=held, out=held.values.view(-1)[64:192].view(BF16).view(4, 16)), held.values
+
+
+def across_scales():
+    memory = torch.full((256,), 127, dtype=torch.uint8, device="cuda")
+    return dict(x=held_from(BF16)._replace(scales=memory[96:112].view(1, 16)), out=memory[:128].view(BF16).view(4, 16)), memory
+
+
+def across_add():
+    add = torch.ones(16, 16, device="cuda")
+    return dict(x=zeros(4, 16), add=add, out=add.view(-1)[64:96].view(BF16).view(4, 16)), add
+
+
+@pytest.mark.parametrize("make, name", [(across_x, "x"), (across_values, "the checkpoint's values"), (across_scales, "the checkpoint's scales"), (across_add, "add")])
+def test_inner_across_what_the_weight_gradient_reads(make, name):
+    args, memory = make()
+    before = memory.clone()
+    with pytest.raises(ValueError, match="gated_linear_backward: out overlaps " + name):
+        ops.gated_linear_backward(zeros(4, 8), zeros(4, 16), args.pop("x"), zeros(16, 16), **args)
+    assert torch.equal(memory, before)
+
+
+@pytest.mark.parametrize("rows", [1, 4])
+def test_inner_beside_what_the_weight_gradient_reads(rows):
+    """Rows of one buffer: x, then kept, in whose place inner goes; and x's place where x has no part."""
+    memory = torch.randn(rows, 32, generator=torch.Generator().manual_seed(1)).to(BF16).cuda()
+    x, kept, grad = memory[:, :16], memory[:, 16:], torch.randn(rows, 8, generator=torch.Generator().manual_seed(3)).to(BF16).cuda()
+    w = torch.randn(16, 16, generator=torch.Generator().manual_seed(2)).to(BF16).cuda()
+    want = ops.gated_linear_backward(grad, kept.clone(), x.clone(), w)
+    before = memory.clone()
+    got = ops.gated_linear_backward(grad, kept, x, w, out=kept)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(x, before[:, :16])
+    elsewhere = ops.gated_linear_backward(grad, before[:, 16:].clone(), x, w, out=x, weights=False)
+    assert torch.equal(elsewhere.inner, want.inner) and torch.equal(elsewhere.x, want.x)

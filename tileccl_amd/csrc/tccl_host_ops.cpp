@@ -100,6 +100,14 @@ struct Matrix {
     return row >= rows || row * step >= to;
   }
   bool clear_of(const at::Tensor* o) const { return !o || clear_of(*o); }
+  // No byte of either's rows lies in the other's; rows of one pitch may lie beside each other.
+  bool clear_of(const Matrix& m) const {
+    if (elsewhere(m)) return true;
+    const int64_t step = pitch * (int64_t)t->element_size(), width = cols * (int64_t)t->element_size(), other = m.cols * (int64_t)m.t->element_size();
+    if (rows < 2 || m.rows < 2 || step != m.pitch * (int64_t)m.t->element_size()) return false;
+    const int64_t ahead = ((m.at - at) % step + step) % step;
+    return ahead >= width && ahead + other <= step;
+  }
   // The same elements in the same places, or none in common.
   bool apart(const Matrix& m) const { return !m.t || elsewhere(m) || (at == m.at && pitch == m.pitch && t->scalar_type() == m.t->scalar_type()); }
 };
@@ -552,6 +560,10 @@ struct WeightGradientWanted {
     return add.open(added, w.kmajor) && add.rows == (w.kmajor ? 2 * w.outputs : w.inputs) && add.cols == (w.kmajor ? w.inputs : 2 * w.outputs) &&
            (add.t->scalar_type() == at::kFloat || add.t->scalar_type() == type) && add.t->device() == device;
   }
+  // Nothing of it lies where inner goes.
+  bool clear_of(const Matrix& inner) const {
+    return (!x.t || inner.clear_of(x)) && inner.clear_of(held.values) && inner.clear_of(held.scales) && (!add.t || inner.clear_of(add));
+  }
 };
 
 // gated_gradient(grad, kept, x, weight, activation, out, weights, out_dtype, add): of the projections.  With kept, weight is not read.  `weights`: weight_gradient()
@@ -587,7 +599,7 @@ PyObject* gated_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       made = empty({grad.rows, 2 * w.outputs}, type, device);
       d.inner = made.data_ptr(), d.ld_inner = 2 * w.outputs;
     }
-    if (weights && !wanted.takes(args[2], w, grad.rows, type, device, out, args[7], args[8])) return none();
+    if (weights && (!wanted.takes(args[2], w, grad.rows, type, device, out, args[7], args[8]) || (out.t && !wanted.clear_of(out)))) return none();
     d.grad = grad.at, d.ld_grad = grad.pitch;
     if (computed)
       d.x = x.at, d.ld_x = x.pitch, d.weight = w.at, d.ld_weight = w.pitch, d.up = w.up;

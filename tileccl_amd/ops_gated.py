@@ -21,7 +21,7 @@ from typing import Any, NamedTuple, NoReturn
 import torch
 
 from tileccl_amd import _lib, ops_training
-from tileccl_amd.ops_training import ActivationCheckpoint, _apart, _held, _matrix, _span, _unexplained, weight_gradient
+from tileccl_amd.ops_training import ActivationCheckpoint, _apart, _bytes_of, _clear, _held, _matrix, _span, _unexplained, weight_gradient
 
 __all__ = ["GatedLinearResult", "GatedLinearGradients", "gated_linear", "gated_linear_backward"]
 
@@ -86,6 +86,18 @@ def _elsewhere(out: torch.Tensor, op: str, **others: "tuple[int, int]") -> None:
             raise ValueError(f"{op}: out overlaps {name}")
 
 
+def _beside(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """No byte of either matrix's rows lies in the other's; rows of one pitch may lie beside each other."""
+    (lo, hi), (start, end) = _span(a), _span(b)
+    if end <= lo or hi <= start:
+        return True
+    step = a.stride(0) * a.element_size()
+    if min(a.shape[0], b.shape[0]) < 2 or step != b.stride(0) * b.element_size():
+        return False
+    ahead = (start - lo) % step
+    return ahead >= a.shape[1] * a.element_size() and ahead + b.shape[1] * b.element_size() <= step
+
+
 def gated_linear(x: torch.Tensor, weight: torch.Tensor, *, activation: str = "silu", keep: bool = False, out: torch.Tensor | None = None) -> GatedLinearResult:
     """``act(x @ weight[:, :F]) * (x @ weight[:, F:])`` for ``x`` (rows, inputs) and ``weight`` (inputs, 2 * F), float16 or bfloat16.
 
@@ -136,7 +148,7 @@ def gated_linear_backward(
 
     ``inner`` (rows, 2 * F): the gradient of ``x @ weight``, made of ``kept``, or, where that is None, of the product computed
     again, which is then not rounded on the way (``x`` must be the tensor itself); rounded once.  ``out`` is where it goes: ``kept``
-    itself, which has no further use, or memory that lies across no operand.
+    itself, which has no further use, or memory that lies across no operand (with ``weights`` ``x``, its checkpoint and ``add`` are some).
     ``x``: ``inner @ weight.t()``, in ``grad``'s type; ``inputs=False``: not wanted, for instance because it is summed over ranks.
     ``weight``: ``x.t() @ inner`` in ``out_dtype`` (float32 or ``grad``'s type; ``add``'s where that is given), of ``weight``'s shape and
     layout, on top of ``add`` (of that layout, too): ``ops.weight_gradient``, from ``x`` in full or its 8-bit checkpoint.
@@ -194,6 +206,12 @@ def _refuse_weight_gradient(grad, x, weight, out, out_dtype, add, op) -> None:
             raise ValueError(f"{op}: x has {x.shape[1]} columns (pitch {pitch}), at most {_MOST_PITCH}")
     if out is not None and out.shape[0] > 1 and out.stride(0) > _MOST_PITCH:
         raise ValueError(f"{op}: out has a pitch of {out.stride(0)} elements, at most {_MOST_PITCH} where the weight's gradient is made of it")
+    if out is not None:
+        if isinstance(x, ActivationCheckpoint):
+            _clear(out, op, **_bytes_of(x))
+        for t, name in ((x, "x"), (add if add is None or _by_rows(weight) else add.t(), "add")):
+            if isinstance(t, torch.Tensor) and not _beside(out, t):
+                raise ValueError(f"{op}: out overlaps {name}")
     if add is None:
         if out_dtype not in (torch.float32, grad.dtype):
             raise ValueError(f"{op}: the weight's gradient must be float32 or {grad.dtype}, got {out_dtype}")
