@@ -618,8 +618,27 @@ PyObject* gated_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
-// input_gradient(inner, weight): inner @ weight.t(), by the kernel that splits the sum where it is the quicker one; else by the library's GEMM, which reads and writes whole 16-byte vectors: an operand that does not lie in
-// these is copied first, both in one launch, and a result whose rows do not has the columns that it wants of wider rows.
+// The same by tccl_gated_input_grad, whose tiles start anew from a 64-bit address in every step.
+PyObject* input_gradient_in_tiles(const Matrix& inner, const GatedWeight& w) {
+  const at::ScalarType type = inner.t->scalar_type();
+  const at::Tensor dx = empty({inner.rows, w.inputs}, type, inner.t->device());
+  tccl_gated_input_grad_desc d;
+  memset(&d, 0, sizeof d);
+  d.inner = inner.at, d.weight = w.at, d.dx = dx.data_ptr();
+  d.ld_inner = inner.pitch, d.ld_weight = w.pitch, d.ld_dx = w.inputs;
+  d.rows = (int32_t)inner.rows, d.inputs = (int32_t)w.inputs, d.outputs = (int32_t)w.outputs, d.dtype = code_of(type), d.kmajor = w.kmajor;
+  at::Tensor workspace;
+  if (!with_workspace(d, entry_input_grad_workspace, "tccl_gated_input_grad", inner.t->device(), workspace)) return nullptr;
+  void* stream;
+  if (!stream_now(stream)) return nullptr;
+  if (failed(entry_input_grad(&d, stream), "tccl_gated_input_grad")) return nullptr;
+  return THPVariable_Wrap(dx);
+}
+
+// input_gradient(inner, weight): inner @ weight.t(), by the kernel that splits the sum where it is the quicker one; else by the library's GEMM, which reads
+// and writes whole 16-byte vectors (an operand that does not lie in these is copied first, both in one launch, and a result whose rows do not has the
+// columns that it wants of wider rows) and reaches 4 GiB far from a tile's base: the rows of a tile, and all of a k-major weight, the last step's 64 of
+// its rows in full.  What is longer is left to the former.
 PyObject* input_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 2) return none();
   return guarded([&]() -> PyObject* {
@@ -630,21 +649,13 @@ PyObject* input_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (w.t->scalar_type() != type || inner.cols != 2 * w.outputs) return none();
     int32_t splits = 0;
     if (failed(entry_input_grad_cut((int32_t)inner.rows, (int32_t)w.inputs, (int32_t)w.outputs, 0, &splits), "tccl_gated_input_grad_cut")) return nullptr;
-    if (splits) {
-      const at::Tensor dx = empty({inner.rows, w.inputs}, type, inner.t->device());
-      tccl_gated_input_grad_desc g;
-      memset(&g, 0, sizeof g);
-      g.inner = inner.at, g.weight = w.at, g.dx = dx.data_ptr();
-      g.ld_inner = inner.pitch, g.ld_weight = w.pitch, g.ld_dx = w.inputs;
-      g.rows = (int32_t)inner.rows, g.inputs = (int32_t)w.inputs, g.outputs = (int32_t)w.outputs, g.dtype = code_of(type), g.kmajor = w.kmajor;
-      at::Tensor workspace;
-      if (!with_workspace(g, entry_input_grad_workspace, "tccl_gated_input_grad", inner.t->device(), workspace)) return nullptr;
-      void* stream;
-      if (!stream_now(stream)) return nullptr;
-      if (failed(entry_input_grad(&g, stream), "tccl_gated_input_grad")) return nullptr;
-      return THPVariable_Wrap(dx);
-    }
+    if (splits) return input_gradient_in_tiles(inner, w);
     const int64_t N = w.inputs, K = inner.cols, width = (N + 7) / 8 * 8, depth = (K + 7) / 8 * 8;
+    const bool copy_a = K != depth || inner.pitch % 8 || (uintptr_t)inner.at % 16, copy_b = N != width || K != depth || w.pitch % 8 || (uintptr_t)w.at % 16;
+    auto on_64_bytes = [](int64_t cols) { return (cols + 31) / 32 * 32; };  // as the GEMM fetches rows
+    const int64_t lda = copy_a ? on_64_bytes(depth) : inner.pitch, ldb = copy_b ? on_64_bytes(w.kmajor ? width : depth) : w.pitch;
+    const int64_t span_a = 255 * lda + depth, span_b = w.kmajor ? ((depth + 63) / 64 * 64 - 1) * ldb + width : 255 * ldb + depth;
+    if (std::max(span_a, span_b) * 2 > 0xfffffff0ll) return input_gradient_in_tiles(inner, w);
     const at::Tensor made = empty({inner.rows, width}, type, inner.t->device());
     const at::Tensor result = width == N ? made : made.narrow(1, 0, N);
     if (!inner.rows) return THPVariable_Wrap(result);
@@ -654,27 +665,20 @@ PyObject* input_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     memset(&d, 0, sizeof d);
     d.A = inner.at, d.B = w.at, d.C = made.data_ptr();
     d.M = (int32_t)inner.rows, d.N = (int32_t)width, d.K = (int32_t)depth;
-    d.lda = inner.pitch, d.ldb = w.pitch, d.ldc = width;
+    d.lda = lda, d.ldb = ldb, d.ldc = width;
     d.in_dtype = d.out_dtype = code_of(type);
     d.alpha = 1.f, d.block_m = d.block_n = 128, d.group_m = 8;
     d.flags = w.kmajor ? 0 : TCCL_GEMM_B_KMAJOR;  // of weight.t(): its columns are the weight's rows
     tccl_pack_desc jobs[2];
     int n = 0;
     at::Tensor a, b;
-    auto copied = [&](at::Tensor& to, const char* from, int64_t pitch, int64_t rows, int64_t cols, int64_t to_rows, int64_t to_cols) {
-      const int64_t to_pitch = (to_cols + 31) / 32 * 32;  // rows on 64 bytes, as the GEMM fetches them
+    auto copied = [&](at::Tensor& to, const char* from, int64_t pitch, int64_t rows, int64_t cols, int64_t to_rows, int64_t to_cols, int64_t to_pitch) {
       to = empty({to_rows, to_pitch}, type, inner.t->device());
       jobs[n++] = {from, to.data_ptr(), pitch, 1, to_pitch, (int32_t)rows, (int32_t)cols, (int32_t)to_rows, (int32_t)to_cols};
-      return to_pitch;
+      return to.data_ptr();
     };
-    if (K != depth || inner.pitch % 8 || (uintptr_t)inner.at % 16) d.lda = copied(a, inner.at, inner.pitch, inner.rows, K, inner.rows, depth), d.A = a.data_ptr();
-    if (N != width || K != depth || w.pitch % 8 || (uintptr_t)w.at % 16) {
-      if (w.kmajor)
-        d.ldb = copied(b, w.at, w.pitch, K, N, depth, width);
-      else
-        d.ldb = copied(b, w.at, w.pitch, N, K, width, depth);
-      d.B = b.data_ptr();
-    }
+    if (copy_a) d.A = copied(a, inner.at, inner.pitch, inner.rows, K, inner.rows, depth, lda);
+    if (copy_b) d.B = w.kmajor ? copied(b, w.at, w.pitch, K, N, depth, width, ldb) : copied(b, w.at, w.pitch, N, K, width, depth, ldb);
     if (n && failed(entry_pack(jobs, n, 2, stream), "tccl_pack_matrices")) return nullptr;
     if (failed(entry_gemm(&d, stream), "tccl_gemm")) return nullptr;
     return THPVariable_Wrap(result);
