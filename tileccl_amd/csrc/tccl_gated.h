@@ -23,6 +23,7 @@ struct GatedArgs {
   int activation;
   int tiles_m, tiles_n, band;
   int xcds, per_xcd;    // dies with an L2 of their own; tiles of one
+  int first, items;     // tiles ahead of this launch, tiles (of every split) up to its end
   // K split over workgroups: blocks of 64 k in each split, and where their sums go: [split][row][2 N] (NULL: nowhere, a workgroup has them all).
   int splits, blocks_per_split;
   float* partial;
@@ -35,7 +36,7 @@ struct InputGradArgs {
   int64_t ld_out, ld_partial;
   int tiles_m, tiles_n, band;
   int splits, blocks_per_split;
-  int xcds, per_xcd;
+  int xcds, per_xcd, first, items;
 };
 
 struct GatedGradArgs {
@@ -224,8 +225,8 @@ __global__ __launch_bounds__(512, 2) void gated_kernel(GatedArgs a) {
   typedef Gated<T, kTile, kBDeep, kBackward> Tile;
   __shared__ __attribute__((aligned(1024))) char gated_lds[Tile::kLds];
   // Workgroups go to the XCDs in turn; each XCD takes a run of neighbouring tiles, which share their operands in its L2.
-  const int id = (int)blockIdx.x % a.xcds * a.per_xcd + (int)blockIdx.x / a.xcds, tiles = a.tiles_m * a.tiles_n;
-  if (id >= tiles * a.splits) return;
+  const int id = a.first + (int)blockIdx.x % a.xcds * a.per_xcd + (int)blockIdx.x / a.xcds, tiles = a.tiles_m * a.tiles_n;
+  if (id >= a.items) return;
   const int split = id / tiles;
   const TileCoord at = tile_coords(id - split * tiles, a.tiles_m, a.tiles_n, a.band);
   Tile(a, gated_lds).tile(at.m * kTile, at.n * (kTile / 2), split);
@@ -445,8 +446,8 @@ __global__ __launch_bounds__(512, 2) void input_grad_kernel(InputGradArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef Product<T, 128, false, kBDeep, false> Tile;
   __shared__ __attribute__((aligned(1024))) char grad_lds[Tile::kLds];
-  const int tiles = a.tiles_m * a.tiles_n, item = (int)blockIdx.x % a.xcds * a.per_xcd + (int)blockIdx.x / a.xcds;
-  if (item >= tiles * a.splits) return;
+  const int tiles = a.tiles_m * a.tiles_n, item = a.first + (int)blockIdx.x % a.xcds * a.per_xcd + (int)blockIdx.x / a.xcds;
+  if (item >= a.items) return;
   const int split = item / tiles;
   const TileCoord at = tile_coords(item - split * tiles, a.tiles_m, a.tiles_n, a.band);
   const int m0 = at.m * 128, n0 = at.n * 128, first = split * a.blocks_per_split, all = (a.p.K + 63) / 64;

@@ -146,18 +146,31 @@ int launch_few(const char* what, GatedArgs& a, const Choice& c, bool kmajor, int
   return launched(what);
 }
 
+// All tiles of every split, in launches of at most 2^22 workgroups (a launch counts its threads in 32 bits); `launch` is given the grid of one.
+template <typename Args, typename Launch>
+int launch_tiles(const char* what, Args& a, int cus, Launch launch) {
+  const int64_t items = (int64_t)a.tiles_m * a.tiles_n * a.splits, most = 1 << 22;
+  if (items > 1 << 30) return reportf(TCCL_ERR_UNSUPPORTED, "%s: %lld tiles of the result", what, (long long)items);
+  a.xcds = cus % 8 ? 1 : 8, a.band = 4;
+  for (int64_t first = 0; first < items; first += most) {
+    const int64_t n = items - first < most ? items - first : most;
+    a.first = (int)first, a.items = (int)(first + n), a.per_xcd = (int)((n + a.xcds - 1) / a.xcds);
+    launch(dim3((unsigned)(a.xcds * a.per_xcd)));
+    const int rc = launched(what);
+    if (rc) return rc;
+  }
+  return 0;
+}
+
 template <typename T, int kTile, bool kBackward>
 int launch_tile(const char* what, GatedArgs& a, bool kmajor, int cus, hipStream_t stream) {
   a.tiles_m = (a.p.M + kTile - 1) / kTile, a.tiles_n = (a.p.N + kTile / 2 - 1) / (kTile / 2);
-  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
-  if (tiles > 1 << 22) return reportf(TCCL_ERR_UNSUPPORTED, "%s: %lld tiles of the result", what, (long long)tiles);
-  a.xcds = cus % 8 ? 1 : 8, a.per_xcd = (int)((tiles * a.splits + a.xcds - 1) / a.xcds), a.band = 4;
-  const dim3 wgs((unsigned)(a.xcds * a.per_xcd));
-  if (kmajor)
-    hipLaunchKernelGGL((gated_kernel<T, kTile, false, kBackward>), wgs, dim3(512), 0, stream, a);
-  else
-    hipLaunchKernelGGL((gated_kernel<T, kTile, true, kBackward>), wgs, dim3(512), 0, stream, a);
-  return launched(what);
+  return launch_tiles(what, a, cus, [&](dim3 wgs) {
+    if (kmajor)
+      hipLaunchKernelGGL((gated_kernel<T, kTile, false, kBackward>), wgs, dim3(512), 0, stream, a);
+    else
+      hipLaunchKernelGGL((gated_kernel<T, kTile, true, kBackward>), wgs, dim3(512), 0, stream, a);
+  });
 }
 
 template <typename T, bool kBackward>
@@ -257,16 +270,13 @@ int set_input_grad(const tccl_gated_input_grad_desc* d, InputGradArgs& a, Copies
 
 template <typename T>
 int launch_input_grad(const char* what, InputGradArgs& a, bool kmajor, int cus, hipStream_t stream) {
-  a.tiles_m = (a.p.M + 127) / 128, a.tiles_n = (a.p.N + 127) / 128, a.band = 4;
-  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
-  if (tiles > 1 << 22) return reportf(TCCL_ERR_UNSUPPORTED, "%s: %lld tiles of the result", what, (long long)tiles);
-  a.xcds = cus % 8 ? 1 : 8, a.per_xcd = (int)((tiles * a.splits + a.xcds - 1) / a.xcds);
-  const dim3 wgs((unsigned)(a.xcds * a.per_xcd));
-  if (kmajor)
-    hipLaunchKernelGGL((input_grad_kernel<T, true>), wgs, dim3(512), 0, stream, a);
-  else
-    hipLaunchKernelGGL((input_grad_kernel<T, false>), wgs, dim3(512), 0, stream, a);
-  const int rc = launched(what);
+  a.tiles_m = (a.p.M + 127) / 128, a.tiles_n = (a.p.N + 127) / 128;
+  const int rc = launch_tiles(what, a, cus, [&](dim3 wgs) {
+    if (kmajor)
+      hipLaunchKernelGGL((input_grad_kernel<T, true>), wgs, dim3(512), 0, stream, a);
+    else
+      hipLaunchKernelGGL((input_grad_kernel<T, false>), wgs, dim3(512), 0, stream, a);
+  });
   if (rc || a.splits == 1) return rc;
   const WeightSumArgs s = {a.partial, nullptr, a.out, a.ld_partial, 0, a.ld_out, a.p.M * a.ld_partial, a.p.M, a.p.N, a.splits};
   const int64_t sums = ((int64_t)a.p.M * ((a.p.N + 3) / 4) + 255) / 256;
