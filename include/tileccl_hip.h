@@ -683,8 +683,8 @@ int64_t tccl_gated_grad_workspace(const tccl_gated_grad_desc* gated);
 int tccl_gated_grad(const tccl_gated_grad_desc* gated, void* stream);
 
 /* The gradient of x from that of z: dx (rows x inputs) = inner times the weight's transpose, in tiles that split the sum over workgroups; for few rows and
- * inputs with many outputs.  `splits` of the host view _cut (compute_units 0: of the current device) is 0 where tccl_gemm is quicker.  The weight is
- * tccl_gated's, both halves in one matrix: kmajor 0: inputs rows of 2 outputs; kmajor 1: 2 outputs rows of inputs.  Alignments and the workspace
+ * inputs with many outputs, and for what tccl_gemm does not take: rows of dx that are no whole 16-byte vectors, operands beyond its 4 GiB.  `splits` of the
+ * host view _cut (compute_units 0: of the current device) is 0 where tccl_gemm is quicker.  The weight is tccl_gated's, both halves in one matrix: kmajor 0: inputs rows of 2 outputs; kmajor 1: 2 outputs rows of inputs.  Alignments and the workspace
  * as tccl_gated's; dx shares no memory with an operand. */
 typedef struct tccl_gated_input_grad_desc {
   const void* inner;

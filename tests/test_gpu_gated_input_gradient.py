@@ -1,4 +1,5 @@
-"""``dx`` of the gated layer where the GEMM does not reach over an operand: 4 GiB from a tile's base on."""
+"""``dx`` of the gated layer: where the GEMM does not reach over an operand, 4 GiB from a tile's base on, and in rows next to each other whichever kernel
+makes it."""
 
 import pytest
 import torch
@@ -59,3 +60,13 @@ def test_rows_of_inner_far_apart(layout):
     d = ops.gated_linear_backward(dh, None, x, wd, out=out)
     assert d.inner is out
     check(d, w, F16)
+
+
+@pytest.mark.parametrize("rows, inputs, outputs, layout", [(0, 13, 8, "kn"), (1, 13, 8, "nk"), (70, 65, 36, "kn"), (530, 263, 201, "nk"), (300, 264, 72, "kn"), (1500, 1001, 24, "nk"),
+                                                            (4, 1001, 4100, "kn"), (60, 333, 2000, "nk"), (3000, 2049, 300, "kn")])
+def test_rows_next_to_each_other(rows, inputs, outputs, layout):
+    w, wd = weight_of(inputs, outputs, BF16, layout, 10)
+    x, dh = rand((rows, inputs), 11, BF16).cuda(), rand((rows, outputs), 12, BF16).cuda()
+    d = ops.gated_linear_backward(dh, None, x, wd, weights=False)
+    assert d.x.shape == (rows, inputs) and d.x.is_contiguous()
+    check(d, w, BF16)

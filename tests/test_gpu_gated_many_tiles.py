@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oracle import layers as ref
-from tests.layer_bounds import BF16, SUM, gated_bounds, inner_bounds, rand, within
+from tests.layer_bounds import BF16, SUM, gated_bounds, inner_bounds, rand, rounded, within
 from tests.test_gpu_gated import weight_of
 from tileccl_amd import ops
 
@@ -50,3 +50,16 @@ def test_projections():
     want, bound = inner_bounds(dhs, g, u, inputs * SUM * s[:, :outputs], inputs * SUM * s[:, outputs:], BF16, "silu")
     within(ends(inner), want, bound, "inner")
     assert nothing_between(inner)
+
+
+@pytest.mark.parametrize("rows, inputs", [((1 << 30) + 300, 8), ((1 << 29) + 300, 13)])
+def test_input_gradient(rows, inputs):
+    outputs = 8
+    _, wd = weight_of(inputs, outputs, BF16, "kn", 4)
+    dh, _ = tall(rows, outputs, 5)
+    kept, _ = tall(rows, 2 * outputs, 6)
+    d = ops.gated_linear_backward(dh, kept, None, wd, out=kept, weights=False)
+    inner = ends(d.inner).cpu().double()
+    want = inner @ wd.cpu().double().t()
+    within(ends(d.x), want, rounded(want, 2 * outputs * SUM * (inner.abs() @ wd.cpu().double().abs().t()), BF16), "dx")
+    assert nothing_between(d.x)

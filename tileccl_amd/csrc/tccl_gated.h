@@ -438,8 +438,9 @@ __global__ __launch_bounds__(kWaves * 64, kMB == 1 && kNB == 2 ? 4 : 2) void gat
 }
 
 // dx = inner W', the tiles of Product without pairs: of few outputs and a long sum, where the GEMM's kernels, which do not split K, leave CUs without
-// work.  Sums of splits are added up by weight_sum_kernel.  Bound by
-// what comes from L2 to a CU, as gated_kernel's 128 tiles: 1024 x 2048 from 8192 42 us (the GEMM 62),
+// work, and of rows that are no whole vectors or operands that reach beyond the GEMM's windows (8192 x 4097 from 8192 545 to 628 us, the GEMM into
+// wider rows 510 to 541; 300 x 1001 from 600 9.4 to 12.7, 9.7 to 10.0; 4 x 1001 from 16384 12.9 to 28, 29 to 44).  Sums of splits are added up by
+// weight_sum_kernel.  Bound by what comes from L2 to a CU, as gated_kernel's 128 tiles: 1024 x 2048 from 8192 42 us (the GEMM 62),
 // 4142 x 232 from 7952 32 to 35 (70 to 77), 8192 x 128 from 16384 62 (81 to 95).
 template <typename T, bool kBDeep>
 __global__ __launch_bounds__(512, 2) void input_grad_kernel(InputGradArgs a) {

@@ -220,6 +220,18 @@ struct Prepared {
   }
 };
 
+// How often these kernels split a sum, from `fewest` on: what the estimate says is quickest.
+int least_splits(int rows, int inputs, int depth, int cus, int fewest) {
+  const int64_t tiles = (int64_t)((rows + 127) / 128) * ((inputs + 127) / 128);
+  const int blocks = (depth + 63) / 64;
+  int best = 0;
+  double least = 1e30;
+  for (int splits = fewest; splits <= 16 && (splits == 1 || blocks >= 4 * splits); ++splits) {
+    const double us = split_takes(tiles, blocks, splits, cus) + (splits > 1 ? join_takes(splits, rows, (inputs + 1) / 2) : 0.0);
+    if (us < least) best = splits, least = us;
+  }
+  return best;
+}
 // The gradient of x by these kernels: how often the sum is split, 0 where the library's GEMM is left to make it, which is as quick where tiles
 // are many or the sum is short (37 shapes of both layouts, this and the GEMM: 1000 x 1000 from 6000 24 to 25 us and 31 to 34, from 4096 21 and 19 to 25,
 // from 1200 16 and 10 to 11; 1 x 4096 from 8192 15 and 14 to 19; 300 x 256 from 4096 12.6 and 7.4 to 8.6; 256 x 256 from 16384 16 and 16 to 29).
@@ -227,13 +239,7 @@ int input_grad_splits(int rows, int inputs, int depth, int cus) {
   const int64_t tiles = (int64_t)((rows + 127) / 128) * ((inputs + 127) / 128);
   const int blocks = (depth + 63) / 64;
   if (rows < 64 || tiles * 2 > cus || tiles * blocks < (blocks < 256 ? 4096 : 1024)) return 0;
-  int best = 0;
-  double least = 1e30;
-  for (int splits = 2; splits <= 16 && blocks >= 4 * splits; ++splits) {
-    const double us = split_takes(tiles, blocks, splits, cus) + join_takes(splits, rows, (inputs + 1) / 2);
-    if (us < least) best = splits, least = us;
-  }
-  return best;
+  return least_splits(rows, inputs, depth, cus, 2);
 }
 
 int check_input_grad(const char* what, const tccl_gated_input_grad_desc* d) {
@@ -260,7 +266,7 @@ int set_input_grad(const tccl_gated_input_grad_desc* d, InputGradArgs& a, Copies
     p.ldb = d->kmajor ? width : whole;
   }
   a.splits = input_grad_splits(d->rows, d->inputs, depth, cus);
-  if (!a.splits) a.splits = 1;
+  if (!a.splits) a.splits = least_splits(d->rows, d->inputs, depth, cus, 1);
   a.blocks_per_split = ((depth + 63) / 64 + a.splits - 1) / a.splits;
   a.ld_partial = ((int64_t)d->inputs + 3) / 4 * 4;
   bytes = copies.bytes + (a.splits > 1 ? 4ll * a.splits * d->rows * a.ld_partial : 0);

@@ -636,9 +636,9 @@ PyObject* input_gradient_in_tiles(const Matrix& inner, const GatedWeight& w) {
 }
 
 // input_gradient(inner, weight): inner @ weight.t(), by the kernel that splits the sum where it is the quicker one; else by the library's GEMM, which reads
-// and writes whole 16-byte vectors (an operand that does not lie in these is copied first, both in one launch, and a result whose rows do not has the
-// columns that it wants of wider rows) and reaches 4 GiB far from a tile's base: the rows of a tile, and all of a k-major weight, the last step's 64 of
-// its rows in full.  What is longer is left to the former.
+// whole 16-byte vectors (an operand that does not lie in these is copied first, both in one launch), writes them and reaches 4 GiB far from a tile's
+// base: the rows of a tile, and all of a k-major weight, the last step's 64 of its rows in full.  What is longer, and rows of a result that are no
+// whole vectors, are left to the former.
 PyObject* input_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 2) return none();
   return guarded([&]() -> PyObject* {
@@ -649,23 +649,22 @@ PyObject* input_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (w.t->scalar_type() != type || inner.cols != 2 * w.outputs) return none();
     int32_t splits = 0;
     if (failed(entry_input_grad_cut((int32_t)inner.rows, (int32_t)w.inputs, (int32_t)w.outputs, 0, &splits), "tccl_gated_input_grad_cut")) return nullptr;
-    if (splits) return input_gradient_in_tiles(inner, w);
-    const int64_t N = w.inputs, K = inner.cols, width = (N + 7) / 8 * 8, depth = (K + 7) / 8 * 8;
-    const bool copy_a = K != depth || inner.pitch % 8 || (uintptr_t)inner.at % 16, copy_b = N != width || K != depth || w.pitch % 8 || (uintptr_t)w.at % 16;
+    const int64_t N = w.inputs, K = inner.cols, depth = (K + 7) / 8 * 8;
+    if (splits || N % 8) return input_gradient_in_tiles(inner, w);
+    const bool copy_a = K != depth || inner.pitch % 8 || (uintptr_t)inner.at % 16, copy_b = K != depth || w.pitch % 8 || (uintptr_t)w.at % 16;
     auto on_64_bytes = [](int64_t cols) { return (cols + 31) / 32 * 32; };  // as the GEMM fetches rows
-    const int64_t lda = copy_a ? on_64_bytes(depth) : inner.pitch, ldb = copy_b ? on_64_bytes(w.kmajor ? width : depth) : w.pitch;
-    const int64_t span_a = 255 * lda + depth, span_b = w.kmajor ? ((depth + 63) / 64 * 64 - 1) * ldb + width : 255 * ldb + depth;
+    const int64_t lda = copy_a ? on_64_bytes(depth) : inner.pitch, ldb = copy_b ? on_64_bytes(w.kmajor ? N : depth) : w.pitch;
+    const int64_t span_a = 255 * lda + depth, span_b = w.kmajor ? ((depth + 63) / 64 * 64 - 1) * ldb + N : 255 * ldb + depth;
     if (std::max(span_a, span_b) * 2 > 0xfffffff0ll) return input_gradient_in_tiles(inner, w);
-    const at::Tensor made = empty({inner.rows, width}, type, inner.t->device());
-    const at::Tensor result = width == N ? made : made.narrow(1, 0, N);
-    if (!inner.rows) return THPVariable_Wrap(result);
+    const at::Tensor dx = empty({inner.rows, N}, type, inner.t->device());
+    if (!inner.rows) return THPVariable_Wrap(dx);
     void* stream;
     if (!stream_now(stream)) return nullptr;
     tccl_gemm_desc d;
     memset(&d, 0, sizeof d);
-    d.A = inner.at, d.B = w.at, d.C = made.data_ptr();
-    d.M = (int32_t)inner.rows, d.N = (int32_t)width, d.K = (int32_t)depth;
-    d.lda = lda, d.ldb = ldb, d.ldc = width;
+    d.A = inner.at, d.B = w.at, d.C = dx.data_ptr();
+    d.M = (int32_t)inner.rows, d.N = (int32_t)N, d.K = (int32_t)depth;
+    d.lda = lda, d.ldb = ldb, d.ldc = N;
     d.in_dtype = d.out_dtype = code_of(type);
     d.alpha = 1.f, d.block_m = d.block_n = 128, d.group_m = 8;
     d.flags = w.kmajor ? 0 : TCCL_GEMM_B_KMAJOR;  // of weight.t(): its columns are the weight's rows
@@ -678,10 +677,10 @@ PyObject* input_gradient(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       return to.data_ptr();
     };
     if (copy_a) d.A = copied(a, inner.at, inner.pitch, inner.rows, K, inner.rows, depth, lda);
-    if (copy_b) d.B = w.kmajor ? copied(b, w.at, w.pitch, K, N, depth, width, ldb) : copied(b, w.at, w.pitch, N, K, width, depth, ldb);
+    if (copy_b) d.B = w.kmajor ? copied(b, w.at, w.pitch, K, N, depth, N, ldb) : copied(b, w.at, w.pitch, N, K, N, depth, ldb);
     if (n && failed(entry_pack(jobs, n, 2, stream), "tccl_pack_matrices")) return nullptr;
     if (failed(entry_gemm(&d, stream), "tccl_gemm")) return nullptr;
-    return THPVariable_Wrap(result);
+    return THPVariable_Wrap(dx);
   });
 }
 

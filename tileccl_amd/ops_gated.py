@@ -149,7 +149,7 @@ def gated_linear_backward(
     ``inner`` (rows, 2 * F): the gradient of ``x @ weight``, made of ``kept``, or, where that is None, of the product computed
     again, which is then not rounded on the way (``x`` must be the tensor itself); rounded once.  ``out`` is where it goes: ``kept``
     itself, which has no further use, or memory that lies across no operand (with ``weights`` ``x``, its checkpoint and ``add`` are some).
-    ``x``: ``inner @ weight.t()``, in ``grad``'s type; ``inputs=False``: not wanted, for instance because it is summed over ranks.
+    ``x``: ``inner @ weight.t()``, contiguous, in ``grad``'s type; ``inputs=False``: not wanted, for instance because it is summed over ranks.
     ``weight``: ``x.t() @ inner`` in ``out_dtype`` (float32 or ``grad``'s type; ``add``'s where that is given), of ``weight``'s shape and
     layout, on top of ``add`` (of that layout, too): ``ops.weight_gradient``, from ``x`` in full or its 8-bit checkpoint.
     ``weights=False``: not wanted.
