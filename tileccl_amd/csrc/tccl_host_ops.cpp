@@ -80,7 +80,7 @@ struct Matrix {
   bool open(PyObject* o, bool turned = false) {
     if (!THPVariable_Check(o)) return false;
     t = &THPVariable_Unpack(o);
-    if (!t->is_cuda() || t->layout() != at::kStrided || t->dim() != 2) return false;
+    if (!t->is_cuda() || t->layout() != at::kStrided || t->dim() != 2 || t->is_neg()) return false;
     rows = t->size(turned), cols = t->size(!turned);
     if (cols < 1 || rows > TCCL_TRAINING_MAX_ROWS || cols > INT32_MAX || (cols > 1 && t->stride(!turned) != 1)) return false;
     pitch = rows > 1 ? t->stride(turned) : cols;
@@ -115,7 +115,7 @@ struct Matrix {
 bool vector_of(PyObject* o, int64_t n, const at::Device& device, const at::Tensor*& t) {
   if (!THPVariable_Check(o)) return false;
   t = &THPVariable_Unpack(o);
-  return t->is_cuda() && t->layout() == at::kStrided && t->dim() == 1 && t->size(0) == n && t->device() == device && (n <= 1 || t->stride(0) == 1);
+  return t->is_cuda() && t->layout() == at::kStrided && t->dim() == 1 && t->size(0) == n && t->device() == device && (n <= 1 || t->stride(0) == 1) && !t->is_neg();
 }
 
 struct Held {
@@ -476,7 +476,7 @@ struct GatedWeight {
   bool open(PyObject* o) {
     if (!THPVariable_Check(o)) return false;
     t = &THPVariable_Unpack(o);
-    if (!on_device0(*t) || t->layout() != at::kStrided || t->dim() != 2) return false;
+    if (!on_device0(*t) || t->layout() != at::kStrided || t->dim() != 2 || t->is_neg()) return false;
     inputs = t->size(0), outputs = t->size(1) / 2;
     if (inputs < 1 || outputs < 1 || t->size(1) % 2 || inputs > TCCL_GATED_MAX_COLS || outputs > TCCL_GATED_MAX_COLS || !sixteen_bits(t->scalar_type())) return false;
     at = (char*)t->data_ptr();
@@ -733,7 +733,7 @@ bool flat_of(PyObject* o, at::ScalarType type, int64_t least, const at::Tensor*&
   if (!THPVariable_Check(o)) return false;
   t = &THPVariable_Unpack(o);
   return on_device0(*t) && t->layout() == at::kStrided && t->dim() == 1 && t->scalar_type() == type && t->numel() >= least && (t->numel() <= 1 || t->stride(0) == 1) &&
-         !((uintptr_t)t->data_ptr() % 16 && type != at::kByte);
+         !t->is_neg() && !((uintptr_t)t->data_ptr() % 16 && type != at::kByte);
 }
 
 // A number, or a device tensor of one element that holds it.

@@ -17,7 +17,7 @@ from typing import Any, NamedTuple, NoReturn, Sequence
 import torch
 
 from tileccl_amd import _lib, ops_training
-from tileccl_amd.ops_training import _unexplained
+from tileccl_amd.ops_training import _not_negated, _unexplained
 
 __all__ = ["AdamWState", "adamw_step", "adamw_moments"]
 
@@ -115,10 +115,11 @@ def _tensor(t: Any, name: str, op: str) -> None:
         raise ValueError(f"{op}: {name} must be a tensor, got {type(t).__name__}")
     if not t.is_cuda or t.device.index != 0:
         raise ValueError(f"{op}: {name} must reside on cuda:0, got {t.device}")
+    _not_negated(t, name, op)
 
 
 def _flat(t: Any, name: str, op: str, dtype: torch.dtype, least: int, aligned: bool = True) -> None:
-    _tensor(t, name, op)
+    _tensor(t, f"the state's {name}", op)
     if t.ndim != 1 or not t.is_contiguous() or t.dtype != dtype or t.numel() < least or (aligned and t.data_ptr() % 16):
         raise ValueError(f"{op}: the state's {name} must be {least} or more contiguous elements of {dtype}{' on 16 bytes' if aligned else ''}, "
                          f"got {t.dtype} {tuple(t.shape)}")
@@ -133,7 +134,7 @@ def _refuse_adamw_step(params, grads, state, step, lr, grad_scale) -> NoReturn:
     for i, (p, g, n) in enumerate(zip(params, grads, state.sizes)):
         for t, name in ((p, f"params[{i}]"), (g, f"grads[{i}]")):
             _tensor(t, name, op)
-            if not t.is_contiguous() or t.is_neg():
+            if not t.is_contiguous():
                 raise ValueError(f"{op}: {name} must be contiguous, got strides {tuple(t.stride())}")
         if p.dtype not in _TYPES or p.dtype != params[0].dtype:
             raise ValueError(f"{op}: params must share float32, float16 or bfloat16, got {p.dtype} in params[{i}]")

@@ -21,7 +21,7 @@ from typing import Any, NamedTuple, NoReturn
 import torch
 
 from tileccl_amd import _lib, ops_training
-from tileccl_amd.ops_training import ActivationCheckpoint, _apart, _bytes_of, _clear, _held, _matrix, _span, _unexplained, weight_gradient
+from tileccl_amd.ops_training import ActivationCheckpoint, _apart, _bytes_of, _clear, _held, _matrix, _not_negated, _span, _unexplained, weight_gradient
 
 __all__ = ["GatedLinearResult", "GatedLinearGradients", "gated_linear", "gated_linear_backward"]
 
@@ -59,6 +59,7 @@ def _weight(w: Any, op: str) -> None:
     if not w.is_cuda:
         raise ValueError(f"{op}: weight must reside on the GPU, got {w.device}")
     _device0(w, "weight", op)
+    _not_negated(w, "weight", op)
     inputs, columns = w.shape
     if columns % 2 or not columns or not inputs:
         raise ValueError(f"{op}: weight must be (inputs, 2 * outputs), got {tuple(w.shape)}")

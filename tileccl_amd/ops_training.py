@@ -117,12 +117,18 @@ def _unexplained(op: str) -> NoReturn:
     raise RuntimeError(f"{op}: arguments were refused for no reason that is known here")
 
 
+def _not_negated(t: torch.Tensor, name: str, op: str) -> None:
+    if t.is_neg():
+        raise ValueError(f"{op}: {name} is a view of negated values, call resolve_neg() on it")
+
+
 def _matrix(t: Any, name: str, op: str, *, like: torch.Tensor | None = None, shape: tuple[int, int] | None = None, dtype=None) -> int:
     """Checks a 2-D device tensor with contiguous rows; its row pitch."""
     if not isinstance(t, torch.Tensor) or t.ndim != 2:
         raise ValueError(f"{op}: {name} must be a 2-D tensor, got {getattr(t, 'ndim', type(t).__name__)}")
     if not t.is_cuda:
         raise ValueError(f"{op}: {name} must reside on the GPU, got {t.device}")
+    _not_negated(t, name, op)
     if like is not None:
         shape, dtype = tuple(like.shape), like.dtype
         if t.device != like.device:
@@ -148,6 +154,7 @@ def _vector(t: Any, name: str, op: str, n: int, device: torch.device, types: tup
     if not isinstance(t, torch.Tensor) or t.shape != (n,) or t.device != device or t.dtype not in types or not t.is_contiguous():
         got = f"{tuple(t.shape)} {t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
         raise ValueError(f"{op}: {name} must be a contiguous vector of {n} elements of {' or '.join(map(str, types))} on {device}, got {got}")
+    _not_negated(t, name, op)
 
 
 def _held(c: Any, op: str, device: torch.device | None = None) -> None:
