@@ -54,7 +54,8 @@ TCCL_D float logistic(float x) { return __builtin_amdgcn_rcpf(1.f + exp_of(-x));
 // act(g) and, if wanted, act'(g).
 //
 // gelu is g Phi(g).  Phi(-a) = erfcx(a / sqrt 2) exp(-a^2 / 2) / 2 keeps its relative accuracy where Phi is small: erfcx(y) is
-// t Q(t) with t = 1 / (1 + y / 2), Q of degree 8 fitted to it over y in [0, 12] (largest relative error 4.4e-8, 4e-7 as it is computed).
+// t Q(t) with t = 1 / (1 + y / 2), Q of degree 8 fitted to it over y in [0, 12] (largest relative error 6.9e-8 with these coefficients, 4e-7 as it is
+// computed; further out exp(-a^2 / 2) is 0).
 // gelu_tanh is g s(2 c (g + k g^3)), s the logistic function: (1 + tanh z) / 2 = s(2 z).  Beyond |g| = 64 s is 0 or 1 and its derivative 0;
 // the bound keeps g^3 finite (and a NaN what it is).
 template <int kAct, bool kSlope>
