@@ -2,7 +2,7 @@
 that read a scalar register too soon.
 
 ``python -m tileccl_amd.csrc.check_spills`` compiles the library's sources to
-assembly (some five minutes) and, for every ``gemm256_kernel`` / ``fused256_kernel`` / ``weight_gradient_kernel`` /
+assembly (some ten minutes) and, for every ``gemm256_kernel`` / ``fused256_kernel`` / ``weight_gradient_kernel`` /
 ``weight_full_kernel`` / ``gated_kernel`` / ``gated_rows_kernel`` / ``input_grad_kernel`` instantiation, counts the scratch-memory instructions that lie between the kernel's first and last
 MFMA, i.e. inside its K loops.  A register that the compiler keeps in scratch memory there is
 reloaded through the same queue as the operand loads, so the reload waits for all of them: a

@@ -217,9 +217,10 @@ struct Gated : Product<T, kTile, false, kBDeep, true> {
 };
 
 // 8192 x 4096 x 8192 bf16, k-major: 803 us, 1.37 PFLOP/s, the matrix pipes busy 67 % of a clock that the load holds at 1.9 GHz (the vendor
-// library's product alone 794).  4096 x 4096 x 4096 by rows with z kept 214 us, 1.28 PFLOP/s.  128 tiles are bound by what comes from L2 to a
-// CU, 64 KiB for 4.2 MFLOP at 67 KB a microsecond: 1003 x 1001 x 1035 16 us.  Of a short sum the epilogue is the larger part, bound by the vector
-// instructions of the activation (silu 13 a value, gelu 25, 30 with its derivative): 12628 x 208 x 808, gelu, 33 us, backward 47, memory 10.
+// library's product alone 794).  4096 x 4096 x 4096 by rows with z kept 214 us, 1.28 PFLOP/s.  128 tiles take 0.95 us for a turn of 4.2 MFLOP and the 64 KiB
+// that it reads, with no other turn's loads under way beneath it and one workgroup a CU: 1003 x 1001 x 1035 16 us.  Of a short sum the start, the
+// few steps and the epilogue follow one another with nothing beneath them: 12628 x 208 x 808, gelu, 33 us, backward 47, where memory takes 10 and the vector
+// instructions of the activation (silu 13 a value, gelu 25, 30 with its derivative) 8, 13 with the second round that does not fill the device.
 template <typename T, int kTile, bool kBDeep, bool kBackward>
 __global__ __launch_bounds__(512, 2) void gated_kernel(GatedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -243,7 +244,8 @@ __global__ __launch_bounds__(512, 2) void gated_kernel(GatedArgs a) {
 // c ^ ((r >> 1) & 7).  A weight by rows: of each k row 16 kNB bytes of either matrix, next to each other in LDS; its 32-byte units are permuted
 // (unit()) so that the rows that a transposing read touches at a time lie in different banks.
 //
-// Bound by memory: 1 x 4096 x 8192 bf16, k-major, 23.3 us, 5.8 TB/s; 13 x 4096 x 4096 fp16 by rows 14.8 us, 4.5 TB/s (rows that are a power of two
+// Bound by memory: 1 x 4096 x 8192 bf16, k-major, 24.0 us, 5.6 TB/s, over weights of 2 GiB in turn (over one, which the last-level cache
+// holds, 21.2); 13 x 4096 x 4096 fp16 by rows 14.8 us, 4.5 TB/s (rows that are a power of two
 // apart lie in few of the L2's channels at a time), and 3 to 4 for the join; in tiles of 32 outputs, that is 64 bytes of a row, 26.
 template <typename T, int kMB, int kNB, int kWaves, bool kBDeep>
 struct GatedRows {
@@ -441,7 +443,7 @@ __global__ __launch_bounds__(kWaves * 64, kMB == 1 && kNB == 2 ? 4 : 2) void gat
 // dx = inner W', the tiles of Product without pairs: of few outputs and a long sum, where the GEMM's kernels, which do not split K, leave CUs without
 // work, and of rows that are no whole vectors or operands that reach beyond the GEMM's windows (8192 x 4097 from 8192 545 to 628 us, the GEMM into
 // wider rows 510 to 541; 300 x 1001 from 600 9.4 to 12.7, 9.7 to 10.0; 4 x 1001 from 16384 12.9 to 28, 29 to 44).  Sums of splits are added up by
-// weight_sum_kernel.  Bound by what comes from L2 to a CU, as gated_kernel's 128 tiles: 1024 x 2048 from 8192 42 us (the GEMM 62),
+// weight_sum_kernel.  Bound by its turns, as gated_kernel's 128 tiles: 1024 x 2048 from 8192 42 us (the GEMM 62),
 // 4142 x 232 from 7952 32 to 35 (70 to 77), 8192 x 128 from 16384 62 (81 to 95).
 template <typename T, bool kBDeep>
 __global__ __launch_bounds__(512, 2) void input_grad_kernel(InputGradArgs a) {

@@ -5,7 +5,7 @@
 //
 // 256 tiles: 8192 x 4096 outputs from 4096 tokens, bf16, 235 us as 16 bits (1.17 PFLOP/s; the vendor library 244 to 248); as fp32 on top of another 252,
 // the matrix pipes busy 48 %: 64 + 64 MiB of fp32 behind the last step, which one tile a CU cannot overlap.  128 tiles, like the gated
-// layer's, are bound by what comes from L2 to a CU: 1024 x 512 from 16384 tokens in eight splits 23.5 us, and 4.4 for the sums.
+// layer's, are bound by turns of 0.95 us with one turn's loads under way: 1024 x 512 from 16384 tokens in eight splits 23.5 us, and 4.4 for the sums.
 #pragma once
 
 #include "tccl_weight.h"
